@@ -23,6 +23,8 @@ ROOT = os.path.dirname(os.path.abspath(__file__))
 PKG = os.path.join(ROOT, "distributeddeeplearning_amd")
 BUILD = os.path.join(ROOT, "build")
 ARCH = "gfx950"
+# the packed fp32 forms (v_pk_fma_f32 and its kin) are kept out of all device code: some of them gave wrong results
+NO_PACKED_FP32 = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 
 
 def _hipcc():
@@ -55,7 +57,7 @@ def build_kernels(force=False, jobs=8, verbose=True):
     os.makedirs(os.path.join(BUILD, "kernels"), exist_ok=True)
     hipcc = _hipcc()
     flags = ["-O3", "-std=c++17", "-fPIC", "--offload-arch=" + ARCH, "-fno-math-errno", "-ffp-contract=fast",
-             "-fno-gpu-sanitize", "-Wno-unused-result", "-I", os.path.join(ROOT, "csrc", "kernels")]
+             "-fno-gpu-sanitize", "-Wno-unused-result", "-I", os.path.join(ROOT, "csrc", "kernels")] + NO_PACKED_FP32
     flags += os.environ.get("DDL_EXTRA_HIPCC_FLAGS", "").split()  # e.g. -DDDL_CONV_PROBES (timing probes)
     todo, objs = [], []
     for s in srcs:
@@ -124,7 +126,7 @@ def build_probes(force=False, verbose=True):
         out = s[:-4]
         if force or _newer(out, [s]):
             _run([hipcc, "-O3", "-std=c++17", "--offload-arch=" + ARCH, "-fno-gpu-sanitize",
-                  "-Wno-unused-result", "-o", out, s])
+                  "-Wno-unused-result"] + NO_PACKED_FP32 + ["-o", out, s])
             if verbose:
                 print("[build] built", os.path.relpath(out, ROOT), flush=True)
         outs.append(out)
