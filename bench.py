@@ -38,7 +38,7 @@ import distributeddeeplearning_amd.torch as hvd  # noqa: E402
 from distributeddeeplearning_amd.data.synthetic import DeviceSyntheticLoader  # noqa: E402
 from distributeddeeplearning_amd.models import build_model  # noqa: E402
 from distributeddeeplearning_amd.ops import functional as ops  # noqa: E402
-from distributeddeeplearning_amd.optim import FusedLARS, FusedSGD  # noqa: E402
+from distributeddeeplearning_amd.optim import FusedLARS, FusedMuon, FusedSGD  # noqa: E402
 
 # Stock PyTorch-ROCm (MIOpen, bf16 autocast, channels_last) ResNet-50 batch 256 on one MI355X,
 # measured with benchmarks/stock_pytorch.py — see BASELINE.md.  The reference itself
@@ -62,7 +62,7 @@ def parse_args(argv=None):
     ap.add_argument("--warmup", type=int, default=8)
     ap.add_argument("--batch", type=int, default=256, help="per-GPU batch (BASELINE config: 256)")
     ap.add_argument("--model", default="resnet50")
-    ap.add_argument("--optimizer", default="sgd", choices=["sgd", "lars"])
+    ap.add_argument("--optimizer", default="sgd", choices=["sgd", "lars", "muon"])
     ap.add_argument("--dtype", default="bf16", choices=["bf16", "fp32"])
     ap.add_argument("--device", default=None, help="cuda|cpu (default: cuda when available)")
     ap.add_argument("--image", type=int, default=224)
@@ -112,6 +112,8 @@ def main(argv=None):
     lr = 0.001 * world
     if args.optimizer == "lars":
         opt = FusedLARS(model.named_parameters(), lr=lr, momentum=0.9, weight_decay=5e-5)
+    elif args.optimizer == "muon":
+        opt = FusedMuon(model.named_parameters(), lr=lr, momentum=0.95)
     else:
         opt = FusedSGD(model.named_parameters(), lr=lr, momentum=0.9)
     opt = hvd.DistributedOptimizer(opt, named_parameters=model.named_parameters())

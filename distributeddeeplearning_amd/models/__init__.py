@@ -1,5 +1,5 @@
 from .resnet import (ResNet, resnet, resnet18, resnet34, resnet50, resnet101, resnet152,
-                     resnet200, DEPTHS, count_parameters)
+                     resnet200, DEPTHS, Int8Linear, count_parameters)
 
 
 def build_model(name: str, **kw):

@@ -29,7 +29,7 @@ import torch.nn as nn
 from ..ops import functional as ops
 
 __all__ = ["ResNet", "resnet", "resnet18", "resnet34", "resnet50", "resnet101", "resnet152",
-           "resnet200", "DEPTHS", "Conv2d", "BatchNormAct", "Linear", "Bottleneck",
+           "resnet200", "DEPTHS", "Conv2d", "BatchNormAct", "Linear", "Int8Linear", "Bottleneck",
            "BasicBlock", "count_parameters"]
 
 DEPTHS = {
@@ -135,6 +135,33 @@ class Linear(nn.Module):
 
     def forward(self, x):
         return ops.linear(x, self.weight, self.bias)
+
+
+class Int8Linear(nn.Module):
+    """Dense layer that answers from 8-bit weights (``ops.linear_int8``): codes with a scale for each output channel,
+    the input's rows quantised on the way.  Buffers only: it does not train."""
+
+    def __init__(self, cin, cout, bias=True):
+        super().__init__()
+        self.in_features = cin
+        # (rows are padded to multiples of 64 bytes, as quantize_int8 lays them out)
+        self.register_buffer("codes", torch.zeros(cout, (cin + 63) // 64 * 64, dtype=torch.int8))
+        self.register_buffer("scale", torch.zeros(cout))
+        self.register_buffer("bias", torch.zeros(cout) if bias else None)
+
+    @classmethod
+    def from_linear(cls, linear):
+        w = linear.weight.detach()
+        m = cls(w.shape[1], w.shape[0], linear.bias is not None).to(w.device)
+        q, scale = ops.quantize_int8(w)
+        m.codes[:, :w.shape[1]].copy_(q)
+        m.scale.copy_(scale)
+        if linear.bias is not None:
+            m.bias.copy_(linear.bias.detach())
+        return m
+
+    def forward(self, x):
+        return ops.linear_int8(x, self.codes[:, :self.in_features], self.scale, self.bias)
 
 
 class _Downsample(nn.Sequential):
@@ -275,6 +302,13 @@ class ResNet(nn.Module):
             elif isinstance(m, Linear):
                 m.weight.data = m.weight.data.to(dtype)
         return self
+
+
+    def int8_head(self):
+        """For answering: the classifier head from 8-bit weights (:class:`Int8Linear`), taken from the present ones.  The
+        model no longer trains afterwards, and its ``state_dict`` holds codes and scales in the place of ``fc.weight``."""
+        self.fc = Int8Linear.from_linear(self.fc)
+        return self.eval()
 
 
 def resnet(depth, **kw):

@@ -25,7 +25,7 @@ import torch
 import torch.nn.functional as F
 
 __all__ = ["use_hip", "conv2d", "conv_bn_act", "residual_block", "batchnorm_act", "maxpool3x3s2", "global_avgpool", "linear",
-           "softmax_cross_entropy", "topk_correct", "topk_hits", "NoHipKernel", "set_backend", "backend"]
+           "orthogonalize", "quantize_int8", "linear_int8", "softmax_cross_entropy", "topk_correct", "topk_hits", "NoHipKernel", "set_backend", "backend"]
 
 _FORCED = os.environ.get("DDL_OPS", "auto").lower()  # auto | hip | aten
 
@@ -198,6 +198,139 @@ def linear(x, weight, bias=None):
             return hip_ops.linear(x, weight, bias)
         _no_kernel("linear", "in=%d out=%d on a %d-d input" % (weight.shape[1], weight.shape[0], x.dim()))
     return F.linear(x, weight.to(x.dtype), None if bias is None else bias.to(x.dtype))
+
+
+ORTHO_COEFFICIENTS = (3.4445, -4.7750, 2.0315)   # five steps take singular values from about 0.002 on into [0.7, 1.2]
+
+
+def _check_steps(steps, coefficients, eps):
+    if not isinstance(steps, int) or not 0 <= steps <= 64:
+        raise ValueError("orthogonalize: steps must be an integer from 0 to 64, got %r" % (steps,))
+    if len(coefficients) != 3:
+        raise ValueError("orthogonalize: three coefficients expected, got %r" % (coefficients,))
+    if not eps >= 1e-30:
+        raise ValueError("orthogonalize: eps must be at least 1e-30, got %r" % (eps,))
+
+
+def orthogonalize_plain(x, steps=5, coefficients=ORTHO_COEFFICIENTS, eps=1e-7):
+    """The steps of :func:`orthogonalize` in plain PyTorch, computed and returned in fp32 (fp64 for an fp64 input)."""
+    a, b, c = coefficients
+    x = x if x.dtype == torch.float64 else x.float()
+    turn = x.shape[-2] > x.shape[-1]
+    if turn:
+        x = x.transpose(-2, -1)
+    x = x / x.double().square().sum(dim=(-2, -1), keepdim=True).sqrt().clamp_min(eps).to(x.dtype)
+    for _ in range(steps):
+        gram = x @ x.transpose(-2, -1).contiguous()
+        x = a * x + (b * gram + c * (gram @ gram)) @ x
+    return x.transpose(-2, -1) if turn else x
+
+
+def orthogonalize(x, steps=5, coefficients=ORTHO_COEFFICIENTS, eps=1e-7):
+    """Newton-Schulz orthogonalisation: ``X = G / max(|G|_F, eps)``, then ``steps`` times ``X <- a X + (b A + c A^2) X``
+    with ``A = X X^T`` over the shorter side - every singular value of ``G`` is driven towards 1, its vectors stay.
+
+    ``x``: a matrix [r, c], a stack [k, r, c], or a list / tuple of matrices of any shapes (they share the launches), fp32 or
+    bf16 of any strides; returns bf16 of the same shape(s).  No gradient flows through it: an input that requires one is
+    refused outside ``torch.no_grad()``.  Matrices do not influence each other; one that holds an infinity or a NaN
+    gives NaN, a zero matrix zeros.  ``coefficients`` whose steps leave the range of 16-bit operands are refused."""
+    many = isinstance(x, (list, tuple))
+    mats = list(x) if many else [x]
+    _check_steps(steps, coefficients, eps)
+    for m in mats:
+        if m.dim() != 2 and (many or m.dim() != 3):
+            raise ValueError("orthogonalize: a matrix, a stack of matrices or a list of matrices expected, got shape %s" % (tuple(m.shape),))
+        if m.dtype not in (torch.float32, torch.bfloat16):
+            raise ValueError("orthogonalize: fp32 or bf16 expected, got %s" % m.dtype)
+        if m.device != mats[0].device or m.dtype != mats[0].dtype:
+            raise ValueError("orthogonalize: the matrices of a list must share device and dtype")
+        if m.requires_grad and torch.is_grad_enabled():
+            raise ValueError("orthogonalize: no gradient flows through it; detach the input or call it under torch.no_grad()")
+    if not mats:
+        return []
+    out = None
+    if mats[0].is_cuda and _FORCED != "aten":
+        from . import kernels
+
+        if kernels.require():
+            from . import hip_ops
+
+            if not kernels.ortho_coefficients_ok(*(float(v) for v in coefficients), steps):
+                raise ValueError("orthogonalize: %d steps with the coefficients %r leave the range of the kernels' 16-bit operands"
+                                 % (steps, tuple(coefficients)))
+            out = hip_ops.orthogonalize(mats, steps, tuple(float(v) for v in coefficients), float(eps))
+    if out is None:
+        with torch.no_grad():
+            out = [orthogonalize_plain(m, steps, coefficients, eps).to(torch.bfloat16).contiguous() for m in mats]
+    return out if many else out[0]
+
+
+_INT8_TINY = 1e-30
+
+
+def quantize_int8(w):
+    """8-bit codes of the rows of ``w`` [n, k] (fp32 or bf16): ``(q, scale)`` with ``q`` int8 [n, k], ``scale`` fp32 [n] and
+    ``w ~ q * scale[:, None]``; ``scale = max|row| / 127``, ``q = round(row * (127 / max|row|))`` to even.  Rows of ``q`` start
+    at multiples of 64 bytes, as :func:`linear_int8` reads them.  A row below 1e-30 counts as zero; one that holds an
+    infinity or a NaN has the scale NaN."""
+    if w.dim() != 2 or w.dtype not in (torch.float32, torch.bfloat16) or w.shape[1] == 0:
+        raise ValueError("quantize_int8: an fp32 or bf16 matrix with columns expected, got %s %s" % (w.dtype, tuple(w.shape)))
+    w = w.detach()
+    n, k = w.shape
+    if w.is_cuda and _FORCED != "aten":
+        from . import kernels
+
+        if kernels.require():
+            from . import hip_ops
+
+            return hip_ops.quantize_int8(w)
+    store = torch.zeros((n, (k + 63) // 64 * 64), dtype=torch.int8, device=w.device)
+    q, scale = _int8_rows_plain(w)
+    store[:, :k] = q
+    return store[:, :k], scale
+
+
+def _int8_rows_plain(x):
+    x = x.float()
+    top = x.abs().amax(dim=1)
+    zero = top < _INT8_TINY
+    bad = ~torch.isfinite(top)
+    inv = torch.where(zero | bad, torch.zeros_like(top), 127.0 / top)
+    q = torch.where((zero | bad)[:, None], torch.zeros_like(x), torch.round(x * inv[:, None]))
+    scale = torch.where(zero, torch.zeros_like(top), torch.where(bad, torch.full_like(top, float("nan")), top / 127.0))
+    return q.to(torch.int8), scale
+
+
+def linear_int8(x, q, scale, bias=None):
+    """Dense layer on 8-bit integers, for answering: the rows of ``x`` [..., k] (fp32 or bf16) are quantised like
+    :func:`quantize_int8` does, each with a scale of its own, multiplied with the codes ``q`` [n, k] and ``scale`` [n] of the weights
+    and summed exactly: ``y = (xq q^T) * sx * scale + bias`` in fp32, returned in ``x``'s dtype [..., n].  ``bias``: fp32 [n].
+    ``q`` as :func:`quantize_int8` returns it (rows start at multiples of 16 bytes).  No gradient flows through it: an input
+    that requires one is refused outside ``torch.no_grad()``.  ``k`` is at most 133 144."""
+    if x.dtype not in (torch.float32, torch.bfloat16) or x.dim() < 1:
+        raise ValueError("linear_int8: fp32 or bf16 rows expected, got %s" % x.dtype)
+    if q.dtype != torch.int8 or q.dim() != 2 or q.shape[1] != x.shape[-1] or not 0 < q.shape[1] <= 133144:
+        raise ValueError("linear_int8: int8 codes [n, %d] of at most 133144 columns expected, got %s %s" % (x.shape[-1], q.dtype, tuple(q.shape)))
+    for name, t in (("scale", scale), ("bias", bias)):
+        if t is not None and (t.dtype != torch.float32 or t.shape != q.shape[:1]):
+            raise ValueError("linear_int8: %s must be fp32 [%d], got %s %s" % (name, q.shape[0], t.dtype, tuple(t.shape)))
+    if any(t is not None and t.device != x.device for t in (q, scale, bias)):
+        raise ValueError("linear_int8: input, codes, scales and bias must be on one device")
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, scale, bias)):
+        raise ValueError("linear_int8: no gradient flows through it; call it under torch.no_grad()")
+    x2 = x.reshape(-1, x.shape[-1]) if x.numel() else x.new_empty((x.shape[:-1].numel(), x.shape[-1]))
+    if x.is_cuda and _FORCED != "aten":
+        from . import kernels
+
+        if kernels.require():
+            from . import hip_ops
+
+            return hip_ops.linear_int8(x2, q, scale, bias).view(x.shape[:-1] + q.shape[:1])
+    xq, sx = _int8_rows_plain(x2)
+    # (fp64 sums: whole numbers up to 2^31 are exact)
+    y = (xq.double() @ q.double().t()).float() * (sx[:, None] * scale[None, :])
+    y = y if bias is None else y + bias
+    return y.to(x.dtype).view(x.shape[:-1] + q.shape[:1])
 
 
 def softmax_cross_entropy(logits, target):

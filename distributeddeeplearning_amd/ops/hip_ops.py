@@ -1847,6 +1847,55 @@ def linear(x, weight, bias):
     return LinearFn.apply(x, weight, bias)
 
 
+def quantize_int8(w):
+    n, k = w.shape
+    if w.stride(1) != 1:
+        w = w.contiguous()
+    store = torch.empty((n, (k + 63) // 64 * 64), dtype=torch.int8, device=w.device)
+    scale = torch.empty(n, dtype=torch.float32, device=w.device)
+    with torch.cuda.device(w.device):
+        K.int8_rows(w, store, scale)
+    return store[:, :k], scale
+
+
+def linear_int8(x, q, scale, bias):
+    """``functional.linear_int8`` of a 2-d input."""
+    n, k = q.shape
+    if q.stride(1) != 1 or q.stride(0) % 16 or q.data_ptr() % 16 or K.storage_numel_from(q) < (n - 1) * q.stride(0) + (k + 15) // 16 * 16:
+        raise K.KernelError("linear_int8: the rows of the codes must start at multiples of 16 bytes and be readable to the next one behind "
+                            "their end: take them from quantize_int8 (strides %s)" % (q.stride(),))
+    if x.stride(1) != 1 or x.stride(0) < 0:
+        x = x.contiguous()
+    y = torch.empty((x.shape[0], n), dtype=x.dtype, device=x.device)
+    with torch.cuda.device(x.device):
+        K.int8_linear(x, q, scale.contiguous(), None if bias is None else bias.contiguous(), y)
+    return y
+
+
+# ----------------------------------------------------------------------------------------------
+# orthogonalisation
+# ----------------------------------------------------------------------------------------------
+def orthogonalize(mats, steps, coefficients, eps):
+    """``functional.orthogonalize`` of a list: all matrices (and stacks) of a call share its launches."""
+    outs = [torch.empty(m.shape, dtype=_BF16, device=m.device) for m in mats]
+    groups, keep = [], []
+    for m, o in zip(mats, outs):
+        if m.numel() == 0:
+            continue
+        m3, o3 = (m, o) if m.dim() == 3 else (m[None], o[None])
+        if max(m3.stride()[1:]) >= 1 << 31:
+            m3 = m3.contiguous()
+            keep.append(m3)
+        groups.append((m3.data_ptr(),) + m3.stride() + (o.data_ptr(),) + o3.stride() + (m3.shape[1], m3.shape[2], m3.shape[0]))
+    per = K.ortho_max_groups()
+    with torch.cuda.device(mats[0].device):
+        for k in range(0, len(groups), per):
+            table, count = K.ortho_table(groups[k:k + per])
+            work = torch.empty(K.ortho_workspace(table, count), dtype=torch.uint8, device=mats[0].device)
+            K.orthogonalize(table, count, mats[0].dtype == _BF16, coefficients, steps, eps, work)
+    return outs
+
+
 # ----------------------------------------------------------------------------------------------
 # loss
 # ----------------------------------------------------------------------------------------------

@@ -250,6 +250,86 @@ def nchw_to_nhwc_normalize(x, mean=None, sd=None, in_scale=1.0):
     return out.permute(0, 3, 1, 2)
 
 
+# ---- orthogonalisation, the optimizer step on it (csrc/kernels/orthogonalize.hip) -------------
+@functools.lru_cache(maxsize=None)
+def ortho_max_groups():
+    """Most groups of equal matrices that one call takes."""
+    return int(lib().ddl_ortho_max_groups())
+
+
+def ortho_table(groups):
+    """Table of a call: ``groups`` = (source address, its batch / row / column strides, destination address and strides,
+    rows, columns, matrices) tuples."""
+    flat = [int(v) for g in groups for v in g]
+    return (ctypes.c_longlong * len(flat))(*flat), len(flat) // 11
+
+
+@functools.lru_cache(maxsize=None)
+def ortho_coefficients_ok(a, b, c, steps):
+    """True when these steps keep every operand in the range of the kernels' scaled fp16 values."""
+    f = _fn("ddl_ortho_coefficients_ok", "fff i")
+    return bool(f(a, b, c, steps))
+
+
+def ortho_workspace(table, count):
+    f = getattr(lib(), "ddl_ortho_workspace")
+    f.restype = ctypes.c_longlong
+    n = int(f(table, _i32(count)))
+    if n < 0:
+        raise KernelError("orthogonalize: sizes out of range")
+    return n
+
+
+def orthogonalize(table, count, src_bf16, coefficients, steps, eps, work):
+    """bf16 destinations <- the orthogonalised sources of ``table`` (:func:`ortho_table`)."""
+    f = _fn("ddl_orthogonalize", "p ii fff i f p q p")
+    check(f(table, count, 1 if src_bf16 else 0, coefficients[0], coefficients[1], coefficients[2], steps, eps, work.data_ptr(),
+            work.numel(), _raw_stream()), "orthogonalize")
+
+
+def muon_step_(table, count, w, g, v, lowp, lr, mu, wd, nesterov, lr_scale, coefficients, steps, eps, work):
+    """One step over the matrices of ``table`` (offsets into the arenas in the place of the source's batch stride):
+    v = mu*v + g; u = g + mu*v (nesterov) or v; w = w*(1 - lr*wd) - lr*sqrt(max(1, rows/columns))*orthogonalize(u)."""
+    n = w.numel()
+    if w.dtype != torch.float32 or v.dtype != torch.float32 or v.numel() != n or g.numel() != n or \
+            g.dtype not in (torch.float32, torch.bfloat16) or (lowp is not None and (lowp.dtype != torch.bfloat16 or lowp.numel() != n)):
+        raise KernelError("muon_step: fp32 weights and momentum, fp32 or bf16 gradients and a bf16 copy of one length expected")
+    for i in range(count):
+        at, r, c = table[11 * i + 1], table[11 * i + 8], table[11 * i + 9]
+        if at + r * c > n:
+            raise KernelError("muon_step: matrix %d ends behind the arenas" % i)
+    f = _fn("ddl_muon_step", "p i pppp i fff i p fff i f p q p")
+    check(f(table, count, w.data_ptr(), g.data_ptr(), v.data_ptr(), _p(lowp), 1 if g.dtype == torch.bfloat16 else 0, lr, mu, wd,
+            1 if nesterov else 0, _p(lr_scale), coefficients[0], coefficients[1], coefficients[2], steps, eps, work.data_ptr(),
+            work.numel(), _raw_stream()), "muon_step")
+
+
+# ---- dense layer on 8-bit integers (csrc/kernels/int8_linear.hip) -----------------------------
+@functools.lru_cache(maxsize=None)
+def int8_max_k():
+    """Longest row whose sum of products of two codes is exact in int32."""
+    return int(lib().ddl_int8_max_k())
+
+
+def int8_rows(x, q, scale):
+    """Codes ``q`` [M, Kp] (zeros behind x's columns) and scales of the rows of ``x`` [M, K]."""
+    f = _fn("ddl_int8_rows", "p i qq ii pp p")
+    check(f(x.data_ptr(), 1 if x.dtype == torch.bfloat16 else 0, x.stride(0), x.shape[0], x.shape[1], q.shape[1], q.data_ptr(),
+            scale.data_ptr(), _raw_stream()), "int8_rows")
+
+
+def int8_linear(x, q, scale, bias, y):
+    M, Kd = x.shape
+    N = q.shape[0]
+    f = getattr(lib(), "ddl_int8_linear_workspace")
+    f.restype = ctypes.c_longlong
+    work = torch.empty(int(f(_i64(M), _i32(N), _i32(Kd))), dtype=torch.uint8, device=x.device)
+    f = _fn("ddl_int8_linear", "p i q p qq pp p q q ii p q p")
+    check(f(x.data_ptr(), 1 if x.dtype == torch.bfloat16 else 0, x.stride(0), q.data_ptr(), q.stride(0), storage_numel_from(q),
+            scale.data_ptr(), _p(bias), y.data_ptr(), y.stride(0), M, N, Kd, work.data_ptr(), work.numel(), _raw_stream()),
+          "int8_linear")
+
+
 # ---- convolution / GEMM (csrc/kernels/conv_igemm.hip, conv_wgrad.hip) ------------------------
 def _i32(v):
     return ctypes.c_int(int(v))

@@ -16,8 +16,8 @@ What differs from Horovod's design (MI355X-first):
 * ``step()`` orders the compute stream after the collectives with event waits — the host
   never blocks.  With ``optim.FusedSGD`` the update runs bucket by bucket: the stream waits for
   bucket k, updates bucket k's slice of the arenas, then waits for bucket k+1 — the update of
-  the early buckets overlaps the tail of the exchange (``FusedLARS`` needs every norm first and
-  updates after the last bucket);
+  the early buckets overlaps the tail of the exchange (``FusedLARS`` needs every norm first,
+  ``FusedMuon`` wants every matrix in one launch: both update after the last bucket);
 * per step the exposed communication time (how long the compute stream actually sat in those
   waits, from HIP events) and the device time of every bucket's collective (from the engine)
   are available through ``comm_metrics()`` and land in ``metrics.jsonl``;

@@ -233,9 +233,12 @@ def build_data(cfg, device, dtype, logger, world, rank):
 
 def build_optimizer(cfg, model, world, fused=True):
     """SGD(lr × world, momentum 0.9) as in the reference (:333), fused over flat arenas."""
-    from ..optim import FusedLARS, FusedSGD
+    from ..optim import FusedLARS, FusedMuon, FusedSGD
 
     lr = cfg.lr * world
+    if cfg.optimizer == "muon":
+        return FusedMuon(model.named_parameters(), lr=lr, momentum=cfg.momentum,
+                         weight_decay=cfg.weight_decay)
     if cfg.optimizer == "lars":
         return FusedLARS(model.named_parameters(), lr=lr, momentum=cfg.momentum,
                          weight_decay=cfg.weight_decay)

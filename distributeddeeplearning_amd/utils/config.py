@@ -89,7 +89,7 @@ class TrainConfig:
     log_interval: int = 100
     model: str = "resnet50"
     dtype: str = "bf16"
-    optimizer: str = "sgd"  # sgd | lars
+    optimizer: str = "sgd"  # sgd | lars | muon
     device_data: bool = True  # on-GPU synthetic generator instead of the host FakeData loader
     prefetch_depth: int = 2  # host batches uploaded + converted ahead on a copy stream (0 = off)
     uint8_transport: bool = True  # real data: ship uint8 pixels, normalise on the GPU (K20)

@@ -14,7 +14,7 @@ import torch  # noqa: E402
 import distributeddeeplearning_amd.torch as hvd  # noqa: E402
 from distributeddeeplearning_amd import callbacks as cb  # noqa: E402
 from distributeddeeplearning_amd.models import build_model  # noqa: E402
-from distributeddeeplearning_amd.optim import FusedLARS, FusedSGD  # noqa: E402
+from distributeddeeplearning_amd.optim import FusedLARS, FusedMuon, FusedSGD  # noqa: E402
 from distributeddeeplearning_amd.training import Trainer, build_data  # noqa: E402
 from distributeddeeplearning_amd.utils import TrainConfig, get_logger  # noqa: E402
 from distributeddeeplearning_amd.utils import checkpoint  # noqa: E402
@@ -51,7 +51,7 @@ def main(argv=None):
     train_loader, val_loader, data_length, _ = build_data(cfg, device, dtype, logger, world, rank)
     model = build_model(cfg.model, num_classes=cfg.num_classes)
     model.to_compute(device, dtype) if dtype == torch.bfloat16 else model.to(device)
-    opt_cls = FusedLARS if cfg.optimizer == "lars" else FusedSGD
+    opt_cls = {"lars": FusedLARS, "muon": FusedMuon}.get(cfg.optimizer, FusedSGD)
     opt = opt_cls(model.named_parameters(), lr=cfg.lr * world, momentum=cfg.momentum,
                   weight_decay=cfg.weight_decay)
     opt = hvd.DistributedOptimizer(opt, named_parameters=model.named_parameters())

@@ -1,0 +1,282 @@
+"""Orthogonalisation kernels and the Muon step against the formula in 64 bits, where they can go wrong: odd sizes, strides,
+spectra, empty and infinite matrices, many matrices, captured graphs, other streams, the launch tape."""
+import math
+
+import pytest
+import torch
+
+from tests.test_orthogonalize import oracle, reference_step
+
+pytestmark = pytest.mark.gpu
+DEV, BF = "cuda", torch.bfloat16
+
+# Result: one rounding to bf16 (half a step: 2^-8 of each value).  Within the five steps the products' operands are rounded to
+# fp16 three times a step (half a step: 2^-11): 15 * 2^-11 = 7.3e-3 if every one of them were at its largest and of one sign.
+TOL = 2 ** -8 + 15 * 2 ** -11
+
+
+def off(out, g, **kw):
+    """Relative 2-norm error."""
+    e = oracle(g.cpu(), **kw)
+    return float((out.double().cpu() - e).norm() / max(float(e.norm()), 1e-30))
+
+
+def spectrum(kind, r, c, seed=0):
+    gen = torch.Generator().manual_seed(seed)
+    k = min(r, c)
+    if kind == "gauss":
+        return torch.randn(r, c, generator=gen)
+    left = torch.linalg.qr(torch.randn(r, k, generator=gen, dtype=torch.float64))[0]
+    right = torch.linalg.qr(torch.randn(c, k, generator=gen, dtype=torch.float64))[0]
+    i = torch.arange(k, dtype=torch.float64)
+    s = {"power": 1 / (i + 1), "exp": 10 ** (-6 * i / max(k - 1, 1)), "rank1": (i == 0).double(),
+         "lowrank": torch.where(i < max(1, k // 16), 1.0, 1e-3)}[kind]
+    return ((left * s) @ right.T).float()
+
+
+SHAPES = [(1, 1), (1, 7), (7, 1), (3, 1000), (64, 64), (65, 63), (63, 130), (128, 128), (129, 257), (257, 129), (64, 147),
+          (300, 1000), (1000, 300), (256, 2304), (512, 513), (640, 640)]
+
+
+@pytest.mark.parametrize("shape", SHAPES, ids=str)
+@pytest.mark.parametrize("dtype", [torch.float32, BF], ids=["fp32", "bf16"])
+def test_sizes(shape, dtype):
+    from distributeddeeplearning_amd.ops import functional as ops
+
+    g = spectrum("gauss", *shape).to(DEV, dtype)
+    keep = g.clone()
+    out = ops.orthogonalize(g)
+    assert out.shape == g.shape and out.dtype == BF and torch.equal(g, keep)
+    assert off(out, g) < TOL
+
+
+@pytest.mark.parametrize("kind", ["power", "exp", "rank1", "lowrank"])
+@pytest.mark.parametrize("shape", [(96, 200), (256, 1024), (400, 256)], ids=str)
+def test_spectra(kind, shape):
+    from distributeddeeplearning_amd.ops import functional as ops
+
+    g = spectrum(kind, *shape, seed=5).to(DEV)
+    assert off(ops.orthogonalize(g), g) < TOL
+
+
+@pytest.mark.parametrize("steps, coef", [(0, (3.4445, -4.7750, 2.0315)), (1, (3.4445, -4.7750, 2.0315)), (7, (3.4445, -4.7750, 2.0315)),
+                                         (12, (2.0, -1.5, 0.5)), (20, (1.5, -0.5, 0.0))])
+def test_steps_and_coefficients(steps, coef):
+    from distributeddeeplearning_amd.ops import functional as ops
+
+    g = spectrum("gauss", 70, 200, 2).to(DEV)
+    out = ops.orthogonalize(g, steps=steps, coefficients=coef)
+    assert off(out, g, steps=steps, coef=coef) < 2 ** -8 + 3 * max(steps, 1) * 2 ** -11
+
+
+@pytest.mark.parametrize("scale", [1e-30, 1e-12, 1e30])
+def test_magnitudes(scale):
+    """Squares of these leave fp32; below eps the matrix is divided by eps."""
+    from distributeddeeplearning_amd.ops import functional as ops
+
+    g = (spectrum("gauss", 40, 90, 3) * scale).to(DEV)
+    out = ops.orthogonalize(g, eps=1e-20)
+    assert off(out, g, eps=1e-20) < TOL
+
+
+def test_strides_stacks_and_lists():
+    from distributeddeeplearning_amd.ops import functional as ops
+
+    base = spectrum("gauss", 200, 331, 4).to(DEV)
+    views = [base.t(), base[3:100, 5:200], base[::2, 1::3], base[:, 7:8], base[10:11], base[:50, :50].expand(50, 50)]
+    for v in views:
+        assert off(ops.orthogonalize(v), v) < TOL
+    stack = spectrum("gauss", 5 * 70, 33, 6).to(DEV).view(5, 70, 33)
+    for s in (stack, stack.transpose(0, 1), stack.transpose(1, 2), stack[::2, 1:, :20], stack[:1].expand(4, 70, 33)):
+        out = ops.orthogonalize(s)
+        assert out.shape == s.shape
+        for k in range(s.shape[0]):
+            assert off(out[k], s[k]) < TOL
+    # more matrices than one launch takes, ragged, some empty
+    mats = [spectrum("gauss", 1 + 7 * (i % 13), 1 + 11 * (i % 17), i).to(DEV) for i in range(150)]
+    mats[20], mats[140] = torch.empty(0, 5, device=DEV), torch.empty(5, 0, device=DEV)
+    outs = ops.orthogonalize(mats)
+    for m, o in zip(mats, outs):
+        assert o.shape == m.shape and (m.numel() == 0 or off(o, m) < TOL)
+    assert ops.orthogonalize([mats[20]])[0].shape == (0, 5)
+
+
+def test_matrices_do_not_touch_each_other():
+    from distributeddeeplearning_amd.ops import functional as ops
+
+    clean = [spectrum("gauss", 65, 130, i).to(DEV) for i in range(4)]
+    want = ops.orthogonalize(clean)
+    bad = [m.clone() for m in clean]
+    bad[1][3, 4] = float("nan")
+    bad[2][64, 129] = float("inf")
+    bad.insert(1, torch.zeros(65, 130, device=DEV))
+    got = ops.orthogonalize(bad)
+    assert torch.equal(got[0], want[0]) and torch.equal(got[4], want[3])
+    assert not got[1].any() and got[2].isnan().all() and got[3].isnan().all()
+
+
+def test_out_of_range_coefficients_are_refused():
+    from distributeddeeplearning_amd.ops import functional as ops
+
+    for coef in ((50.0, 0.0, 0.0), (3.0, 3.0, 3.0), (float("nan"), 0.0, 0.0), (1.0, -40.0, 0.0)):
+        with pytest.raises(ValueError, match="range"):
+            ops.orthogonalize(torch.zeros(4, 4, device=DEV), coefficients=coef)
+
+
+def test_repeated_calls_are_equal_and_other_streams_work():
+    from distributeddeeplearning_amd.ops import functional as ops
+
+    g = [spectrum("gauss", 300, 700, 1).to(DEV), spectrum("power", 512, 64, 2).to(DEV)]
+    a = ops.orthogonalize(g)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        b = ops.orthogonalize(g)
+    torch.cuda.current_stream().wait_stream(side)
+    c = ops.orthogonalize(g)
+    for x, y, z in zip(a, b, c):
+        assert torch.equal(x, y) and torch.equal(x, z)
+
+
+def test_two_captured_graphs():
+    from distributeddeeplearning_amd.ops import functional as ops
+
+    xs = [torch.zeros(130, 260, device=DEV), torch.zeros(3, 64, 70, device=DEV)]
+    graphs, outs = [], []
+    for x in xs:
+        ops.orthogonalize(x)
+    torch.cuda.synchronize()
+    for x in xs:
+        gr = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(gr):
+            outs.append(ops.orthogonalize(x))
+        graphs.append(gr)
+    for rep in range(4):
+        for x in xs:
+            x.copy_(torch.randn(x.shape, generator=torch.Generator().manual_seed(rep)))
+        for gr in graphs if rep % 2 else graphs[::-1]:
+            gr.replay()
+        eager = [ops.orthogonalize(x) for x in xs]
+        torch.cuda.synchronize()
+        for o, e in zip(outs, eager):
+            assert torch.equal(o, e)
+
+
+# ---------------------------------------------------------------------------------------------------- the optimizer
+def _params(shapes, dtype, seed=0, many=0):
+    gen = torch.Generator().manual_seed(seed)
+    out = []
+    for i, s in enumerate(list(shapes) + [(6 + i % 5, 9 + i % 7) for i in range(many)]):
+        t = (0.1 * torch.randn(s, generator=gen)).to(DEV)
+        t = t.to(dtype) if len(s) > 1 else t
+        if len(s) == 4:
+            t = t.contiguous(memory_format=torch.channels_last)
+        out.append(("p%d" % i, torch.nn.Parameter(t)))
+    return out
+
+
+MUON_SHAPES = [(64,), (64, 3, 7, 7), (130, 64, 3, 3), (200, 130, 1, 1), (200,), (10, 200), (257, 31), (1, 5), (5, 1)]
+
+
+@pytest.mark.parametrize("dtype, grads", [(BF, "auto"), (BF, "fp32"), (torch.float32, "auto")], ids=["bf16", "bf16-fp32-grads", "fp32"])
+@pytest.mark.parametrize("nesterov, wd, many", [(True, 0.0, 0), (False, 0.05, 0), (True, 0.05, 70)])
+def test_muon_steps(dtype, grads, nesterov, wd, many):
+    from distributeddeeplearning_amd.optim import FusedMuon
+    from distributeddeeplearning_amd.utils.config import EngineConfig
+
+    named = _params(MUON_SHAPES, dtype, many=many)
+    opt = FusedMuon(named, lr=0.02, momentum=0.9, weight_decay=wd, nesterov=nesterov, vector_lr_scale=0.25,
+                    engine_config=EngineConfig(comm_dtype=grads))
+    ref = {n: p.detach().double().cpu() for n, p in named}
+    vel = {n: torch.zeros_like(w) for n, w in ref.items()}
+    change = {n: 0.0 for n in ref}
+    for step in range(3):
+        gen = torch.Generator().manual_seed(100 + step)
+        for n, p in named:
+            p.grad.copy_(1e-3 * torch.randn(p.shape, generator=gen))
+            before = ref[n].clone()
+            reference_step(ref[n], p.grad.double().cpu(), vel[n], 0.02, 0.9, wd, nesterov, p.dim() > 1, 0.25)
+            change[n] += float((ref[n] - before).norm())
+        opt.step()
+    torch.cuda.synchronize()
+    for dt, plan in opt.arena.plans.items():
+        covered = torch.zeros(plan.numel, dtype=torch.bool)
+        for seg in plan.segments:
+            w = opt._weights(dt)[seg.offset:seg.offset + seg.numel]
+            v = opt.momentum_buf[dt][seg.offset:seg.offset + seg.numel]
+            covered[seg.offset:seg.offset + seg.numel] = True
+
+            def flat(t):
+                return (t.permute(0, 2, 3, 1) if t.dim() == 4 else t).reshape(-1)
+
+            # the weights are fp32: off by the direction's error (16-bit products; no final rounding) times how far they went,
+            # and three roundings a step
+            err = float((w.double().cpu() - flat(ref[seg.name])).norm())
+            assert err <= 15 * 2 ** -11 * change[seg.name] + 9 * 2 ** -24 * float(ref[seg.name].norm()) + 1e-12, seg.name
+            torch.testing.assert_close(v.double().cpu(), flat(vel[seg.name]), rtol=1e-6, atol=1e-9)
+            if dt in opt.master:
+                assert torch.equal(opt.arena.params[dt][seg.offset:seg.offset + seg.numel], w.to(BF))
+        assert not opt.momentum_buf[dt].cpu()[~covered].any() and not opt.arena.params[dt].cpu()[~covered].any()
+
+
+def test_muon_frozen_lr_follows_the_schedule_bit_for_bit():
+    from distributeddeeplearning_amd.optim import FusedMuon
+
+    results = []
+    for frozen in (False, True):
+        named = _params(MUON_SHAPES, BF)
+        opt = FusedMuon(named, lr=0.02, weight_decay=0.01)
+        if frozen:
+            opt.freeze_lr()
+        for step, lr in enumerate((0.02, 0.013, 0.004)):
+            opt.param_groups[0]["lr"] = lr
+            opt.sync_lr()
+            gen = torch.Generator().manual_seed(step)
+            for _, p in named:
+                p.grad.copy_(torch.randn(p.shape, generator=gen))
+            opt.step()
+        results.append([opt.master[BF].clone(), opt.arena.params[torch.float32].clone()])
+    for a, b in zip(*results):
+        assert torch.equal(a, b)
+
+
+def _train(taped, graphed=False, steps=7):
+    from distributeddeeplearning_amd.data.synthetic import DeviceSyntheticLoader
+    from distributeddeeplearning_amd.models import resnet18
+    from distributeddeeplearning_amd.ops import functional as ops, hip_ops
+    from distributeddeeplearning_amd.optim import FusedMuon
+    from distributeddeeplearning_amd.training.graph import GraphedTrainStep
+    from distributeddeeplearning_amd.training.tape import TapedTrainStep
+
+    hip_ops.reset_caches()
+    torch.manual_seed(3)
+    model = resnet18(num_classes=16).to_compute(torch.device(DEV), BF).train()
+    opt = FusedMuon(model.named_parameters(), lr=0.01, momentum=0.9, weight_decay=1e-3)
+    loader = DeviceSyntheticLoader(8, length=8 * 64, pool_size=32, height=64, width=64, n_classes=16, device=DEV, dtype=BF, seed=11)
+    if graphed:
+        step = GraphedTrainStep(model, opt, ops.softmax_cross_entropy, warmup=2)
+    else:
+        step = TapedTrainStep(model, opt, ops.softmax_cross_entropy, loader=loader, warmup=2, enabled=taped)
+    for s in range(steps):
+        if s == 4:
+            opt.param_groups[0]["lr"] = 0.003
+        if graphed:
+            step(*loader.batch())
+        else:
+            step()
+    torch.cuda.synchronize()
+    return step, opt
+
+
+def test_muon_step_on_the_launch_tape_is_the_eager_step():
+    eager, a = _train(False)
+    taped, b = _train(True)
+    assert taped.taped and not eager.taped
+    assert torch.equal(a.master[BF], b.master[BF]) and torch.equal(a.momentum_buf[BF], b.momentum_buf[BF])
+
+
+def test_muon_step_in_a_captured_graph_is_the_eager_step():
+    _, a = _train(False)
+    graphed, b = _train(False, graphed=True)
+    assert graphed.graphed
+    assert torch.equal(a.master[BF], b.master[BF]) and torch.equal(a.momentum_buf[BF], b.momentum_buf[BF])
