@@ -50,6 +50,7 @@ struct MulGroup {
     unsigned first;
     unsigned mat;
     int tiles;                      // workgroups of a matrix
+    int batch;
 };
 struct MulTable { MulGroup g[MAXG]; int count; };
 
@@ -212,118 +213,240 @@ __global__ void __launch_bounds__(256) ortho_unpack_kernel(const IoTable t, cons
 }
 
 // ---- products ---------------------------------------------------------------------------------------------------------
-constexpr int LDK = 40;   // LDS row of 32 reduction elements, padded to 80 bytes
+// D = F S^T over K (a multiple of 32): 4 waves as 2 x 2, a BF x BS tile in steps of 32, NST stages filled by LDS-DMA (tile
+// t + NST - 1 is on its way while tile t is multiplied; counted waits, one barrier a step).
+//   S and, with TRF = false, F: row-major, k-contiguous rows.  LDS rows of 64 bytes, 16-byte chunk c of row r at c ^ -(r / 4)
+//   (16 rows x one chunk are free of bank conflicts).
+//   TRF = true: F is given transposed, [k][columns].  Its rows of k stay as they are in LDS and are read by the transposing
+//   load: 16 lanes take 4 rows x 16 columns; a half-wave touches rows 0-3 and 8-11 (+ 4, + 16), whose 32-byte windows
+//   the swizzle spreads over all banks.
+// A lane ends with D[i][j][e]: F index 16 i + 4 (lane / 16) + e, S index 16 j + lane % 16 of its wave's quarter.
+typedef __fp16 half4 __attribute__((ext_vector_type(4)));      // (the type that the transposing load is declared with)
+typedef __attribute__((address_space(3))) half4* lds_half4_ptr;
+constexpr unsigned OUT = 0x80000000u;      // an offset behind the descriptor's range: reads as zero
 
-// 64 x 64 tile of rows a[..][k] times rows b[..][k] (both k-contiguous), 4 waves of 32 x 32
-template <bool TRANS_B>
-__device__ __forceinline__ void tile_mul(const f16_t* __restrict__ a, int lda, const f16_t* __restrict__ b, int ldb, int K, f16_t* As,
-                                         f16_t* Bs, f32x4 (&acc)[2][2]) {
-    const int tid = threadIdx.x, lane = tid & 63, wid = tid >> 6, wm = wid >> 1, wn = wid & 1;
-    const int row = tid >> 2, ch = tid & 3;
-    for (int k0 = 0; k0 < K; k0 += 32) {
-        const f16x8 va = *reinterpret_cast<const f16x8*>(a + (long long)row * lda + k0 + ch * 8);
-        f16x8 vb;
-        if (TRANS_B) vb = *reinterpret_cast<const f16x8*>(b + (long long)(k0 + (tid >> 3)) * ldb + (tid & 7) * 8);
-        else vb = *reinterpret_cast<const f16x8*>(b + (long long)row * ldb + k0 + ch * 8);
-        __syncthreads();
-        *reinterpret_cast<f16x8*>(As + row * LDK + ch * 8) = va;
-        if (TRANS_B) {
-#pragma unroll
-            for (int e = 0; e < 8; ++e) Bs[((tid & 7) * 8 + e) * LDK + (tid >> 3)] = vb[e];
-        } else {
-            *reinterpret_cast<f16x8*>(Bs + row * LDK + ch * 8) = vb;
-        }
-        __syncthreads();
-        f16x8 fa[2], fb[2];
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            fa[i] = *reinterpret_cast<const f16x8*>(As + (wm * 32 + i * 16 + (lane & 15)) * LDK + (lane >> 4) * 8);
-            fb[i] = *reinterpret_cast<const f16x8*>(Bs + (wn * 32 + i * 16 + (lane & 15)) * LDK + (lane >> 4) * 8);
-        }
-#pragma unroll
-        for (int i = 0; i < 2; ++i)
-#pragma unroll
-            for (int j = 0; j < 2; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(fa[i], fb[j], acc[i][j], 0, 0, 0);
-    }
+__device__ __forceinline__ int nt_off(int row, int ch) { return row * 64 + ((ch ^ ((0 - (row >> 2)) & 3)) << 4); }
+template <int B>
+__device__ __forceinline__ int tr_swz(int row) {
+    return B == 128 ? (row & 3) | ((row >> 1) & 4) : ((row >> 1) & 1) | ((row >> 2) & 2);
 }
 
-__device__ __forceinline__ void tri_tile(int idx, int& ti, int& tj) {    // idx -> (ti >= tj) of a lower triangle
-    ti = (int)((sqrtf(8.f * (float)idx + 1.f) - 1.f) * 0.5f);
-    while ((ti + 1) * (ti + 2) / 2 <= idx) ++ti;
-    while (ti * (ti + 1) / 2 > idx) --ti;
-    tj = idx - ti * (ti + 1) / 2;
+template <int BF, int BS, int NST, bool TRF>
+struct Mul {
+    static constexpr int FBYTES = BF * 64, SBYTES = BS * 64, STAGE = FBYTES + SBYTES;
+    static constexpr int FL = BF / 64, SL = BS / 64, L = FL + SL;       // LDS-DMA instructions of a wave and stage
+    static constexpr int NF = BF / 32, NS = BS / 32;                    // fragments of a wave
+    f32x4 acc[NF][NS];
+
+    // f: first row (TRF: first column) of the tile, ldf its row length, fleft rows (columns) that exist; s likewise
+    __device__ __forceinline__ void run(unsigned char* smem, const f16_t* f, long long ldf, int fleft, const f16_t* s, long long lds, int sleft, int K) {
+        const int tid = threadIdx.x, lane = tid & 63, wid = __builtin_amdgcn_readfirstlane(tid >> 6), w0 = wid >> 1, w1 = wid & 1;
+        const int fr = lane & 15, fq = lane >> 4;
+        const int KT = K / 32;
+        const unsigned lds0 = (unsigned)(uintptr_t)(__attribute__((address_space(3))) void*)smem;
+        unsigned fo[FL], so[SL];
+#pragma unroll
+        for (int i = 0; i < FL; ++i) {
+            const int slot = (i * 4 + wid) * 64 + lane;
+            if (TRF) {
+                constexpr int CPR = BF / 8;
+                const int row = slot / CPR, ch = slot % CPR, c = (((ch >> 1) ^ tr_swz<BF>(row)) << 1) | (ch & 1);
+                fo[i] = c * 8 < fleft ? (unsigned)((row * ldf + c * 8) * 2) : OUT;
+            } else {
+                const int row = slot >> 2, c = (slot & 3) ^ ((0 - (row >> 2)) & 3);
+                fo[i] = row < fleft ? (unsigned)((row * ldf + c * 8) * 2) : OUT;
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < SL; ++i) {
+            const int slot = (i * 4 + wid) * 64 + lane, row = slot >> 2, c = (slot & 3) ^ ((0 - (row >> 2)) & 3);
+            so[i] = row < sleft ? (unsigned)((row * lds + c * 8) * 2) : OUT;
+        }
+        // every stage is exactly L instructions a wave (zeros behind the end): the counted waits rely on it
+        auto fetch = [&](int kt, int stage) {
+            const bool live = kt < KT;
+            const u32x4 rf = raw_rsrc(f + (live ? (TRF ? (long long)kt * 32 * ldf : (long long)kt * 32) : 0), OUT - 16);
+            const u32x4 rs = raw_rsrc(s + (live ? (long long)kt * 32 : 0), OUT - 16);
+            const unsigned at = lds0 + (unsigned)(stage * STAGE + wid * 1024);
+#pragma unroll
+            for (int i = 0; i < FL; ++i) lds_dma16(rf, at + i * 4096, live ? fo[i] : OUT, 0u);
+#pragma unroll
+            for (int i = 0; i < SL; ++i) lds_dma16(rs, at + FBYTES + i * 4096, live ? so[i] : OUT, 0u);
+        };
+        int foff[NF], soff[NS];
+        const int trow = 8 * fq + ((lane >> 2) & 3);
+#pragma unroll
+        for (int i = 0; i < NF; ++i)
+            foff[i] = TRF ? trow * (BF * 2) + (((w0 * NF + i) ^ tr_swz<BF>(trow)) * 32) + 8 * (lane & 3) : nt_off(w0 * (BF / 2) + i * 16 + fr, fq);
+#pragma unroll
+        for (int j = 0; j < NS; ++j) soff[j] = FBYTES + nt_off(w1 * (BS / 2) + j * 16 + fr, fq);
+#pragma unroll
+        for (int i = 0; i < NF; ++i)
+#pragma unroll
+            for (int j = 0; j < NS; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+
+#pragma unroll
+        for (int k = 0; k < NST - 1; ++k) fetch(k, k);
+        asm volatile("s_waitcnt vmcnt(%0)" ::"n"((NST - 2) * L) : "memory");
+        __builtin_amdgcn_s_barrier();
+        int cur = 0, nxt = NST - 1;
+        for (int kt = 0; kt < KT; ++kt) {
+            fetch(kt + NST - 1, nxt);          // into the stage whose reads ended before the last barrier
+            unsigned char* st = smem + cur * STAGE;
+            f16x8 a[NF], b[NS];
+#pragma unroll
+            for (int j = 0; j < NS; ++j) b[j] = *reinterpret_cast<const f16x8*>(st + soff[j]);
+#pragma unroll
+            for (int i = 0; i < NF; ++i) {
+                if (TRF) {
+                    // (row + 4 has the swizzle of row: bit 2 of the row does not take part in it)
+                    const f16x4 lo = __builtin_bit_cast(f16x4, __builtin_amdgcn_ds_read_tr16_b64_v4f16((lds_half4_ptr)(st + foff[i])));
+                    const f16x4 hi = __builtin_bit_cast(f16x4, __builtin_amdgcn_ds_read_tr16_b64_v4f16((lds_half4_ptr)(st + foff[i] + 4 * BF * 2)));
+                    a[i] = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+                } else {
+                    a[i] = *reinterpret_cast<const f16x8*>(st + foff[i]);
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < NF; ++i)
+#pragma unroll
+                for (int j = 0; j < NS; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a[i], b[j], acc[i][j], 0, 0, 0);
+            asm volatile("s_waitcnt vmcnt(%0)" ::"n"((NST - 2) * L) : "memory");
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+            __builtin_amdgcn_s_barrier();
+            nxt = cur;
+            cur = cur + 1 == NST ? 0 : cur + 1;
+        }
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    }
+};
+
+// Tiles of a matrix in bands of 8 rows, a band column by column: the tiles that an XCD works on at a time are about as many
+// rows as columns.  A matrix of many tiles is dealt to the XCDs (workgroup number modulo 8) in runs of neighbours.
+__device__ __forceinline__ int deal(int idx, int tiles) {
+    if (tiles < 64) return idx;
+    const int q = tiles >> 3, r = tiles & 7, xcd = idx & 7;
+    return xcd * q + (xcd < r ? xcd : r) + (idx >> 3);
+}
+__device__ __forceinline__ void band_tile(int idx, int rows, int cols, int& ti, int& tj) {
+    const int band = idx / (8 * cols), rem = idx - band * 8 * cols, h = rows - band * 8 < 8 ? rows - band * 8 : 8;
+    tj = rem / h;
+    ti = band * 8 + rem - tj * h;
+}
+// the same of a lower triangle (ti >= tj): band b is 8 b whole columns and a triangle
+__device__ __forceinline__ void tri_tile(int idx, int rows, int& ti, int& tj) {
+    int band = (int)((sqrtf(16.f + 128.f * (float)idx) - 4.f) * (1.f / 64.f));
+    while (32 * (band + 1) * (band + 1) + 4 * (band + 1) <= idx) ++band;
+    while (32 * band * band + 4 * band > idx) --band;
+    const int rem = idx - 32 * band * band - 4 * band, h = rows - band * 8 < 8 ? rows - band * 8 : 8;
+    if (rem < h * 8 * band) {
+        tj = rem / h;
+        ti = band * 8 + rem - tj * h;
+        return;
+    }
+    const int left = rem - h * 8 * band;
+    int i = 0;
+    while ((i + 1) * (i + 2) / 2 <= left) ++i;
+    ti = band * 8 + i;
+    tj = band * 8 + left - i * (i + 1) / 2;
 }
 
 // SQUARE = false: O, d of A = X X^T.  SQUARE = true: O, d of P = b A + c A^2 (diagonal: + a) from those of A
-template <bool SQUARE>
-__global__ void __launch_bounds__(256) ortho_sym_kernel(const MulTable t, const f16_t* __restrict__ in, const float* __restrict__ din,
-                                                       f16_t* __restrict__ out, float* __restrict__ dout, const int* __restrict__ ex, int down,
-                                                       float ca, float cb, float cc) {
-    __shared__ __attribute__((aligned(16))) f16_t As[64 * LDK], Bs[64 * LDK];
+template <int B, int NST, bool SQUARE>
+__global__ void __launch_bounds__(256, 2) ortho_sym_kernel(const MulTable t, const f16_t* __restrict__ in, const float* __restrict__ din,
+                                                          f16_t* __restrict__ out, float* __restrict__ dout, const int* __restrict__ ex, int down,
+                                                          float ca, float cb, float cc) {
+    typedef Mul<B, B, NST, false> M;
+    __shared__ __attribute__((aligned(16))) unsigned char smem[NST * M::STAGE];
     const int gi = find_group(t, blockIdx.x);
     const MulGroup g = t.g[gi];
     const unsigned idx = blockIdx.x - g.first;
     const int b = idx / g.tiles;
+    if (b >= g.batch) return;              // (groups are padded to multiples of 8 workgroups)
     int ti, tj;
-    tri_tile(idx - b * g.tiles, ti, tj);
+    tri_tile(deal(idx - b * g.tiles, g.tiles), (g.np + B - 1) / B, ti, tj);
     const int K = SQUARE ? g.np : g.mp;
     const long long ao = (long long)g.ao * 64 + (long long)b * g.np * g.np;
     const f16_t* src = SQUARE ? in + ao : in + (long long)g.xo * 64 + (long long)b * g.np * g.mp;
-    f32x4 acc[2][2] = {};
-    tile_mul<false>(src + (long long)ti * 64 * K, K, src + (long long)tj * 64 * K, K, K, As, Bs, acc);
-    const int lane = threadIdx.x & 63, wid = threadIdx.x >> 6, wm = wid >> 1, wn = wid & 1;
+    M m;
+    m.run(smem, src + (long long)ti * B * K, K, g.np - ti * B, src + (long long)tj * B * K, K, g.np - tj * B, K);
+    const int lane = threadIdx.x & 63, wid = threadIdx.x >> 6, w0 = wid >> 1, w1 = wid & 1;
     const float* d = SQUARE ? din + g.dof + (long long)b * g.np : nullptr;
     const float unscale = SQUARE ? USC * USC : ldexpf(USC * USC, -2 * shift_of(ex, g.mat + b, down));
+    f16_t* o = out + ao;
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
+    for (int i = 0; i < M::NF; ++i)
 #pragma unroll
-        for (int j = 0; j < 2; ++j)
+        for (int j = 0; j < M::NS; ++j) {
+            const int r = ti * B + w0 * (B / 2) + i * 16 + (lane >> 4) * 4, c = tj * B + w1 * (B / 2) + j * 16 + (lane & 15);
+            if (B > 64 && (r >= g.np || c >= g.np)) continue;
+            f32x4 v = m.acc[i][j] * unscale;
+            if (SQUARE) {
+                // (A is symmetric: its row c holds this lane's column)
+                const f16x4 a = *reinterpret_cast<const f16x4*>(src + (long long)c * K + r);
+                const f32x4 dr = *reinterpret_cast<const f32x4*>(d + r);
+                const float dc = d[c];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const float af = (float)a[e] * USC;
+                    v[e] = r + e == c ? ca + cb * dc + cc * (v[e] + dc * dc) : cb * af + cc * (v[e] + (dr[e] + dc) * af);
+                }
+            }
+            f16x4 h;
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                const int r = ti * 64 + wm * 32 + i * 16 + (lane >> 4) * 4 + e, c = tj * 64 + wn * 32 + j * 16 + (lane & 15);
-                float v = acc[i][j][e] * unscale;
-                if (SQUARE) {
-                    const float o = (float)src[(long long)r * K + c] * USC;
-                    const float dr = d[r], dc = d[c];
-                    v = r == c ? ca + cb * dr + cc * (v + dr * dr) : cb * o + cc * (v + (dr + dc) * o);
-                }
-                if (r == c) dout[g.dof + (long long)b * g.np + r] = v;
-                const f16_t h = r == c ? (f16_t)0.f : (f16_t)(v * SC);
-                out[ao + (long long)r * g.np + c] = h;
-                if (ti != tj) out[ao + (long long)c * g.np + r] = h;
+                if (r + e == c) dout[g.dof + (long long)b * g.np + c] = v[e];
+                h[e] = r + e == c ? (f16_t)0.f : (f16_t)(v[e] * SC);
+                if (ti != tj) o[(long long)(r + e) * g.np + c] = h[e];
             }
+            *reinterpret_cast<f16x4*>(o + (long long)c * g.np + r) = h;
+        }
 }
 
-// X' = pd X + offdiag(P) X_hi
-__global__ void __launch_bounds__(256) ortho_apply_kernel(const MulTable t, const f16_t* __restrict__ P, const float* __restrict__ pd,
-                                                         const f16_t* __restrict__ xh, const f16_t* __restrict__ xl,
-                                                         f16_t* __restrict__ yh, f16_t* __restrict__ yl,
-                                                         const int* __restrict__ ex, int down, int down1) {
-    __shared__ __attribute__((aligned(16))) f16_t As[64 * LDK], Bs[64 * LDK];
+// X' = pd X + offdiag(P) X_hi; tile: BF columns of X times BS rows of P
+template <int BF, int BS, int NST>
+__global__ void __launch_bounds__(256, 2) ortho_apply_kernel(const MulTable t, const f16_t* __restrict__ P, const float* __restrict__ pd,
+                                                            const f16_t* __restrict__ xh, const f16_t* __restrict__ xl,
+                                                            f16_t* __restrict__ yh, f16_t* __restrict__ yl,
+                                                            const int* __restrict__ ex, int down, int down1) {
+    typedef Mul<BF, BS, NST, true> M;
+    __shared__ __attribute__((aligned(16))) unsigned char smem[NST * M::STAGE];
     const int gi = find_group(t, blockIdx.x);
     const MulGroup g = t.g[gi];
     const unsigned idx = blockIdx.x - g.first;
-    const int b = idx / g.tiles, rem = idx - b * g.tiles, tm = g.mp >> 6;
-    const int ti = rem / tm, tj = rem - ti * tm;
-    const f16_t* A = P + (long long)g.ao * 64 + (long long)b * g.np * g.np + (long long)ti * 64 * g.np;
+    const int b = idx / g.tiles;
+    if (b >= g.batch) return;              // (groups are padded to multiples of 8 workgroups)
+    int ti, tj;
+    band_tile(deal(idx - b * g.tiles, g.tiles), (g.np + BS - 1) / BS, (g.mp + BF - 1) / BF, ti, tj);
+    const f16_t* A = P + (long long)g.ao * 64 + (long long)b * g.np * g.np + (long long)ti * BS * g.np;
     const long long xo = (long long)g.xo * 64 + (long long)b * g.np * g.mp;
-    f32x4 acc[2][2] = {};
-    tile_mul<true>(A, g.np, xh + xo + tj * 64, g.mp, g.np, As, Bs, acc);
+    M m;
+    m.run(smem, xh + xo + tj * BF, g.mp, g.mp - tj * BF, A, g.np, g.np - ti * BS, g.np);
     const float rescale = ldexpf(1.f, shift_of(ex, g.mat + b, down1) - shift_of(ex, g.mat + b, down));
-    const int lane = threadIdx.x & 63, wid = threadIdx.x >> 6, wm = wid >> 1, wn = wid & 1;
+    const int lane = threadIdx.x & 63, wid = threadIdx.x >> 6, w0 = wid >> 1, w1 = wid & 1;
+    const float* d = pd + g.dof + (long long)b * g.np;
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
+    for (int j = 0; j < M::NS; ++j) {
+        const int r = ti * BS + w1 * (BS / 2) + j * 16 + (lane & 15);
+        if (BS > 64 && r >= g.np) continue;
+        const float dr = d[r];
 #pragma unroll
-        for (int j = 0; j < 2; ++j)
+        for (int i = 0; i < M::NF; ++i) {
+            const int c = tj * BF + w0 * (BF / 2) + i * 16 + (lane >> 4) * 4;
+            if (BF > 64 && c >= g.mp) continue;
+            const long long at = xo + (long long)r * g.mp + c;
+            const f16x4 h0 = *reinterpret_cast<const f16x4*>(xh + at), l0 = *reinterpret_cast<const f16x4*>(xl + at);
+            f16x4 h, l;
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                const int r = ti * 64 + wm * 32 + i * 16 + (lane >> 4) * 4 + e, c = tj * 64 + wn * 32 + j * 16 + (lane & 15);
-                const long long at = xo + (long long)r * g.mp + c;
-                const float v = (pd[g.dof + (long long)b * g.np + r] * ((float)xh[at] + (float)xl[at]) + acc[i][j][e] * USC) * rescale;
-                const f16_t h = (f16_t)v;
-                yh[at] = h;
-                yl[at] = (f16_t)(v - (float)h);
+                const float v = (dr * ((float)h0[e] + (float)l0[e]) + m.acc[i][j][e] * USC) * rescale;
+                h[e] = (f16_t)v;
+                l[e] = (f16_t)(v - (float)h[e]);
             }
+            *reinterpret_cast<f16x4*>(yh + at) = h;
+            *reinterpret_cast<f16x4*>(yl + at) = l;
+        }
+    }
 }
 
 // ---- host -------------------------------------------------------------------------------------------------------------
@@ -403,6 +526,7 @@ int run_all(const Desc* q, int count, int kind, const Muon& mu, float a, float b
     if (!plan_of(q, count, pl)) return DDL_EINVAL;
     IoTable in, tiles, outt;
     MulTable sym, app;
+    static const int sb = getenv("ORTHO_SB") ? atoi(getenv("ORTHO_SB")) : 64, ab = getenv("ORTHO_AB") ? atoi(getenv("ORTHO_AB")) : 64;
     in.count = tiles.count = outt.count = sym.count = app.count = count;
     long long nin = 0, nio = 0, nsym = 0, napp = 0, xo = 0, ao = 0, dof = 0, po = 0, mat = 0;
     for (int i = 0; i < count; ++i) {
@@ -417,11 +541,12 @@ int run_all(const Desc* q, int count, int kind, const Muon& mu, float a, float b
         if (kind < 2) { io.p = (const void*)s.dst; io.bs = s.db; io.rs = (int)s.drs; io.cs = (int)s.dcs; }
         outt.g[i] = io;
         MulGroup mg;
-        mg.np = (int)np; mg.mp = (int)mp; mg.xo = (unsigned)(xo / 64); mg.ao = (unsigned)(ao / 64); mg.dof = (unsigned)dof; mg.mat = (unsigned)mat;
-        mg.tiles = (int)(tn * (tn + 1) / 2); mg.first = (unsigned)nsym; sym.g[i] = mg;
-        nsym += s.batch * mg.tiles;
-        mg.tiles = (int)(tn * tm); mg.first = (unsigned)napp; app.g[i] = mg;
-        napp += s.batch * mg.tiles;
+        mg.np = (int)np; mg.mp = (int)mp; mg.xo = (unsigned)(xo / 64); mg.ao = (unsigned)(ao / 64); mg.dof = (unsigned)dof; mg.mat = (unsigned)mat; mg.batch = (int)s.batch;
+        const long long sn = (np + sb - 1) / sb, an = (np + ab - 1) / ab, am = (mp + ab - 1) / ab;
+        mg.tiles = (int)(sn * (sn + 1) / 2); mg.first = (unsigned)nsym; sym.g[i] = mg;
+        nsym += (s.batch * mg.tiles + 7) / 8 * 8;
+        mg.tiles = (int)(an * am); mg.first = (unsigned)napp; app.g[i] = mg;
+        napp += (s.batch * mg.tiles + 7) / 8 * 8;
         nin += s.batch * parts; nio += s.batch * tn * tm;
         xo += s.batch * np * mp; ao += s.batch * np * np; dof += s.batch * np; po += s.batch * parts; mat += s.batch;
         if (nin > 0x7fffffffLL || nio > 0x7fffffffLL || nsym > 0x7fffffffLL || napp > 0x7fffffffLL) return DDL_EINVAL;
@@ -439,9 +564,11 @@ int run_all(const Desc* q, int count, int kind, const Muon& mu, float a, float b
     if (kind == 0) { IO(0); } else if (kind == 1) { IO(1); } else if (kind == 2) { IO(2); } else { IO(3); }
 #undef IO
     for (int k = 0; k < steps; ++k) {
-        DDL_KLAUNCH(ortho_sym_kernel<false>, dim3((unsigned)nsym), block, 0, stream, sym, xh, (const float*)nullptr, O, d, ex, k * fall, a, b, c);
-        DDL_KLAUNCH(ortho_sym_kernel<true>, dim3((unsigned)nsym), block, 0, stream, sym, O, d, P, pd, ex, 0, a, b, c);
-        DDL_KLAUNCH(ortho_apply_kernel, dim3((unsigned)napp), block, 0, stream, app, P, pd, xh, xl, yh, yl, ex, k * fall, (k + 1) * fall);
+#define SYM(B, NST, SQ, IN, DIN, OUTP, DOUT, DOWN) DDL_KLAUNCH((ortho_sym_kernel<B, NST, SQ>), dim3((unsigned)nsym), block, 0, stream, sym, IN, DIN, OUTP, DOUT, ex, DOWN, a, b, c)
+        if (sb == 64) { SYM(64, 4, false, xh, (const float*)nullptr, O, d, k * fall); SYM(64, 4, true, O, d, P, pd, 0); }
+        else { SYM(128, 4, false, xh, (const float*)nullptr, O, d, k * fall); SYM(128, 4, true, O, d, P, pd, 0); }
+        if (ab == 64) DDL_KLAUNCH((ortho_apply_kernel<64, 64, 4>), dim3((unsigned)napp), block, 0, stream, app, P, pd, xh, xl, yh, yl, ex, k * fall, (k + 1) * fall);
+        else DDL_KLAUNCH((ortho_apply_kernel<128, 128, 4>), dim3((unsigned)napp), block, 0, stream, app, P, pd, xh, xl, yh, yl, ex, k * fall, (k + 1) * fall);
         f16_t* s = xh; xh = yh; yh = s;
         s = xl; xl = yl; yl = s;
     }
