@@ -20,6 +20,7 @@
 // keep (0 = a 0 + 0), so the products have no edges.
 #include "common.h"
 #include <math.h>
+#include <string.h>
 
 namespace {
 
@@ -27,39 +28,84 @@ typedef _Float16 f16_t;
 typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 
-constexpr int MAXG = 64;            // groups of a launch: one lane each in find_group
+constexpr int MAXG = 64;            // groups of a call: one lane each where a workgroup looks its group up
+constexpr int CHUNK = 32;           // groups that travel in one launch's arguments
 constexpr int PARTS = 1024;         // most partial sums of squares of a matrix
 constexpr float SC = 4096.f, USC = 1.f / 4096.f;
 
-struct IoGroup {                    // where a group's matrices come from / go to
-    const void* p;                  // first matrix (K23: unused)
-    long long bs;                   // elements from a matrix to the next (K23: offset in the arenas)
-    int rs, cs;                     // strides of a row, of a column
-    int r, c;
-    int part_elems;                 // elements of a partial sum of squares
-    unsigned xo;                    // first matrix in the workspace, in 64 elements
-    unsigned po;                    // its first partial sum
-    unsigned first;                 // first workgroup of the group in this launch
-    unsigned mat;                   // its first matrix among all
-};
-struct IoTable { IoGroup g[MAXG]; int count; };
-
-struct MulGroup {
-    int np, mp;                     // padded sizes
-    unsigned xo, ao, dof;           // first matrix in the X and A workspaces (64 elements), in the diagonals (elements)
-    unsigned first;
-    unsigned mat;
-    int tiles;                      // workgroups of a matrix
+struct Group {                      // `batch` equal matrices
+    const void* src;                // K23: unused
+    bf16_t* dst;                    // dense
+    long long sb;                   // elements from a matrix to the next (K23: offset in the arenas)
+    int rs, cs;                     // strides of a row, of a column of src
+    int r, c, np, mp;               // sizes; padded shorter and longer side
     int batch;
+    int vec;                        // src (K23: the arenas) can be read 8 elements of a row at a time
+    int part_elems, parts;          // elements of a partial sum of squares, partial sums of a matrix
+    unsigned xo, ao, dof, po, mat;  // first matrix in the X and square workspaces (64 elements), in the diagonals, the partial sums, among all
+    int tsym, tapp;                 // tiles of a matrix in the symmetric products and in P X
+    int hsym, happ;                 // the XCD that computes them, -1: all
+    unsigned fin, fio;              // first workgroup of the sums, of the packing
 };
-struct MulTable { MulGroup g[MAXG]; int count; };
+struct Chunk { Group g[CHUNK]; int base, n, last; };
 
-// the group whose workgroups contain `bid`: groups are in ascending order of `first`
-template <typename T>
-__device__ __forceinline__ int find_group(const T& t, unsigned bid) {
-    const int lane = threadIdx.x & 63;
-    const bool mine = lane < t.count && t.g[lane < t.count ? lane : 0].first <= bid;
+// What the kernels of a call read.  Workgroup w of a product runs on XCD w mod 8 as that XCD's item w / 8: fsym / fapp say at
+// which item a group begins there.  Tiles of a small matrix all go to one XCD, whose L2 then holds it; those of a large one are
+// cut into 8 runs of neighbours.
+struct Table {
+    Group g[MAXG];
+    unsigned fin[MAXG], fio[MAXG], fsym[8][MAXG], fapp[8][MAXG];
+};
+
+__host__ __device__ __forceinline__ unsigned run_start(unsigned total, int home, int xcd) {
+    return home < 0 ? (unsigned)((unsigned long long)total * xcd / 8) : (xcd > home ? total : 0u);
+}
+
+__global__ void __launch_bounds__(256) ortho_table_kernel(const Chunk ch, Table* __restrict__ t) {
+    const unsigned* from = reinterpret_cast<const unsigned*>(ch.g);
+    unsigned* to = reinterpret_cast<unsigned*>(t->g + ch.base);
+    for (int i = threadIdx.x; i < ch.n * (int)(sizeof(Group) / 4); i += 256) to[i] = from[i];
+    if (!ch.last) return;
+    __syncthreads();
+    if (threadIdx.x >= 64) return;
+    const int lane = threadIdx.x, count = ch.base + ch.n;
+    const bool live = lane < count;
+    const Group* g = t->g + (live ? lane : 0);
+    t->fin[lane] = live ? g->fin : 0xffffffffu;
+    t->fio[lane] = live ? g->fio : 0xffffffffu;
+#pragma unroll 1
+    for (int k = 0; k < 16; ++k) {
+        const int xcd = k & 7, home = k < 8 ? g->hsym : g->happ;
+        const unsigned total = live ? (unsigned)g->batch * (unsigned)(k < 8 ? g->tsym : g->tapp) : 0u;
+        const unsigned mine = run_start(total, home, xcd + 1) - run_start(total, home, xcd);
+        unsigned sum = mine;
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) {
+            const unsigned v = __shfl_up(sum, o, 64);
+            if (lane >= o) sum += v;
+        }
+        (k < 8 ? t->fsym : t->fapp)[xcd][lane] = live ? sum - mine : 0xffffffffu;
+    }
+}
+
+// the last of the groups that begin at or before `at`
+__device__ __forceinline__ int find_group(const unsigned* first, unsigned at) {
+    const bool mine = first[threadIdx.x & 63] <= at;
     return __builtin_amdgcn_readfirstlane(__popcll(__ballot(mine)) - 1);
+}
+// item of a product -> group, matrix, tile; false: this XCD has no such item
+__device__ __forceinline__ bool find_tile(const Table* t, bool sym, int& gi, int& b, int& tile) {
+    const unsigned xcd = blockIdx.x & 7, at = blockIdx.x >> 3;
+    const unsigned* first = sym ? t->fsym[xcd] : t->fapp[xcd];
+    gi = find_group(first, at);
+    const Group* g = t->g + gi;
+    const unsigned tiles = sym ? g->tsym : g->tapp, total = (unsigned)g->batch * tiles;
+    const int home = sym ? g->hsym : g->happ;
+    const unsigned idx = at - first[gi] + run_start(total, home, xcd);
+    if (idx >= run_start(total, home, xcd + 1)) return false;
+    b = idx / tiles;
+    tile = idx - b * tiles;
+    return true;
 }
 
 __device__ __forceinline__ double wave_sum_d(double v) {
@@ -84,250 +130,375 @@ __device__ __forceinline__ int shift_of(const int* ex, unsigned mat, int down) {
     return e > 0 ? e : 0;
 }
 
-// ---- element (i, j) of the matrix that is orthogonalised --------------------------------------------------------------
-// kind 0 / 1: an fp32 / bf16 tensor; 2 / 3: the momentum direction from an fp32 / bf16 gradient arena
-template <int KIND>
-__device__ __forceinline__ float load_u(const IoGroup& g, const Muon& mu, int b, int i, int j) {
-    if (KIND >= 2) {
-        const long long e = g.bs + (long long)i * g.c + j;
-        const float v = mu.v[e];
-        if (!mu.nesterov) return v;
-        const float gr = KIND == 3 ? bf2f(((const bf16_t*)mu.g)[e]) : ((const float*)mu.g)[e];
-        return gr + mu.mu * v;
+// ---- the matrix that is orthogonalised --------------------------------------------------------------------------------
+// KIND 0 / 1: an fp32 / bf16 tensor; 2 / 3: the momentum direction from an fp32 / bf16 gradient arena
+template <bool BF>
+__device__ __forceinline__ void load8(const void* p, long long e, float (&v)[8]) {
+    if (BF) {
+        const bf16x8 b = *reinterpret_cast<const bf16x8*>((const bf16_t*)p + e);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = bf2f(b[j]);
+    } else {
+        load8f((const float*)p + e, v);
     }
-    const long long e = b * g.bs + (long long)i * g.rs + (long long)j * g.cs;
-    return KIND == 1 ? bf2f(((const bf16_t*)g.p)[e]) : ((const float*)g.p)[e];
 }
+template <bool BF>
+__device__ __forceinline__ float load1(const void* p, long long e) { return BF ? bf2f(((const bf16_t*)p)[e]) : ((const float*)p)[e]; }
 
-// sums of squares in 64 bits (an fp32 square overflows from 1.8e19 on and vanishes below 1e-23): one partial a workgroup
+__device__ __forceinline__ float momentum_of(const Muon& mu, float g, float v) { return mu.mu * v + g; }
+__device__ __forceinline__ float direction_of(const Muon& mu, float g, float v) { return mu.nesterov ? g + mu.mu * v : v; }   // v: new
+
+// sums of squares in 64 bits (an fp32 square overflows from 1.8e19 on and vanishes below 1e-23): one partial a workgroup.
+// (The new momentum is not stored here: ortho_pack_kernel computes it again, and what this pass read may still be in the
+// memory-side cache then.)
 template <int KIND>
-__global__ void __launch_bounds__(256) ortho_sqsum_kernel(const IoTable t, const Muon mu, double* __restrict__ part) {
-    const int gi = find_group(t, blockIdx.x);
-    const IoGroup g = t.g[gi];
+__global__ void __launch_bounds__(256) ortho_sqsum_kernel(const Table* __restrict__ t, const Muon mu, double* __restrict__ part) {
+    constexpr bool BF = KIND & 1;
+    const int gi = find_group(t->fin, blockIdx.x);
+    const Group& g = t->g[gi];
     const long long numel = (long long)g.r * g.c;
-    const int np = (int)((numel + g.part_elems - 1) / g.part_elems);
-    const unsigned idx = blockIdx.x - g.first;
-    const int b = idx / np, pi = idx - b * np;
+    const unsigned idx = blockIdx.x - t->fin[gi];
+    const int b = idx / g.parts, pi = idx - b * g.parts;
     const long long lo = (long long)pi * g.part_elems, hi = lo + g.part_elems < numel ? lo + g.part_elems : numel;
     double s = 0.0;
-    for (long long e = lo + threadIdx.x; e < hi; e += 256) {
-        float u;
-        if (KIND >= 2) {
-            const long long at = g.bs + e;
-            const float gr = KIND == 3 ? bf2f(((const bf16_t*)mu.g)[at]) : ((const float*)mu.g)[at];
-            const float v = mu.mu * mu.v[at] + gr;
-            mu.v[at] = v;
-            u = mu.nesterov ? gr + mu.mu * v : v;
-        } else {
-            const int i = (int)(e / g.c), j = (int)(e - (long long)i * g.c);
-            u = load_u<KIND>(g, mu, b, i, j);
+    if (KIND >= 2) {
+        const long long end8 = lo + ((hi - lo) & ~7LL);
+        for (long long e = lo + threadIdx.x * 8; e < end8; e += 2048) {
+            float gr[8], v[8];
+            load8<BF>(mu.g, g.sb + e, gr);
+            load8f(mu.v + g.sb + e, v);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const float u = direction_of(mu, gr[j], momentum_of(mu, gr[j], v[j]));
+                s += (double)u * (double)u;
+            }
         }
-        s += (double)u * (double)u;
+        if (threadIdx.x < hi - end8) {
+            const long long e = g.sb + end8 + threadIdx.x;
+            const float gr = load1<BF>(mu.g, e), u = direction_of(mu, gr, momentum_of(mu, gr, mu.v[e]));
+            s += (double)u * (double)u;
+        }
+    } else if (g.vec && g.rs == g.c) {       // dense
+        const long long end8 = lo + ((hi - lo) & ~7LL);
+        for (long long e = lo + threadIdx.x * 8; e < end8; e += 2048) {
+            float u[8];
+            load8<BF>(g.src, b * g.sb + e, u);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) s += (double)u[j] * (double)u[j];
+        }
+        if (threadIdx.x < hi - end8) {
+            const float u = load1<BF>(g.src, b * g.sb + end8 + threadIdx.x);
+            s += (double)u * (double)u;
+        }
+    } else {
+        for (long long e = lo + threadIdx.x; e < hi; e += 256) {
+            const int i = (int)(e / g.c), j = (int)(e - (long long)i * g.c);
+            const float u = load1<BF>(g.src, b * g.sb + (long long)i * g.rs + (long long)j * g.cs);
+            s += (double)u * (double)u;
+        }
     }
     __shared__ double red[4];
     s = wave_sum_d(s);
     if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = s;
     __syncthreads();
-    if (threadIdx.x == 0) part[g.po + (unsigned)b * np + pi] = (red[0] + red[1]) + (red[2] + red[3]);
+    if (threadIdx.x == 0) part[g.po + (unsigned)b * g.parts + pi] = (red[0] + red[1]) + (red[2] + red[3]);
 }
 
-// hi + lo of the scaled, normalised matrix; one 64 x 64 tile of the padded workspace a workgroup
+// scale and further shift of a matrix of this norm: X in the workspace is 2^(12 + shift) X
+__device__ __forceinline__ double inverse_of(double norm, float eps, int& shift) {
+    shift = norm < (double)eps && norm > 0.0 ? ilogb((double)eps / norm) : 0;
+    return ldexp((double)SC, shift) / (norm > (double)eps ? norm : (norm == norm ? (double)eps : norm));   // (a NaN stays one)
+}
+
+// hi + lo of the scaled, normalised matrix; one 64 x 64 tile of the padded workspace a workgroup.  A lane's 8 elements run along
+// the source's rows in both orientations.
 template <int KIND>
-__global__ void __launch_bounds__(256) ortho_pack_kernel(const IoTable t, const Muon mu, const double* __restrict__ part, float eps,
+__global__ void __launch_bounds__(256) ortho_pack_kernel(const Table* __restrict__ t, const Muon mu, const double* __restrict__ part, float eps,
                                                         int* __restrict__ ex, f16_t* __restrict__ xh, f16_t* __restrict__ xl) {
-    __shared__ float tile[64][65];
+    constexpr bool BF = KIND & 1;
+    __shared__ __attribute__((aligned(16))) float tile[64][68];
     __shared__ double red[4];
-    const int gi = find_group(t, blockIdx.x);
-    const IoGroup g = t.g[gi];
+    const int gi = find_group(t->fio, blockIdx.x);
+    const Group& g = t->g[gi];
     const bool turn = g.r > g.c;
-    const int n = turn ? g.c : g.r, m = turn ? g.r : g.c;
-    const int tn = (n + 63) >> 6, tm = (m + 63) >> 6;
-    const unsigned idx = blockIdx.x - g.first;
+    const int tn = g.np >> 6, tm = g.mp >> 6;
+    const unsigned idx = blockIdx.x - t->fio[gi];
     const int b = idx / (tn * tm), ti = (idx - b * (tn * tm)) / tm, tj = idx - b * (tn * tm) - ti * tm;
-    const long long numel = (long long)g.r * g.c;
-    const int np = (int)((numel + g.part_elems - 1) / g.part_elems);
     double s = 0.0;
-    for (int k = threadIdx.x; k < np; k += 256) s += part[g.po + (unsigned)b * np + k];
+    for (int k = threadIdx.x; k < g.parts; k += 256) s += part[g.po + (unsigned)b * g.parts + k];
     s = wave_sum_d(s);
     if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = s;
-    __syncthreads();
-    const double norm = sqrt((red[0] + red[1]) + (red[2] + red[3]));
-    const bool small = norm < (double)eps && norm > 0.0;
-    const int shift = small ? ilogb((double)eps / norm) : 0;
-    const double inv = ldexp((double)SC, shift) / (norm > (double)eps ? norm : (norm == norm ? (double)eps : norm));   // (a NaN stays one)
-    if (ti == 0 && tj == 0 && threadIdx.x == 0) ex[g.mat + b] = shift;
-    const int x = threadIdx.x & 63, y0 = threadIdx.x >> 6;
-    for (int y = y0; y < 64; y += 4) {
-        // the lane index runs along the source's rows (its usual contiguous direction) in both orientations
-        const int i = turn ? tj * 64 + y : ti * 64 + y, j = turn ? ti * 64 + x : tj * 64 + x;
-        const float u = i < g.r && j < g.c ? (float)(load_u<KIND>(g, mu, b, i, j) * inv) : 0.f;
-        if (turn) tile[x][y] = u; else tile[y][x] = u;
+    // the source: rows i0 .. i0 + 63, columns j0 .. j0 + 63
+    const int i0 = (turn ? tj : ti) * 64, j0 = (turn ? ti : tj) * 64;
+    const int x = (threadIdx.x & 7) * 8, y0 = threadIdx.x >> 3;
+    float u[2][8];
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+        const int i = i0 + y0 + k * 32, j = j0 + x;
+#pragma unroll
+        for (int q = 0; q < 8; ++q) u[k][q] = 0.f;
+        if (i >= g.r || j >= g.c) continue;
+        const long long e = KIND >= 2 ? g.sb + (long long)i * g.c + j : b * g.sb + (long long)i * g.rs + (long long)j * g.cs;
+        if (g.vec && j + 8 <= g.c) {
+            if (KIND >= 2) {
+                float v[8];
+                load8<BF>(mu.g, e, u[k]);
+                load8f(mu.v + e, v);
+#pragma unroll
+                for (int q = 0; q < 8; ++q) {
+                    v[q] = momentum_of(mu, u[k][q], v[q]);
+                    u[k][q] = direction_of(mu, u[k][q], v[q]);
+                }
+                *reinterpret_cast<f32x4*>(mu.v + e) = f32x4{v[0], v[1], v[2], v[3]};
+                *reinterpret_cast<f32x4*>(mu.v + e + 4) = f32x4{v[4], v[5], v[6], v[7]};
+            } else {
+                load8<BF>(g.src, e, u[k]);
+            }
+        } else {
+#pragma unroll
+            for (int q = 0; q < 8; ++q) {
+                if (j + q >= g.c) continue;
+                if (KIND >= 2) {
+                    const float gr = load1<BF>(mu.g, e + q), v = momentum_of(mu, gr, mu.v[e + q]);
+                    mu.v[e + q] = v;
+                    u[k][q] = direction_of(mu, gr, v);
+                } else {
+                    u[k][q] = load1<BF>(g.src, e + (long long)q * g.cs);
+                }
+            }
+        }
     }
     __syncthreads();
-    const int mp = tm * 64;
-    const long long base = (long long)g.xo * 64 + (long long)b * (tn * 64) * mp + (long long)(ti * 64) * mp + tj * 64;
-    for (int y = y0; y < 64; y += 4) {
-        const float u = tile[y][x];
-        const f16_t h = (f16_t)u;
-        xh[base + (long long)y * mp + x] = h;
-        xl[base + (long long)y * mp + x] = (f16_t)(u - (float)h);
+    int shift;
+    const double inv = inverse_of(sqrt((red[0] + red[1]) + (red[2] + red[3])), eps, shift);
+    if (ti == 0 && tj == 0 && threadIdx.x == 0) ex[g.mat + b] = shift;
+    const long long base = (long long)g.xo * 64 + ((long long)b * g.np + ti * 64) * g.mp + tj * 64;
+    if (turn) {
+#pragma unroll
+        for (int k = 0; k < 2; ++k)
+#pragma unroll
+            for (int q = 0; q < 8; ++q) tile[x + q][y0 + k * 32] = (float)(u[k][q] * inv);
+        __syncthreads();
+    }
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+        const int y = y0 + k * 32;
+        f16x8 h, l;
+#pragma unroll
+        for (int q = 0; q < 8; ++q) {
+            const float v = turn ? tile[y][x + q] : (float)(u[k][q] * inv);
+            h[q] = (f16_t)v;
+            l[q] = (f16_t)(v - (float)h[q]);
+        }
+        *reinterpret_cast<f16x8*>(xh + base + (long long)y * g.mp + x) = h;
+        *reinterpret_cast<f16x8*>(xl + base + (long long)y * g.mp + x) = l;
     }
 }
 
-// result of the last step -> the output tensor (bf16), or the weights (K23)
+// 8 consecutive elements of the result (row i from column j on, `live` of them inside) -> the output, or the weights (K23)
 template <bool MUON>
-__global__ void __launch_bounds__(256) ortho_unpack_kernel(const IoTable t, const Muon mu, const int* __restrict__ ex, int down,
-                                                          const f16_t* __restrict__ xh, const f16_t* __restrict__ xl) {
-    __shared__ float tile[64][65];
-    const int gi = find_group(t, blockIdx.x);
-    const IoGroup g = t.g[gi];
-    const bool turn = g.r > g.c;
-    const int n = turn ? g.c : g.r, m = turn ? g.r : g.c;
-    const int tn = (n + 63) >> 6, tm = (m + 63) >> 6;
-    const unsigned idx = blockIdx.x - g.first;
-    const int b = idx / (tn * tm), ti = (idx - b * (tn * tm)) / tm, tj = idx - b * (tn * tm) - ti * tm;
-    const int mp = tm * 64;
-    const long long base = (long long)g.xo * 64 + (long long)b * (tn * 64) * mp + (long long)(ti * 64) * mp + tj * 64;
-    const int x = threadIdx.x & 63, y0 = threadIdx.x >> 6;
-    const float scale = ldexpf(USC, -shift_of(ex, g.mat + b, down));
-    for (int y = y0; y < 64; y += 4) {
-        const float u = ((float)xh[base + (long long)y * mp + x] + (float)xl[base + (long long)y * mp + x]) * scale;
-        if (turn) tile[x][y] = u; else tile[y][x] = u;
-    }
-    __syncthreads();
-    for (int y = y0; y < 64; y += 4) {
-        const int i = turn ? tj * 64 + y : ti * 64 + y, j = turn ? ti * 64 + x : tj * 64 + x;
-        if (i >= g.r || j >= g.c) continue;
-        const float u = tile[y][x];
-        if (MUON) {
-            const float lr = mu.lr_scale ? mu.lr * *mu.lr_scale : mu.lr;
-            const float s = lr * sqrtf(g.r > g.c ? (float)g.r / (float)g.c : 1.f);
-            const long long e = g.bs + (long long)i * g.c + j;
-            const float w = mu.w[e] * (1.f - lr * mu.wd) - s * u;
-            mu.w[e] = w;
-            if (mu.lowp) mu.lowp[e] = f2bf(w);
+__device__ __forceinline__ void store_result(const Group& g, const Muon& mu, int b, int i, int j, int live, float lr, float step, const float (&u)[8]) {
+    if (MUON) {
+        const long long e = g.sb + (long long)i * g.c + j;
+        const float keep = 1.f - lr * mu.wd;
+        if (g.vec && live == 8) {
+            float w[8];
+            load8f(mu.w + e, w);
+            bf16x8 lo;
+#pragma unroll
+            for (int q = 0; q < 8; ++q) {
+                w[q] = w[q] * keep - step * u[q];
+                lo[q] = f2bf(w[q]);
+            }
+            *reinterpret_cast<f32x4*>(mu.w + e) = f32x4{w[0], w[1], w[2], w[3]};
+            *reinterpret_cast<f32x4*>(mu.w + e + 4) = f32x4{w[4], w[5], w[6], w[7]};
+            if (mu.lowp) *reinterpret_cast<bf16x8*>(mu.lowp + e) = lo;
         } else {
-            ((bf16_t*)g.p)[b * g.bs + (long long)i * g.rs + (long long)j * g.cs] = f2bf(u);
+#pragma unroll
+            for (int q = 0; q < 8; ++q)
+                if (q < live) {
+                    const float w = mu.w[e + q] * keep - step * u[q];
+                    mu.w[e + q] = w;
+                    if (mu.lowp) mu.lowp[e + q] = f2bf(w);
+                }
+        }
+    } else {
+        bf16_t* o = g.dst + ((long long)b * g.r + i) * g.c + j;
+        bf16x8 v;
+#pragma unroll
+        for (int q = 0; q < 8; ++q) v[q] = f2bf(u[q]);
+        if (live == 8 && (g.c & 7) == 0) {
+            *reinterpret_cast<bf16x8*>(o) = v;
+        } else {
+#pragma unroll
+            for (int q = 0; q < 8; ++q)
+                if (q < live) o[q] = v[q];
         }
     }
 }
 
 // ---- products ---------------------------------------------------------------------------------------------------------
-// D = F S^T over K (a multiple of 32): 4 waves as 2 x 2, a BF x BS tile in steps of 32, NST stages filled by LDS-DMA (tile
-// t + NST - 1 is on its way while tile t is multiplied; counted waits, one barrier a step).
-//   S and, with TRF = false, F: row-major, k-contiguous rows.  LDS rows of 64 bytes, 16-byte chunk c of row r at c ^ -(r / 4)
-//   (16 rows x one chunk are free of bank conflicts).
+// D = F S^T over K (a multiple of 64): W0 x W1 waves, a BF x BS tile, NST stages of 64 filled by LDS-DMA (128-byte pieces of
+// rows: a stage of 32 fetched each line twice), counted waits, one barrier a stage.
+//   S and, with TRF = false, F: row-major, k-contiguous rows.  16-byte chunk c of row r lies at c ^ (r / 2 mod 8): the 16 rows x
+//   one chunk that a quarter of a wave reads are free of bank conflicts.
 //   TRF = true: F is given transposed, [k][columns].  Its rows of k stay as they are in LDS and are read by the transposing
 //   load: 16 lanes take 4 rows x 16 columns; a half-wave touches rows 0-3 and 8-11 (+ 4, + 16), whose 32-byte windows
 //   the swizzle spreads over all banks.
-// A lane ends with D[i][j][e]: F index 16 i + 4 (lane / 16) + e, S index 16 j + lane % 16 of its wave's quarter.
+// A lane ends with D[i][j][e]: F index 16 i + 4 (lane / 16) + e, S index 16 j + lane % 16 of its wave's part.
 typedef __fp16 half4 __attribute__((ext_vector_type(4)));      // (the type that the transposing load is declared with)
 typedef __attribute__((address_space(3))) half4* lds_half4_ptr;
 constexpr unsigned OUT = 0x80000000u;      // an offset behind the descriptor's range: reads as zero
 
-__device__ __forceinline__ int nt_off(int row, int ch) { return row * 64 + ((ch ^ ((0 - (row >> 2)) & 3)) << 4); }
+__device__ __forceinline__ int nt_off(int row, int ch) { return row * 128 + ((ch ^ ((row >> 1) & 7)) << 4); }
 template <int B>
 __device__ __forceinline__ int tr_swz(int row) {
-    return B == 128 ? (row & 3) | ((row >> 1) & 4) : ((row >> 1) & 1) | ((row >> 2) & 2);
+    return B >= 128 ? (row & 3) | ((row >> 1) & 4) : ((row >> 1) & 1) | ((row >> 2) & 2);
 }
 
-template <int BF, int BS, int NST, bool TRF>
+template <int BF, int BS, int W0, int W1, int NST, bool TRF>
 struct Mul {
-    static constexpr int FBYTES = BF * 64, SBYTES = BS * 64, STAGE = FBYTES + SBYTES;
-    static constexpr int FL = BF / 64, SL = BS / 64, L = FL + SL;       // LDS-DMA instructions of a wave and stage
-    static constexpr int NF = BF / 32, NS = BS / 32;                    // fragments of a wave
+    static constexpr int WAVES = W0 * W1, THREADS = WAVES * 64;
+    static constexpr int FBYTES = BF * 128, SBYTES = BS * 128, STAGE = FBYTES + SBYTES;
+    static constexpr int FL = BF / 8 / WAVES, SL = BS / 8 / WAVES, L = FL + SL;         // LDS-DMA instructions of a wave and stage
+    static constexpr int NF = BF / W0 / 16, NS = BS / W1 / 16;                          // fragments of a wave
+    static_assert(FL * 8 * WAVES == BF && SL * 8 * WAVES == BS && L % NF == 0, "whole instructions, spread over the fragments");
+    static_assert(NST >= 2 && NST * STAGE <= 160 * 1024, "LDS");
     f32x4 acc[NF][NS];
 
     // f: first row (TRF: first column) of the tile, ldf its row length, fleft rows (columns) that exist; s likewise
-    __device__ __forceinline__ void run(unsigned char* smem, const f16_t* f, long long ldf, int fleft, const f16_t* s, long long lds, int sleft, int K) {
-        const int tid = threadIdx.x, lane = tid & 63, wid = __builtin_amdgcn_readfirstlane(tid >> 6), w0 = wid >> 1, w1 = wid & 1;
+    __device__ __forceinline__ void run(unsigned char* smem, const f16_t* f, int ldf, int fleft, const f16_t* s, int lds, int sleft, int K) {
+        const int tid = threadIdx.x, lane = tid & 63, wid = __builtin_amdgcn_readfirstlane(tid >> 6), w0 = wid / W1, w1 = wid % W1;
         const int fr = lane & 15, fq = lane >> 4;
-        const int KT = K / 32;
+        const int KT = K / 64;
         const unsigned lds0 = (unsigned)(uintptr_t)(__attribute__((address_space(3))) void*)smem;
-        unsigned fo[FL], so[SL];
+        unsigned vo[L];
 #pragma unroll
         for (int i = 0; i < FL; ++i) {
-            const int slot = (i * 4 + wid) * 64 + lane;
+            const int slot = (i * WAVES + wid) * 64 + lane;
             if (TRF) {
                 constexpr int CPR = BF / 8;
                 const int row = slot / CPR, ch = slot % CPR, c = (((ch >> 1) ^ tr_swz<BF>(row)) << 1) | (ch & 1);
-                fo[i] = c * 8 < fleft ? (unsigned)((row * ldf + c * 8) * 2) : OUT;
+                vo[i] = c * 8 < fleft ? (unsigned)((row * ldf + c * 8) * 2) : OUT;
             } else {
-                const int row = slot >> 2, c = (slot & 3) ^ ((0 - (row >> 2)) & 3);
-                fo[i] = row < fleft ? (unsigned)((row * ldf + c * 8) * 2) : OUT;
+                const int row = slot >> 3, c = (slot & 7) ^ ((row >> 1) & 7);
+                vo[i] = row < fleft ? (unsigned)((row * ldf + c * 8) * 2) : OUT;
             }
         }
 #pragma unroll
         for (int i = 0; i < SL; ++i) {
-            const int slot = (i * 4 + wid) * 64 + lane, row = slot >> 2, c = (slot & 3) ^ ((0 - (row >> 2)) & 3);
-            so[i] = row < sleft ? (unsigned)((row * lds + c * 8) * 2) : OUT;
+            const int slot = (i * WAVES + wid) * 64 + lane, row = slot >> 3, c = (slot & 7) ^ ((row >> 1) & 7);
+            vo[FL + i] = row < sleft ? (unsigned)((row * lds + c * 8) * 2) : OUT;
         }
-        // every stage is exactly L instructions a wave (zeros behind the end): the counted waits rely on it
-        auto fetch = [&](int kt, int stage) {
-            const bool live = kt < KT;
-            const u32x4 rf = raw_rsrc(f + (live ? (TRF ? (long long)kt * 32 * ldf : (long long)kt * 32) : 0), OUT - 16);
-            const u32x4 rs = raw_rsrc(s + (live ? (long long)kt * 32 : 0), OUT - 16);
-            const unsigned at = lds0 + (unsigned)(stage * STAGE + wid * 1024);
-#pragma unroll
-            for (int i = 0; i < FL; ++i) lds_dma16(rf, at + i * 4096, live ? fo[i] : OUT, 0u);
-#pragma unroll
-            for (int i = 0; i < SL; ++i) lds_dma16(rs, at + FBYTES + i * 4096, live ? so[i] : OUT, 0u);
+        const u32x4 rf = raw_rsrc(f, OUT - 16), rs = raw_rsrc(s, OUT - 16);
+        const unsigned fstep = TRF ? (unsigned)ldf * 128u : 128u;              // bytes from a tile to the next
+        // every stage is exactly L instructions a wave (behind the end: the last tile again): the counted waits rely on it
+        auto piece = [&](unsigned kt, unsigned at, int i) {                    // at: LDS address of the wave's part of the stage
+            if (i < FL) lds_dma16(rf, at + i * WAVES * 1024, vo[i], kt * fstep);
+            else lds_dma16(rs, at + FBYTES + (i - FL) * WAVES * 1024, vo[i], kt * 128u);
         };
-        int foff[NF], soff[NS];
+        // a fragment's offset in a stage, half h: i-th of f at fbase[h] + 2048 i (TRF: foff[i] + 64 BF h), of s at sbase[h] + 2048 j
+        int fbase[2], sbase[2], foff[NF];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            fbase[h] = nt_off(w0 * (BF / W0) + fr, h * 4 + fq);
+            sbase[h] = FBYTES + nt_off(w1 * (BS / W1) + fr, h * 4 + fq);
+        }
         const int trow = 8 * fq + ((lane >> 2) & 3);
 #pragma unroll
-        for (int i = 0; i < NF; ++i)
-            foff[i] = TRF ? trow * (BF * 2) + (((w0 * NF + i) ^ tr_swz<BF>(trow)) * 32) + 8 * (lane & 3) : nt_off(w0 * (BF / 2) + i * 16 + fr, fq);
-#pragma unroll
-        for (int j = 0; j < NS; ++j) soff[j] = FBYTES + nt_off(w1 * (BS / 2) + j * 16 + fr, fq);
+        for (int i = 0; i < NF; ++i) foff[i] = trow * (BF * 2) + (((w0 * NF + i) ^ tr_swz<BF>(trow)) * 32) + 8 * (lane & 3);
+        auto read_f = [&](unsigned char* st, int h, int i) -> f16x8 {
+            if (!TRF) return *reinterpret_cast<const f16x8*>(st + fbase[h] + i * 2048);
+            // (row + 4 has the swizzle of row: bit 2 of the row takes no part in it; nor does bit 5)
+            unsigned char* p = st + foff[i] + h * (BF * 64);
+            const f16x4 lo = __builtin_bit_cast(f16x4, __builtin_amdgcn_ds_read_tr16_b64_v4f16((lds_half4_ptr)p));
+            const f16x4 hi = __builtin_bit_cast(f16x4, __builtin_amdgcn_ds_read_tr16_b64_v4f16((lds_half4_ptr)(p + 4 * BF * 2)));
+            return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+        };
+        auto read_s = [&](unsigned char* st, int h, int j) -> f16x8 { return *reinterpret_cast<const f16x8*>(st + sbase[h] + j * 2048); };
 #pragma unroll
         for (int i = 0; i < NF; ++i)
 #pragma unroll
             for (int j = 0; j < NS; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
 
+        // The fragments of the next half are read while a half is multiplied: s into a second set of registers, each of f into
+        // its own behind its last use.  A stage is free once both halves are in registers: behind the barrier that ends
+        // the first one, tile t + NST goes where tile t was.
+        const unsigned at0 = lds0 + wid * 1024;
 #pragma unroll
-        for (int k = 0; k < NST - 1; ++k) fetch(k, k);
-        asm volatile("s_waitcnt vmcnt(%0)" ::"n"((NST - 2) * L) : "memory");
+        for (int k = 0; k < NST; ++k)
+#pragma unroll
+            for (int i = 0; i < L; ++i) piece(k < KT ? k : KT - 1, at0 + k * STAGE, i);
+        asm volatile("s_waitcnt vmcnt(%0)" ::"n"((NST - 1) * L) : "memory");
         __builtin_amdgcn_s_barrier();
-        int cur = 0, nxt = NST - 1;
-        for (int kt = 0; kt < KT; ++kt) {
-            fetch(kt + NST - 1, nxt);          // into the stage whose reads ended before the last barrier
-            unsigned char* st = smem + cur * STAGE;
-            f16x8 a[NF], b[NS];
+        f16x8 a[NF], b0[NS], b1[NS];
 #pragma unroll
-            for (int j = 0; j < NS; ++j) b[j] = *reinterpret_cast<const f16x8*>(st + soff[j]);
+        for (int j = 0; j < NS; ++j) b0[j] = read_s(smem, 0, j);
+#pragma unroll
+        for (int i = 0; i < NF; ++i) a[i] = read_f(smem, 0, i);
+        int cur = 0;                               // offset of tile kt's stage
+        for (int kt = 0; kt < KT; ++kt) {
+            unsigned char* st = smem + cur;
+#pragma unroll
+            for (int j = 0; j < NS; ++j) b1[j] = read_s(st, 1, j);
 #pragma unroll
             for (int i = 0; i < NF; ++i) {
-                if (TRF) {
-                    // (row + 4 has the swizzle of row: bit 2 of the row does not take part in it)
-                    const f16x4 lo = __builtin_bit_cast(f16x4, __builtin_amdgcn_ds_read_tr16_b64_v4f16((lds_half4_ptr)(st + foff[i])));
-                    const f16x4 hi = __builtin_bit_cast(f16x4, __builtin_amdgcn_ds_read_tr16_b64_v4f16((lds_half4_ptr)(st + foff[i] + 4 * BF * 2)));
-                    a[i] = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
-                } else {
-                    a[i] = *reinterpret_cast<const f16x8*>(st + foff[i]);
-                }
+#pragma unroll
+                for (int j = 0; j < NS; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a[i], b0[j], acc[i][j], 0, 0, 0);
+                a[i] = read_f(st, 1, i);
             }
-#pragma unroll
-            for (int i = 0; i < NF; ++i)
-#pragma unroll
-                for (int j = 0; j < NS; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a[i], b[j], acc[i][j], 0, 0, 0);
             asm volatile("s_waitcnt vmcnt(%0)" ::"n"((NST - 2) * L) : "memory");
             asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
             __builtin_amdgcn_s_barrier();
-            nxt = cur;
-            cur = cur + 1 == NST ? 0 : cur + 1;
+            const int ns = cur + STAGE == NST * STAGE ? 0 : cur + STAGE;
+            const unsigned next = kt + NST < KT ? kt + NST : KT - 1;
+            unsigned char* sn = smem + ns;
+#pragma unroll
+            for (int j = 0; j < NS; ++j) b0[j] = read_s(sn, 0, j);
+#pragma unroll
+            for (int i = 0; i < NF; ++i) {
+#pragma unroll
+                for (int j = 0; j < NS; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a[i], b1[j], acc[i][j], 0, 0, 0);
+                a[i] = read_f(sn, 0, i);
+#pragma unroll
+                for (int q = 0; q < L / NF; ++q) piece(next, at0 + cur, i * (L / NF) + q);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            cur = ns;
         }
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        __builtin_amdgcn_s_barrier();              // the LDS is the epilogue's from here
     }
+
+    // The epilogues go through LDS (fp32, rows of S, 16-byte chunk q of row s at q ^ fold(s)): whole rows are read back and
+    // written, and their loops stay rolled - a tile's code runs once, so its length is paid for in instruction fetches
+    // (an unrolled epilogue of 8 KB took 4 us).  PASSES parts of BS / PASSES rows where the tile is larger than the stages.
+    static constexpr int PASSES = BF * BS * 4 > NST * STAGE ? BF * BS * 4 / (NST * STAGE) : 1;
+    static_assert(NS % PASSES == 0, "whole fragments a pass");
+    static constexpr int ROWS = BS / PASSES;       // rows of a pass: those of fragments j with j / (NS / PASSES) == pass of every wave
+    __device__ __forceinline__ void to_lds(float* t, int pass) const {
+        const int lane = threadIdx.x & 63, wid = threadIdx.x >> 6, w0 = wid / W1, w1 = wid % W1;
+        const int s0 = w1 * (ROWS / W1) + (lane & 15), f0 = w0 * (BF / W0 / 4) + (lane >> 4);
+#pragma unroll
+        for (int p = 0; p < PASSES; ++p)
+            if (p == pass)
+#pragma unroll
+                for (int j = 0; j < NS / PASSES; ++j)
+#pragma unroll
+                    for (int i = 0; i < NF; ++i)
+                        *reinterpret_cast<f32x4*>(t + (s0 + j * 16) * BF + (((f0 + i * 4) ^ fold(s0 + j * 16)) * 4)) = acc[i][p * (NS / PASSES) + j];
+    }
+    static __device__ __forceinline__ int fold(int s) { return (s ^ (s >> 3)) & 15; }     // rows 1 apart and rows 8 apart on different banks
+    // row of the tile that row `s` of a pass holds
+    static __device__ __forceinline__ int tile_row(int s, int pass) { return (s / (ROWS / W1)) * (BS / W1) + pass * (ROWS / W1) + s % (ROWS / W1); }
+    static __device__ __forceinline__ void put(float* t, int s, int q, f32x4 v) { *reinterpret_cast<f32x4*>(t + s * BF + ((q ^ fold(s)) * 4)) = v; }
+    static __device__ __forceinline__ float at1(const float* t, int s, int f) { return t[s * BF + (((f >> 2) ^ fold(s)) * 4) + (f & 3)]; }
+    static __device__ __forceinline__ f32x4 at(const float* t, int s, int q) { return *reinterpret_cast<const f32x4*>(t + s * BF + ((q ^ fold(s)) * 4)); }
 };
 
 // Tiles of a matrix in bands of 8 rows, a band column by column: the tiles that an XCD works on at a time are about as many
-// rows as columns.  A matrix of many tiles is dealt to the XCDs (workgroup number modulo 8) in runs of neighbours.
-__device__ __forceinline__ int deal(int idx, int tiles) {
-    if (tiles < 64) return idx;
-    const int q = tiles >> 3, r = tiles & 7, xcd = idx & 7;
-    return xcd * q + (xcd < r ? xcd : r) + (idx >> 3);
-}
+// rows as columns.
 __device__ __forceinline__ void band_tile(int idx, int rows, int cols, int& ti, int& tj) {
     const int band = idx / (8 * cols), rem = idx - band * 8 * cols, h = rows - band * 8 < 8 ? rows - band * 8 : 8;
     tj = rem / h;
@@ -352,99 +523,164 @@ __device__ __forceinline__ void tri_tile(int idx, int rows, int& ti, int& tj) {
 }
 
 // SQUARE = false: O, d of A = X X^T.  SQUARE = true: O, d of P = b A + c A^2 (diagonal: + a) from those of A
-template <int B, int NST, bool SQUARE>
-__global__ void __launch_bounds__(256, 2) ortho_sym_kernel(const MulTable t, const f16_t* __restrict__ in, const float* __restrict__ din,
+template <int B, int W0, int W1, int NST, bool SQUARE>
+__global__ void __launch_bounds__(W0 * W1 * 64, 2) ortho_sym_kernel(const Table* __restrict__ t, const f16_t* __restrict__ in, const float* __restrict__ din,
                                                           f16_t* __restrict__ out, float* __restrict__ dout, const int* __restrict__ ex, int down,
                                                           float ca, float cb, float cc) {
-    typedef Mul<B, B, NST, false> M;
+    typedef Mul<B, B, W0, W1, NST, false> M;
     __shared__ __attribute__((aligned(16))) unsigned char smem[NST * M::STAGE];
-    const int gi = find_group(t, blockIdx.x);
-    const MulGroup g = t.g[gi];
-    const unsigned idx = blockIdx.x - g.first;
-    const int b = idx / g.tiles;
-    if (b >= g.batch) return;              // (groups are padded to multiples of 8 workgroups)
-    int ti, tj;
-    tri_tile(deal(idx - b * g.tiles, g.tiles), (g.np + B - 1) / B, ti, tj);
-    const int K = SQUARE ? g.np : g.mp;
-    const long long ao = (long long)g.ao * 64 + (long long)b * g.np * g.np;
-    const f16_t* src = SQUARE ? in + ao : in + (long long)g.xo * 64 + (long long)b * g.np * g.mp;
+    int gi, b, tidx, ti, tj;
+    if (!find_tile(t, true, gi, b, tidx)) return;
+    const Group& g = t->g[gi];
+    const int np = g.np, lda = np, ld = SQUARE ? np : g.mp, K = ld;
+    tri_tile(tidx, (np + B - 1) / B, ti, tj);
+    const long long ao = (long long)g.ao * 64 + (long long)b * np * lda;
+    const f16_t* src = SQUARE ? in + ao : in + (long long)g.xo * 64 + (long long)b * np * ld;
     M m;
-    m.run(smem, src + (long long)ti * B * K, K, g.np - ti * B, src + (long long)tj * B * K, K, g.np - tj * B, K);
-    const int lane = threadIdx.x & 63, wid = threadIdx.x >> 6, w0 = wid >> 1, w1 = wid & 1;
+    m.run(smem, src + (long long)ti * B * ld, ld, g.np - ti * B, src + (long long)tj * B * ld, ld, g.np - tj * B, K);
     const float* d = SQUARE ? din + g.dof + (long long)b * g.np : nullptr;
     const float unscale = SQUARE ? USC * USC : ldexpf(USC * USC, -2 * shift_of(ex, g.mat + b, down));
     f16_t* o = out + ao;
-#pragma unroll
-    for (int i = 0; i < M::NF; ++i)
-#pragma unroll
-        for (int j = 0; j < M::NS; ++j) {
-            const int r = ti * B + w0 * (B / 2) + i * 16 + (lane >> 4) * 4, c = tj * B + w1 * (B / 2) + j * 16 + (lane & 15);
-            if (B > 64 && (r >= g.np || c >= g.np)) continue;
-            f32x4 v = m.acc[i][j] * unscale;
-            if (SQUARE) {
-                // (A is symmetric: its row c holds this lane's column)
-                const f16x4 a = *reinterpret_cast<const f16x4*>(src + (long long)c * K + r);
-                const f32x4 dr = *reinterpret_cast<const f32x4*>(d + r);
-                const float dc = d[c];
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const float af = (float)a[e] * USC;
-                    v[e] = r + e == c ? ca + cb * dc + cc * (v[e] + dc * dc) : cb * af + cc * (v[e] + (dr[e] + dc) * af);
-                }
-            }
-            f16x4 h;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                if (r + e == c) dout[g.dof + (long long)b * g.np + c] = v[e];
-                h[e] = r + e == c ? (f16_t)0.f : (f16_t)(v[e] * SC);
-                if (ti != tj) o[(long long)(r + e) * g.np + c] = h[e];
-            }
-            *reinterpret_cast<f16x4*>(o + (long long)c * g.np + r) = h;
+    float* dst = dout + g.dof + (long long)b * g.np;
+    float* tile = reinterpret_cast<float*>(smem);
+    // value (r, c) of the result from the product's
+    auto value = [&](float v, int r, int c, float a, float dr, float dc) {
+        v *= unscale;
+        if (SQUARE) {
+            a *= USC;
+            v = r == c ? ca + cb * dc + cc * (v + dc * dc) : cb * a + cc * (v + (dr + dc) * a);
         }
+        return v;
+    };
+#pragma unroll
+    for (int pass = 0; pass < M::PASSES; ++pass) {
+        if (M::PASSES > 1 && pass > 0) __syncthreads();
+        m.to_lds(tile, pass);
+        __syncthreads();
+        // block (tj, ti): rows c, 8 of r a thread
+        for (int k = threadIdx.x; k < M::ROWS * B / 8; k += M::THREADS) {
+            const int s = k / (B / 8), q = (k % (B / 8)) * 2, c = tj * B + M::tile_row(s, pass), r = ti * B + q * 4;
+            if (B > 64 && (c >= g.np || r >= g.np)) continue;
+            const f32x4 v0 = M::at(tile, s, q), v1 = M::at(tile, s, q + 1);
+            f16x8 av = {};
+            f32x4 d0 = {}, d1 = {};
+            float dc = 0.f;
+            if (SQUARE) {
+                av = *reinterpret_cast<const f16x8*>(src + (long long)c * ld + r);        // (A is symmetric)
+                d0 = *reinterpret_cast<const f32x4*>(d + r);
+                d1 = *reinterpret_cast<const f32x4*>(d + r + 4);
+                dc = d[c];
+            }
+            f16x8 h;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const float v = value(e < 4 ? v0[e & 3] : v1[e & 3], r + e, c, (float)av[e], e < 4 ? d0[e & 3] : d1[e & 3], dc);
+                h[e] = r + e == c ? (f16_t)0.f : (f16_t)(v * SC);
+                if (ti == tj && r + e == c) dst[c] = v;
+            }
+            *reinterpret_cast<f16x8*>(o + (long long)c * lda + r) = h;
+        }
+        if (ti == tj) continue;
+        // block (ti, tj): 4 rows r x 8 of c a thread, 8 threads side by side along c
+        for (int k = threadIdx.x; k < M::ROWS * B / 32; k += M::THREADS) {
+            const int s = ((k & 7) + (k >> 3) % (M::ROWS / 64) * 8) * 8, q = (k >> 3) / (M::ROWS / 64);
+            const int c = tj * B + M::tile_row(s, pass), r = ti * B + q * 4;
+            if (B > 64 && (c >= g.np || r >= g.np)) continue;
+            f32x4 v[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] = M::at(tile, s + e, q);
+            f16x8 av[4] = {};
+            f32x4 d0 = {}, d1 = {}, dr = {};
+            if (SQUARE) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) av[i] = *reinterpret_cast<const f16x8*>(src + (long long)(r + i) * ld + c);
+                d0 = *reinterpret_cast<const f32x4*>(d + c);
+                d1 = *reinterpret_cast<const f32x4*>(d + c + 4);
+                dr = *reinterpret_cast<const f32x4*>(d + r);
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                f16x8 h;
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                    h[e] = (f16_t)(value(v[e][i], r + i, c + e, (float)av[i][e], dr[i], e < 4 ? d0[e & 3] : d1[e & 3]) * SC);
+                *reinterpret_cast<f16x8*>(o + (long long)(r + i) * lda + c) = h;
+            }
+        }
+    }
 }
 
-// X' = pd X + offdiag(P) X_hi; tile: BF columns of X times BS rows of P
-template <int BF, int BS, int NST>
-__global__ void __launch_bounds__(256, 2) ortho_apply_kernel(const MulTable t, const f16_t* __restrict__ P, const float* __restrict__ pd,
-                                                            const f16_t* __restrict__ xh, const f16_t* __restrict__ xl,
+// X' = pd X + offdiag(P) X_hi; tile: BF columns of X times BS rows of P.  FINAL 0: the next X; 1: the output; 2: the weights (K23)
+template <int BF, int BS, int W0, int W1, int NST, int FINAL>
+__global__ void __launch_bounds__(W0 * W1 * 64, 2) ortho_apply_kernel(const Table* __restrict__ t, const Muon mu, const f16_t* __restrict__ P,
+                                                            const float* __restrict__ pd, const f16_t* __restrict__ xh, const f16_t* __restrict__ xl,
                                                             f16_t* __restrict__ yh, f16_t* __restrict__ yl,
                                                             const int* __restrict__ ex, int down, int down1) {
-    typedef Mul<BF, BS, NST, true> M;
+    typedef Mul<BF, BS, W0, W1, NST, true> M;
     __shared__ __attribute__((aligned(16))) unsigned char smem[NST * M::STAGE];
-    const int gi = find_group(t, blockIdx.x);
-    const MulGroup g = t.g[gi];
-    const unsigned idx = blockIdx.x - g.first;
-    const int b = idx / g.tiles;
-    if (b >= g.batch) return;              // (groups are padded to multiples of 8 workgroups)
-    int ti, tj;
-    band_tile(deal(idx - b * g.tiles, g.tiles), (g.np + BS - 1) / BS, (g.mp + BF - 1) / BF, ti, tj);
-    const f16_t* A = P + (long long)g.ao * 64 + (long long)b * g.np * g.np + (long long)ti * BS * g.np;
-    const long long xo = (long long)g.xo * 64 + (long long)b * g.np * g.mp;
+    int gi, b, tidx, ti, tj;
+    if (!find_tile(t, false, gi, b, tidx)) return;
+    const Group& g = t->g[gi];
+    const int np = g.np, mp = g.mp;
+    band_tile(tidx, (np + BS - 1) / BS, (mp + BF - 1) / BF, ti, tj);
+    const f16_t* A = P + (long long)g.ao * 64 + ((long long)b * np + ti * BS) * np;
+    const long long xo = (long long)g.xo * 64 + (long long)b * np * mp;
     M m;
-    m.run(smem, xh + xo + tj * BF, g.mp, g.mp - tj * BF, A, g.np, g.np - ti * BS, g.np);
-    const float rescale = ldexpf(1.f, shift_of(ex, g.mat + b, down1) - shift_of(ex, g.mat + b, down));
-    const int lane = threadIdx.x & 63, wid = threadIdx.x >> 6, w0 = wid >> 1, w1 = wid & 1;
-    const float* d = pd + g.dof + (long long)b * g.np;
+    m.run(smem, xh + xo + tj * BF, mp, mp - tj * BF, A, np, np - ti * BS, np);
+    const int e0 = shift_of(ex, g.mat + b, down), e1 = shift_of(ex, g.mat + b, down1);
+    const float rescale = FINAL ? ldexpf(USC, -e0) : ldexpf(1.f, e1 - e0);
+    const float* d = pd + g.dof + (long long)b * np;
+    float* tile = reinterpret_cast<float*>(smem);
+    const bool turn = g.r > g.c;
+    float lr = 0.f, step = 0.f;
+    if (FINAL == 2) {
+        lr = mu.lr_scale ? mu.lr * *mu.lr_scale : mu.lr;
+        step = lr * sqrtf(turn ? (float)g.r / (float)g.c : 1.f);
+    }
 #pragma unroll
-    for (int j = 0; j < M::NS; ++j) {
-        const int r = ti * BS + w1 * (BS / 2) + j * 16 + (lane & 15);
-        if (BS > 64 && r >= g.np) continue;
-        const float dr = d[r];
+    for (int pass = 0; pass < M::PASSES; ++pass) {
+        if (M::PASSES > 1 && pass > 0) __syncthreads();
+        m.to_lds(tile, pass);
+        __syncthreads();
+#pragma unroll 2
+        for (int k = threadIdx.x; k < M::ROWS * BF / 8; k += M::THREADS) {
+            const int s = k / (BF / 8), q = (k % (BF / 8)) * 2, r = ti * BS + M::tile_row(s, pass), c = tj * BF + q * 4;
+            if ((BS > 64 && r >= np) || (BF > 64 && c >= mp)) continue;
+            const long long at = xo + (long long)r * mp + c;
+            const f16x8 h0 = *reinterpret_cast<const f16x8*>(xh + at), l0 = *reinterpret_cast<const f16x8*>(xl + at);
+            const float dr = d[r];
+            const f32x4 v0 = M::at(tile, s, q), v1 = M::at(tile, s, q + 1);
+            float v[8];
 #pragma unroll
-        for (int i = 0; i < M::NF; ++i) {
-            const int c = tj * BF + w0 * (BF / 2) + i * 16 + (lane >> 4) * 4;
-            if (BF > 64 && c >= g.mp) continue;
-            const long long at = xo + (long long)r * g.mp + c;
-            const f16x4 h0 = *reinterpret_cast<const f16x4*>(xh + at), l0 = *reinterpret_cast<const f16x4*>(xl + at);
-            f16x4 h, l;
+            for (int e = 0; e < 8; ++e) v[e] = (dr * ((float)h0[e] + (float)l0[e]) + (e < 4 ? v0[e & 3] : v1[e & 3]) * USC) * rescale;
+            if (FINAL == 0) {
+                f16x8 h, l;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const float v = (dr * ((float)h0[e] + (float)l0[e]) + m.acc[i][j][e] * USC) * rescale;
-                h[e] = (f16_t)v;
-                l[e] = (f16_t)(v - (float)h[e]);
+                for (int e = 0; e < 8; ++e) {
+                    h[e] = (f16_t)v[e];
+                    l[e] = (f16_t)(v[e] - (float)h[e]);
+                }
+                *reinterpret_cast<f16x8*>(yh + at) = h;
+                *reinterpret_cast<f16x8*>(yl + at) = l;
+            } else if (!turn) {
+                if (r < g.r && c < g.c) store_result<FINAL == 2>(g, mu, b, r, c, g.c - c < 8 ? g.c - c : 8, lr, step, v);
+            } else {
+                M::put(tile, s, q, f32x4{v[0], v[1], v[2], v[3]});
+                M::put(tile, s, q + 1, f32x4{v[4], v[5], v[6], v[7]});
             }
-            *reinterpret_cast<f16x4*>(yh + at) = h;
-            *reinterpret_cast<f16x4*>(yl + at) = l;
+        }
+        if (FINAL == 0 || !turn) continue;
+        // a tall matrix: the tile's columns are the result's rows; 8 threads side by side along them
+        __syncthreads();
+#pragma unroll 1
+        for (int k = threadIdx.x; k < M::ROWS * BF / 8; k += M::THREADS) {
+            const int s = ((k & 7) + (k >> 3) % (M::ROWS / 64) * 8) * 8, f = (k >> 3) / (M::ROWS / 64);
+            const int j = ti * BS + M::tile_row(s, pass), i = tj * BF + f;
+            if (i >= g.r || j >= g.c) continue;
+            float v[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] = M::at1(tile, s + e, f);
+            store_result<FINAL == 2>(g, mu, b, i, j, g.c - j < 8 ? g.c - j : 8, lr, step, v);
         }
     }
 }
@@ -455,7 +691,7 @@ struct Desc { long long src, sb, srs, scs, dst, db, drs, dcs, r, c, batch; };
 
 struct Plan {
     long long x_elems = 0, a_elems = 0, d_elems = 0, parts = 0, mats = 0;
-    long long xa_h, xa_l, xb_h, xb_l, o, p, d, pd, part, ex, bytes;
+    long long table, xa_h, xa_l, xb_h, xb_l, o, p, d, pd, part, ex, bytes;
 };
 
 long long part_elems_of(long long numel) {
@@ -469,9 +705,9 @@ bool plan_of(const Desc* q, int count, Plan& pl) {
     if (count < 0 || count > MAXG || (count && !q)) return false;
     for (int i = 0; i < count; ++i) {
         const Desc& s = q[i];
-        if (s.r <= 0 || s.c <= 0 || s.batch <= 0 || s.r > (1 << 20) || s.c > (1 << 20)) return false;
-        if (s.batch > (1LL << 31) || (s.r * s.c) > (1LL << 33)) return false;
+        if (s.r <= 0 || s.c <= 0 || s.batch <= 0 || s.r >= (1LL << 30) || s.c >= (1LL << 30)) return false;
         const long long np = pad64(s.r < s.c ? s.r : s.c), mp = pad64(s.r < s.c ? s.c : s.r);
+        if (s.batch > 0x7fffffffLL || np * mp >= (1LL << 30)) return false;        // (a matrix's byte offsets have 31 bits)
         pl.x_elems += s.batch * np * mp;
         pl.a_elems += s.batch * np * np;
         pl.d_elems += s.batch * np;
@@ -482,6 +718,7 @@ bool plan_of(const Desc* q, int count, Plan& pl) {
     }
     auto up = [](long long b) { return (b + 255) / 256 * 256; };
     long long at = 0;
+    pl.table = at; at += up(sizeof(Table));
     pl.xa_h = at; at += up(pl.x_elems * 2);
     pl.xa_l = at; at += up(pl.x_elems * 2);
     pl.xb_h = at; at += up(pl.x_elems * 2);
@@ -494,6 +731,36 @@ bool plan_of(const Desc* q, int count, Plan& pl) {
     pl.ex = at; at += up(pl.mats * 4);
     pl.bytes = at;
     return true;
+}
+
+// XCDs for the groups' tiles, the costliest first: a group of more than a sixteenth of all cost is cut over all of them, another
+// goes to the one with the least so far.  Returns the workgroups of the launch.
+long long homes(Group* g, int count, bool sym, const double* cost) {
+    double all = 0.0, load[8] = {};
+    int order[MAXG];
+    for (int i = 0; i < count; ++i) { all += cost[i]; order[i] = i; }
+    for (int i = 1; i < count; ++i)
+        for (int k = i; k > 0 && cost[order[k]] > cost[order[k - 1]]; --k) { const int s = order[k]; order[k] = order[k - 1]; order[k - 1] = s; }
+    for (int k = 0; k < count; ++k) {
+        int home = -1;
+        if (cost[order[k]] * 16.0 <= all) {
+            home = 0;
+            for (int x = 1; x < 8; ++x) if (load[x] < load[home]) home = x;
+            load[home] += cost[order[k]];
+        }
+        (sym ? g[order[k]].hsym : g[order[k]].happ) = home;
+    }
+    long long most = 0;
+    for (int x = 0; x < 8; ++x) {
+        long long items = 0;
+        for (int i = 0; i < count; ++i) {
+            const unsigned total = (unsigned)g[i].batch * (unsigned)(sym ? g[i].tsym : g[i].tapp);
+            const int home = sym ? g[i].hsym : g[i].happ;
+            items += run_start(total, home, x + 1) - run_start(total, home, x);
+        }
+        if (items > most) most = items;
+    }
+    return most * 8;
 }
 
 // The polynomial over [0, top], top = what the step before leaves: the largest |f(s)|, |b s^2 + c s^4| (X and P have to stay
@@ -524,33 +791,40 @@ int growth_bits(float a, float b, float c, int steps) {
 int run_all(const Desc* q, int count, int kind, const Muon& mu, float a, float b, float c, int steps, float eps, char* ws, hipStream_t stream) {
     Plan pl;
     if (!plan_of(q, count, pl)) return DDL_EINVAL;
-    IoTable in, tiles, outt;
-    MulTable sym, app;
     static const int sb = getenv("ORTHO_SB") ? atoi(getenv("ORTHO_SB")) : 64, ab = getenv("ORTHO_AB") ? atoi(getenv("ORTHO_AB")) : 64;
-    in.count = tiles.count = outt.count = sym.count = app.count = count;
+    // the groups with the longest sums first
+    int order[MAXG];
+    for (int i = 0; i < count; ++i) order[i] = i;
+    auto longer = [&](int i) { return q[i].r > q[i].c ? q[i].r : q[i].c; };
+    for (int i = 1; i < count; ++i)
+        for (int k = i; k > 0 && longer(order[k]) > longer(order[k - 1]); --k) { const int s = order[k]; order[k] = order[k - 1]; order[k - 1] = s; }
+    Group g[MAXG];
+    double csym[MAXG], capp[MAXG];
     long long nin = 0, nio = 0, nsym = 0, napp = 0, xo = 0, ao = 0, dof = 0, po = 0, mat = 0;
     for (int i = 0; i < count; ++i) {
-        const Desc& s = q[i];
-        const long long n = s.r < s.c ? s.r : s.c, m = s.r < s.c ? s.c : s.r, np = pad64(n), mp = pad64(m), tn = np / 64, tm = mp / 64;
+        const Desc& s = q[order[i]];
+        Group& o = g[i];
+        const long long n = s.r < s.c ? s.r : s.c, m = s.r < s.c ? s.c : s.r, np = pad64(n), mp = pad64(m);
         const long long pe = part_elems_of(s.r * s.c), parts = (s.r * s.c + pe - 1) / pe;
-        IoGroup io;
-        io.p = (const void*)s.src; io.bs = s.sb; io.rs = (int)s.srs; io.cs = (int)s.scs; io.r = (int)s.r; io.c = (int)s.c;
-        io.part_elems = (int)pe; io.xo = (unsigned)(xo / 64); io.po = (unsigned)po; io.mat = (unsigned)mat;
-        io.first = (unsigned)nin; in.g[i] = io;
-        io.first = (unsigned)nio; tiles.g[i] = io;
-        if (kind < 2) { io.p = (const void*)s.dst; io.bs = s.db; io.rs = (int)s.drs; io.cs = (int)s.dcs; }
-        outt.g[i] = io;
-        MulGroup mg;
-        mg.np = (int)np; mg.mp = (int)mp; mg.xo = (unsigned)(xo / 64); mg.ao = (unsigned)(ao / 64); mg.dof = (unsigned)dof; mg.mat = (unsigned)mat; mg.batch = (int)s.batch;
         const long long sn = (np + sb - 1) / sb, an = (np + ab - 1) / ab, am = (mp + ab - 1) / ab;
-        mg.tiles = (int)(sn * (sn + 1) / 2); mg.first = (unsigned)nsym; sym.g[i] = mg;
-        nsym += (s.batch * mg.tiles + 7) / 8 * 8;
-        mg.tiles = (int)(an * am); mg.first = (unsigned)napp; app.g[i] = mg;
-        napp += (s.batch * mg.tiles + 7) / 8 * 8;
-        nin += s.batch * parts; nio += s.batch * tn * tm;
+        o.src = (const void*)s.src; o.dst = (bf16_t*)s.dst; o.sb = s.sb; o.rs = (int)s.srs; o.cs = (int)s.scs;
+        o.r = (int)s.r; o.c = (int)s.c; o.np = (int)np; o.mp = (int)mp; o.batch = (int)s.batch;
+        o.vec = kind >= 2 ? s.c % 8 == 0                                   // (offsets and arenas are checked)
+                          : s.scs == 1 && s.srs % 8 == 0 && (s.batch == 1 || s.sb % 8 == 0) && ((uintptr_t)s.src & 15) == 0;
+        o.part_elems = (int)pe; o.parts = (int)parts;
+        o.xo = (unsigned)(xo / 64); o.ao = (unsigned)(ao / 64); o.dof = (unsigned)dof; o.po = (unsigned)po; o.mat = (unsigned)mat;
+        o.tsym = (int)(sn * (sn + 1) / 2); o.tapp = (int)(an * am);
+        o.fin = (unsigned)nin; o.fio = (unsigned)nio;
+        csym[i] = (double)s.batch * o.tsym * (double)(np + mp + 512);      // (512: what a tile costs beside its sum)
+        capp[i] = (double)s.batch * o.tapp * (double)(np + 512);
+        nin += s.batch * parts; nio += s.batch * (np / 64) * (mp / 64);
+        nsym += s.batch * o.tsym; napp += s.batch * o.tapp;
         xo += s.batch * np * mp; ao += s.batch * np * np; dof += s.batch * np; po += s.batch * parts; mat += s.batch;
-        if (nin > 0x7fffffffLL || nio > 0x7fffffffLL || nsym > 0x7fffffffLL || napp > 0x7fffffffLL) return DDL_EINVAL;
+        if (nin > 0x7fffffffLL || nio > 0x7fffffffLL || nsym > 0x0fffffffLL || napp > 0x0fffffffLL) return DDL_EINVAL;
     }
+    nsym = homes(g, count, true, csym);
+    napp = homes(g, count, false, capp);
+    Table* t = (Table*)(ws + pl.table);
     f16_t *xh = (f16_t*)(ws + pl.xa_h), *xl = (f16_t*)(ws + pl.xa_l), *yh = (f16_t*)(ws + pl.xb_h), *yl = (f16_t*)(ws + pl.xb_l);
     f16_t *O = (f16_t*)(ws + pl.o), *P = (f16_t*)(ws + pl.p);
     float *d = (float*)(ws + pl.d), *pd = (float*)(ws + pl.pd);
@@ -558,22 +832,34 @@ int run_all(const Desc* q, int count, int kind, const Muon& mu, float a, float b
     int* ex = (int*)(ws + pl.ex);
     const int fall = growth_bits(a, b, c, steps);
     const dim3 block(256);
+    for (int base = 0; base < count; base += CHUNK) {
+        Chunk ch;
+        ch.base = base;
+        ch.n = count - base < CHUNK ? count - base : CHUNK;
+        ch.last = base + CHUNK >= count;
+        memcpy(ch.g, g + base, ch.n * sizeof(Group));
+        memset(ch.g + ch.n, 0, (CHUNK - ch.n) * sizeof(Group));
+        DDL_KLAUNCH(ortho_table_kernel, dim3(1), block, 0, stream, ch, t);
+    }
 #define IO(K)                                                                                              \
-    DDL_KLAUNCH(ortho_sqsum_kernel<K>, dim3((unsigned)nin), block, 0, stream, in, mu, part);               \
-    DDL_KLAUNCH(ortho_pack_kernel<K>, dim3((unsigned)nio), block, 0, stream, tiles, mu, part, eps, ex, xh, xl)
+    DDL_KLAUNCH(ortho_sqsum_kernel<K>, dim3((unsigned)nin), block, 0, stream, t, mu, part);                \
+    DDL_KLAUNCH(ortho_pack_kernel<K>, dim3((unsigned)nio), block, 0, stream, t, mu, part, eps, ex, xh, xl)
     if (kind == 0) { IO(0); } else if (kind == 1) { IO(1); } else if (kind == 2) { IO(2); } else { IO(3); }
 #undef IO
     for (int k = 0; k < steps; ++k) {
-#define SYM(B, NST, SQ, IN, DIN, OUTP, DOUT, DOWN) DDL_KLAUNCH((ortho_sym_kernel<B, NST, SQ>), dim3((unsigned)nsym), block, 0, stream, sym, IN, DIN, OUTP, DOUT, ex, DOWN, a, b, c)
-        if (sb == 64) { SYM(64, 4, false, xh, (const float*)nullptr, O, d, k * fall); SYM(64, 4, true, O, d, P, pd, 0); }
-        else { SYM(128, 4, false, xh, (const float*)nullptr, O, d, k * fall); SYM(128, 4, true, O, d, P, pd, 0); }
-        if (ab == 64) DDL_KLAUNCH((ortho_apply_kernel<64, 64, 4>), dim3((unsigned)napp), block, 0, stream, app, P, pd, xh, xl, yh, yl, ex, k * fall, (k + 1) * fall);
-        else DDL_KLAUNCH((ortho_apply_kernel<128, 128, 4>), dim3((unsigned)napp), block, 0, stream, app, P, pd, xh, xl, yh, yl, ex, k * fall, (k + 1) * fall);
+        const int fin = k < steps - 1 ? 0 : (kind < 2 ? 1 : 2);
+#define SYM(B, W0, W1, NST, SQ, IN, DIN, OUTP, DOUT, DOWN) DDL_KLAUNCH((ortho_sym_kernel<B, W0, W1, NST, SQ>), dim3((unsigned)nsym), dim3(W0 * W1 * 64), 0, stream, t, IN, DIN, OUTP, DOUT, ex, DOWN, a, b, c)
+#define APP1(B, W0, W1, NST, FIN) DDL_KLAUNCH((ortho_apply_kernel<B, B, W0, W1, NST, FIN>), dim3((unsigned)napp), dim3(W0 * W1 * 64), 0, stream, t, mu, P, pd, xh, xl, yh, yl, ex, k * fall, (k + 1) * fall)
+#define APP(B, W0, W1, NST) { if (fin == 0) APP1(B, W0, W1, NST, 0); else if (fin == 1) APP1(B, W0, W1, NST, 1); else APP1(B, W0, W1, NST, 2); }
+        if (sb == 64) { SYM(64, 2, 2, 3, false, xh, (const float*)nullptr, O, d, k * fall); SYM(64, 2, 2, 3, true, O, d, P, pd, 0); }
+        else if (sb == 128) { SYM(128, 2, 2, 2, false, xh, (const float*)nullptr, O, d, k * fall); SYM(128, 2, 2, 2, true, O, d, P, pd, 0); }
+        else { SYM(256, 2, 4, 2, false, xh, (const float*)nullptr, O, d, k * fall); SYM(256, 2, 4, 2, true, O, d, P, pd, 0); }
+        if (ab == 64) APP(64, 2, 2, 3)
+        else if (ab == 128) APP(128, 2, 2, 2)
+        else APP(256, 2, 4, 2)
         f16_t* s = xh; xh = yh; yh = s;
         s = xl; xl = yl; yl = s;
     }
-    if (kind < 2) DDL_KLAUNCH(ortho_unpack_kernel<false>, dim3((unsigned)nio), block, 0, stream, outt, mu, ex, steps * fall, xh, xl);
-    else DDL_KLAUNCH(ortho_unpack_kernel<true>, dim3((unsigned)nio), block, 0, stream, outt, mu, ex, steps * fall, xh, xl);
     return ddl_launch_status();
 }
 
@@ -586,7 +872,7 @@ extern "C" int ddl_ortho_max_groups() { return MAXG; }
 // 1 when the steps keep every operand in the range of scaled fp16 (see range_of)
 extern "C" int ddl_ortho_coefficients_ok(float a, float b, float c, int steps) {
     double growth;
-    return isfinite(a) && isfinite(b) && isfinite(c) && steps >= 0 && steps <= 64 && range_of(a, b, c, steps, growth);
+    return isfinite(a) && isfinite(b) && isfinite(c) && steps >= 1 && steps <= 64 && range_of(a, b, c, steps, growth);
 }
 
 // bytes of workspace of a call with these groups (`desc`: count x 11 int64: source address, its batch / row / column
@@ -626,7 +912,7 @@ extern "C" int ddl_muon_step(const long long* desc, int count, void* w, const vo
     if ((reinterpret_cast<uintptr_t>(ws) & 255) || !ddl_aligned16(w) || !ddl_aligned16(g) || !ddl_aligned16(v) || (lowp && !ddl_aligned16(lowp)))
         return DDL_EALIGN;
     for (int i = 0; i < count; ++i)
-        if (q[i].batch != 1 || q[i].sb < 0) return DDL_EINVAL;
+        if (q[i].batch != 1 || q[i].sb < 0 || q[i].sb % 8) return DDL_EINVAL;
     Muon m;
     m.g = g; m.v = (float*)v; m.w = (float*)w; m.lowp = (bf16_t*)lowp;
     m.lr = lr; m.mu = mu; m.wd = wd; m.nesterov = nesterov; m.lr_scale = (const float*)lr_scale;

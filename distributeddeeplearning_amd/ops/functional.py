@@ -204,8 +204,8 @@ ORTHO_COEFFICIENTS = (3.4445, -4.7750, 2.0315)   # five steps take singular valu
 
 
 def _check_steps(steps, coefficients, eps):
-    if not isinstance(steps, int) or not 0 <= steps <= 64:
-        raise ValueError("orthogonalize: steps must be an integer from 0 to 64, got %r" % (steps,))
+    if not isinstance(steps, int) or not 1 <= steps <= 64:
+        raise ValueError("orthogonalize: steps must be an integer from 1 to 64, got %r" % (steps,))
     if len(coefficients) != 3:
         raise ValueError("orthogonalize: three coefficients expected, got %r" % (coefficients,))
     if not eps >= 1e-30:

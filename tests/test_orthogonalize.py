@@ -50,6 +50,7 @@ def test_cpu_forms_and_types():
     (lambda: ops.orthogonalize(torch.zeros(2, 2, dtype=torch.float64)), "fp32 or bf16"),
     (lambda: ops.orthogonalize([torch.zeros(2, 2), torch.zeros(2, 2, dtype=torch.bfloat16)]), "share"),
     (lambda: ops.orthogonalize(torch.zeros(2, 2, requires_grad=True)), "gradient"),
+    (lambda: ops.orthogonalize(torch.zeros(2, 2), steps=0), "steps"),
     (lambda: ops.orthogonalize(torch.zeros(2, 2), steps=-1), "steps"),
     (lambda: ops.orthogonalize(torch.zeros(2, 2), steps=65), "steps"),
     (lambda: ops.orthogonalize(torch.zeros(2, 2), steps=2.5), "steps"),
