@@ -1,6 +1,6 @@
 // K24: dense layer on 8-bit integers (gfx950): a scale for each row of the input and for each output channel.
 //
-//   top_m = max_k |x[m][k]|,  xq[m][k] = rne(x[m][k] * (127 / top_m)),  sx_m = top_m / 127
+//   top_m = max_k |x[m][k]|,  xq[m][k] = rne(x[m][k] * (127 * (1 / top_m))),  sx_m = top_m / 127      (fp32, a rounding each)
 //   y[m][n] = (sum_k xq[m][k] q[n][k]) * (sx_m * s[n]) + bias[n]
 //
 // The sum is exact in int32 for K <= 133 144 (127^2 K < 2^31) whatever its order; rows below 1e-30 count as zero (127 / top
@@ -36,7 +36,7 @@ __global__ void __launch_bounds__(256) int8_rows_kernel(const T* __restrict__ x,
     top = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
     bad = redb[0] | redb[1] | redb[2] | redb[3];
     const bool zero = bad || top < 1e-30f;
-    const float inv = zero ? 0.f : 127.f / top;
+    const float inv = zero ? 0.f : 127.f * (1.f / top);
     if (threadIdx.x == 0) scale[m] = bad ? __builtin_nanf("") : (zero ? 0.f : top / 127.f);
     signed char* out = q + m * Kp;
     for (int k = threadIdx.x; k < Kp; k += 256) out[k] = k < K && !zero ? (signed char)(int)rintf(ld_in(row + k) * inv) : (signed char)0;

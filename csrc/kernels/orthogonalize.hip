@@ -55,6 +55,8 @@ struct Chunk { Group g[CHUNK]; int base, n, last; };
 struct Table {
     Group g[MAXG];
     unsigned fin[MAXG], fio[MAXG], fsym[8][MAXG], fapp[8][MAXG];
+    int batch[MAXG], np[MAXG], mp[MAXG], tsym[MAXG], tapp[MAXG], hsym[MAXG], happ[MAXG];      // copies out of g: a lane a group (find_tile)
+    unsigned xo[MAXG], ao[MAXG], dof[MAXG], mat[MAXG];
 };
 
 __host__ __device__ __forceinline__ unsigned run_start(unsigned total, int home, int xcd) {
@@ -73,6 +75,9 @@ __global__ void __launch_bounds__(256) ortho_table_kernel(const Chunk ch, Table*
     const Group* g = t->g + (live ? lane : 0);
     t->fin[lane] = live ? g->fin : 0xffffffffu;
     t->fio[lane] = live ? g->fio : 0xffffffffu;
+    t->batch[lane] = g->batch; t->np[lane] = g->np; t->mp[lane] = g->mp;
+    t->tsym[lane] = g->tsym; t->tapp[lane] = g->tapp; t->hsym[lane] = g->hsym; t->happ[lane] = g->happ;
+    t->xo[lane] = g->xo; t->ao[lane] = g->ao; t->dof[lane] = g->dof; t->mat[lane] = g->mat;
 #pragma unroll 1
     for (int k = 0; k < 16; ++k) {
         const int xcd = k & 7, home = k < 8 ? g->hsym : g->happ;
@@ -93,20 +98,35 @@ __device__ __forceinline__ int find_group(const unsigned* first, unsigned at) {
     const bool mine = first[threadIdx.x & 63] <= at;
     return __builtin_amdgcn_readfirstlane(__popcll(__ballot(mine)) - 1);
 }
-// item of a product -> group, matrix, tile; false: this XCD has no such item
-__device__ __forceinline__ bool find_tile(const Table* t, bool sym, int& gi, int& b, int& tile) {
-    const unsigned xcd = blockIdx.x & 7, at = blockIdx.x >> 3;
-    const unsigned* first = sym ? t->fsym[xcd] : t->fapp[xcd];
-    gi = find_group(first, at);
-    const Group* g = t->g + gi;
-    const unsigned tiles = sym ? g->tsym : g->tapp, total = (unsigned)g->batch * tiles;
-    const int home = sym ? g->hsym : g->happ;
-    const unsigned idx = at - first[gi] + run_start(total, home, xcd);
-    if (idx >= run_start(total, home, xcd + 1)) return false;
-    b = idx / tiles;
-    tile = idx - b * tiles;
-    return true;
-}
+// item of a product -> group, matrix, tile and what the product needs to know.  Every lane reads its group's values at once and
+// the one that is meant is picked afterwards: a tile waits for one load, not for two in a row.
+struct Item {
+    int gi, b, tile, np, mp;
+    unsigned xo, ao, dof, mat;
+    __device__ __forceinline__ bool find(const Table* t, bool sym) {      // false: this XCD has no such item
+        const unsigned xcd = blockIdx.x & 7, at = blockIdx.x >> 3;
+        const int lane = threadIdx.x & 63;
+        const unsigned first = sym ? t->fsym[xcd][lane] : t->fapp[xcd][lane];
+        const int l_tiles = sym ? t->tsym[lane] : t->tapp[lane], l_home = sym ? t->hsym[lane] : t->happ[lane];
+        const int l_np = t->np[lane], l_mp = t->mp[lane], l_xo = t->xo[lane], l_ao = t->ao[lane], l_dof = t->dof[lane], l_mat = t->mat[lane];
+        const int l_batch = t->batch[lane];
+        gi = __builtin_amdgcn_readfirstlane(__popcll(__ballot(first <= at)) - 1);
+        const unsigned tiles = __builtin_amdgcn_readlane(l_tiles, gi);
+        const int home = __builtin_amdgcn_readlane(l_home, gi);
+        np = __builtin_amdgcn_readlane(l_np, gi);
+        mp = __builtin_amdgcn_readlane(l_mp, gi);
+        xo = __builtin_amdgcn_readlane(l_xo, gi);
+        ao = __builtin_amdgcn_readlane(l_ao, gi);
+        dof = __builtin_amdgcn_readlane(l_dof, gi);
+        mat = __builtin_amdgcn_readlane(l_mat, gi);
+        const unsigned total = (unsigned)__builtin_amdgcn_readlane(l_batch, gi) * tiles;
+        const unsigned idx = at - (unsigned)__builtin_amdgcn_readlane((int)first, gi) + run_start(total, home, xcd);
+        if (idx >= run_start(total, home, xcd + 1)) return false;
+        b = idx / tiles;
+        tile = idx - b * tiles;
+        return true;
+    }
+};
 
 __device__ __forceinline__ double wave_sum_d(double v) {
 #pragma unroll
@@ -141,6 +161,12 @@ __device__ __forceinline__ void load8(const void* p, long long e, float (&v)[8])
     } else {
         load8f((const float*)p + e, v);
     }
+}
+template <bool BF>
+__device__ __forceinline__ f32x4 load4(const void* p, long long e) {
+    if (!BF) return *reinterpret_cast<const f32x4*>((const float*)p + e);
+    const bf16x4 b = *reinterpret_cast<const bf16x4*>((const bf16_t*)p + e);
+    return f32x4{bf2f(b[0]), bf2f(b[1]), bf2f(b[2]), bf2f(b[3])};
 }
 template <bool BF>
 __device__ __forceinline__ float load1(const void* p, long long e) { return BF ? bf2f(((const bf16_t*)p)[e]) : ((const float*)p)[e]; }
@@ -529,19 +555,19 @@ __global__ void __launch_bounds__(W0 * W1 * 64, 2) ortho_sym_kernel(const Table*
                                                           float ca, float cb, float cc) {
     typedef Mul<B, B, W0, W1, NST, false> M;
     __shared__ __attribute__((aligned(16))) unsigned char smem[NST * M::STAGE];
-    int gi, b, tidx, ti, tj;
-    if (!find_tile(t, true, gi, b, tidx)) return;
-    const Group& g = t->g[gi];
-    const int np = g.np, lda = np, ld = SQUARE ? np : g.mp, K = ld;
-    tri_tile(tidx, (np + B - 1) / B, ti, tj);
-    const long long ao = (long long)g.ao * 64 + (long long)b * np * lda;
-    const f16_t* src = SQUARE ? in + ao : in + (long long)g.xo * 64 + (long long)b * np * ld;
+    Item it;
+    if (!it.find(t, true)) return;
+    const int np = it.np, lda = np, ld = SQUARE ? np : it.mp, K = ld, b = it.b;
+    int ti, tj;
+    tri_tile(it.tile, (np + B - 1) / B, ti, tj);
+    const long long ao = (long long)it.ao * 64 + (long long)b * np * lda;
+    const f16_t* src = SQUARE ? in + ao : in + (long long)it.xo * 64 + (long long)b * np * ld;
     M m;
-    m.run(smem, src + (long long)ti * B * ld, ld, g.np - ti * B, src + (long long)tj * B * ld, ld, g.np - tj * B, K);
-    const float* d = SQUARE ? din + g.dof + (long long)b * g.np : nullptr;
-    const float unscale = SQUARE ? USC * USC : ldexpf(USC * USC, -2 * shift_of(ex, g.mat + b, down));
+    m.run(smem, src + (long long)ti * B * ld, ld, np - ti * B, src + (long long)tj * B * ld, ld, np - tj * B, K);
+    const float* d = SQUARE ? din + it.dof + (long long)b * np : nullptr;
+    const float unscale = SQUARE ? USC * USC : ldexpf(USC * USC, -2 * shift_of(ex, it.mat + b, down));
     f16_t* o = out + ao;
-    float* dst = dout + g.dof + (long long)b * g.np;
+    float* dst = dout + it.dof + (long long)b * np;
     float* tile = reinterpret_cast<float*>(smem);
     // value (r, c) of the result from the product's
     auto value = [&](float v, int r, int c, float a, float dr, float dc) {
@@ -560,7 +586,7 @@ __global__ void __launch_bounds__(W0 * W1 * 64, 2) ortho_sym_kernel(const Table*
         // block (tj, ti): rows c, 8 of r a thread
         for (int k = threadIdx.x; k < M::ROWS * B / 8; k += M::THREADS) {
             const int s = k / (B / 8), q = (k % (B / 8)) * 2, c = tj * B + M::tile_row(s, pass), r = ti * B + q * 4;
-            if (B > 64 && (c >= g.np || r >= g.np)) continue;
+            if (B > 64 && (c >= np || r >= np)) continue;
             const f32x4 v0 = M::at(tile, s, q), v1 = M::at(tile, s, q + 1);
             f16x8 av = {};
             f32x4 d0 = {}, d1 = {};
@@ -585,7 +611,7 @@ __global__ void __launch_bounds__(W0 * W1 * 64, 2) ortho_sym_kernel(const Table*
         for (int k = threadIdx.x; k < M::ROWS * B / 32; k += M::THREADS) {
             const int s = ((k & 7) + (k >> 3) % (M::ROWS / 64) * 8) * 8, q = (k >> 3) / (M::ROWS / 64);
             const int c = tj * B + M::tile_row(s, pass), r = ti * B + q * 4;
-            if (B > 64 && (c >= g.np || r >= g.np)) continue;
+            if (B > 64 && (c >= np || r >= np)) continue;
             f32x4 v[8];
 #pragma unroll
             for (int e = 0; e < 8; ++e) v[e] = M::at(tile, s + e, q);
@@ -618,20 +644,21 @@ __global__ void __launch_bounds__(W0 * W1 * 64, 2) ortho_apply_kernel(const Tabl
                                                             const int* __restrict__ ex, int down, int down1) {
     typedef Mul<BF, BS, W0, W1, NST, true> M;
     __shared__ __attribute__((aligned(16))) unsigned char smem[NST * M::STAGE];
-    int gi, b, tidx, ti, tj;
-    if (!find_tile(t, false, gi, b, tidx)) return;
-    const Group& g = t->g[gi];
-    const int np = g.np, mp = g.mp;
-    band_tile(tidx, (np + BS - 1) / BS, (mp + BF - 1) / BF, ti, tj);
-    const f16_t* A = P + (long long)g.ao * 64 + ((long long)b * np + ti * BS) * np;
-    const long long xo = (long long)g.xo * 64 + (long long)b * np * mp;
+    Item it;
+    if (!it.find(t, false)) return;
+    const int np = it.np, mp = it.mp, b = it.b;
+    int ti, tj;
+    band_tile(it.tile, (np + BS - 1) / BS, (mp + BF - 1) / BF, ti, tj);
+    const f16_t* A = P + (long long)it.ao * 64 + ((long long)b * np + ti * BS) * np;
+    const long long xo = (long long)it.xo * 64 + (long long)b * np * mp;
     M m;
     m.run(smem, xh + xo + tj * BF, mp, mp - tj * BF, A, np, np - ti * BS, np);
-    const int e0 = shift_of(ex, g.mat + b, down), e1 = shift_of(ex, g.mat + b, down1);
+    const int e0 = shift_of(ex, it.mat + b, down), e1 = shift_of(ex, it.mat + b, down1);
     const float rescale = FINAL ? ldexpf(USC, -e0) : ldexpf(1.f, e1 - e0);
-    const float* d = pd + g.dof + (long long)b * np;
+    const float* d = pd + it.dof + (long long)b * np;
     float* tile = reinterpret_cast<float*>(smem);
-    const bool turn = g.r > g.c;
+    const Group& g = t->g[it.gi];
+    const bool turn = FINAL && g.r > g.c;
     float lr = 0.f, step = 0.f;
     if (FINAL == 2) {
         lr = mu.lr_scale ? mu.lr * *mu.lr_scale : mu.lr;
@@ -685,6 +712,242 @@ __global__ void __launch_bounds__(W0 * W1 * 64, 2) ortho_apply_kernel(const Tabl
     }
 }
 
+// ---- small matrices: all steps in one launch ----------------------------------------------------------------------------
+// One workgroup of 8 waves a matrix: np = NP padded rows, up to 128 CB columns.  X stays in registers in fp32 (in the layout of the
+// products' results: wave w has the 16-column blocks w, w + 8, ..; a lane 4 columns of rows lane % 16 + 16 j), X_hi, O and
+// P in LDS; pd X is the accumulator that P X is added to.  What bounds it is latency: the other path is 19 launches of 4 us.
+template <int NP, int CB, int KIND>
+__global__ void __launch_bounds__(512, 2) ortho_small_kernel(const Chunk ch, const Muon mu, float ca, float cb, float cc, int steps, int fall, float eps) {
+    constexpr bool BF = KIND & 1;
+    constexpr int LDX = 128 * CB + 8, LDO = NP + 8, NS = NP / 16, GF = NS * NS / 8;      // GF: blocks of A a wave
+    __shared__ __attribute__((aligned(16))) f16_t Xs[NP * LDX], Os[NP * LDO];
+    __shared__ __attribute__((aligned(16))) float ds[NP], pds[NP];
+    __shared__ double red[8];
+    const int tid = threadIdx.x, lane = tid & 63, wid = __builtin_amdgcn_readfirstlane(tid >> 6), fr = lane & 15, fq = lane >> 4;
+    const bool mine = lane < ch.n && ch.g[lane < CHUNK ? lane : 0].fin <= blockIdx.x;
+    const int gi = __builtin_amdgcn_readfirstlane(__popcll(__ballot(mine)) - 1);
+    const Group g = ch.g[gi];
+    const int b = blockIdx.x - g.fin;
+    const bool turn = g.r > g.c;
+    const int n = turn ? g.c : g.r, m = turn ? g.r : g.c;
+    const int blocks = g.mp >> 4;
+    // row r, columns c .. c + 3 of X in the source
+    f32x4 x[CB][NS];
+    double sq = 0.0;
+    const long long rs = turn ? g.cs : g.rs, cs = turn ? g.rs : g.cs;
+    const long long ar = turn ? 1 : g.c, ac = turn ? g.c : 1;             // the same strides in a dense array
+#pragma unroll
+    for (int k = 0; k < CB; ++k)
+#pragma unroll
+        for (int j = 0; j < NS; ++j) {
+            x[k][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+            const int r = j * 16 + fr, c = (wid + 8 * k) * 16 + fq * 4;
+            if (r >= n) continue;
+            if (!turn && g.vec) {                                         // (whole fours: the columns are a multiple of 8)
+                if (c >= m) continue;
+                f32x4 u;
+                if (KIND >= 2) {
+                    const long long at = g.sb + r * ar + c;
+                    const f32x4 gr = load4<BF>(mu.g, at);
+                    f32x4 v = *reinterpret_cast<const f32x4*>(mu.v + at);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        v[e] = momentum_of(mu, gr[e], v[e]);
+                        u[e] = direction_of(mu, gr[e], v[e]);
+                    }
+                    *reinterpret_cast<f32x4*>(mu.v + at) = v;
+                } else {
+                    u = load4<BF>(g.src, b * g.sb + r * rs + c);
+                }
+                x[k][j] = u;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) sq += (double)u[e] * (double)u[e];
+                continue;
+            }
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                if (c + e >= m) continue;
+                float u;
+                if (KIND >= 2) {
+                    const long long at = g.sb + r * ar + (c + e) * ac;
+                    const float gr = load1<BF>(mu.g, at), v = momentum_of(mu, gr, mu.v[at]);
+                    mu.v[at] = v;
+                    u = direction_of(mu, gr, v);
+                } else {
+                    u = load1<BF>(g.src, b * g.sb + r * rs + (c + e) * cs);
+                }
+                x[k][j][e] = u;
+                sq += (double)u * (double)u;
+            }
+        }
+    sq = wave_sum_d(sq);
+    if (lane == 0) red[wid] = sq;
+    __syncthreads();
+    int shift;
+    const double inv = inverse_of(sqrt(((red[0] + red[1]) + (red[2] + red[3])) + ((red[4] + red[5]) + (red[6] + red[7]))), eps, shift);
+    auto put_x = [&]() {
+#pragma unroll
+        for (int k = 0; k < CB; ++k)
+            if (wid + 8 * k < blocks)
+#pragma unroll
+                for (int j = 0; j < NS; ++j) {
+                    f16x4 h;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) h[e] = (f16_t)x[k][j][e];
+                    *reinterpret_cast<f16x4*>(Xs + (j * 16 + fr) * LDX + (wid + 8 * k) * 16 + fq * 4) = h;
+                }
+    };
+#pragma unroll
+    for (int k = 0; k < CB; ++k)
+#pragma unroll
+        for (int j = 0; j < NS; ++j)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x[k][j][e] = (float)(x[k][j][e] * inv);
+    put_x();
+    __syncthreads();
+    const int fi = wid * NS / 8, s0 = NP == 64 ? (wid & 1) * 2 : 0;          // this wave's blocks of A: row block fi, columns s0 .. s0 + GF - 1
+#pragma unroll 1
+    for (int step = 0; step < steps; ++step) {
+        const int e0 = shift > step * fall ? shift - step * fall : 0, e1 = shift > (step + 1) * fall ? shift - (step + 1) * fall : 0;
+        // A
+        f32x4 acc[GF];
+#pragma unroll
+        for (int j = 0; j < GF; ++j) acc[j] = f32x4{0.f, 0.f, 0.f, 0.f};
+        for (int k0 = 0; k0 < g.mp; k0 += 32) {
+            const f16x8 a = *reinterpret_cast<const f16x8*>(Xs + (fi * 16 + fr) * LDX + k0 + fq * 8);
+#pragma unroll
+            for (int j = 0; j < GF; ++j) {
+                const f16x8 q = *reinterpret_cast<const f16x8*>(Xs + ((s0 + j) * 16 + fr) * LDX + k0 + fq * 8);
+                acc[j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, q, acc[j], 0, 0, 0);
+            }
+        }
+        const int r0 = fi * 16 + fq * 4;
+        const float unscale = ldexpf(USC * USC, -2 * e0);
+        f32x4 av[GF];                                                         // A's values, rows r0 .. r0 + 3, column (s0 + j) 16 + fr
+#pragma unroll
+        for (int j = 0; j < GF; ++j) {
+            const int c = (s0 + j) * 16 + fr;
+            f16x4 h;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                av[j][e] = acc[j][e] * unscale;
+                if (r0 + e == c) ds[c] = av[j][e];
+                h[e] = r0 + e == c ? (f16_t)0.f : (f16_t)(av[j][e] * SC);
+            }
+            *reinterpret_cast<f16x4*>(Os + c * LDO + r0) = h;                 // (symmetric)
+        }
+        __syncthreads();
+        // P
+#pragma unroll
+        for (int j = 0; j < GF; ++j) acc[j] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int k0 = 0; k0 < NP; k0 += 32) {
+            const f16x8 a = *reinterpret_cast<const f16x8*>(Os + (fi * 16 + fr) * LDO + k0 + fq * 8);
+#pragma unroll
+            for (int j = 0; j < GF; ++j) {
+                const f16x8 q = *reinterpret_cast<const f16x8*>(Os + ((s0 + j) * 16 + fr) * LDO + k0 + fq * 8);
+                acc[j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, q, acc[j], 0, 0, 0);
+            }
+        }
+        const f32x4 dr = *reinterpret_cast<const f32x4*>(ds + r0);
+        float dc[GF];
+#pragma unroll
+        for (int j = 0; j < GF; ++j) dc[j] = ds[(s0 + j) * 16 + fr];
+        __syncthreads();
+#pragma unroll
+        for (int j = 0; j < GF; ++j) {
+            const int c = (s0 + j) * 16 + fr;
+            f16x4 h;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const float v = acc[j][e] * (USC * USC), o = av[j][e];
+                if (r0 + e == c) pds[c] = ca + cb * dc[j] + cc * (v + dc[j] * dc[j]);
+                h[e] = r0 + e == c ? (f16_t)0.f : (f16_t)((cb * o + cc * (v + (dr[e] + dc[j]) * o)) * SC);
+            }
+            *reinterpret_cast<f16x4*>(Os + c * LDO + r0) = h;
+        }
+        __syncthreads();
+        // X: D rows = columns of X, D columns = rows of P
+        const float rescale = ldexpf(USC, e1 - e0);
+#pragma unroll
+        for (int j = 0; j < NS; ++j) {
+            const float pd = pds[j * 16 + fr] * SC;
+#pragma unroll
+            for (int k = 0; k < CB; ++k) x[k][j] *= pd;
+        }
+#pragma unroll
+        for (int h = 0; h < NP / 32; ++h) {
+            f16x8 q[NS];
+#pragma unroll
+            for (int j = 0; j < NS; ++j) q[j] = *reinterpret_cast<const f16x8*>(Os + (j * 16 + fr) * LDO + h * 32 + fq * 8);
+#pragma unroll
+            for (int k = 0; k < CB; ++k) {
+                if (wid + 8 * k >= blocks) continue;
+                f16_t* at = Xs + (h * 32 + 8 * fq + ((lane >> 2) & 3)) * LDX + (wid + 8 * k) * 16 + 4 * (lane & 3);
+                const f16x4 lo = __builtin_bit_cast(f16x4, __builtin_amdgcn_ds_read_tr16_b64_v4f16((lds_half4_ptr)at));
+                const f16x4 hi = __builtin_bit_cast(f16x4, __builtin_amdgcn_ds_read_tr16_b64_v4f16((lds_half4_ptr)(at + 4 * LDX)));
+                const f16x8 a = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+#pragma unroll
+                for (int j = 0; j < NS; ++j) x[k][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, q[j], x[k][j], 0, 0, 0);
+            }
+        }
+#pragma unroll
+        for (int k = 0; k < CB; ++k)
+#pragma unroll
+            for (int j = 0; j < NS; ++j) x[k][j] *= rescale;
+        if (step == steps - 1) break;
+        __syncthreads();
+        put_x();
+        __syncthreads();
+    }
+    const float scale = ldexpf(USC, -(shift > steps * fall ? shift - steps * fall : 0));
+    float lr = 0.f, by = 0.f;
+    if (KIND >= 2) {
+        lr = mu.lr_scale ? mu.lr * *mu.lr_scale : mu.lr;
+        by = lr * sqrtf(turn ? (float)g.r / (float)g.c : 1.f);
+    }
+#pragma unroll
+    for (int k = 0; k < CB; ++k)
+#pragma unroll
+        for (int j = 0; j < NS; ++j) {
+            const int r = j * 16 + fr, c = (wid + 8 * k) * 16 + fq * 4;
+            if (r >= n) continue;
+            if (!turn && g.vec) {
+                if (c >= m) continue;
+                const long long at = (KIND >= 2 ? g.sb : (long long)b * g.r * g.c) + r * ar + c;
+                bf16x4 o;
+                if (KIND >= 2) {
+                    f32x4 w = *reinterpret_cast<const f32x4*>(mu.w + at);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        w[e] = w[e] * (1.f - lr * mu.wd) - by * (x[k][j][e] * scale);
+                        o[e] = f2bf(w[e]);
+                    }
+                    *reinterpret_cast<f32x4*>(mu.w + at) = w;
+                    if (mu.lowp) *reinterpret_cast<bf16x4*>(mu.lowp + at) = o;
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) o[e] = f2bf(x[k][j][e] * scale);
+                    *reinterpret_cast<bf16x4*>(g.dst + at) = o;
+                }
+                continue;
+            }
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                if (c + e >= m) continue;
+                const long long at = r * ar + (c + e) * ac;
+                const float u = x[k][j][e] * scale;
+                if (KIND >= 2) {
+                    const float w = mu.w[g.sb + at] * (1.f - lr * mu.wd) - by * u;
+                    mu.w[g.sb + at] = w;
+                    if (mu.lowp) mu.lowp[g.sb + at] = f2bf(w);
+                } else {
+                    g.dst[(long long)b * g.r * g.c + at] = f2bf(u);
+                }
+            }
+        }
+}
+
 // ---- host -------------------------------------------------------------------------------------------------------------
 // one group as the callers describe it: 11 int64 values
 struct Desc { long long src, sb, srs, scs, dst, db, drs, dcs, r, c, batch; };
@@ -733,6 +996,12 @@ bool plan_of(const Desc* q, int count, Plan& pl) {
     return true;
 }
 
+// whether the source's rows (K23: the arenas', whose offsets are checked) can be read 8 elements at a time
+bool vec_of(const Desc& s, int kind) {
+    if (kind >= 2) return s.c % 8 == 0;
+    return s.scs == 1 && s.srs % 8 == 0 && (s.batch == 1 || s.sb % 8 == 0) && ((uintptr_t)s.src & 15) == 0;
+}
+
 // XCDs for the groups' tiles, the costliest first: a group of more than a sixteenth of all cost is cut over all of them, another
 // goes to the one with the least so far.  Returns the workgroups of the launch.
 long long homes(Group* g, int count, bool sym, const double* cost) {
@@ -763,20 +1032,31 @@ long long homes(Group* g, int count, bool sym, const double* cost) {
     return most * 8;
 }
 
-// The polynomial over [0, top], top = what the step before leaves: the largest |f(s)|, |b s^2 + c s^4| (X and P have to stay
-// in fp16's range) and |f(s) / s|, the most that X grows by.  False: out of range
-bool range_of(float a, float b, float c, int steps, double& growth) {
+// The polynomial over [0, top], top = what the step before leaves (1 at first): the largest |f(s)| and |b s^2 + c s^4| (X and P
+// have to stay in fp16's range) and |f(s) / s|, the most that X grows by - at the ends or where a derivative vanishes.
+// False: out of range
+bool range_of(double a, double b, double c, int steps, double& growth) {
     double top = 1.0;
     growth = 1.0;
     for (int k = 0; k < steps; ++k) {
+        const double end = top * top;
+        double l[4] = {0.0, end, 0.0, 0.0};                            // squares of the candidates
         double f = 0.0, p = 0.0, q = 0.0;
-        for (int i = 0; i <= 4096; ++i) {
-            const double s = top * i / 4096.0, l = s * s, r = fabs(a + b * l + c * l * l);
-            f = fmax(f, s * r);
-            p = fmax(p, fabs(b * l + c * l * l));
-            q = fmax(q, r);
+        const double root = 9.0 * b * b - 20.0 * a * c;               // f' = a + 3 b l + 5 c l^2
+        if (c != 0.0) {
+            if (root >= 0.0) { l[2] = (-3.0 * b + sqrt(root)) / (10.0 * c); l[3] = (-3.0 * b - sqrt(root)) / (10.0 * c); }
+        } else if (b != 0.0) {
+            l[2] = -a / (3.0 * b);
         }
-        if (!(f * 1.02 <= 8.0) || !(p * 1.02 <= 15.0) || !(top * top <= 15.0) || !(q <= 1024.0)) return false;
+        for (int i = 0; i < 4; ++i) {
+            const double s = l[i] >= 0.0 && l[i] <= end ? l[i] : 0.0;
+            f = fmax(f, sqrt(s) * fabs(a + b * s + c * s * s));
+        }
+        const double mid = c != 0.0 && -b / (2.0 * c) > 0.0 && -b / (2.0 * c) < end ? -b / (2.0 * c) : 0.0;
+        p = fmax(fabs(b * end + c * end * end), fabs(b * mid + c * mid * mid));
+        q = fmax(fmax(fabs(a), fabs(a + b * end + c * end * end)), fabs(a + b * mid + c * mid * mid));
+        // (the products' roundings may pass the exact range by a little)
+        if (!(f * 1.02 <= 8.0) || !(p * 1.02 <= 15.0) || !(end <= 15.0) || !(q <= 1024.0)) return false;
         growth = fmax(growth, q);
         top = f * 1.02 > 1.0 ? f * 1.02 : 1.0;
     }
@@ -787,11 +1067,89 @@ int growth_bits(float a, float b, float c, int steps) {
     return range_of(a, b, c, steps, growth) ? (int)ceil(log2(growth)) : 0;
 }
 
-// kind as in load_u
+// Tile sizes of a call.  Larger tiles need less LDS and L2 traffic a product (256 CUs full: 64 x 64 650, 128 x 128 890, 256 x 256
+// 1050 TFLOP/s), smaller ones fill the chip with less work.  Measured (us, 64 / 128 / 256): P X of 12 512 x 512 (768 tiles of 64)
+// 12.3 / 14.2 / 25.6, of 2048 x 2048 (1024) 35 / 32 / 55, of all of ResNet-50 (6200) 75 / 65 / 72, of 4096 x 8192 (8192; 512
+// of 256) 468 / 311 / 274; A and A^2 of ResNet-50 (880) 52 / 79 / 134, of 2048 x 2048 (528) 51 / 56 / 108, of two
+// 2048 x 4096 and 1000 x 4096 (1192) 116 / 107 / 152, of 4096 x 8192 (2080; 136 of 256) 374 / 318 / 311.
+void tiles_of(const Desc* q, int count, int& sym, int& app) {
+    long long s64 = 0, s256 = 0, a64 = 0, a256 = 0;
+    for (int i = 0; i < count; ++i) {
+        const long long n = q[i].r < q[i].c ? q[i].r : q[i].c, m = q[i].r < q[i].c ? q[i].c : q[i].r;
+        const long long n64 = (n + 63) / 64, n256 = (n + 255) / 256;
+        s64 += q[i].batch * n64 * (n64 + 1) / 2;
+        s256 += q[i].batch * n256 * (n256 + 1) / 2;
+        a64 += q[i].batch * n64 * ((m + 63) / 64);
+        a256 += q[i].batch * n256 * ((m + 255) / 256);
+    }
+    sym = s256 >= 128 && s64 >= 12 * s256 ? 256 : (s64 >= 1100 ? 128 : 64);      // (12 of 16: the larger tiles are mostly filled)
+    app = a256 >= 384 && a64 >= 12 * a256 ? 256 : (a64 >= 1024 ? 128 : 64);
+}
+
+// Calls that ortho_small_kernel serves: every matrix of up to 64 rows (its shorter side) and 512 columns, or 128 and 256
+int small_class(const Desc& s) {            // 0: none, else 8 * padded rows / 64 + the smallest CB
+    const long long n = s.r < s.c ? s.r : s.c, m = s.r < s.c ? s.c : s.r;
+    if (n <= 64 && m <= 512) return 8 + (m <= 128 ? 0 : m <= 256 ? 1 : 2);
+    if (n <= 128 && m <= 256) return 16 + (m <= 128 ? 0 : 1);
+    return 0;
+}
+bool all_small(const Desc* q, int count) {
+    for (int i = 0; i < count; ++i)
+        if (!small_class(q[i])) return false;
+    return true;
+}
+template <int KIND>
+int launch_small(int cls, const Chunk& ch, unsigned grid, const Muon& mu, float a, float b, float c, int steps, int fall, float eps, hipStream_t stream) {
+#define SMALL(NP, CB) DDL_KLAUNCH((ortho_small_kernel<NP, CB, KIND>), dim3(grid), dim3(512), 0, stream, ch, mu, a, b, c, steps, fall, eps)
+    switch (cls) {
+        case 8: SMALL(64, 1); break;
+        case 9: SMALL(64, 2); break;
+        case 10: SMALL(64, 4); break;
+        case 16: SMALL(128, 1); break;
+        default: SMALL(128, 2); break;
+    }
+#undef SMALL
+    return ddl_launch_status();
+}
+int run_small(const Desc* q, int count, int kind, const Muon& mu, float a, float b, float c, int steps, float eps, hipStream_t stream) {
+    const int fall = growth_bits(a, b, c, steps);
+    static const int classes[5] = {8, 9, 10, 16, 17};
+    for (int k = 0; k < 5; ++k) {
+        Chunk ch;
+        memset(&ch, 0, sizeof(ch));
+        long long grid = 0;
+        for (int i = 0; i <= count; ++i) {
+            if (ch.n && (i == count || ch.n == CHUNK)) {
+                const int rc = kind == 0 ? launch_small<0>(classes[k], ch, (unsigned)grid, mu, a, b, c, steps, fall, eps, stream)
+                             : kind == 1 ? launch_small<1>(classes[k], ch, (unsigned)grid, mu, a, b, c, steps, fall, eps, stream)
+                             : kind == 2 ? launch_small<2>(classes[k], ch, (unsigned)grid, mu, a, b, c, steps, fall, eps, stream)
+                                         : launch_small<3>(classes[k], ch, (unsigned)grid, mu, a, b, c, steps, fall, eps, stream);
+                if (rc != DDL_OK) return rc;
+                ch.n = 0;
+                grid = 0;
+            }
+            if (i == count || small_class(q[i]) != classes[k]) continue;
+            Group& o = ch.g[ch.n++];
+            const Desc& s = q[i];
+            o.src = (const void*)s.src; o.dst = (bf16_t*)s.dst; o.sb = s.sb; o.rs = (int)s.srs; o.cs = (int)s.scs;
+            o.r = (int)s.r; o.c = (int)s.c; o.batch = (int)s.batch;
+            o.vec = vec_of(s, kind) && s.c % 8 == 0;
+            o.np = (int)pad64(s.r < s.c ? s.r : s.c); o.mp = (int)pad64(s.r < s.c ? s.c : s.r);
+            o.fin = (unsigned)grid;
+            grid += s.batch;
+            if (grid > 0x7fffffffLL) return DDL_EINVAL;
+        }
+    }
+    return DDL_OK;
+}
+
+// kind as in load8
 int run_all(const Desc* q, int count, int kind, const Muon& mu, float a, float b, float c, int steps, float eps, char* ws, hipStream_t stream) {
     Plan pl;
     if (!plan_of(q, count, pl)) return DDL_EINVAL;
-    static const int sb = getenv("ORTHO_SB") ? atoi(getenv("ORTHO_SB")) : 64, ab = getenv("ORTHO_AB") ? atoi(getenv("ORTHO_AB")) : 64;
+    if (all_small(q, count)) return run_small(q, count, kind, mu, a, b, c, steps, eps, stream);
+    int sb = 64, ab = 64;
+    tiles_of(q, count, sb, ab);
     // the groups with the longest sums first
     int order[MAXG];
     for (int i = 0; i < count; ++i) order[i] = i;
@@ -809,8 +1167,7 @@ int run_all(const Desc* q, int count, int kind, const Muon& mu, float a, float b
         const long long sn = (np + sb - 1) / sb, an = (np + ab - 1) / ab, am = (mp + ab - 1) / ab;
         o.src = (const void*)s.src; o.dst = (bf16_t*)s.dst; o.sb = s.sb; o.rs = (int)s.srs; o.cs = (int)s.scs;
         o.r = (int)s.r; o.c = (int)s.c; o.np = (int)np; o.mp = (int)mp; o.batch = (int)s.batch;
-        o.vec = kind >= 2 ? s.c % 8 == 0                                   // (offsets and arenas are checked)
-                          : s.scs == 1 && s.srs % 8 == 0 && (s.batch == 1 || s.sb % 8 == 0) && ((uintptr_t)s.src & 15) == 0;
+        o.vec = vec_of(s, kind);
         o.part_elems = (int)pe; o.parts = (int)parts;
         o.xo = (unsigned)(xo / 64); o.ao = (unsigned)(ao / 64); o.dof = (unsigned)dof; o.po = (unsigned)po; o.mat = (unsigned)mat;
         o.tsym = (int)(sn * (sn + 1) / 2); o.tapp = (int)(an * am);

@@ -270,7 +270,7 @@ _INT8_TINY = 1e-30
 
 def quantize_int8(w):
     """8-bit codes of the rows of ``w`` [n, k] (fp32 or bf16): ``(q, scale)`` with ``q`` int8 [n, k], ``scale`` fp32 [n] and
-    ``w ~ q * scale[:, None]``; ``scale = max|row| / 127``, ``q = round(row * (127 / max|row|))`` to even.  Rows of ``q`` start
+    ``w ~ q * scale[:, None]``; ``scale = max|row| / 127``, ``q = round(row * (127 * (1 / max|row|)))`` to even, in fp32.  Rows of ``q`` start
     at multiples of 64 bytes, as :func:`linear_int8` reads them.  A row below 1e-30 counts as zero; one that holds an
     infinity or a NaN has the scale NaN."""
     if w.dim() != 2 or w.dtype not in (torch.float32, torch.bfloat16) or w.shape[1] == 0:
@@ -295,7 +295,7 @@ def _int8_rows_plain(x):
     top = x.abs().amax(dim=1)
     zero = top < _INT8_TINY
     bad = ~torch.isfinite(top)
-    inv = torch.where(zero | bad, torch.zeros_like(top), 127.0 / top)
+    inv = torch.where(zero | bad, torch.zeros_like(top), 127.0 * top.reciprocal())
     q = torch.where((zero | bad)[:, None], torch.zeros_like(x), torch.round(x * inv[:, None]))
     scale = torch.where(zero, torch.zeros_like(top), torch.where(bad, torch.full_like(top, float("nan")), top / 127.0))
     return q.to(torch.int8), scale

@@ -15,7 +15,7 @@ def rows_oracle(x):
             s[i] = float("nan")
         elif top >= 1e-30:
             s[i] = top / 127.0
-            q[i] = torch.round(row * (torch.tensor(127.0) / top)).to(torch.int8)
+            q[i] = torch.round(row * (127.0 * top.reciprocal())).to(torch.int8)
     return q, s
 
 
