@@ -5,94 +5,271 @@
 //
 // The sum is exact in int32 for K <= 133 144 (127^2 K < 2^31) whatever its order; rows below 1e-30 count as zero (127 / top
 // would overflow), a row with an infinity or a NaN gives NaN (its scale is NaN).
+//
+// Up to 16 rows: one launch that is bound by reading the weights once (int8_skinny_kernel).  More: the rows are quantised first
+// (int8_rows_kernel, bound by memory), then multiplied tile by tile (int8_gemm_kernel, bound by the matrix pipe).
 #include "common.h"
+#include "tile_mul.h"
 
 namespace {
 
-typedef int i32x4 __attribute__((ext_vector_type(4)));
-
-__device__ __forceinline__ float ld_in(const float* p) { return *p; }
-__device__ __forceinline__ float ld_in(const bf16_t* p) { return bf2f(*p); }
-
-// one row a workgroup: codes [M][Kp] (zeros from K on) and the scales
 template <typename T>
-__global__ void __launch_bounds__(256) int8_rows_kernel(const T* __restrict__ x, long long ldx, int K, int Kp, signed char* __restrict__ q,
-                                                       float* __restrict__ scale) {
-    __shared__ float red[4];
-    __shared__ int redb[4];
-    const long long m = blockIdx.x;
-    const T* row = x + m * ldx;
+__device__ __forceinline__ void ld8(const T* p, float (&v)[8]) {
+    if constexpr (sizeof(T) == 2) {
+        const bf16x8 b = *reinterpret_cast<const bf16x8*>(p);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = bf2f(b[j]);
+    } else {
+        load8f(p, v);
+    }
+}
+__device__ __forceinline__ float ld1(const float* p) { return *p; }
+__device__ __forceinline__ float ld1(const bf16_t* p) { return bf2f(*p); }
+__device__ __forceinline__ void st1(float* p, float v) { *p = v; }
+__device__ __forceinline__ void st1(bf16_t* p, float v) { *p = f2bf(v); }
+__device__ __forceinline__ unsigned code_of(float v, float inv) { return (unsigned)(int)rintf(v * inv) & 255u; }
+
+// One wave: the codes of a row (K values, zeros up to Kp, a multiple of 16) to q, which starts at a multiple of 16 bytes; returns
+// its scale.  The first 2048 values stay in registers between the two passes.  vec: the row starts at a multiple of 16 bytes.
+template <typename T>
+__device__ __forceinline__ float quantize_row(const T* __restrict__ row, int K, int Kp, bool vec, signed char* q) {
+    const int lane = threadIdx.x & 63;
     float top = 0.f;
     int bad = 0;
-    for (int k = threadIdx.x; k < K; k += 256) {
-        const float v = fabsf(ld_in(row + k));
+    auto see = [&](float v) {
+        v = fabsf(v);
         bad |= !(v < __builtin_inff());
         top = fmaxf(top, v);
+    };
+    constexpr int HOLD = 4;
+    float held[HOLD][8];
+    const int k8 = vec ? K & ~7 : 0;
+#pragma unroll
+    for (int h = 0; h < HOLD; ++h) {
+        const int k = (h * 64 + lane) * 8;
+        if (k < k8) {
+            ld8(row + k, held[h]);
+        } else {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) held[h][j] = 0.f;
+        }
     }
+#pragma unroll
+    for (int h = 0; h < HOLD; ++h)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) see(held[h][j]);
+#pragma unroll 2
+    for (int k = (HOLD * 64 + lane) * 8; k < k8; k += 512) {
+        float v[8];
+        ld8(row + k, v);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) see(v[j]);
+    }
+#pragma unroll 4
+    for (int k = k8 + lane; k < K; k += 64) see(ld1(row + k));
     top = wave_max(top);
     bad = __any(bad);
-    if ((threadIdx.x & 63) == 0) { red[threadIdx.x >> 6] = top; redb[threadIdx.x >> 6] = bad; }
-    __syncthreads();
-    top = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
-    bad = redb[0] | redb[1] | redb[2] | redb[3];
     const bool zero = bad || top < 1e-30f;
     const float inv = zero ? 0.f : 127.f * (1.f / top);
-    if (threadIdx.x == 0) scale[m] = bad ? __builtin_nanf("") : (zero ? 0.f : top / 127.f);
-    signed char* out = q + m * Kp;
-    for (int k = threadIdx.x; k < Kp; k += 256) out[k] = k < K && !zero ? (signed char)(int)rintf(ld_in(row + k) * inv) : (signed char)0;
+    auto pack = [&](const float (&v)[8]) {
+        u32x2 o;
+#pragma unroll
+        for (int p = 0; p < 2; ++p)
+            o[p] = zero ? 0u : code_of(v[4 * p], inv) | code_of(v[4 * p + 1], inv) << 8 | code_of(v[4 * p + 2], inv) << 16 | code_of(v[4 * p + 3], inv) << 24;
+        return o;
+    };
+#pragma unroll
+    for (int h = 0; h < HOLD; ++h) {
+        const int k = (h * 64 + lane) * 8;
+        if (k < k8) *reinterpret_cast<u32x2*>(q + k) = pack(held[h]);
+    }
+    for (int k = (HOLD * 64 + lane) * 8; k < k8; k += 512) {
+        float v[8];
+        ld8(row + k, v);
+        *reinterpret_cast<u32x2*>(q + k) = pack(v);
+    }
+    // the rest, four values a lane, zeros from K on
+    for (int k = k8 + lane * 4; k < Kp; k += 256) {
+        unsigned o = 0;
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            if (k + j < K && !zero) o |= code_of(ld1(row + k + j), inv) << (8 * j);
+        *reinterpret_cast<unsigned*>(q + k) = o;
+    }
+    return bad ? __builtin_nanf("") : (zero ? 0.f : top / 127.f);
 }
 
-// 64 x 64 tile of y, 4 waves of 32 x 32; both operands row-major and k-contiguous
+// a row a wave: codes [M][Kp], scales.  12 544 rows of 4096 bf16 values (154 MB): 94 -> ROWS_US us
 template <typename T>
-__global__ void __launch_bounds__(256) int8_gemm_kernel(const signed char* __restrict__ xq, const float* __restrict__ sx, const signed char* __restrict__ q,
-                                                       long long ldq, const float* __restrict__ s, const float* __restrict__ bias,
-                                                       T* __restrict__ y, long long ldy, int M, int N, int K, int Kp, int tiles_n) {
-    constexpr int LD = 80;
-    __shared__ __attribute__((aligned(16))) signed char As[64 * LD], Bs[64 * LD];
-    const int tid = threadIdx.x, lane = tid & 63, wid = tid >> 6, wm = wid >> 1, wn = wid & 1;
-    const int tm = blockIdx.x / tiles_n, tn = blockIdx.x - tm * tiles_n, m0 = tm * 64, n0 = tn * 64;
-    const int row = tid >> 2, ch = (tid & 3) * 16;
-    i32x4 acc[2][2] = {};
-    for (int k0 = 0; k0 < Kp; k0 += 64) {
-        i32x4 va = {}, vb = {};
-        if (m0 + row < M) va = *reinterpret_cast<const i32x4*>(xq + (long long)(m0 + row) * Kp + k0 + ch);
-        if (n0 + row < N && k0 + ch < K) vb = *reinterpret_cast<const i32x4*>(q + (n0 + row) * ldq + k0 + ch);
+__global__ void __launch_bounds__(256) int8_rows_kernel(const T* __restrict__ x, long long ldx, int M, int K, int Kp, int vec, signed char* __restrict__ q,
+                                                       float* __restrict__ scale) {
+    const int m = blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (m >= M) return;
+    const float s = quantize_row(x + m * ldx, K, Kp, vec, q + (long long)m * Kp);
+    if ((threadIdx.x & 63) == 0) scale[m] = s;
+}
+
+// B x B tile of y: F = output channels, S = rows of x
+template <typename T, int B, int W0, int W1, int NST>
+__global__ void __launch_bounds__(W0 * W1 * 64, 2) int8_gemm_kernel(const signed char* __restrict__ xq, const float* __restrict__ sx,
+                                                                   const signed char* __restrict__ q, long long ldq, long long q_bytes,
+                                                                   const float* __restrict__ s, const float* __restrict__ bias, T* __restrict__ y, long long ldy,
+                                                                   int M, int N, int Kp, int tm, int tn) {
+    typedef TileMul<MulI8, B, B, W0, W1, NST, false> Mu;
+    __shared__ __attribute__((aligned(16))) unsigned char smem[NST * Mu::STAGE];
+    // an XCD (workgroup number modulo 8) has a run of tiles, in bands of 8 rows, a band column by column
+    const int all = tm * tn, per = (all + 7) >> 3, idx = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
+    if ((int)(blockIdx.x >> 3) >= per || idx >= all) return;
+    const int band = idx / (8 * tn), rem = idx - band * 8 * tn, h = tm - band * 8 < 8 ? tm - band * 8 : 8;
+    const int ni = rem / h, mi = band * 8 + rem - ni * h, m0 = mi * B, n0 = ni * B;
+    const long long left = q_bytes - n0 * ldq;
+    Mu mu;
+    mu.run(smem, q + n0 * ldq, (unsigned)ldq, N - n0, left < (long long)DESC_BYTES ? (unsigned)left : DESC_BYTES, xq + (long long)m0 * Kp, Kp, M - m0, DESC_BYTES,
+           Kp / 128);
+    const bool vec = (N & 7) == 0 && (ldy & 7) == 0;
+#pragma unroll
+    for (int pass = 0; pass < Mu::PASSES; ++pass) {
+        if (Mu::PASSES > 1 && pass > 0) __syncthreads();
+        mu.to_lds(smem, pass);
         __syncthreads();
-        *reinterpret_cast<i32x4*>(As + row * LD + ch) = va;
-        *reinterpret_cast<i32x4*>(Bs + row * LD + ch) = vb;
-        __syncthreads();
-        i32x4 fa[2], fb[2];
+#pragma unroll 1
+        for (int k = threadIdx.x; k < Mu::ROWS * B / 8; k += Mu::THREADS) {
+            const int r = k / (B / 8), c = (k % (B / 8)) * 2, m = m0 + Mu::tile_row(r, pass), n = n0 + c * 4;
+            if (m >= M || n >= N) continue;
+            const i32x4 v0 = Mu::at(smem, r, c), v1 = Mu::at(smem, r, c + 1);
+            const float rs = sx[m];
+            float o[8];
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            fa[i] = *reinterpret_cast<const i32x4*>(As + (wm * 32 + i * 16 + (lane & 15)) * LD + (lane >> 4) * 16);
-            fb[i] = *reinterpret_cast<const i32x4*>(Bs + (wn * 32 + i * 16 + (lane & 15)) * LD + (lane >> 4) * 16);
-        }
-#pragma unroll
-        for (int i = 0; i < 2; ++i)
-#pragma unroll
-            for (int j = 0; j < 2; ++j) acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(fa[i], fb[j], acc[i][j], 0, 0, 0);
-    }
-#pragma unroll
-    for (int i = 0; i < 2; ++i)
-#pragma unroll
-        for (int j = 0; j < 2; ++j)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const int m = m0 + wm * 32 + i * 16 + (lane >> 4) * 4 + e, n = n0 + wn * 32 + j * 16 + (lane & 15);
-                if (m >= M || n >= N) continue;
-                const float v = (float)acc[i][j][e] * (sx[m] * s[n]) + (bias ? bias[n] : 0.f);
-                if constexpr (sizeof(T) == 4) y[m * ldy + n] = v; else y[m * ldy + n] = f2bf(v);
+            for (int e = 0; e < 8; ++e) {
+                const int ne = n + e < N ? n + e : N - 1;
+                o[e] = (float)(e < 4 ? v0[e & 3] : v1[e & 3]) * (rs * s[ne]) + (bias ? bias[ne] : 0.f);
             }
+            T* out = y + m * ldy + n;
+            if (vec) {
+                if constexpr (sizeof(T) == 2) {
+                    bf16x8 w;
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) w[e] = f2bf(o[e]);
+                    *reinterpret_cast<bf16x8*>(out) = w;
+                } else {
+                    *reinterpret_cast<f32x4*>(out) = f32x4{o[0], o[1], o[2], o[3]};
+                    *reinterpret_cast<f32x4*>(out + 4) = f32x4{o[4], o[5], o[6], o[7]};
+                }
+            } else {
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                    if (n + e < N) st1(out + e, o[e]);
+            }
+        }
+    }
+}
+
+// Up to 16 rows.  A workgroup of 8 waves takes tiles of 16 output channels (tile w, w + grid, ..); a wave 128-byte pieces of their
+// rows, every 8th, straight from memory into the matrix pipe's operand (16 channels x 64 values), three pieces ahead; the rows of x
+// are quantised into LDS meanwhile, once a workgroup.  The waves' integer sums are added in LDS.
+template <typename T>
+__global__ void __launch_bounds__(512) int8_skinny_kernel(const T* __restrict__ x, long long ldx, int vec, const signed char* __restrict__ q, long long ldq,
+                                                         const float* __restrict__ s, const float* __restrict__ bias, T* __restrict__ y, long long ldy,
+                                                         int M, int N, int K, int tiles) {
+    extern __shared__ __attribute__((aligned(16))) signed char xs[];       // [M][Kp + 16]
+    __shared__ __attribute__((aligned(16))) i32x4 red[2][8][64];
+    __shared__ float sx[16];
+    const int Kp = (K + 127) & ~127, LD = Kp + 16, pieces = Kp >> 7, P = (pieces + 7) >> 3;
+    const int lane = threadIdx.x & 63, wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), fr = lane & 15, fq = lane >> 4;
+    const int total = ((tiles - (int)blockIdx.x + (int)gridDim.x - 1) / (int)gridDim.x) * P;
+    struct Pair { i32x4 a, b; };
+    auto load = [&](int it) {
+        Pair p = {};
+        const int n = ((int)blockIdx.x + it / P * (int)gridDim.x) * 16 + fr, k = (wid + 8 * (it % P)) * 128 + fq * 16;
+        if (it < total && n < N) {
+            const signed char* at = q + n * ldq + k;
+            if (k < K) p.a = *reinterpret_cast<const i32x4*>(at);
+            if (k + 64 < K) p.b = *reinterpret_cast<const i32x4*>(at + 64);
+        }
+        return p;
+    };
+    Pair buf[4];
+#pragma unroll
+    for (int u = 0; u < 3; ++u) buf[u] = load(u);
+    for (int m = wid; m < M; m += 8) {
+        const float t = quantize_row(x + m * ldx, K, Kp, vec, xs + m * LD);
+        if (lane == 0) sx[m] = t;
+    }
+    __syncthreads();
+    const signed char* row = xs + (fr < M ? fr : 0) * LD + fq * 16;        // (columns from M on repeat row 0 and are not stored)
+    i32x4 acc = {0, 0, 0, 0};
+    int done = 0;                                                          // tiles finished
+    for (int base = 0; base < total; base += 4) {
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            const int it = base + u;
+            if (it >= total) break;
+            buf[(u + 3) & 3] = load(it + 3);
+            const int k = (wid + 8 * (it % P)) * 128;
+            if (k < Kp) {
+                acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(buf[u].a, *reinterpret_cast<const i32x4*>(row + k), acc, 0, 0, 0);
+                acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(buf[u].b, *reinterpret_cast<const i32x4*>(row + k + 64), acc, 0, 0, 0);
+            }
+            if (it % P != P - 1) continue;
+            i32x4(&mine)[8][64] = red[done & 1];
+            mine[wid][lane] = acc;
+            acc = i32x4{0, 0, 0, 0};
+            __syncthreads();
+            // channel 4 (lane / 16) + e of row lane % 16 lies at [lane][e]; the buffer of two tiles ago is free behind this barrier
+            if (threadIdx.x < 256) {
+                const int c = threadIdx.x & 15, m = threadIdx.x >> 4, n = ((int)blockIdx.x + done * (int)gridDim.x) * 16 + c;
+                if (m < M && n < N) {
+                    const int l = (c >> 2) * 16 + m, e = c & 3;
+                    int sum = 0;
+#pragma unroll
+                    for (int w = 0; w < 8; ++w) sum += mine[w][l][e];
+                    st1(y + m * ldy + n, (float)sum * (sx[m] * s[n]) + (bias ? bias[n] : 0.f));
+                }
+            }
+            ++done;
+        }
+    }
+}
+
+constexpr int SKINNY = 16, SKINNY_LDS = 40 * 1024;
+bool skinny(long long M, int K) { return M <= SKINNY && M * ((K + 127LL) / 128 * 128 + 16) <= SKINNY_LDS; }
+bool rows_vec(const void* x, int bf16, long long ldx) { return ddl_aligned16(x) && ldx % (bf16 ? 8 : 4) == 0; }
+
+template <typename T>
+int run(const T* x, long long ldx, const signed char* q, long long ldq, long long q_bytes, const float* s, const float* bias, T* y, long long ldy, int M, int N,
+        int K, char* ws, hipStream_t stream) {
+    const int vec = rows_vec(x, sizeof(T) == 2, ldx), Kp = (K + 127) / 128 * 128;
+    if (skinny(M, K)) {
+        const int tiles = (N + 15) / 16, grid = tiles < 512 ? tiles : 512;
+        DDL_KLAUNCH(int8_skinny_kernel<T>, dim3(grid), dim3(512), (size_t)M * (Kp + 16), stream, x, ldx, vec, q, ldq, s, bias, y, ldy, M, N, K, tiles);
+        return ddl_launch_status();
+    }
+    signed char* xq = (signed char*)ws;
+    float* sx = (float*)(ws + ((long long)M * Kp + 255) / 256 * 256);
+    DDL_KLAUNCH(int8_rows_kernel<T>, dim3((M + 3) / 4), dim3(256), 0, stream, x, ldx, M, K, Kp, vec, xq, sx);
+    // the larger the tile the less LDS and L2 traffic a product; it has to fill the chip twice (256 x 256: once and a half)
+    const long long t256 = ((M + 255LL) / 256) * ((N + 255) / 256), t128 = ((M + 127LL) / 128) * ((N + 127) / 128), t64 = ((M + 63LL) / 64) * ((N + 63) / 64);
+    if ((t64 + 7) / 8 * 8 > 0x7fffffffLL) return DDL_EINVAL;
+#define GEMM(B, W0, W1, NST, t) DDL_KLAUNCH((int8_gemm_kernel<T, B, W0, W1, NST>), dim3((unsigned)((t + 7) / 8 * 8)), dim3(W0 * W1 * 64), 0, stream, xq, sx, q, \
+                                            ldq, q_bytes, s, bias, y, ldy, M, N, Kp, (M + B - 1) / B, (N + B - 1) / B)
+    if (t256 >= 384) GEMM(256, 2, 4, 2, t256);
+    else if (t128 >= 256) GEMM(128, 2, 2, 2, t128);
+    else GEMM(64, 2, 2, 3, t64);
+#undef GEMM
+    return ddl_launch_status();
 }
 
 }  // namespace
 
-// codes and scales of the rows of x [M][K] (row stride ldx elements); q [M][Kp], zeros from K on
+// codes and scales of the rows of x [M][K] (row stride ldx elements); q [M][Kp], zeros from K on, Kp a multiple of 16, q aligned
 extern "C" int ddl_int8_rows(const void* x, int x_bf16, long long ldx, long long M, int K, int Kp, void* q, void* scale, hipStream_t stream) {
     if (M == 0) return DDL_OK;
-    if (!x || !q || !scale || M < 0 || M > 0x7fffffffLL || K <= 0 || Kp < K || ldx < 0) return DDL_EINVAL;
-    if (x_bf16) DDL_KLAUNCH(int8_rows_kernel<bf16_t>, dim3((unsigned)M), dim3(256), 0, stream, (const bf16_t*)x, ldx, K, Kp, (signed char*)q, (float*)scale);
-    else DDL_KLAUNCH(int8_rows_kernel<float>, dim3((unsigned)M), dim3(256), 0, stream, (const float*)x, ldx, K, Kp, (signed char*)q, (float*)scale);
+    if (!x || !q || !scale || M < 0 || M > 0x7fffff00LL || K <= 0 || Kp < K || Kp % 16 || ldx < 0) return DDL_EINVAL;
+    if (!ddl_aligned16(q)) return DDL_EALIGN;
+    const int vec = rows_vec(x, x_bf16, ldx);
+    const dim3 grid((unsigned)((M + 3) / 4)), block(256);
+    if (x_bf16) DDL_KLAUNCH(int8_rows_kernel<bf16_t>, grid, block, 0, stream, (const bf16_t*)x, ldx, (int)M, K, Kp, vec, (signed char*)q, (float*)scale);
+    else DDL_KLAUNCH(int8_rows_kernel<float>, grid, block, 0, stream, (const float*)x, ldx, (int)M, K, Kp, vec, (signed char*)q, (float*)scale);
     return ddl_launch_status();
 }
 
@@ -100,7 +277,8 @@ extern "C" int ddl_int8_max_k() { return 133144; }
 
 // bytes of workspace of ddl_int8_linear
 extern "C" long long ddl_int8_linear_workspace(long long M, int N, int K) {
-    const long long Kp = (K + 63LL) / 64 * 64;
+    if (skinny(M, K)) return 0;
+    const long long Kp = (K + 127LL) / 128 * 128;
     return (M * Kp + 255) / 256 * 256 + M * 4;
 }
 
@@ -109,23 +287,14 @@ extern "C" long long ddl_int8_linear_workspace(long long M, int N, int K) {
 extern "C" int ddl_int8_linear(const void* x, int x_bf16, long long ldx, const void* q, long long ldq, long long q_bytes, const void* s, const void* bias,
                                void* y, long long ldy, long long M, int N, int K, void* ws, long long ws_bytes, hipStream_t stream) {
     if (M == 0 || N == 0) return DDL_OK;
-    if (!x || !q || !s || !y || !ws || M < 0 || N < 0 || K <= 0 || K > ddl_int8_max_k() || ldx < 0 || ldq < K || ldy < N) return DDL_EINVAL;
-    if (M > 0x7fffffffLL - 256 || N > 0x7fffffff - 256) return DDL_EINVAL;
-    if (!ddl_aligned16(q) || ldq % 16 || (reinterpret_cast<uintptr_t>(ws) & 255)) return DDL_EALIGN;
-    if (q_bytes < (N - 1LL) * ldq + (K + 15) / 16 * 16 || ws_bytes < ddl_int8_linear_workspace(M, N, K)) return DDL_EINVAL;
-    const int Kp = (K + 63) / 64 * 64;
-    signed char* xq = (signed char*)ws;
-    float* sx = (float*)((char*)ws + (M * Kp + 255) / 256 * 256);
-    const int rc = ddl_int8_rows(x, x_bf16, ldx, M, K, Kp, xq, sx, stream);
-    if (rc != DDL_OK) return rc;
-    const long long tn = (N + 63) / 64, tiles = (M + 63) / 64 * tn;
-    if (tiles > 0x7fffffffLL) return DDL_EINVAL;
-    const dim3 grid((unsigned)tiles), block(256);
+    if (!x || !q || !s || !y || M < 0 || N < 0 || K <= 0 || K > ddl_int8_max_k() || ldx < 0 || ldq < K || ldy < N) return DDL_EINVAL;
+    // (a tile's byte offsets have 31 bits)
+    if (M > 0x7fffff00LL || N > 0x7fffff00 || ldq >= (1 << 22)) return DDL_EINVAL;
+    if (!ddl_aligned16(q) || ldq % 16 || !ddl_aligned16(y) || (reinterpret_cast<uintptr_t>(ws) & 255)) return DDL_EALIGN;
+    if (q_bytes < (N - 1LL) * ldq + (K + 15) / 16 * 16) return DDL_EINVAL;
+    const long long need = ddl_int8_linear_workspace(M, N, K);
+    if (need > 0 && (!ws || ws_bytes < need)) return DDL_EINVAL;
     if (x_bf16)
-        DDL_KLAUNCH(int8_gemm_kernel<bf16_t>, grid, block, 0, stream, xq, sx, (const signed char*)q, ldq, (const float*)s, (const float*)bias, (bf16_t*)y, ldy,
-                    (int)M, N, K, Kp, (int)tn);
-    else
-        DDL_KLAUNCH(int8_gemm_kernel<float>, grid, block, 0, stream, xq, sx, (const signed char*)q, ldq, (const float*)s, (const float*)bias, (float*)y, ldy,
-                    (int)M, N, K, Kp, (int)tn);
-    return ddl_launch_status();
+        return run((const bf16_t*)x, ldx, (const signed char*)q, ldq, q_bytes, (const float*)s, (const float*)bias, (bf16_t*)y, ldy, (int)M, N, K, (char*)ws, stream);
+    return run((const float*)x, ldx, (const signed char*)q, ldq, q_bytes, (const float*)s, (const float*)bias, (float*)y, ldy, (int)M, N, K, (char*)ws, stream);
 }

@@ -19,14 +19,11 @@
 // kept scaled by a further 2^e (shift_of), which falls from step to step as X can grow.  Workspace copies are padded to multiples of 64 with zeros, which the steps
 // keep (0 = a 0 + 0), so the products have no edges.
 #include "common.h"
+#include "tile_mul.h"
 #include <math.h>
 #include <string.h>
 
 namespace {
-
-typedef _Float16 f16_t;
-typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
-typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 
 constexpr int MAXG = 64;            // groups of a call: one lane each where a workgroup looks its group up
 constexpr int CHUNK = 32;           // groups that travel in one launch's arguments
@@ -364,165 +361,6 @@ __device__ __forceinline__ void store_result(const Group& g, const Muon& mu, int
 }
 
 // ---- products ---------------------------------------------------------------------------------------------------------
-// D = F S^T over K (a multiple of 64): W0 x W1 waves, a BF x BS tile, NST stages of 64 filled by LDS-DMA (128-byte pieces of
-// rows: a stage of 32 fetched each line twice), counted waits, one barrier a stage.
-//   S and, with TRF = false, F: row-major, k-contiguous rows.  16-byte chunk c of row r lies at c ^ (r / 2 mod 8): the 16 rows x
-//   one chunk that a quarter of a wave reads are free of bank conflicts.
-//   TRF = true: F is given transposed, [k][columns].  Its rows of k stay as they are in LDS and are read by the transposing
-//   load: 16 lanes take 4 rows x 16 columns; a half-wave touches rows 0-3 and 8-11 (+ 4, + 16), whose 32-byte windows
-//   the swizzle spreads over all banks.
-// A lane ends with D[i][j][e]: F index 16 i + 4 (lane / 16) + e, S index 16 j + lane % 16 of its wave's part.
-typedef __fp16 half4 __attribute__((ext_vector_type(4)));      // (the type that the transposing load is declared with)
-typedef __attribute__((address_space(3))) half4* lds_half4_ptr;
-constexpr unsigned OUT = 0x80000000u;      // an offset behind the descriptor's range: reads as zero
-
-__device__ __forceinline__ int nt_off(int row, int ch) { return row * 128 + ((ch ^ ((row >> 1) & 7)) << 4); }
-template <int B>
-__device__ __forceinline__ int tr_swz(int row) {
-    return B >= 128 ? (row & 3) | ((row >> 1) & 4) : ((row >> 1) & 1) | ((row >> 2) & 2);
-}
-
-template <int BF, int BS, int W0, int W1, int NST, bool TRF>
-struct Mul {
-    static constexpr int WAVES = W0 * W1, THREADS = WAVES * 64;
-    static constexpr int FBYTES = BF * 128, SBYTES = BS * 128, STAGE = FBYTES + SBYTES;
-    static constexpr int FL = BF / 8 / WAVES, SL = BS / 8 / WAVES, L = FL + SL;         // LDS-DMA instructions of a wave and stage
-    static constexpr int NF = BF / W0 / 16, NS = BS / W1 / 16;                          // fragments of a wave
-    static_assert(FL * 8 * WAVES == BF && SL * 8 * WAVES == BS && L % NF == 0, "whole instructions, spread over the fragments");
-    static_assert(NST >= 2 && NST * STAGE <= 160 * 1024, "LDS");
-    f32x4 acc[NF][NS];
-
-    // f: first row (TRF: first column) of the tile, ldf its row length, fleft rows (columns) that exist; s likewise
-    __device__ __forceinline__ void run(unsigned char* smem, const f16_t* f, int ldf, int fleft, const f16_t* s, int lds, int sleft, int K) {
-        const int tid = threadIdx.x, lane = tid & 63, wid = __builtin_amdgcn_readfirstlane(tid >> 6), w0 = wid / W1, w1 = wid % W1;
-        const int fr = lane & 15, fq = lane >> 4;
-        const int KT = K / 64;
-        const unsigned lds0 = (unsigned)(uintptr_t)(__attribute__((address_space(3))) void*)smem;
-        unsigned vo[L];
-#pragma unroll
-        for (int i = 0; i < FL; ++i) {
-            const int slot = (i * WAVES + wid) * 64 + lane;
-            if (TRF) {
-                constexpr int CPR = BF / 8;
-                const int row = slot / CPR, ch = slot % CPR, c = (((ch >> 1) ^ tr_swz<BF>(row)) << 1) | (ch & 1);
-                vo[i] = c * 8 < fleft ? (unsigned)((row * ldf + c * 8) * 2) : OUT;
-            } else {
-                const int row = slot >> 3, c = (slot & 7) ^ ((row >> 1) & 7);
-                vo[i] = row < fleft ? (unsigned)((row * ldf + c * 8) * 2) : OUT;
-            }
-        }
-#pragma unroll
-        for (int i = 0; i < SL; ++i) {
-            const int slot = (i * WAVES + wid) * 64 + lane, row = slot >> 3, c = (slot & 7) ^ ((row >> 1) & 7);
-            vo[FL + i] = row < sleft ? (unsigned)((row * lds + c * 8) * 2) : OUT;
-        }
-        const u32x4 rf = raw_rsrc(f, OUT - 16), rs = raw_rsrc(s, OUT - 16);
-        const unsigned fstep = TRF ? (unsigned)ldf * 128u : 128u;              // bytes from a tile to the next
-        // every stage is exactly L instructions a wave (behind the end: the last tile again): the counted waits rely on it
-        auto piece = [&](unsigned kt, unsigned at, int i) {                    // at: LDS address of the wave's part of the stage
-            if (i < FL) lds_dma16(rf, at + i * WAVES * 1024, vo[i], kt * fstep);
-            else lds_dma16(rs, at + FBYTES + (i - FL) * WAVES * 1024, vo[i], kt * 128u);
-        };
-        // a fragment's offset in a stage, half h: i-th of f at fbase[h] + 2048 i (TRF: foff[i] + 64 BF h), of s at sbase[h] + 2048 j
-        int fbase[2], sbase[2], foff[NF];
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            fbase[h] = nt_off(w0 * (BF / W0) + fr, h * 4 + fq);
-            sbase[h] = FBYTES + nt_off(w1 * (BS / W1) + fr, h * 4 + fq);
-        }
-        const int trow = 8 * fq + ((lane >> 2) & 3);
-#pragma unroll
-        for (int i = 0; i < NF; ++i) foff[i] = trow * (BF * 2) + (((w0 * NF + i) ^ tr_swz<BF>(trow)) * 32) + 8 * (lane & 3);
-        auto read_f = [&](unsigned char* st, int h, int i) -> f16x8 {
-            if (!TRF) return *reinterpret_cast<const f16x8*>(st + fbase[h] + i * 2048);
-            // (row + 4 has the swizzle of row: bit 2 of the row takes no part in it; nor does bit 5)
-            unsigned char* p = st + foff[i] + h * (BF * 64);
-            const f16x4 lo = __builtin_bit_cast(f16x4, __builtin_amdgcn_ds_read_tr16_b64_v4f16((lds_half4_ptr)p));
-            const f16x4 hi = __builtin_bit_cast(f16x4, __builtin_amdgcn_ds_read_tr16_b64_v4f16((lds_half4_ptr)(p + 4 * BF * 2)));
-            return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
-        };
-        auto read_s = [&](unsigned char* st, int h, int j) -> f16x8 { return *reinterpret_cast<const f16x8*>(st + sbase[h] + j * 2048); };
-#pragma unroll
-        for (int i = 0; i < NF; ++i)
-#pragma unroll
-            for (int j = 0; j < NS; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-
-        // The fragments of the next half are read while a half is multiplied: s into a second set of registers, each of f into
-        // its own behind its last use.  A stage is free once both halves are in registers: behind the barrier that ends
-        // the first one, tile t + NST goes where tile t was.
-        const unsigned at0 = lds0 + wid * 1024;
-#pragma unroll
-        for (int k = 0; k < NST; ++k)
-#pragma unroll
-            for (int i = 0; i < L; ++i) piece(k < KT ? k : KT - 1, at0 + k * STAGE, i);
-        asm volatile("s_waitcnt vmcnt(%0)" ::"n"((NST - 1) * L) : "memory");
-        __builtin_amdgcn_s_barrier();
-        f16x8 a[NF], b0[NS], b1[NS];
-#pragma unroll
-        for (int j = 0; j < NS; ++j) b0[j] = read_s(smem, 0, j);
-#pragma unroll
-        for (int i = 0; i < NF; ++i) a[i] = read_f(smem, 0, i);
-        int cur = 0;                               // offset of tile kt's stage
-        for (int kt = 0; kt < KT; ++kt) {
-            unsigned char* st = smem + cur;
-#pragma unroll
-            for (int j = 0; j < NS; ++j) b1[j] = read_s(st, 1, j);
-#pragma unroll
-            for (int i = 0; i < NF; ++i) {
-#pragma unroll
-                for (int j = 0; j < NS; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a[i], b0[j], acc[i][j], 0, 0, 0);
-                a[i] = read_f(st, 1, i);
-            }
-            asm volatile("s_waitcnt vmcnt(%0)" ::"n"((NST - 2) * L) : "memory");
-            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-            __builtin_amdgcn_s_barrier();
-            const int ns = cur + STAGE == NST * STAGE ? 0 : cur + STAGE;
-            const unsigned next = kt + NST < KT ? kt + NST : KT - 1;
-            unsigned char* sn = smem + ns;
-#pragma unroll
-            for (int j = 0; j < NS; ++j) b0[j] = read_s(sn, 0, j);
-#pragma unroll
-            for (int i = 0; i < NF; ++i) {
-#pragma unroll
-                for (int j = 0; j < NS; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a[i], b1[j], acc[i][j], 0, 0, 0);
-                a[i] = read_f(sn, 0, i);
-#pragma unroll
-                for (int q = 0; q < L / NF; ++q) piece(next, at0 + cur, i * (L / NF) + q);
-                __builtin_amdgcn_sched_barrier(0);
-            }
-            cur = ns;
-        }
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-        __builtin_amdgcn_s_barrier();              // the LDS is the epilogue's from here
-    }
-
-    // The epilogues go through LDS (fp32, rows of S, 16-byte chunk q of row s at q ^ fold(s)): whole rows are read back and
-    // written, and their loops stay rolled - a tile's code runs once, so its length is paid for in instruction fetches
-    // (an unrolled epilogue of 8 KB took 4 us).  PASSES parts of BS / PASSES rows where the tile is larger than the stages.
-    static constexpr int PASSES = BF * BS * 4 > NST * STAGE ? BF * BS * 4 / (NST * STAGE) : 1;
-    static_assert(NS % PASSES == 0, "whole fragments a pass");
-    static constexpr int ROWS = BS / PASSES;       // rows of a pass: those of fragments j with j / (NS / PASSES) == pass of every wave
-    __device__ __forceinline__ void to_lds(float* t, int pass) const {
-        const int lane = threadIdx.x & 63, wid = threadIdx.x >> 6, w0 = wid / W1, w1 = wid % W1;
-        const int s0 = w1 * (ROWS / W1) + (lane & 15), f0 = w0 * (BF / W0 / 4) + (lane >> 4);
-#pragma unroll
-        for (int p = 0; p < PASSES; ++p)
-            if (p == pass)
-#pragma unroll
-                for (int j = 0; j < NS / PASSES; ++j)
-#pragma unroll
-                    for (int i = 0; i < NF; ++i)
-                        *reinterpret_cast<f32x4*>(t + (s0 + j * 16) * BF + (((f0 + i * 4) ^ fold(s0 + j * 16)) * 4)) = acc[i][p * (NS / PASSES) + j];
-    }
-    static __device__ __forceinline__ int fold(int s) { return (s ^ (s >> 3)) & 15; }     // rows 1 apart and rows 8 apart on different banks
-    // row of the tile that row `s` of a pass holds
-    static __device__ __forceinline__ int tile_row(int s, int pass) { return (s / (ROWS / W1)) * (BS / W1) + pass * (ROWS / W1) + s % (ROWS / W1); }
-    static __device__ __forceinline__ void put(float* t, int s, int q, f32x4 v) { *reinterpret_cast<f32x4*>(t + s * BF + ((q ^ fold(s)) * 4)) = v; }
-    static __device__ __forceinline__ float at1(const float* t, int s, int f) { return t[s * BF + (((f >> 2) ^ fold(s)) * 4) + (f & 3)]; }
-    static __device__ __forceinline__ f32x4 at(const float* t, int s, int q) { return *reinterpret_cast<const f32x4*>(t + s * BF + ((q ^ fold(s)) * 4)); }
-};
-
 // Tiles of a matrix in bands of 8 rows, a band column by column: the tiles that an XCD works on at a time are about as many
 // rows as columns.
 __device__ __forceinline__ void band_tile(int idx, int rows, int cols, int& ti, int& tj) {
@@ -553,7 +391,7 @@ template <int B, int W0, int W1, int NST, bool SQUARE>
 __global__ void __launch_bounds__(W0 * W1 * 64, 2) ortho_sym_kernel(const Table* __restrict__ t, const f16_t* __restrict__ in, const float* __restrict__ din,
                                                           f16_t* __restrict__ out, float* __restrict__ dout, const int* __restrict__ ex, int down,
                                                           float ca, float cb, float cc) {
-    typedef Mul<B, B, W0, W1, NST, false> M;
+    typedef TileMul<MulF16, B, B, W0, W1, NST, false> M;
     __shared__ __attribute__((aligned(16))) unsigned char smem[NST * M::STAGE];
     Item it;
     if (!it.find(t, true)) return;
@@ -563,7 +401,7 @@ __global__ void __launch_bounds__(W0 * W1 * 64, 2) ortho_sym_kernel(const Table*
     const long long ao = (long long)it.ao * 64 + (long long)b * np * lda;
     const f16_t* src = SQUARE ? in + ao : in + (long long)it.xo * 64 + (long long)b * np * ld;
     M m;
-    m.run(smem, src + (long long)ti * B * ld, ld, np - ti * B, src + (long long)tj * B * ld, ld, np - tj * B, K);
+    m.run(smem, src + (long long)ti * B * ld, ld * 2, np - ti * B, DESC_BYTES, src + (long long)tj * B * ld, ld * 2, np - tj * B, DESC_BYTES, K / 64);
     const float* d = SQUARE ? din + it.dof + (long long)b * np : nullptr;
     const float unscale = SQUARE ? USC * USC : ldexpf(USC * USC, -2 * shift_of(ex, it.mat + b, down));
     f16_t* o = out + ao;
@@ -642,7 +480,7 @@ __global__ void __launch_bounds__(W0 * W1 * 64, 2) ortho_apply_kernel(const Tabl
                                                             const float* __restrict__ pd, const f16_t* __restrict__ xh, const f16_t* __restrict__ xl,
                                                             f16_t* __restrict__ yh, f16_t* __restrict__ yl,
                                                             const int* __restrict__ ex, int down, int down1) {
-    typedef Mul<BF, BS, W0, W1, NST, true> M;
+    typedef TileMul<MulF16, BF, BS, W0, W1, NST, true> M;
     __shared__ __attribute__((aligned(16))) unsigned char smem[NST * M::STAGE];
     Item it;
     if (!it.find(t, false)) return;
@@ -652,7 +490,7 @@ __global__ void __launch_bounds__(W0 * W1 * 64, 2) ortho_apply_kernel(const Tabl
     const f16_t* A = P + (long long)it.ao * 64 + ((long long)b * np + ti * BS) * np;
     const long long xo = (long long)it.xo * 64 + (long long)b * np * mp;
     M m;
-    m.run(smem, xh + xo + tj * BF, mp, mp - tj * BF, A, np, np - ti * BS, np);
+    m.run(smem, xh + xo + tj * BF, mp * 2, mp - tj * BF, DESC_BYTES, A, np * 2, np - ti * BS, DESC_BYTES, np / 64);
     const int e0 = shift_of(ex, it.mat + b, down), e1 = shift_of(ex, it.mat + b, down1);
     const float rescale = FINAL ? ldexpf(USC, -e0) : ldexpf(1.f, e1 - e0);
     const float* d = pd + it.dof + (long long)b * np;

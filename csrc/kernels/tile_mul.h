@@ -1,0 +1,189 @@
+// Tile product on the matrix pipe, shared by the kernels whose operands are rows of 16-bit or 8-bit values (gfx950).
+//
+// D = F S^T: W0 x W1 waves, a BF x BS tile, NST stages of 128 bytes of every row (64 fp16 or 128 int8 values) filled by LDS-DMA
+// (64-byte pieces fetched each line twice), counted waits, one barrier a stage.
+//   S and, with TRF = false, F: row-major, k-contiguous rows.  16-byte chunk c of row r lies at c ^ (r / 2 mod 8): the 16 rows x
+//   one chunk that a quarter of a wave reads are free of bank conflicts.
+//   TRF = true (fp16): F is given transposed, [k][columns].  Its rows of k stay as they are in LDS and are read by the transposing
+//   load: 16 lanes take 4 rows x 16 columns; a half-wave touches rows 0-3 and 8-11 (+ 4, + 16), whose 32-byte windows
+//   the swizzle spreads over all banks.
+// A lane ends with D[i][j][e]: F index 16 i + 4 (lane / 16) + e, S index 16 j + lane % 16 of its wave's part.
+#pragma once
+#include "common.h"
+
+typedef _Float16 f16_t;
+typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef int i32x4 __attribute__((ext_vector_type(4)));
+
+namespace {
+
+typedef __fp16 half4 __attribute__((ext_vector_type(4)));      // (the type that the transposing load is declared with)
+typedef __attribute__((address_space(3))) half4* lds_half4_ptr;
+constexpr unsigned OUT = 0x80000000u, DESC_BYTES = OUT - 16;      // an offset behind every descriptor's range (reads as zero); the longest range
+
+__device__ __forceinline__ int nt_off(int row, int ch) { return row * 128 + ((ch ^ ((row >> 1) & 7)) << 4); }
+template <int B>
+__device__ __forceinline__ int tr_swz(int row) {
+    return B >= 128 ? (row & 3) | ((row >> 1) & 4) : ((row >> 1) & 1) | ((row >> 2) & 2);
+}
+
+struct MulF16 {
+    typedef f16x8 frag;
+    typedef f32x4 acc;
+    static __device__ __forceinline__ acc mma(frag a, frag b, acc c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
+};
+struct MulI8 {
+    typedef i32x4 frag;
+    typedef i32x4 acc;
+    static __device__ __forceinline__ acc mma(frag a, frag b, acc c) { return __builtin_amdgcn_mfma_i32_16x16x64_i8(a, b, c, 0, 0, 0); }
+};
+
+template <typename OP, int BF, int BS, int W0, int W1, int NST, bool TRF>
+struct TileMul {
+    typedef typename OP::frag frag;
+    typedef typename OP::acc vec;
+    static constexpr int WAVES = W0 * W1, THREADS = WAVES * 64;
+    static constexpr int FBYTES = BF * 128, SBYTES = BS * 128, STAGE = FBYTES + SBYTES;
+    static constexpr int FL = BF / 8 / WAVES, SL = BS / 8 / WAVES, L = FL + SL;         // LDS-DMA instructions of a wave and stage
+    static constexpr int NF = BF / W0 / 16, NS = BS / W1 / 16;                          // fragments of a wave
+    static_assert(FL * 8 * WAVES == BF && SL * 8 * WAVES == BS && L % NF == 0, "whole instructions, spread over the fragments");
+    static_assert(NST >= 2 && NST * STAGE <= 160 * 1024, "LDS");
+    vec acc[NF][NS];
+
+    // f: first row (TRF: first column) of the tile, ldf bytes from a row to the next, fleft rows (columns) that exist, fbytes: what
+    // may be read from f on (behind it and behind the rows that exist: zeros); s likewise; KT stages.  All offsets < 2^31.
+    __device__ __forceinline__ void run(unsigned char* smem, const void* f, unsigned ldf, int fleft, unsigned fbytes, const void* s, unsigned lds, int sleft,
+                                        unsigned sbytes, int KT) {
+        const int tid = threadIdx.x, lane = tid & 63, wid = __builtin_amdgcn_readfirstlane(tid >> 6), w0 = wid / W1, w1 = wid % W1;
+        const int fr = lane & 15, fq = lane >> 4;
+        const unsigned lds0 = (unsigned)(uintptr_t)(__attribute__((address_space(3))) void*)smem;
+        unsigned vo[L];
+#pragma unroll
+        for (int i = 0; i < FL; ++i) {
+            const int slot = (i * WAVES + wid) * 64 + lane;
+            if (TRF) {
+                constexpr int CPR = BF / 8;
+                const int row = slot / CPR, ch = slot % CPR, c = (((ch >> 1) ^ tr_swz<BF>(row)) << 1) | (ch & 1);
+                vo[i] = c * 8 < fleft ? row * ldf + c * 16 : OUT;
+            } else {
+                const int row = slot >> 3, c = (slot & 7) ^ ((row >> 1) & 7);
+                vo[i] = row < fleft ? row * ldf + c * 16 : OUT;
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < SL; ++i) {
+            const int slot = (i * WAVES + wid) * 64 + lane, row = slot >> 3, c = (slot & 7) ^ ((row >> 1) & 7);
+            vo[FL + i] = row < sleft ? row * lds + c * 16 : OUT;
+        }
+        const u32x4 rf = raw_rsrc(f, fbytes), rs = raw_rsrc(s, sbytes);
+        const unsigned fstep = TRF ? ldf * 64u : 128u;                         // bytes from a tile to the next
+        // every stage is exactly L instructions a wave (behind the end: the last tile again): the counted waits rely on it
+        auto piece = [&](unsigned kt, unsigned at, int i) {                    // at: LDS address of the wave's part of the stage
+            if (i < FL) lds_dma16(rf, at + i * WAVES * 1024, vo[i], kt * fstep);
+            else lds_dma16(rs, at + FBYTES + (i - FL) * WAVES * 1024, vo[i], kt * 128u);
+        };
+        // a fragment's offset in a stage, half h: i-th of f at fbase[h] + 2048 i (TRF: foff[i] + 64 BF h), of s at sbase[h] + 2048 j
+        int fbase[2], sbase[2], foff[NF];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            fbase[h] = nt_off(w0 * (BF / W0) + fr, h * 4 + fq);
+            sbase[h] = FBYTES + nt_off(w1 * (BS / W1) + fr, h * 4 + fq);
+        }
+        const int trow = 8 * fq + ((lane >> 2) & 3);
+#pragma unroll
+        for (int i = 0; i < NF; ++i) foff[i] = trow * (BF * 2) + (((w0 * NF + i) ^ tr_swz<BF>(trow)) * 32) + 8 * (lane & 3);
+        auto read_f = [&](unsigned char* st, int h, int i) -> frag {
+            if constexpr (!TRF) {
+                return *reinterpret_cast<const frag*>(st + fbase[h] + i * 2048);
+            } else {
+            // (row + 4 has the swizzle of row: bit 2 of the row takes no part in it; nor does bit 5)
+            unsigned char* p = st + foff[i] + h * (BF * 64);
+            const f16x4 lo = __builtin_bit_cast(f16x4, __builtin_amdgcn_ds_read_tr16_b64_v4f16((lds_half4_ptr)p));
+            const f16x4 hi = __builtin_bit_cast(f16x4, __builtin_amdgcn_ds_read_tr16_b64_v4f16((lds_half4_ptr)(p + 4 * BF * 2)));
+            return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+            }
+        };
+        auto read_s = [&](unsigned char* st, int h, int j) -> frag { return *reinterpret_cast<const frag*>(st + sbase[h] + j * 2048); };
+#pragma unroll
+        for (int i = 0; i < NF; ++i)
+#pragma unroll
+            for (int j = 0; j < NS; ++j) acc[i][j] = vec{0, 0, 0, 0};
+
+        // The fragments of the next half are read while a half is multiplied: s into a second set of registers, each of f into
+        // its own behind its last use.  A stage is free once both halves are in registers: behind the barrier that ends
+        // the first one, tile t + NST goes where tile t was.
+        const unsigned at0 = lds0 + wid * 1024;
+#pragma unroll
+        for (int k = 0; k < NST; ++k)
+#pragma unroll
+            for (int i = 0; i < L; ++i) piece(k < KT ? k : KT - 1, at0 + k * STAGE, i);
+        asm volatile("s_waitcnt vmcnt(%0)" ::"n"((NST - 1) * L) : "memory");
+        __builtin_amdgcn_s_barrier();
+        frag a[NF], b0[NS], b1[NS];
+#pragma unroll
+        for (int j = 0; j < NS; ++j) b0[j] = read_s(smem, 0, j);
+#pragma unroll
+        for (int i = 0; i < NF; ++i) a[i] = read_f(smem, 0, i);
+        int cur = 0;                               // offset of tile kt's stage
+        for (int kt = 0; kt < KT; ++kt) {
+            unsigned char* st = smem + cur;
+#pragma unroll
+            for (int j = 0; j < NS; ++j) b1[j] = read_s(st, 1, j);
+#pragma unroll
+            for (int i = 0; i < NF; ++i) {
+#pragma unroll
+                for (int j = 0; j < NS; ++j) acc[i][j] = OP::mma(a[i], b0[j], acc[i][j]);
+                a[i] = read_f(st, 1, i);
+            }
+            asm volatile("s_waitcnt vmcnt(%0)" ::"n"((NST - 2) * L) : "memory");
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+            __builtin_amdgcn_s_barrier();
+            const int ns = cur + STAGE == NST * STAGE ? 0 : cur + STAGE;
+            const unsigned next = kt + NST < KT ? kt + NST : KT - 1;
+            unsigned char* sn = smem + ns;
+#pragma unroll
+            for (int j = 0; j < NS; ++j) b0[j] = read_s(sn, 0, j);
+#pragma unroll
+            for (int i = 0; i < NF; ++i) {
+#pragma unroll
+                for (int j = 0; j < NS; ++j) acc[i][j] = OP::mma(a[i], b1[j], acc[i][j]);
+                a[i] = read_f(sn, 0, i);
+#pragma unroll
+                for (int q = 0; q < L / NF; ++q) piece(next, at0 + cur, i * (L / NF) + q);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            cur = ns;
+        }
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        __builtin_amdgcn_s_barrier();              // the LDS is the epilogue's from here
+    }
+
+    // The epilogues go through LDS (32-bit values, rows of S, 16-byte chunk q of row s at q ^ fold(s)): whole rows are read back and
+    // written, and their loops stay rolled - a tile's code runs once, so its length is paid for in instruction fetches
+    // (an unrolled epilogue of 8 KB took 4 us).  PASSES parts of BS / PASSES rows where the tile is larger than the stages.
+    static constexpr int PASSES = BF * BS * 4 > NST * STAGE ? BF * BS * 4 / (NST * STAGE) : 1;
+    static_assert(NS % PASSES == 0, "whole fragments a pass");
+    static constexpr int ROWS = BS / PASSES;       // rows of a pass: those of fragments j with j / (NS / PASSES) == pass of every wave
+    __device__ __forceinline__ void to_lds(void* t, int pass) const {
+        const int lane = threadIdx.x & 63, wid = threadIdx.x >> 6, w0 = wid / W1, w1 = wid % W1;
+        const int s0 = w1 * (ROWS / W1) + (lane & 15), f0 = w0 * (BF / W0 / 4) + (lane >> 4);
+#pragma unroll
+        for (int p = 0; p < PASSES; ++p)
+            if (p == pass)
+#pragma unroll
+                for (int j = 0; j < NS / PASSES; ++j)
+#pragma unroll
+                    for (int i = 0; i < NF; ++i)
+                        *reinterpret_cast<vec*>((unsigned*)t + (s0 + j * 16) * BF + (((f0 + i * 4) ^ fold(s0 + j * 16)) * 4)) = acc[i][p * (NS / PASSES) + j];
+    }
+    static __device__ __forceinline__ int fold(int s) { return (s ^ (s >> 3)) & 15; }     // rows 1 apart and rows 8 apart on different banks
+    // row of the tile that row `s` of a pass holds
+    static __device__ __forceinline__ int tile_row(int s, int pass) { return (s / (ROWS / W1)) * (BS / W1) + pass * (ROWS / W1) + s % (ROWS / W1); }
+    static __device__ __forceinline__ void put(float* t, int s, int q, f32x4 v) { *reinterpret_cast<f32x4*>(t + s * BF + ((q ^ fold(s)) * 4)) = v; }
+    static __device__ __forceinline__ float at1(const float* t, int s, int f) { return t[s * BF + (((f >> 2) ^ fold(s)) * 4) + (f & 3)]; }
+    static __device__ __forceinline__ vec at(const void* t, int s, int q) { return *reinterpret_cast<const vec*>((const unsigned*)t + s * BF + ((q ^ fold(s)) * 4)); }
+};
+
+}  // namespace

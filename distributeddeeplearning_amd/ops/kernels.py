@@ -318,16 +318,22 @@ def int8_rows(x, q, scale):
             scale.data_ptr(), _raw_stream()), "int8_rows")
 
 
-def int8_linear(x, q, scale, bias, y):
-    M, Kd = x.shape
-    N = q.shape[0]
+@functools.lru_cache(maxsize=1024)
+def _int8_workspace(M, N, Kd):
     f = getattr(lib(), "ddl_int8_linear_workspace")
     f.restype = ctypes.c_longlong
-    work = torch.empty(int(f(_i64(M), _i32(N), _i32(Kd))), dtype=torch.uint8, device=x.device)
+    return int(f(_i64(M), _i32(N), _i32(Kd)))
+
+
+def int8_linear(x, q, scale, bias, y):
+    """``y`` [M, N] (dense) from ``x`` [M, K] and the codes ``q`` [N, K]; see ``functional.linear_int8``."""
+    M, Kd = x.shape
+    N = q.shape[0]
+    nbytes = _int8_workspace(M, N, Kd)
+    work = torch.empty(nbytes, dtype=torch.uint8, device=x.device) if nbytes else None
     f = _fn("ddl_int8_linear", "p i q p qq pp p q q ii p q p")
     check(f(x.data_ptr(), 1 if x.dtype == torch.bfloat16 else 0, x.stride(0), q.data_ptr(), q.stride(0), storage_numel_from(q),
-            scale.data_ptr(), _p(bias), y.data_ptr(), y.stride(0), M, N, Kd, work.data_ptr(), work.numel(), _raw_stream()),
-          "int8_linear")
+            scale.data_ptr(), _p(bias), y.data_ptr(), N, M, N, Kd, _p(work), nbytes, _raw_stream()), "int8_linear")
 
 
 # ---- convolution / GEMM (csrc/kernels/conv_igemm.hip, conv_wgrad.hip) ------------------------
