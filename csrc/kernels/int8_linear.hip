@@ -247,13 +247,14 @@ int run(const T* x, long long ldx, const signed char* q, long long ldq, long lon
     signed char* xq = (signed char*)ws;
     float* sx = (float*)(ws + ((long long)M * Kp + 255) / 256 * 256);
     DDL_KLAUNCH(int8_rows_kernel<T>, dim3((M + 3) / 4), dim3(256), 0, stream, x, ldx, M, K, Kp, vec, xq, sx);
-    // the larger the tile the less LDS and L2 traffic a product; it has to fill the chip twice (256 x 256: once and a half)
-    const long long t256 = ((M + 255LL) / 256) * ((N + 255) / 256), t128 = ((M + 127LL) / 128) * ((N + 127) / 128), t64 = ((M + 63LL) / 64) * ((N + 63) / 64);
+    // 128 x 128 tiles, two a CU, unless they are fewer than the CUs.  (256 x 256 in 8 waves is no faster where it fills whole rounds,
+    // 4096^3 in 100 / 101 us, and 12 544 x 4096 x 4096 takes 4 rounds for 3.06: 333 / 304 us.  256 x 128: 328; 4 waves of 128 x 128:
+    // 396, copies between register halves.)
+    const long long t128 = ((M + 127LL) / 128) * ((N + 127) / 128), t64 = ((M + 63LL) / 64) * ((N + 63) / 64);
     if ((t64 + 7) / 8 * 8 > 0x7fffffffLL) return DDL_EINVAL;
 #define GEMM(B, W0, W1, NST, t) DDL_KLAUNCH((int8_gemm_kernel<T, B, W0, W1, NST>), dim3((unsigned)((t + 7) / 8 * 8)), dim3(W0 * W1 * 64), 0, stream, xq, sx, q, \
                                             ldq, q_bytes, s, bias, y, ldy, M, N, Kp, (M + B - 1) / B, (N + B - 1) / B)
-    if (t256 >= 384) GEMM(256, 2, 4, 2, t256);
-    else if (t128 >= 256) GEMM(128, 2, 2, 2, t128);
+    if (t128 >= 256) GEMM(128, 2, 2, 2, t128);
     else GEMM(64, 2, 2, 3, t64);
 #undef GEMM
     return ddl_launch_status();

@@ -60,34 +60,36 @@ __host__ __device__ __forceinline__ unsigned run_start(unsigned total, int home,
     return home < 0 ? (unsigned)((unsigned long long)total * xcd / 8) : (xcd > home ? total : 0u);
 }
 
-__global__ void __launch_bounds__(256) ortho_table_kernel(const Chunk ch, Table* __restrict__ t) {
+// One workgroup writes its chunk's groups; that of the last chunk also where the groups begin on each XCD.  1024 threads: one
+// wave a prefix sum.
+__device__ __forceinline__ void write_table(const Chunk& ch, Table* __restrict__ t) {
     const unsigned* from = reinterpret_cast<const unsigned*>(ch.g);
     unsigned* to = reinterpret_cast<unsigned*>(t->g + ch.base);
-    for (int i = threadIdx.x; i < ch.n * (int)(sizeof(Group) / 4); i += 256) to[i] = from[i];
+    for (int i = threadIdx.x; i < ch.n * (int)(sizeof(Group) / 4); i += 1024) to[i] = from[i];
     if (!ch.last) return;
-    __syncthreads();
-    if (threadIdx.x >= 64) return;
-    const int lane = threadIdx.x, count = ch.base + ch.n;
+    const int lane = threadIdx.x & 63, k = threadIdx.x >> 6, count = ch.base + ch.n;
     const bool live = lane < count;
-    const Group* g = t->g + (live ? lane : 0);
-    t->fin[lane] = live ? g->fin : 0xffffffffu;
-    t->fio[lane] = live ? g->fio : 0xffffffffu;
-    t->batch[lane] = g->batch; t->np[lane] = g->np; t->mp[lane] = g->mp;
-    t->tsym[lane] = g->tsym; t->tapp[lane] = g->tapp; t->hsym[lane] = g->hsym; t->happ[lane] = g->happ;
-    t->xo[lane] = g->xo; t->ao[lane] = g->ao; t->dof[lane] = g->dof; t->mat[lane] = g->mat;
-#pragma unroll 1
-    for (int k = 0; k < 16; ++k) {
-        const int xcd = k & 7, home = k < 8 ? g->hsym : g->happ;
-        const unsigned total = live ? (unsigned)g->batch * (unsigned)(k < 8 ? g->tsym : g->tapp) : 0u;
-        const unsigned mine = run_start(total, home, xcd + 1) - run_start(total, home, xcd);
-        unsigned sum = mine;
-#pragma unroll
-        for (int o = 1; o < 64; o <<= 1) {
-            const unsigned v = __shfl_up(sum, o, 64);
-            if (lane >= o) sum += v;
-        }
-        (k < 8 ? t->fsym : t->fapp)[xcd][lane] = live ? sum - mine : 0xffffffffu;
+    // (groups of earlier chunks: written by earlier launches)
+    Group g = {};
+    if (lane < ch.base) g = t->g[lane];
+    else if (live) g = ch.g[lane - ch.base];
+    if (k == 0) {
+        t->fin[lane] = live ? g.fin : 0xffffffffu;
+        t->fio[lane] = live ? g.fio : 0xffffffffu;
+        t->batch[lane] = g.batch; t->np[lane] = g.np; t->mp[lane] = g.mp;
+        t->tsym[lane] = g.tsym; t->tapp[lane] = g.tapp; t->hsym[lane] = g.hsym; t->happ[lane] = g.happ;
+        t->xo[lane] = g.xo; t->ao[lane] = g.ao; t->dof[lane] = g.dof; t->mat[lane] = g.mat;
     }
+    const int xcd = k & 7, home = k < 8 ? g.hsym : g.happ;
+    const unsigned total = live ? (unsigned)g.batch * (unsigned)(k < 8 ? g.tsym : g.tapp) : 0u;
+    const unsigned mine = run_start(total, home, xcd + 1) - run_start(total, home, xcd);
+    unsigned sum = mine;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const unsigned v = __shfl_up(sum, o, 64);
+        if (lane >= o) sum += v;
+    }
+    (k < 8 ? t->fsym : t->fapp)[xcd][lane] = live ? sum - mine : 0xffffffffu;
 }
 
 // the last of the groups that begin at or before `at`
@@ -174,19 +176,27 @@ __device__ __forceinline__ float direction_of(const Muon& mu, float g, float v) 
 // sums of squares in 64 bits (an fp32 square overflows from 1.8e19 on and vanishes below 1e-23): one partial a workgroup.
 // (The new momentum is not stored here: ortho_pack_kernel computes it again, and what this pass read may still be in the
 // memory-side cache then.)
+// A chunk of groups a launch; its first workgroup writes the table for the kernels behind it.
 template <int KIND>
-__global__ void __launch_bounds__(256) ortho_sqsum_kernel(const Table* __restrict__ t, const Muon mu, double* __restrict__ part) {
+__global__ void __launch_bounds__(1024) ortho_sqsum_kernel(const Chunk ch, const Muon mu, double* __restrict__ part, Table* __restrict__ t) {
     constexpr bool BF = KIND & 1;
-    const int gi = find_group(t->fin, blockIdx.x);
-    const Group& g = t->g[gi];
+    if (blockIdx.x == 0) {
+        write_table(ch, t);
+        return;
+    }
+    const unsigned wg = blockIdx.x - 1 + ch.g[0].fin;
+    const int lane = threadIdx.x & 63;
+    const bool mine = lane < ch.n && ch.g[lane < CHUNK ? lane : 0].fin <= wg;
+    const int gi = __builtin_amdgcn_readfirstlane(__popcll(__ballot(mine)) - 1);
+    const Group& g = ch.g[gi];
     const long long numel = (long long)g.r * g.c;
-    const unsigned idx = blockIdx.x - t->fin[gi];
+    const unsigned idx = wg - g.fin;
     const int b = idx / g.parts, pi = idx - b * g.parts;
     const long long lo = (long long)pi * g.part_elems, hi = lo + g.part_elems < numel ? lo + g.part_elems : numel;
     double s = 0.0;
     if (KIND >= 2) {
         const long long end8 = lo + ((hi - lo) & ~7LL);
-        for (long long e = lo + threadIdx.x * 8; e < end8; e += 2048) {
+        for (long long e = lo + threadIdx.x * 8; e < end8; e += 8192) {
             float gr[8], v[8];
             load8<BF>(mu.g, g.sb + e, gr);
             load8f(mu.v + g.sb + e, v);
@@ -203,7 +213,7 @@ __global__ void __launch_bounds__(256) ortho_sqsum_kernel(const Table* __restric
         }
     } else if (g.vec && g.rs == g.c) {       // dense
         const long long end8 = lo + ((hi - lo) & ~7LL);
-        for (long long e = lo + threadIdx.x * 8; e < end8; e += 2048) {
+        for (long long e = lo + threadIdx.x * 8; e < end8; e += 8192) {
             float u[8];
             load8<BF>(g.src, b * g.sb + e, u);
 #pragma unroll
@@ -214,17 +224,22 @@ __global__ void __launch_bounds__(256) ortho_sqsum_kernel(const Table* __restric
             s += (double)u * (double)u;
         }
     } else {
-        for (long long e = lo + threadIdx.x; e < hi; e += 256) {
+        for (long long e = lo + threadIdx.x; e < hi; e += 1024) {
             const int i = (int)(e / g.c), j = (int)(e - (long long)i * g.c);
             const float u = load1<BF>(g.src, b * g.sb + (long long)i * g.rs + (long long)j * g.cs);
             s += (double)u * (double)u;
         }
     }
-    __shared__ double red[4];
+    __shared__ double red[16];
     s = wave_sum_d(s);
-    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = s;
+    if (lane == 0) red[threadIdx.x >> 6] = s;
     __syncthreads();
-    if (threadIdx.x == 0) part[g.po + (unsigned)b * g.parts + pi] = (red[0] + red[1]) + (red[2] + red[3]);
+    if (threadIdx.x == 0) {
+        double all = 0.0;
+#pragma unroll
+        for (int w = 0; w < 16; ++w) all += red[w];
+        part[g.po + (unsigned)b * g.parts + pi] = all;
+    }
 }
 
 // scale and further shift of a matrix of this norm: X in the workspace is 2^(12 + shift) X
@@ -797,8 +812,8 @@ struct Plan {
 
 long long part_elems_of(long long numel) {
     long long e = (numel + PARTS - 1) / PARTS;
-    e = (e + 2047) / 2048 * 2048;
-    return e < 4096 ? 4096 : e;
+    e = (e + 8191) / 8192 * 8192;
+    return e < 16384 ? 16384 : e;
 }
 long long pad64(long long v) { return (v + 63) / 64 * 64; }
 
@@ -1026,7 +1041,6 @@ int run_all(const Desc* q, int count, int kind, const Muon& mu, float a, float b
     double* part = (double*)(ws + pl.part);
     int* ex = (int*)(ws + pl.ex);
     const int fall = growth_bits(a, b, c, steps);
-    const dim3 block(256);
     for (int base = 0; base < count; base += CHUNK) {
         Chunk ch;
         ch.base = base;
@@ -1034,13 +1048,14 @@ int run_all(const Desc* q, int count, int kind, const Muon& mu, float a, float b
         ch.last = base + CHUNK >= count;
         memcpy(ch.g, g + base, ch.n * sizeof(Group));
         memset(ch.g + ch.n, 0, (CHUNK - ch.n) * sizeof(Group));
-        DDL_KLAUNCH(ortho_table_kernel, dim3(1), block, 0, stream, ch, t);
+        const dim3 grid((unsigned)((ch.last ? nin : g[base + CHUNK].fin) - g[base].fin) + 1);
+#define SUMS(K) DDL_KLAUNCH(ortho_sqsum_kernel<K>, grid, dim3(1024), 0, stream, ch, mu, part, t)
+        if (kind == 0) SUMS(0); else if (kind == 1) SUMS(1); else if (kind == 2) SUMS(2); else SUMS(3);
+#undef SUMS
     }
-#define IO(K)                                                                                              \
-    DDL_KLAUNCH(ortho_sqsum_kernel<K>, dim3((unsigned)nin), block, 0, stream, t, mu, part);                \
-    DDL_KLAUNCH(ortho_pack_kernel<K>, dim3((unsigned)nio), block, 0, stream, t, mu, part, eps, ex, xh, xl)
-    if (kind == 0) { IO(0); } else if (kind == 1) { IO(1); } else if (kind == 2) { IO(2); } else { IO(3); }
-#undef IO
+#define PACK(K) DDL_KLAUNCH(ortho_pack_kernel<K>, dim3((unsigned)nio), dim3(256), 0, stream, t, mu, part, eps, ex, xh, xl)
+    if (kind == 0) PACK(0); else if (kind == 1) PACK(1); else if (kind == 2) PACK(2); else PACK(3);
+#undef PACK
     for (int k = 0; k < steps; ++k) {
         const int fin = k < steps - 1 ? 0 : (kind < 2 ? 1 : 2);
 #define SYM(B, W0, W1, NST, SQ, IN, DIN, OUTP, DOUT, DOWN) DDL_KLAUNCH((ortho_sym_kernel<B, W0, W1, NST, SQ>), dim3((unsigned)nsym), dim3(W0 * W1 * 64), 0, stream, t, IN, DIN, OUTP, DOUT, ex, DOWN, a, b, c)
