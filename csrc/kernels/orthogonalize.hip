@@ -403,7 +403,7 @@ __device__ __forceinline__ void tri_tile(int idx, int rows, int& ti, int& tj) {
 
 // SQUARE = false: O, d of A = X X^T.  SQUARE = true: O, d of P = b A + c A^2 (diagonal: + a) from those of A
 template <int B, int W0, int W1, int NST, bool SQUARE>
-__global__ void __launch_bounds__(W0 * W1 * 64, 2) ortho_sym_kernel(const Table* __restrict__ t, const f16_t* __restrict__ in, const float* __restrict__ din,
+__global__ void __launch_bounds__(W0 * W1 * 64, B == 128 ? 4 : 2) ortho_sym_kernel(const Table* __restrict__ t, const f16_t* __restrict__ in, const float* __restrict__ din,
                                                           f16_t* __restrict__ out, float* __restrict__ dout, const int* __restrict__ ex, int down,
                                                           float ca, float cb, float cc) {
     typedef TileMul<MulF16, B, B, W0, W1, NST, false> M;
@@ -491,7 +491,7 @@ __global__ void __launch_bounds__(W0 * W1 * 64, 2) ortho_sym_kernel(const Table*
 
 // X' = pd X + offdiag(P) X_hi; tile: BF columns of X times BS rows of P.  FINAL 0: the next X; 1: the output; 2: the weights (K23)
 template <int BF, int BS, int W0, int W1, int NST, int FINAL>
-__global__ void __launch_bounds__(W0 * W1 * 64, 2) ortho_apply_kernel(const Table* __restrict__ t, const Muon mu, const f16_t* __restrict__ P,
+__global__ void __launch_bounds__(W0 * W1 * 64, BF == 128 ? 4 : 2) ortho_apply_kernel(const Table* __restrict__ t, const Muon mu, const f16_t* __restrict__ P,
                                                             const float* __restrict__ pd, const f16_t* __restrict__ xh, const f16_t* __restrict__ xl,
                                                             f16_t* __restrict__ yh, f16_t* __restrict__ yl,
                                                             const int* __restrict__ ex, int down, int down1) {
@@ -936,7 +936,7 @@ void tiles_of(const Desc* q, int count, int& sym, int& app) {
         a256 += q[i].batch * n256 * ((m + 255) / 256);
     }
     sym = s256 >= 128 && s64 >= 12 * s256 ? 256 : (s64 >= 1100 ? 128 : 64);      // (12 of 16: the larger tiles are mostly filled)
-    app = a256 >= 384 && a64 >= 12 * a256 ? 256 : (a64 >= 1024 ? 128 : 64);
+    app = a256 >= 512 && a64 >= 12 * a256 ? 256 : (a64 >= 1024 ? 128 : 64);
 }
 
 // Calls that ortho_small_kernel serves: every matrix of up to 64 rows (its shorter side) and 512 columns, or 128 and 256
@@ -1062,10 +1062,10 @@ int run_all(const Desc* q, int count, int kind, const Muon& mu, float a, float b
 #define APP1(B, W0, W1, NST, FIN) DDL_KLAUNCH((ortho_apply_kernel<B, B, W0, W1, NST, FIN>), dim3((unsigned)napp), dim3(W0 * W1 * 64), 0, stream, t, mu, P, pd, xh, xl, yh, yl, ex, k * fall, (k + 1) * fall)
 #define APP(B, W0, W1, NST) { if (fin == 0) APP1(B, W0, W1, NST, 0); else if (fin == 1) APP1(B, W0, W1, NST, 1); else APP1(B, W0, W1, NST, 2); }
         if (sb == 64) { SYM(64, 2, 2, 3, false, xh, (const float*)nullptr, O, d, k * fall); SYM(64, 2, 2, 3, true, O, d, P, pd, 0); }
-        else if (sb == 128) { SYM(128, 2, 2, 2, false, xh, (const float*)nullptr, O, d, k * fall); SYM(128, 2, 2, 2, true, O, d, P, pd, 0); }
+        else if (sb == 128) { SYM(128, 2, 4, 2, false, xh, (const float*)nullptr, O, d, k * fall); SYM(128, 2, 4, 2, true, O, d, P, pd, 0); }
         else { SYM(256, 2, 4, 2, false, xh, (const float*)nullptr, O, d, k * fall); SYM(256, 2, 4, 2, true, O, d, P, pd, 0); }
         if (ab == 64) APP(64, 2, 2, 3)
-        else if (ab == 128) APP(128, 2, 2, 2)
+        else if (ab == 128) APP(128, 2, 4, 2)
         else APP(256, 2, 4, 2)
         f16_t* s = xh; xh = yh; yh = s;
         s = xl; xl = yl; yl = s;

@@ -307,25 +307,31 @@ def linear_int8(x, q, scale, bias=None):
     and summed exactly: ``y = (xq q^T) * sx * scale + bias`` in fp32, returned in ``x``'s dtype [..., n].  ``bias``: fp32 [n].
     ``q`` as :func:`quantize_int8` returns it (rows start at multiples of 16 bytes).  No gradient flows through it: an input
     that requires one is refused outside ``torch.no_grad()``.  ``k`` is at most 133 144."""
-    if x.dtype not in (torch.float32, torch.bfloat16) or x.dim() < 1:
+    if (x.dtype is not torch.float32 and x.dtype is not torch.bfloat16) or x.dim() < 1:
         raise ValueError("linear_int8: fp32 or bf16 rows expected, got %s" % x.dtype)
-    if q.dtype != torch.int8 or q.dim() != 2 or q.shape[1] != x.shape[-1] or not 0 < q.shape[1] <= 133144:
-        raise ValueError("linear_int8: int8 codes [n, %d] of at most 133144 columns expected, got %s %s" % (x.shape[-1], q.dtype, tuple(q.shape)))
+    shape, k = x.shape, x.shape[-1]
+    if q.dtype is not torch.int8 or q.dim() != 2 or q.shape[1] != k or not 0 < k <= 133144:
+        raise ValueError("linear_int8: int8 codes [n, %d] of 1 to 133144 columns expected, got %s %s" % (k, q.dtype, tuple(q.shape)))
     for name, t in (("scale", scale), ("bias", bias)):
-        if t is not None and (t.dtype != torch.float32 or t.shape != q.shape[:1]):
+        if t is None:
+            continue
+        if t.dtype is not torch.float32 or t.dim() != 1 or t.shape[0] != q.shape[0]:
             raise ValueError("linear_int8: %s must be fp32 [%d], got %s %s" % (name, q.shape[0], t.dtype, tuple(t.shape)))
-    if any(t is not None and t.device != x.device for t in (q, scale, bias)):
+        if t.device != x.device:
+            raise ValueError("linear_int8: input, codes, scales and bias must be on one device")
+    if q.device != x.device:
         raise ValueError("linear_int8: input, codes, scales and bias must be on one device")
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, scale, bias)):
+    if torch.is_grad_enabled() and (x.requires_grad or scale.requires_grad or (bias is not None and bias.requires_grad)):
         raise ValueError("linear_int8: no gradient flows through it; call it under torch.no_grad()")
-    x2 = x.reshape(-1, x.shape[-1]) if x.numel() else x.new_empty((x.shape[:-1].numel(), x.shape[-1]))
+    x2 = x if x.dim() == 2 else x.reshape(shape[:-1].numel(), k)
     if x.is_cuda and _FORCED != "aten":
         from . import kernels
 
         if kernels.require():
             from . import hip_ops
 
-            return hip_ops.linear_int8(x2, q, scale, bias).view(x.shape[:-1] + q.shape[:1])
+            y = hip_ops.linear_int8(x2, q, scale, bias)
+            return y if x.dim() == 2 else y.view(shape[:-1] + q.shape[:1])
     xq, sx = _int8_rows_plain(x2)
     # (fp64 sums: whole numbers up to 2^31 are exact)
     y = (xq.double() @ q.double().t()).float() * (sx[:, None] * scale[None, :])

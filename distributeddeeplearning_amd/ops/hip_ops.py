@@ -1847,13 +1847,29 @@ def linear(x, weight, bias):
     return LinearFn.apply(x, weight, bias)
 
 
+class _NoSwitch:
+    def __enter__(self):
+        return self
+
+    def __exit__(self, *exc):
+        return False
+
+
+_NO_SWITCH = _NoSwitch()
+
+
+def _on(device):
+    """Context in which ``device`` is the current one (nothing where it is already)."""
+    return _NO_SWITCH if device.index == torch._C._cuda_getDevice() else torch.cuda.device(device)
+
+
 def quantize_int8(w):
     n, k = w.shape
     if w.stride(1) != 1:
         w = w.contiguous()
     store = torch.empty((n, (k + 63) // 64 * 64), dtype=torch.int8, device=w.device)
     scale = torch.empty(n, dtype=torch.float32, device=w.device)
-    with torch.cuda.device(w.device):
+    with _on(w.device):
         K.int8_rows(w, store, scale)
     return store[:, :k], scale
 
@@ -1861,14 +1877,19 @@ def quantize_int8(w):
 def linear_int8(x, q, scale, bias):
     """``functional.linear_int8`` of a 2-d input."""
     n, k = q.shape
-    if q.stride(1) != 1 or q.stride(0) % 16 or q.data_ptr() % 16 or K.storage_numel_from(q) < (n - 1) * q.stride(0) + (k + 15) // 16 * 16:
-        raise K.KernelError("linear_int8: the rows of the codes must start at multiples of 16 bytes and be readable to the next one behind "
-                            "their end: take them from quantize_int8 (strides %s)" % (q.stride(),))
+    ldq, s1 = q.stride()
+    if s1 != 1 or ldq % 16 or ldq >= 1 << 22 or q.data_ptr() % 16 or K.storage_numel_from(q) < (n - 1) * ldq + (k + 15) // 16 * 16:
+        raise K.KernelError("linear_int8: the rows of the codes must start at multiples of 16 bytes, less than 4 MiB apart, and be readable to "
+                            "the next multiple behind their end: take them from quantize_int8 (strides %s)" % (q.stride(),))
     if x.stride(1) != 1 or x.stride(0) < 0:
         x = x.contiguous()
     y = torch.empty((x.shape[0], n), dtype=x.dtype, device=x.device)
-    with torch.cuda.device(x.device):
-        K.int8_linear(x, q, scale.contiguous(), None if bias is None else bias.contiguous(), y)
+    if not scale.is_contiguous():
+        scale = scale.contiguous()
+    if bias is not None and not bias.is_contiguous():
+        bias = bias.contiguous()
+    with _on(x.device):
+        K.int8_linear(x, q, scale, bias, y)
     return y
 
 
@@ -1888,7 +1909,7 @@ def orthogonalize(mats, steps, coefficients, eps):
             keep.append(m3)
         groups.append((m3.data_ptr(),) + m3.stride() + (o.data_ptr(),) + o3.stride() + (m3.shape[1], m3.shape[2], m3.shape[0]))
     per = K.ortho_max_groups()
-    with torch.cuda.device(mats[0].device):
+    with _on(mats[0].device):
         for k in range(0, len(groups), per):
             table, count = K.ortho_table(groups[k:k + per])
             work = torch.empty(K.ortho_workspace(table, count), dtype=torch.uint8, device=mats[0].device)
