@@ -29,77 +29,68 @@ __device__ __forceinline__ void st1(float* p, float v) { *p = v; }
 __device__ __forceinline__ void st1(bf16_t* p, float v) { *p = f2bf(v); }
 __device__ __forceinline__ unsigned code_of(float v, float inv) { return (unsigned)(int)rintf(v * inv) & 255u; }
 
+// 8 values of a row from k on, zeros from K on; vec: the row starts at a multiple of 16 bytes
+template <typename T>
+__device__ __forceinline__ void ld_row(const T* __restrict__ row, int k, int K, bool vec, float (&v)[8]) {
+    if (vec && k + 8 <= K) {
+        ld8(row + k, v);
+    } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = k + j < K ? ld1(row + k + j) : 0.f;
+    }
+}
+
 // One wave: the codes of a row (K values, zeros up to Kp, a multiple of 16) to q, which starts at a multiple of 16 bytes; returns
-// its scale.  The first 2048 values stay in registers between the two passes.  vec: the row starts at a multiple of 16 bytes.
+// its scale.  The first 2048 values are read at once and stay in registers between the two passes.
 template <typename T>
 __device__ __forceinline__ float quantize_row(const T* __restrict__ row, int K, int Kp, bool vec, signed char* q) {
     const int lane = threadIdx.x & 63;
-    float top = 0.f;
-    int bad = 0;
-    auto see = [&](float v) {
-        v = fabsf(v);
-        bad |= !(v < __builtin_inff());
-        top = fmaxf(top, v);
-    };
     constexpr int HOLD = 4;
-    float held[HOLD][8];
-    const int k8 = vec ? K & ~7 : 0;
+    float held[HOLD][8], top = 0.f;
+    int bad = 0;
 #pragma unroll
-    for (int h = 0; h < HOLD; ++h) {
-        const int k = (h * 64 + lane) * 8;
-        if (k < k8) {
-            ld8(row + k, held[h]);
-        } else {
+    for (int h = 0; h < HOLD; ++h) ld_row(row, (h * 64 + lane) * 8, K, vec, held[h]);
+    auto see = [&](const float (&v)[8]) {
 #pragma unroll
-            for (int j = 0; j < 8; ++j) held[h][j] = 0.f;
+        for (int j = 0; j < 8; ++j) {
+            const float a = fabsf(v[j]);
+            bad |= !(a < __builtin_inff());
+            top = fmaxf(top, a);
         }
-    }
+    };
 #pragma unroll
-    for (int h = 0; h < HOLD; ++h)
-#pragma unroll
-        for (int j = 0; j < 8; ++j) see(held[h][j]);
+    for (int h = 0; h < HOLD; ++h) see(held[h]);
 #pragma unroll 2
-    for (int k = (HOLD * 64 + lane) * 8; k < k8; k += 512) {
+    for (int k = (HOLD * 64 + lane) * 8; k < K; k += 512) {
         float v[8];
-        ld8(row + k, v);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) see(v[j]);
+        ld_row(row, k, K, vec, v);
+        see(v);
     }
-#pragma unroll 4
-    for (int k = k8 + lane; k < K; k += 64) see(ld1(row + k));
     top = wave_max(top);
     bad = __any(bad);
     const bool zero = bad || top < 1e-30f;
     const float inv = zero ? 0.f : 127.f * (1.f / top);
-    auto pack = [&](const float (&v)[8]) {
+    auto put = [&](int k, const float (&v)[8]) {
+        if (k >= Kp) return;
         u32x2 o;
 #pragma unroll
         for (int p = 0; p < 2; ++p)
             o[p] = zero ? 0u : code_of(v[4 * p], inv) | code_of(v[4 * p + 1], inv) << 8 | code_of(v[4 * p + 2], inv) << 16 | code_of(v[4 * p + 3], inv) << 24;
-        return o;
+        *reinterpret_cast<u32x2*>(q + k) = o;
     };
 #pragma unroll
-    for (int h = 0; h < HOLD; ++h) {
-        const int k = (h * 64 + lane) * 8;
-        if (k < k8) *reinterpret_cast<u32x2*>(q + k) = pack(held[h]);
-    }
-    for (int k = (HOLD * 64 + lane) * 8; k < k8; k += 512) {
+    for (int h = 0; h < HOLD; ++h) put((h * 64 + lane) * 8, held[h]);
+#pragma unroll 2
+    for (int k = (HOLD * 64 + lane) * 8; k < Kp; k += 512) {
         float v[8];
-        ld8(row + k, v);
-        *reinterpret_cast<u32x2*>(q + k) = pack(v);
-    }
-    // the rest, four values a lane, zeros from K on
-    for (int k = k8 + lane * 4; k < Kp; k += 256) {
-        unsigned o = 0;
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-            if (k + j < K && !zero) o |= code_of(ld1(row + k + j), inv) << (8 * j);
-        *reinterpret_cast<unsigned*>(q + k) = o;
+        ld_row(row, k, K, vec, v);
+        put(k, v);
     }
     return bad ? __builtin_nanf("") : (zero ? 0.f : top / 127.f);
 }
 
-// a row a wave: codes [M][Kp], scales.  12 544 rows of 4096 bf16 values (154 MB): 94 -> ROWS_US us
+// a row a wave: codes [M][Kp], scales.  12 544 rows of 4096 bf16 values (154 MB): 31 us (values of a row held in registers between its largest
+// and its codes; read a second time: 94)
 template <typename T>
 __global__ void __launch_bounds__(256) int8_rows_kernel(const T* __restrict__ x, long long ldx, int M, int K, int Kp, int vec, signed char* __restrict__ q,
                                                        float* __restrict__ scale) {
@@ -110,13 +101,13 @@ __global__ void __launch_bounds__(256) int8_rows_kernel(const T* __restrict__ x,
 }
 
 // B x B tile of y: F = output channels, S = rows of x
-template <typename T, int B, int W0, int W1, int NST>
-__global__ void __launch_bounds__(W0 * W1 * 64, 2) int8_gemm_kernel(const signed char* __restrict__ xq, const float* __restrict__ sx,
+template <typename T, int B, int W0, int W1, int NST, int KS>
+__global__ void __launch_bounds__(KS * W0 * W1 * 64, 2) int8_gemm_kernel(const signed char* __restrict__ xq, const float* __restrict__ sx,
                                                                    const signed char* __restrict__ q, long long ldq, long long q_bytes,
                                                                    const float* __restrict__ s, const float* __restrict__ bias, T* __restrict__ y, long long ldy,
                                                                    int M, int N, int Kp, int tm, int tn) {
-    typedef TileMul<MulI8, B, B, W0, W1, NST, false> Mu;
-    __shared__ __attribute__((aligned(16))) unsigned char smem[NST * Mu::STAGE];
+    typedef TileMul<MulI8, B, B, W0, W1, NST, false, KS> Mu;
+    __shared__ __attribute__((aligned(16))) unsigned char smem[Mu::LDS];
     // an XCD (workgroup number modulo 8) has a run of tiles, in bands of 8 rows, a band column by column
     const int all = tm * tn, per = (all + 7) >> 3, idx = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
     if ((int)(blockIdx.x >> 3) >= per || idx >= all) return;
@@ -247,15 +238,16 @@ int run(const T* x, long long ldx, const signed char* q, long long ldq, long lon
     signed char* xq = (signed char*)ws;
     float* sx = (float*)(ws + ((long long)M * Kp + 255) / 256 * 256);
     DDL_KLAUNCH(int8_rows_kernel<T>, dim3((M + 3) / 4), dim3(256), 0, stream, x, ldx, M, K, Kp, vec, xq, sx);
-    // 128 x 128 tiles, two a CU, unless they are fewer than the CUs.  (256 x 256 in 8 waves is no faster where it fills whole rounds,
+    // 128 x 128 tiles, two a CU, unless they are fewer than the CUs; two groups of waves a tile where even 64 x 64 are.  (256 x 256 in 8 waves is no faster where it fills whole rounds,
     // 4096^3 in 100 / 101 us, and 12 544 x 4096 x 4096 takes 4 rounds for 3.06: 333 / 304 us.  256 x 128: 328; 4 waves of 128 x 128:
     // 396, copies between register halves.)
     const long long t128 = ((M + 127LL) / 128) * ((N + 127) / 128), t64 = ((M + 63LL) / 64) * ((N + 63) / 64);
     if ((t64 + 7) / 8 * 8 > 0x7fffffffLL) return DDL_EINVAL;
-#define GEMM(B, W0, W1, NST, t) DDL_KLAUNCH((int8_gemm_kernel<T, B, W0, W1, NST>), dim3((unsigned)((t + 7) / 8 * 8)), dim3(W0 * W1 * 64), 0, stream, xq, sx, q, \
+#define GEMM(B, W0, W1, NST, KS, t) DDL_KLAUNCH((int8_gemm_kernel<T, B, W0, W1, NST, KS>), dim3((unsigned)((t + 7) / 8 * 8)), dim3(KS * W0 * W1 * 64), 0, stream, xq, sx, q, \
                                             ldq, q_bytes, s, bias, y, ldy, M, N, Kp, (M + B - 1) / B, (N + B - 1) / B)
-    if (t128 >= 256) GEMM(128, 2, 2, 2, t128);
-    else GEMM(64, 2, 2, 3, t64);
+    if (t128 >= 256) GEMM(128, 2, 2, 2, 1, t128);
+    else if (t64 <= 256 && Kp > 128) GEMM(64, 2, 2, 3, 2, t64);
+    else GEMM(64, 2, 2, 3, 1, t64);
 #undef GEMM
     return ddl_launch_status();
 }

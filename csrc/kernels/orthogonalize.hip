@@ -13,11 +13,15 @@
 // Against 64 bits the result is 2e-4 .. 1e-3 off (2-norm; Gaussian, power-law, exponential, low-rank and gradient-like
 // spectra), below half a bf16 step (1.7e-3 on average); bf16 operands throughout give 8e-3 .. 0.3, plain fp16 1e-3 .. 4e-2.
 //
-// A call takes up to 64 groups of equal matrices; all of them share each launch (a table of shapes and offsets travels by
-// value in the kernel arguments, so a call can be captured or recorded and needs no copy to the device): sums of squares,
-// packing, three products a step, result.  A matrix whose norm is below eps starts at X_0 = G / eps, far below 1: it is
-// kept scaled by a further 2^e (shift_of), which falls from step to step as X can grow.  Workspace copies are padded to multiples of 64 with zeros, which the steps
-// keep (0 = a 0 + 0), so the products have no edges.
+// A call takes up to 64 groups of equal matrices; all of them share each launch.  Three forms, by sizes alone:
+//   * every matrix of up to 64 x 512 or 128 x 256: a workgroup a matrix, one launch (ortho_small_kernel);
+//   * else, every matrix of up to 32 rows: four launches, all steps on the Gram matrix (ortho_thin_*_kernel);
+//   * else tiles: sums of squares (whose first workgroup writes the table of shapes and offsets, from the kernel's arguments: a
+//     call can be captured or recorded and copies nothing to the device), packing, three products a step; the last product
+//     writes the result or the weights.
+// A matrix whose norm is below eps starts at X_0 = G / eps, far below 1: it is kept scaled by a further 2^e (shift_of), which
+// falls from step to step as X can grow.  Workspace copies are padded to multiples of 64 with zeros, which the steps keep
+// (0 = a 0 + 0), so the products have no edges.
 #include "common.h"
 #include "tile_mul.h"
 #include <math.h>
@@ -42,7 +46,8 @@ struct Group {                      // `batch` equal matrices
     unsigned xo, ao, dof, po, mat;  // first matrix in the X and square workspaces (64 elements), in the diagonals, the partial sums, among all
     int tsym, tapp;                 // tiles of a matrix in the symmetric products and in P X
     int hsym, happ;                 // the XCD that computes them, -1: all
-    unsigned fin, fio;              // first workgroup of the sums, of the packing
+    unsigned fin, fio;              // first workgroup of the sums, of the packing (thin form: of the chunks)
+    int tcols, chunks;              // thin form: columns of a chunk, chunks of a matrix
 };
 struct Chunk { Group g[CHUNK]; int base, n, last; };
 
@@ -78,7 +83,7 @@ __device__ __forceinline__ void write_table(const Chunk& ch, Table* __restrict__
         t->fio[lane] = live ? g.fio : 0xffffffffu;
         t->batch[lane] = g.batch; t->np[lane] = g.np; t->mp[lane] = g.mp;
         t->tsym[lane] = g.tsym; t->tapp[lane] = g.tapp; t->hsym[lane] = g.hsym; t->happ[lane] = g.happ;
-        t->xo[lane] = g.xo; t->ao[lane] = g.ao; t->dof[lane] = g.dof; t->mat[lane] = g.mat;
+        t->xo[lane] = g.xo; t->ao[lane] = g.ao; t->dof[lane] = g.dof; t->mat[lane] = live ? g.mat : 0xffffffffu;
     }
     const int xcd = k & 7, home = k < 8 ? g.hsym : g.happ;
     const unsigned total = live ? (unsigned)g.batch * (unsigned)(k < 8 ? g.tsym : g.tapp) : 0u;
@@ -402,12 +407,12 @@ __device__ __forceinline__ void tri_tile(int idx, int rows, int& ti, int& tj) {
 }
 
 // SQUARE = false: O, d of A = X X^T.  SQUARE = true: O, d of P = b A + c A^2 (diagonal: + a) from those of A
-template <int B, int W0, int W1, int NST, bool SQUARE>
-__global__ void __launch_bounds__(W0 * W1 * 64, B == 128 ? 4 : 2) ortho_sym_kernel(const Table* __restrict__ t, const f16_t* __restrict__ in, const float* __restrict__ din,
+template <int B, int W0, int W1, int NST, int KS, bool SQUARE>
+__global__ void __launch_bounds__(KS * W0 * W1 * 64, B == 128 ? 4 : 2) ortho_sym_kernel(const Table* __restrict__ t, const f16_t* __restrict__ in, const float* __restrict__ din,
                                                           f16_t* __restrict__ out, float* __restrict__ dout, const int* __restrict__ ex, int down,
                                                           float ca, float cb, float cc) {
-    typedef TileMul<MulF16, B, B, W0, W1, NST, false> M;
-    __shared__ __attribute__((aligned(16))) unsigned char smem[NST * M::STAGE];
+    typedef TileMul<MulF16, B, B, W0, W1, NST, false, KS> M;
+    __shared__ __attribute__((aligned(16))) unsigned char smem[M::LDS];
     Item it;
     if (!it.find(t, true)) return;
     const int np = it.np, lda = np, ld = SQUARE ? np : it.mp, K = ld, b = it.b;
@@ -490,13 +495,13 @@ __global__ void __launch_bounds__(W0 * W1 * 64, B == 128 ? 4 : 2) ortho_sym_kern
 }
 
 // X' = pd X + offdiag(P) X_hi; tile: BF columns of X times BS rows of P.  FINAL 0: the next X; 1: the output; 2: the weights (K23)
-template <int BF, int BS, int W0, int W1, int NST, int FINAL>
-__global__ void __launch_bounds__(W0 * W1 * 64, BF == 128 ? 4 : 2) ortho_apply_kernel(const Table* __restrict__ t, const Muon mu, const f16_t* __restrict__ P,
+template <int BF, int BS, int W0, int W1, int NST, int KS, int FINAL>
+__global__ void __launch_bounds__(KS * W0 * W1 * 64, BF == 128 ? 4 : 2) ortho_apply_kernel(const Table* __restrict__ t, const Muon mu, const f16_t* __restrict__ P,
                                                             const float* __restrict__ pd, const f16_t* __restrict__ xh, const f16_t* __restrict__ xl,
                                                             f16_t* __restrict__ yh, f16_t* __restrict__ yl,
                                                             const int* __restrict__ ex, int down, int down1) {
-    typedef TileMul<MulF16, BF, BS, W0, W1, NST, true> M;
-    __shared__ __attribute__((aligned(16))) unsigned char smem[NST * M::STAGE];
+    typedef TileMul<MulF16, BF, BS, W0, W1, NST, true, KS> M;
+    __shared__ __attribute__((aligned(16))) unsigned char smem[M::LDS];
     Item it;
     if (!it.find(t, false)) return;
     const int np = it.np, mp = it.mp, b = it.b;
@@ -801,6 +806,213 @@ __global__ void __launch_bounds__(512, 2) ortho_small_kernel(const Chunk ch, con
         }
 }
 
+// ---- thin matrices: all steps on the Gram matrix ------------------------------------------------------------------------
+// Up to 32 rows of any length.  X_k = Q_k X_0 with Q_k and A_k polynomials in A_0: A <- P A P, Q <- P Q on np x np matrices, so the
+// long side is read twice and never iterated on: Gram matrix a chunk of columns a workgroup, all steps in one workgroup a matrix,
+// result a chunk of columns a workgroup.  An error of A_0 grows by up to 3e4 where a singular value vanishes, so A and Q are
+// computed in fp64 (its matrix instruction); Q reaches a^steps = 485 with cancelling entries: the result's product is fp32.
+// Bound by the latency of four launches.  Measured against the
+// tiles below: 17 x 2762 105 -> 46 us, 32 x 2048 94 -> 37, 59 of 1 x 3157 209 -> 34, 1000 of 32 x 600 602 -> 192, 32 x 100000
+// 1186 -> 131; 64 rows: 86 -> 80 us in fp32, and too few digits.  Error against 64 bits: 1e-5 before the rounding to bf16.
+typedef double f64x4 __attribute__((ext_vector_type(4)));
+
+// value of X (before its scale) at row r, column c; STORE: the new momentum is stored
+template <int KIND, bool STORE>
+__device__ __forceinline__ float thin_value(const Group& g, const Muon& mu, int b, bool turn, int r, int c) {
+    constexpr bool BF = KIND & 1;
+    const int i = turn ? c : r, j = turn ? r : c;
+    if (KIND >= 2) {
+        const long long at = g.sb + (long long)i * g.c + j;
+        const float gr = load1<BF>(mu.g, at), v = momentum_of(mu, gr, mu.v[at]);
+        if (STORE) mu.v[at] = v;
+        return direction_of(mu, gr, v);
+    }
+    return load1<BF>(g.src, b * g.sb + (long long)i * g.rs + (long long)j * g.cs);
+}
+__device__ __forceinline__ double thin_scale(const Group& g, const double* __restrict__ part, int b, float eps) {   // by one whole wave
+    double s = 0.0;
+    for (int k = threadIdx.x & 63; k < g.parts; k += 64) s += part[g.po + (unsigned)b * g.parts + k];
+    const double norm = sqrt(wave_sum_d(s));
+    return 1.0 / (norm > (double)eps ? norm : (norm == norm ? (double)eps : norm));
+}
+
+// slab [NP][NP] of X X^T over a chunk of columns.  A lane has 4 columns of a row; the e-th of all lanes are the reduction's 4
+// values of one matrix instruction (the columns' order does not matter).  Its result: rows lane / 16 + 4 e, column lane % 16.
+template <int NP, int KIND>
+__global__ void __launch_bounds__(256) ortho_thin_gram_kernel(const Table* __restrict__ t, const Muon mu, const double* __restrict__ part, float eps,
+                                                             double* __restrict__ slabs) {
+    constexpr int NS = NP / 16;
+    __shared__ double red[4][NP][NP + 2];
+    const int gi = find_group(t->fio, blockIdx.x);
+    const Group& g = t->g[gi];
+    const bool turn = g.r > g.c;
+    const int n = turn ? g.c : g.r, m = turn ? g.r : g.c, chunks = g.chunks, width = g.tcols;
+    const unsigned idx = blockIdx.x - t->fio[gi];
+    const int b = idx / chunks, c0 = (idx - b * chunks) * width, end = c0 + width < m ? c0 + width : m;
+    const int lane = threadIdx.x & 63, wid = threadIdx.x >> 6, fr = lane & 15, fq = lane >> 4;
+    const double scale = thin_scale(g, part, b, eps);
+    f64x4 acc[NS][NS];
+#pragma unroll
+    for (int i = 0; i < NS; ++i)
+#pragma unroll
+        for (int j = 0; j < NS; ++j) acc[i][j] = f64x4{0.0, 0.0, 0.0, 0.0};
+    for (int k = c0 + wid * 16; k < end; k += 64) {
+        f32x4 x[NS];
+#pragma unroll
+        for (int i = 0; i < NS; ++i)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int r = i * 16 + fr, c = k + fq * 4 + e;
+                x[i][e] = r < n && c < end ? (float)(thin_value<KIND, false>(g, mu, b, turn, r, c) * scale) : 0.f;
+            }
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+#pragma unroll
+            for (int i = 0; i < NS; ++i)
+#pragma unroll
+                for (int j = 0; j <= i; ++j) acc[i][j] = __builtin_amdgcn_mfma_f64_16x16x4f64((double)x[i][e], (double)x[j][e], acc[i][j], 0, 0, 0);
+    }
+#pragma unroll
+    for (int i = 0; i < NS; ++i)
+#pragma unroll
+        for (int j = 0; j <= i; ++j)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int r = i * 16 + fq + 4 * e, c = j * 16 + fr;
+                red[wid][r][c] = acc[i][j][e];
+                if (i != j) red[wid][c][r] = acc[i][j][e];
+            }
+    __syncthreads();
+    double* out = slabs + (long long)blockIdx.x * NP * NP;
+    for (int k = threadIdx.x; k < NP * NP; k += 256) {
+        const int r = k / NP, c = k % NP;
+        out[k] = (red[0][r][c] + red[1][r][c]) + (red[2][r][c] + red[3][r][c]);
+    }
+}
+
+// C = M N for symmetric N, all [NP][NP + 2] in LDS; lower block triangle, mirrored (products of polynomials in A are symmetric).
+// post(r, c, value) gives what is stored.
+template <int NP, typename F>
+__device__ __forceinline__ void thin_mul(const double (*M)[NP + 2], const double (*N)[NP + 2], double (*C)[NP + 2], F post) {
+    constexpr int NS = NP / 16, BLOCKS = NS * (NS + 1) / 2;
+    const int lane = threadIdx.x & 63, blk = threadIdx.x >> 6, fr = lane & 15, fq = lane >> 4;
+    if (blk < BLOCKS) {
+        const int i = blk > 0, j = blk > 1;
+        f64x4 acc = {0.0, 0.0, 0.0, 0.0}, odd = acc;  // two sums: half the instruction's latency
+#pragma unroll
+        for (int k = 0; k < NP; k += 8) {
+            acc = __builtin_amdgcn_mfma_f64_16x16x4f64(M[i * 16 + fr][k + fq], N[j * 16 + fr][k + fq], acc, 0, 0, 0);
+            odd = __builtin_amdgcn_mfma_f64_16x16x4f64(M[i * 16 + fr][k + 4 + fq], N[j * 16 + fr][k + 4 + fq], odd, 0, 0, 0);
+        }
+        acc += odd;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const int r = i * 16 + fq + 4 * e, c = j * 16 + fr;
+            const double v = post(r, c, acc[e]);
+            C[r][c] = v;
+            if (i != j) C[c][r] = v;
+        }
+    }
+    __syncthreads();
+}
+
+template <int NP>
+__global__ void __launch_bounds__(256) ortho_thin_steps_kernel(const Table* __restrict__ t, const double* __restrict__ slabs, float* __restrict__ Qout, float ca,
+                                                              float cb, float cc, int steps) {
+    typedef double Mat[NP][NP + 2];
+    __shared__ Mat A, P, T, Q[2];
+    const int gi = find_group(t->mat, blockIdx.x);
+    const Group& g = t->g[gi];
+    const int b = blockIdx.x - g.mat, chunks = g.chunks;
+    const double* from = slabs + ((long long)g.fio + (long long)b * chunks) * NP * NP;
+    for (int k = threadIdx.x; k < NP * NP; k += 256) {
+        double s = 0.0;
+#pragma unroll 8
+        for (int i = 0; i < chunks; ++i) s += from[(long long)i * NP * NP + k];
+        A[k / NP][k % NP] = s;
+    }
+    __syncthreads();
+    const double da = ca, db = cb, dc = cc;
+    auto same = [](int, int, double v) { return v; };
+    auto poly = [&](int r, int c, double v) { return db * A[r][c] + dc * v + (r == c ? da : 0.0); };
+    thin_mul<NP>(A, A, Q[0], poly);
+    int at = 0;
+#pragma unroll 1
+    for (int k = 1; k < steps; ++k) {
+        // A <- P A P; P of the first step is Q
+        const Mat& last = k == 1 ? Q[0] : P;
+        thin_mul<NP>(A, last, T, same);
+        thin_mul<NP>(last, T, A, same);
+        thin_mul<NP>(A, A, P, poly);
+        thin_mul<NP>(P, Q[at], Q[at ^ 1], same);
+        at ^= 1;
+    }
+    float* out = Qout + (long long)blockIdx.x * NP * NP;
+    for (int k = threadIdx.x; k < NP * NP; k += 256) out[k] = (float)Q[at][k / NP][k % NP];
+}
+
+// result = Q X: D rows = columns of X (4 a lane), D columns = rows
+template <int NP, int KIND>
+__global__ void __launch_bounds__(256) ortho_thin_apply_kernel(const Table* __restrict__ t, const Muon mu, const double* __restrict__ part, float eps,
+                                                              const float* __restrict__ Qin) {
+    constexpr int NS = NP / 16;
+    __shared__ __attribute__((aligned(16))) float Q[NP][NP + 4];
+    const int gi = find_group(t->fio, blockIdx.x);
+    const Group& g = t->g[gi];
+    const bool turn = g.r > g.c;
+    const int n = turn ? g.c : g.r, m = turn ? g.r : g.c, chunks = g.chunks, width = g.tcols;
+    const unsigned idx = blockIdx.x - t->fio[gi];
+    const int b = idx / chunks, c0 = (idx - b * chunks) * width, end = c0 + width < m ? c0 + width : m;
+    const int lane = threadIdx.x & 63, wid = threadIdx.x >> 6, fr = lane & 15, fq = lane >> 4;
+    const float* from = Qin + ((long long)g.mat + b) * NP * NP;
+    for (int k = threadIdx.x; k < NP * NP; k += 256) Q[k / NP][k % NP] = from[k];
+    const double scale = thin_scale(g, part, b, eps);
+    float lr = 0.f, by = 0.f;
+    if (KIND >= 2) {
+        lr = mu.lr_scale ? mu.lr * *mu.lr_scale : mu.lr;
+        by = lr * sqrtf(turn ? (float)g.r / (float)g.c : 1.f);
+    }
+    __syncthreads();
+#pragma unroll 1
+    for (int k = c0 + wid * 16; k < end; k += 64) {
+        f32x4 acc[NS];
+        float x[NS][4];
+#pragma unroll
+        for (int i = 0; i < NS; ++i) {
+            acc[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int r = i * 16 + fq * 4 + e, c = k + fr;
+                x[i][e] = r < n && c < end ? (float)(thin_value<KIND, true>(g, mu, b, turn, r, c) * scale) : 0.f;
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < NS; ++i) {
+#pragma unroll
+            for (int j = 0; j < NS; ++j) {
+                const f32x4 q = *reinterpret_cast<const f32x4*>(&Q[j * 16 + fr][i * 16 + fq * 4]);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) acc[j] = __builtin_amdgcn_mfma_f32_16x16x4f32(x[i][e], q[e], acc[j], 0, 0, 0);
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < NS; ++j)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int r = j * 16 + fr, c = k + fq * 4 + e;
+                if (r >= n || c >= end) continue;
+                const long long at = turn ? (long long)c * g.c + r : (long long)r * g.c + c;
+                if (KIND >= 2) {
+                    const float w = mu.w[g.sb + at] * (1.f - lr * mu.wd) - by * acc[j][e];
+                    mu.w[g.sb + at] = w;
+                    if (mu.lowp) mu.lowp[g.sb + at] = f2bf(w);
+                } else {
+                    g.dst[(long long)b * g.r * g.c + at] = f2bf(acc[j][e]);
+                }
+            }
+    }
+}
+
 // ---- host -------------------------------------------------------------------------------------------------------------
 // one group as the callers describe it: 11 int64 values
 struct Desc { long long src, sb, srs, scs, dst, db, drs, dcs, r, c, batch; };
@@ -808,6 +1020,8 @@ struct Desc { long long src, sb, srs, scs, dst, db, drs, dcs, r, c, batch; };
 struct Plan {
     long long x_elems = 0, a_elems = 0, d_elems = 0, parts = 0, mats = 0;
     long long table, xa_h, xa_l, xb_h, xb_l, o, p, d, pd, part, ex, bytes;
+    int thin = 0;                   // padded rows of the thin form, 0: not taken
+    long long slabs = 0;
 };
 
 long long part_elems_of(long long numel) {
@@ -817,7 +1031,20 @@ long long part_elems_of(long long numel) {
 }
 long long pad64(long long v) { return (v + 63) / 64 * 64; }
 
-bool plan_of(const Desc* q, int count, Plan& pl) {
+// Padded rows of the thin form, or 0: some matrix has more than 32
+int thin_rows(const Desc* q, int count) {
+    long long most = 0;
+    for (int i = 0; i < count; ++i) {
+        const long long n = q[i].r < q[i].c ? q[i].r : q[i].c;
+        if (n > most) most = n;
+    }
+    return most > 32 ? 0 : most > 16 ? 32 : 16;
+}
+
+// columns of a chunk: a 16-column block for each of a workgroup's waves, but 128 chunks at most
+long long thin_cols(long long m) { return (m + 8191) / 8192 * 64; }
+
+bool plan_of(const Desc* q, int count, bool thin, Plan& pl) {
     if (count < 0 || count > MAXG || (count && !q)) return false;
     for (int i = 0; i < count; ++i) {
         const Desc& s = q[i];
@@ -835,6 +1062,18 @@ bool plan_of(const Desc* q, int count, Plan& pl) {
     auto up = [](long long b) { return (b + 255) / 256 * 256; };
     long long at = 0;
     pl.table = at; at += up(sizeof(Table));
+    if (thin && (pl.thin = thin_rows(q, count)) != 0) {
+        for (int i = 0; i < count; ++i) {
+            const long long m = q[i].r > q[i].c ? q[i].r : q[i].c, w = thin_cols(m);
+            pl.slabs += q[i].batch * ((m + w - 1) / w);
+        }
+        if (pl.slabs > 0x7fffffffLL) return false;
+        pl.part = at; at += up(pl.parts * 8);
+        pl.o = at; at += up(pl.slabs * pl.thin * pl.thin * 8);
+        pl.p = at; at += up(pl.mats * pl.thin * pl.thin * 4);
+        pl.bytes = at;
+        return true;
+    }
     pl.xa_h = at; at += up(pl.x_elems * 2);
     pl.xa_l = at; at += up(pl.x_elems * 2);
     pl.xb_h = at; at += up(pl.x_elems * 2);
@@ -920,11 +1159,19 @@ int growth_bits(float a, float b, float c, int steps) {
     return range_of(a, b, c, steps, growth) ? (int)ceil(log2(growth)) : 0;
 }
 
+// Whether the thin form serves these steps: the Gram matrix's rounding, 2^-53, grows by the square of what X grows by (3.4445 ^ 10 =
+// 2^18 for five steps of the usual coefficients), and Q, rounded to fp32, by what X grows by (485)
+bool thin_steps(float a, float b, float c, int steps) {
+    double growth;
+    return range_of(a, b, c, steps, growth) && steps * log2(growth) <= 10.0;
+}
+
 // Tile sizes of a call.  Larger tiles need less LDS and L2 traffic a product (256 CUs full: 64 x 64 650, 128 x 128 890, 256 x 256
 // 1050 TFLOP/s), smaller ones fill the chip with less work.  Measured (us, 64 / 128 / 256): P X of 12 512 x 512 (768 tiles of 64)
 // 12.3 / 14.2 / 25.6, of 2048 x 2048 (1024) 35 / 32 / 55, of all of ResNet-50 (6200) 75 / 65 / 72, of 4096 x 8192 (8192; 512
 // of 256) 468 / 311 / 274; A and A^2 of ResNet-50 (880) 52 / 79 / 134, of 2048 x 2048 (528) 51 / 56 / 108, of two
 // 2048 x 4096 and 1000 x 4096 (1192) 116 / 107 / 152, of 4096 x 8192 (2080; 136 of 256) 374 / 318 / 311.
+// Tiles of 64 that have a CU each (up to 256) are computed by two groups of waves: 512 x 4608 alone 201 -> 182 us in all.
 void tiles_of(const Desc* q, int count, int& sym, int& app) {
     long long s64 = 0, s256 = 0, a64 = 0, a256 = 0;
     for (int i = 0; i < count; ++i) {
@@ -999,7 +1246,7 @@ int run_small(const Desc* q, int count, int kind, const Muon& mu, float a, float
 // kind as in load8
 int run_all(const Desc* q, int count, int kind, const Muon& mu, float a, float b, float c, int steps, float eps, char* ws, hipStream_t stream) {
     Plan pl;
-    if (!plan_of(q, count, pl)) return DDL_EINVAL;
+    if (!plan_of(q, count, thin_steps(a, b, c, steps), pl)) return DDL_EINVAL;
     if (all_small(q, count)) return run_small(q, count, kind, mu, a, b, c, steps, eps, stream);
     int sb = 64, ab = 64;
     tiles_of(q, count, sb, ab);
@@ -1027,7 +1274,9 @@ int run_all(const Desc* q, int count, int kind, const Muon& mu, float a, float b
         o.fin = (unsigned)nin; o.fio = (unsigned)nio;
         csym[i] = (double)s.batch * o.tsym * (double)(np + mp + 512);      // (512: what a tile costs beside its sum)
         capp[i] = (double)s.batch * o.tapp * (double)(np + 512);
-        nin += s.batch * parts; nio += s.batch * (np / 64) * (mp / 64);
+        o.tcols = (int)thin_cols(m);
+        o.chunks = (int)((m + o.tcols - 1) / o.tcols);
+        nin += s.batch * parts; nio += s.batch * (pl.thin ? o.chunks : (np / 64) * (mp / 64));
         nsym += s.batch * o.tsym; napp += s.batch * o.tapp;
         xo += s.batch * np * mp; ao += s.batch * np * np; dof += s.batch * np; po += s.batch * parts; mat += s.batch;
         if (nin > 0x7fffffffLL || nio > 0x7fffffffLL || nsym > 0x0fffffffLL || napp > 0x0fffffffLL) return DDL_EINVAL;
@@ -1053,20 +1302,38 @@ int run_all(const Desc* q, int count, int kind, const Muon& mu, float a, float b
         if (kind == 0) SUMS(0); else if (kind == 1) SUMS(1); else if (kind == 2) SUMS(2); else SUMS(3);
 #undef SUMS
     }
+    if (pl.thin) {
+        double* slabs = (double*)(ws + pl.o);
+        float* Q = (float*)(ws + pl.p);
+#define THIN1(NP, K)                                                                                                             \
+        {                                                                                                                        \
+            DDL_KLAUNCH((ortho_thin_gram_kernel<NP, K>), dim3((unsigned)nio), dim3(256), 0, stream, t, mu, part, eps, slabs);    \
+            DDL_KLAUNCH(ortho_thin_steps_kernel<NP>, dim3((unsigned)mat), dim3(256), 0, stream, t, slabs, Q, a, b, c, steps);    \
+            DDL_KLAUNCH((ortho_thin_apply_kernel<NP, K>), dim3((unsigned)nio), dim3(256), 0, stream, t, mu, part, eps, Q);       \
+        }
+#define THIN(K) { if (pl.thin == 16) THIN1(16, K) else THIN1(32, K) }
+        if (kind == 0) THIN(0) else if (kind == 1) THIN(1) else if (kind == 2) THIN(2) else THIN(3)
+#undef THIN
+#undef THIN1
+        return ddl_launch_status();
+    }
 #define PACK(K) DDL_KLAUNCH(ortho_pack_kernel<K>, dim3((unsigned)nio), dim3(256), 0, stream, t, mu, part, eps, ex, xh, xl)
     if (kind == 0) PACK(0); else if (kind == 1) PACK(1); else if (kind == 2) PACK(2); else PACK(3);
 #undef PACK
     for (int k = 0; k < steps; ++k) {
         const int fin = k < steps - 1 ? 0 : (kind < 2 ? 1 : 2);
-#define SYM(B, W0, W1, NST, SQ, IN, DIN, OUTP, DOUT, DOWN) DDL_KLAUNCH((ortho_sym_kernel<B, W0, W1, NST, SQ>), dim3((unsigned)nsym), dim3(W0 * W1 * 64), 0, stream, t, IN, DIN, OUTP, DOUT, ex, DOWN, a, b, c)
-#define APP1(B, W0, W1, NST, FIN) DDL_KLAUNCH((ortho_apply_kernel<B, B, W0, W1, NST, FIN>), dim3((unsigned)napp), dim3(W0 * W1 * 64), 0, stream, t, mu, P, pd, xh, xl, yh, yl, ex, k * fall, (k + 1) * fall)
-#define APP(B, W0, W1, NST) { if (fin == 0) APP1(B, W0, W1, NST, 0); else if (fin == 1) APP1(B, W0, W1, NST, 1); else APP1(B, W0, W1, NST, 2); }
-        if (sb == 64) { SYM(64, 2, 2, 3, false, xh, (const float*)nullptr, O, d, k * fall); SYM(64, 2, 2, 3, true, O, d, P, pd, 0); }
-        else if (sb == 128) { SYM(128, 2, 4, 2, false, xh, (const float*)nullptr, O, d, k * fall); SYM(128, 2, 4, 2, true, O, d, P, pd, 0); }
-        else { SYM(256, 2, 4, 2, false, xh, (const float*)nullptr, O, d, k * fall); SYM(256, 2, 4, 2, true, O, d, P, pd, 0); }
-        if (ab == 64) APP(64, 2, 2, 3)
-        else if (ab == 128) APP(128, 2, 4, 2)
-        else APP(256, 2, 4, 2)
+#define SYM(B, W0, W1, NST, KS, SQ, IN, DIN, OUTP, DOUT, DOWN) DDL_KLAUNCH((ortho_sym_kernel<B, W0, W1, NST, KS, SQ>), dim3((unsigned)nsym), dim3(KS * W0 * W1 * 64), 0, stream, t, IN, DIN, OUTP, DOUT, ex, DOWN, a, b, c)
+#define SYMS(B, W0, W1, NST, KS) { SYM(B, W0, W1, NST, KS, false, xh, (const float*)nullptr, O, d, k * fall); SYM(B, W0, W1, NST, KS, true, O, d, P, pd, 0); }
+#define APP1(B, W0, W1, NST, KS, FIN) DDL_KLAUNCH((ortho_apply_kernel<B, B, W0, W1, NST, KS, FIN>), dim3((unsigned)napp), dim3(KS * W0 * W1 * 64), 0, stream, t, mu, P, pd, xh, xl, yh, yl, ex, k * fall, (k + 1) * fall)
+#define APP(B, W0, W1, NST, KS) { if (fin == 0) APP1(B, W0, W1, NST, KS, 0); else if (fin == 1) APP1(B, W0, W1, NST, KS, 1); else APP1(B, W0, W1, NST, KS, 2); }
+        if (sb == 64 && nsym <= 256) SYMS(64, 2, 2, 3, 2)
+        else if (sb == 64) SYMS(64, 2, 2, 3, 1)
+        else if (sb == 128) SYMS(128, 2, 4, 2, 1)
+        else SYMS(256, 2, 4, 2, 1)
+        if (ab == 64 && napp <= 256) APP(64, 2, 2, 3, 2)
+        else if (ab == 64) APP(64, 2, 2, 3, 1)
+        else if (ab == 128) APP(128, 2, 4, 2, 1)
+        else APP(256, 2, 4, 2, 1)
         f16_t* s = xh; xh = yh; yh = s;
         s = xl; xl = yl; yl = s;
     }
@@ -1088,17 +1355,18 @@ extern "C" int ddl_ortho_coefficients_ok(float a, float b, float c, int steps) {
 // bytes of workspace of a call with these groups (`desc`: count x 11 int64: source address, its batch / row / column
 // strides, destination address and strides, rows, columns, matrices), -1: sizes out of range
 extern "C" long long ddl_ortho_workspace(const long long* desc, int count) {
-    Plan pl;
-    return plan_of((const Desc*)desc, count, pl) ? pl.bytes : -1;
+    Plan one, other;               // (which of the forms is taken depends on the steps too)
+    if (!plan_of((const Desc*)desc, count, true, one) || !plan_of((const Desc*)desc, count, false, other)) return -1;
+    return one.bytes > other.bytes ? one.bytes : other.bytes;
 }
 
 // kind 0 / 1: fp32 / bf16 sources; destinations are bf16
 extern "C" int ddl_orthogonalize(const long long* desc, int count, int kind, float a, float b, float c, int steps, float eps, void* ws,
                                  long long ws_bytes, hipStream_t stream) {
     if (count == 0) return DDL_OK;
-    Plan pl;
     const Desc* q = (const Desc*)desc;
-    if (kind < 0 || kind > 1 || !ws || !plan_of(q, count, pl) || ws_bytes < pl.bytes) return DDL_EINVAL;
+    const long long need = ddl_ortho_workspace(desc, count);
+    if (kind < 0 || kind > 1 || !ws || need < 0 || ws_bytes < need) return DDL_EINVAL;
     if (!ddl_ortho_coefficients_ok(a, b, c, steps) || !(eps >= 1e-30f)) return DDL_EINVAL;
     if (reinterpret_cast<uintptr_t>(ws) & 255) return DDL_EALIGN;
     for (int i = 0; i < count; ++i)
@@ -1115,9 +1383,9 @@ extern "C" int ddl_muon_step(const long long* desc, int count, void* w, const vo
                              float wd, int nesterov, const void* lr_scale, float a, float b, float c, int steps, float eps, void* ws,
                              long long ws_bytes, hipStream_t stream) {
     if (count == 0) return DDL_OK;
-    Plan pl;
     const Desc* q = (const Desc*)desc;
-    if (!w || !g || !v || !ws || !plan_of(q, count, pl) || ws_bytes < pl.bytes) return DDL_EINVAL;
+    const long long need = ddl_ortho_workspace(desc, count);
+    if (!w || !g || !v || !ws || need < 0 || ws_bytes < need) return DDL_EINVAL;
     if (!ddl_ortho_coefficients_ok(a, b, c, steps) || !(eps >= 1e-30f)) return DDL_EINVAL;
     if ((reinterpret_cast<uintptr_t>(ws) & 255) || !ddl_aligned16(w) || !ddl_aligned16(g) || !ddl_aligned16(v) || (lowp && !ddl_aligned16(lowp)))
         return DDL_EALIGN;

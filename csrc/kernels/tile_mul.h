@@ -39,23 +39,44 @@ struct MulI8 {
     static __device__ __forceinline__ acc mma(frag a, frag b, acc c) { return __builtin_amdgcn_mfma_i32_16x16x64_i8(a, b, c, 0, 0, 0); }
 };
 
-template <typename OP, int BF, int BS, int W0, int W1, int NST, bool TRF>
+// KS = 2: two such groups of waves with stages of their own take half of the sum each and are added at the end - a tile
+// that has a CU to itself is bound by the latency of its stages, one after another, not by their bytes.
+template <typename OP, int BF, int BS, int W0, int W1, int NST, bool TRF, int KS = 1>
 struct TileMul {
     typedef typename OP::frag frag;
     typedef typename OP::acc vec;
-    static constexpr int WAVES = W0 * W1, THREADS = WAVES * 64;
-    static constexpr int FBYTES = BF * 128, SBYTES = BS * 128, STAGE = FBYTES + SBYTES;
+    static constexpr int WAVES = W0 * W1, THREADS = KS * WAVES * 64;
+    static constexpr int FBYTES = BF * 128, SBYTES = BS * 128, STAGE = FBYTES + SBYTES, LDS = KS * NST * STAGE;
     static constexpr int FL = BF / 8 / WAVES, SL = BS / 8 / WAVES, L = FL + SL;         // LDS-DMA instructions of a wave and stage
     static constexpr int NF = BF / W0 / 16, NS = BS / W1 / 16;                          // fragments of a wave
     static_assert(FL * 8 * WAVES == BF && SL * 8 * WAVES == BS, "whole instructions");
-    static_assert(NST >= 2 && NST * STAGE <= 160 * 1024, "LDS");
+    static_assert(NST >= 2 && LDS <= 160 * 1024 && KS <= 2, "LDS");
     vec acc[NF][NS];
 
+    static __device__ __forceinline__ u32x4 uniform(u32x4 r) {               // (it is: tells the compiler so)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) r[i] = __builtin_amdgcn_readfirstlane(r[i]);
+        return r;
+    }
+    static __device__ __forceinline__ unsigned behind(unsigned bytes, unsigned by) { return bytes > by ? bytes - by : 0u; }
     // f: first row (TRF: first column) of the tile, ldf bytes from a row to the next, fleft rows (columns) that exist, fbytes: what
-    // may be read from f on (behind it and behind the rows that exist: zeros); s likewise; KT stages.  All offsets < 2^31.
+    // may be read from f on (behind it and behind the rows that exist: zeros); s likewise; `total` stages.  All offsets < 2^31.
     __device__ __forceinline__ void run(unsigned char* smem, const void* f, unsigned ldf, int fleft, unsigned fbytes, const void* s, unsigned lds, int sleft,
-                                        unsigned sbytes, int KT) {
-        const int tid = threadIdx.x, lane = tid & 63, wid = __builtin_amdgcn_readfirstlane(tid >> 6), w0 = wid / W1, w1 = wid % W1;
+                                        unsigned sbytes, int total) {
+        int KT = total;
+        const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), wid = wave % WAVES, w0 = wid / W1, w1 = wid % W1;
+        int live = KT;                                                         // stages of this group that exist
+        if (KS == 2) {
+            live = KT = (KT + 1) >> 1;
+            if (wave >= WAVES) {
+                live = total - KT;
+                smem += NST * STAGE;
+                f = (const char*)f + (size_t)KT * (TRF ? ldf * 64u : 128u);
+                s = (const char*)s + (size_t)KT * 128u;
+                fbytes = behind(fbytes, KT * (TRF ? ldf * 64u : 128u));
+                sbytes = behind(sbytes, KT * 128u);
+            }
+        }
         const int fr = lane & 15, fq = lane >> 4;
         const unsigned lds0 = (unsigned)(uintptr_t)(__attribute__((address_space(3))) void*)smem;
         unsigned vo[L];
@@ -76,12 +97,13 @@ struct TileMul {
             const int slot = (i * WAVES + wid) * 64 + lane, row = slot >> 3, c = (slot & 7) ^ ((row >> 1) & 7);
             vo[FL + i] = row < sleft ? row * lds + c * 16 : OUT;
         }
-        const u32x4 rf = raw_rsrc(f, fbytes), rs = raw_rsrc(s, sbytes);
+        const u32x4 rf = uniform(raw_rsrc(f, fbytes)), rs = uniform(raw_rsrc(s, sbytes));
         const unsigned fstep = TRF ? ldf * 64u : 128u;                         // bytes from a tile to the next
         // every stage is exactly L instructions a wave (behind the end: the last tile again): the counted waits rely on it
         auto piece = [&](unsigned kt, unsigned at, int i) {                    // at: LDS address of the wave's part of the stage
-            if (i < FL) lds_dma16(rf, at + i * WAVES * 1024, vo[i], kt * fstep);
-            else lds_dma16(rs, at + FBYTES + (i - FL) * WAVES * 1024, vo[i], kt * 128u);
+            const unsigned o = KS == 1 || (int)kt < live ? vo[i] : OUT;        // (the second group may have a stage less: zeros)
+            if (i < FL) lds_dma16(rf, at + i * WAVES * 1024, o, kt * fstep);
+            else lds_dma16(rs, at + FBYTES + (i - FL) * WAVES * 1024, o, kt * 128u);
         };
         // a fragment's offset in a stage, half h: i-th of f at fbase[h] + 2048 i (TRF: foff[i] + 64 BF h), of s at sbase[h] + 2048 j
         int fbase[2], sbase[2], foff[NF];
@@ -168,20 +190,33 @@ struct TileMul {
     // The epilogues go through LDS (32-bit values, rows of S, 16-byte chunk q of row s at q ^ fold(s)): whole rows are read back and
     // written, and their loops stay rolled - a tile's code runs once, so its length is paid for in instruction fetches
     // (an unrolled epilogue of 8 KB took 4 us).  PASSES parts of BS / PASSES rows where the tile is larger than the stages.
-    static constexpr int PASSES = BF * BS * 4 > NST * STAGE ? BF * BS * 4 / (NST * STAGE) : 1;
-    static_assert(NS % PASSES == 0, "whole fragments a pass");
+    static constexpr int PASSES = BF * BS * 4 > LDS ? BF * BS * 4 / LDS : 1;
+    static_assert(NS % PASSES == 0 && (KS == 1 || PASSES == 1), "whole fragments a pass");
     static constexpr int ROWS = BS / PASSES;       // rows of a pass: those of fragments j with j / (NS / PASSES) == pass of every wave
     __device__ __forceinline__ void to_lds(void* t, int pass) const {
-        const int lane = threadIdx.x & 63, wid = threadIdx.x >> 6, w0 = wid / W1, w1 = wid % W1;
+        const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wid = wave % WAVES, w0 = wid / W1, w1 = wid % W1;
         const int s0 = w1 * (ROWS / W1) + (lane & 15), f0 = w0 * (BF / W0 / 4) + (lane >> 4);
+        auto place = [&](int i, int j) { return reinterpret_cast<vec*>((unsigned*)t + (s0 + j * 16) * BF + (((f0 + i * 4) ^ fold(s0 + j * 16)) * 4)); };
+        if (KS == 2) {
+            if (wave >= WAVES) {
+#pragma unroll
+                for (int j = 0; j < NS; ++j)
+#pragma unroll
+                    for (int i = 0; i < NF; ++i) *place(i, j) = acc[i][j];
+            }
+            __syncthreads();
+            if (wave >= WAVES) return;
+        }
 #pragma unroll
         for (int p = 0; p < PASSES; ++p)
             if (p == pass)
 #pragma unroll
                 for (int j = 0; j < NS / PASSES; ++j)
 #pragma unroll
-                    for (int i = 0; i < NF; ++i)
-                        *reinterpret_cast<vec*>((unsigned*)t + (s0 + j * 16) * BF + (((f0 + i * 4) ^ fold(s0 + j * 16)) * 4)) = acc[i][p * (NS / PASSES) + j];
+                    for (int i = 0; i < NF; ++i) {
+                        if (KS == 2) *place(i, j) += acc[i][j];
+                        else *place(i, j) = acc[i][p * (NS / PASSES) + j];
+                    }
     }
     static __device__ __forceinline__ int fold(int s) { return (s ^ (s >> 3)) & 15; }     // rows 1 apart and rows 8 apart on different banks
     // row of the tile that row `s` of a pass holds

@@ -145,3 +145,44 @@ def test_int8_head_answers_on_the_gpu():
     from distributeddeeplearning_amd.ops import functional as ops
 
     check(got, seen[0], *ops.quantize_int8(w.detach()), b.detach())
+
+
+# tiles of 128 (256 of them or more); the last sizes that a workgroup's LDS takes whole, and the next
+@pytest.mark.parametrize("dtype", [torch.float32, BF], ids=["fp32", "bf16"])
+@pytest.mark.parametrize("m, n, k", [(2100, 2100, 200), (9000, 500, 130), (16, 300, 2432), (16, 300, 2560), (1, 200, 40832), (1, 200, 41000), (15, 77, 100),
+                                     (1030, 1000, 128), (1024, 1024, 1), (600, 600, 129)])
+def test_borders_between_the_forms(m, n, k, dtype):
+    from distributeddeeplearning_amd.ops import functional as ops
+
+    x, q, s, b = make(m, n, k, dtype, k, bias=n % 3 != 0)
+    check(ops.linear_int8(x, q, s, b), x, q, s, b)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, BF], ids=["fp32", "bf16"])
+@pytest.mark.parametrize("m", [1, 6, 16, 40])
+def test_unaligned_rows(m, dtype):
+    from distributeddeeplearning_amd.ops import functional as ops
+
+    x, q, s, b = make(m, 50, 700, dtype, 9)
+    wide = torch.full((2 * m, 1003), float("nan"), device=DEV, dtype=dtype)
+    for at in (1, 3, 8):
+        v = wide[::2, at:at + 700]
+        v.copy_(x)
+        check(ops.linear_int8(v, q, s, b), x, q, s, b)
+        assert torch.equal(ops.quantize_int8(v)[0], ops.quantize_int8(x)[0])
+    every = torch.full((m, 1400), float("nan"), device=DEV, dtype=dtype)
+    every[:, ::2] = x
+    check(ops.linear_int8(every[:, ::2], q, s, b), x, q, s, b)
+
+
+def test_a_row_out_of_range_leaves_the_others():
+    from distributeddeeplearning_amd.ops import functional as ops
+
+    for m in (4, 16, 100, 2200):
+        x, q, s, b = make(m, 2100, 260, BF, 5)
+        want = ops.linear_int8(x, q, s, b)
+        x[m // 2, 259] = float("inf")
+        got = ops.linear_int8(x, q, s, b)
+        assert got[m // 2].isnan().all()
+        got[m // 2] = want[m // 2]
+        assert torch.equal(got, want)

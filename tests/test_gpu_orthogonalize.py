@@ -280,3 +280,179 @@ def test_muon_step_in_a_captured_graph_is_the_eager_step():
     graphed, b = _train(False, graphed=True)
     assert graphed.graphed
     assert torch.equal(a.master[BF], b.master[BF]) and torch.equal(a.momentum_buf[BF], b.momentum_buf[BF])
+
+
+# ------------------------------------------------------------------------------------------ each of the kernels' forms
+# A workgroup a matrix, the Gram matrix's steps (all up to 32 rows), tiles: sizes on both sides of their borders.
+# Up to 32 rows the steps are fp64; the matrix that they make (entries up to 3.4445^5 = 485) is rounded to fp32 and multiplied with
+# fp32 values in sums of 32 terms: 34 * 2^-24 * 485 = 2^-10 at most, and the rounding to bf16.
+TOL_THIN = 2 ** -8 + 2 ** -10
+THIN = [(1, 513), (1, 3157), (5, 100001), (16, 2304), (17, 2762), (2762, 17), (31, 1000), (32, 520), (700, 32), (32, 8193)]
+
+
+@pytest.mark.parametrize("kind", ["gauss", "power", "exp", "rank1", "lowrank"])
+@pytest.mark.parametrize("shape", THIN, ids=str)
+def test_few_rows(shape, kind):
+    from distributeddeeplearning_amd.ops import functional as ops
+
+    for dtype in (torch.float32, BF):
+        g = spectrum(kind, *shape, seed=7).to(DEV, dtype)
+        assert off(ops.orthogonalize(g), g) < TOL_THIN
+
+
+def test_few_rows_stacks_strides_and_lists():
+    from distributeddeeplearning_amd.ops import functional as ops
+
+    stack = spectrum("gauss", 21 * 9, 1400, 1).to(DEV).view(9, 21, 1400)
+    for s in (stack, stack.transpose(1, 2), stack[::3, 2:, 1::2], stack[:1].expand(4, 21, 1400)):
+        out = ops.orthogonalize(s)
+        for k in range(s.shape[0]):
+            assert off(out[k], s[k]) < TOL_THIN
+    mats = [spectrum("gauss", 1 + i % 32, 513 + 37 * i, i).to(DEV) for i in range(80)]       # more than one call's groups
+    for m, o in zip(mats, ops.orthogonalize([m.t() if i % 2 else m for i, m in enumerate(mats)])):
+        assert off(o if o.shape == m.shape else o.t(), m) < TOL_THIN
+
+
+@pytest.mark.parametrize("shape", [(32, 512), (33, 512), (64, 512), (64, 513), (65, 256), (128, 256), (128, 260), (129, 129), (200, 1111), (321, 4500)], ids=str)
+@pytest.mark.parametrize("kind", ["gauss", "exp", "lowrank"])
+def test_borders_between_the_forms(shape, kind):
+    from distributeddeeplearning_amd.ops import functional as ops
+
+    g = spectrum(kind, *shape, seed=8).to(DEV)
+    assert off(ops.orthogonalize(g), g) < TOL
+    assert off(ops.orthogonalize(g.t()), g.t()) < TOL
+
+
+FORMS = [(40, 90), (20, 700), (200, 300)]
+
+
+@pytest.mark.parametrize("shape", FORMS, ids=str)
+@pytest.mark.parametrize("scale", [1e-30, 1e-12, 1e30])
+def test_magnitudes_in_each_form(shape, scale):
+    from distributeddeeplearning_amd.ops import functional as ops
+
+    g = (spectrum("gauss", *shape, 3) * scale).to(DEV)
+    assert off(ops.orthogonalize(g, eps=1e-20), g, eps=1e-20) < TOL
+
+
+@pytest.mark.parametrize("shape", FORMS, ids=str)
+def test_matrices_do_not_touch_each_other_in_each_form(shape):
+    from distributeddeeplearning_amd.ops import functional as ops
+
+    clean = [spectrum("gauss", *shape, i).to(DEV) for i in range(4)]
+    want = ops.orthogonalize(clean)
+    bad = [m.clone() for m in clean]
+    bad[1][3, 4] = float("nan")
+    bad[2][-1, -1] = float("inf")
+    bad.insert(1, torch.zeros(shape, device=DEV))
+    got = ops.orthogonalize(bad)
+    assert torch.equal(got[0], want[0]) and torch.equal(got[4], want[3])
+    assert not got[1].any() and got[2].isnan().all() and got[3].isnan().all()
+
+
+@pytest.mark.parametrize("shape", FORMS, ids=str)
+@pytest.mark.parametrize("steps, coef", [(1, (3.4445, -4.7750, 2.0315)), (7, (3.4445, -4.7750, 2.0315)), (10, (2.0, -1.5, 0.5)), (3, (1.5, -0.5, 0.0))])
+def test_steps_and_coefficients_in_each_form(shape, steps, coef):
+    from distributeddeeplearning_amd.ops import functional as ops
+
+    g = spectrum("gauss", *shape, 2).to(DEV)
+    assert off(ops.orthogonalize(g, steps=steps, coefficients=coef), g, steps=steps, coef=coef) < 2 ** -8 + 3 * steps * 2 ** -11
+
+
+def on_the_card(g, steps=5):
+    """The steps themselves in 64 bits, for sizes whose singular values take too long."""
+    x = g.double()
+    x = x / x.norm()
+    a, b, c = 3.4445, -4.7750, 2.0315
+    x = x.t().contiguous() if x.shape[0] > x.shape[1] else x
+    for _ in range(steps):
+        aa = torch.mm(x, x.t().contiguous())
+        x = a * x + torch.mm(b * aa + c * torch.mm(aa, aa), x)
+    return x if x.shape == g.shape else x.t()
+
+
+# tiles of 128 in P X; of 128 in A and A^2 too; of 256 in all (odd sizes; tall)
+@pytest.mark.parametrize("shapes", [[(2040, 2001)], [(2048, 4096), (4001, 2000), (1000, 4090)], [(4000, 8100)], [(8191, 4001)]], ids=str)
+def test_larger_tiles(shapes):
+    from distributeddeeplearning_amd.ops import functional as ops
+
+    gen = torch.Generator(DEV).manual_seed(4)
+    mats = [torch.randn(s, generator=gen, device=DEV) * torch.logspace(0, -4, s[1], device=DEV) for s in shapes]
+    for m, o in zip(mats, ops.orthogonalize(mats)):
+        want = on_the_card(m)
+        assert float((o.double() - want).norm() / want.norm()) < TOL
+
+
+@pytest.mark.parametrize("shapes", [[(8, 16), (64, 300), (300, 64), (100, 250), (127, 127), (1, 1)], [(16, 3, 7, 7), (16, 64, 3, 3), (700, 30), (5, 2000)],
+                                    [(4000, 8100)]], ids=["small", "few-rows", "large"])
+@pytest.mark.parametrize("dtype", [BF, torch.float32], ids=["bf16", "fp32"])
+def test_muon_in_each_form(shapes, dtype):
+    from distributeddeeplearning_amd.optim import FusedMuon
+
+    large = max(max(s) for s in shapes) > 4000
+    named = _params(shapes if large else shapes * 12, dtype)
+    opt = FusedMuon(named, lr=0.02, momentum=0.9, weight_decay=0.05)
+    ref = {n: p.detach().double().clone() for n, p in named}
+    vel = {n: torch.zeros_like(w) for n, w in ref.items()}
+    change = {n: 0.0 for n in ref}
+    for step in range(2):
+        gen = torch.Generator(DEV).manual_seed(step)
+        for n, p in named:
+            p.grad.copy_(1e-3 * torch.randn(p.shape, generator=gen, device=DEV))
+            before, g = ref[n].clone(), p.grad.double()
+            vel[n].mul_(0.9).add_(g)
+            u = (g + 0.9 * vel[n]).flatten(1)
+            o = (on_the_card(u) if large else oracle(u.cpu()).to(DEV)).reshape(g.shape)
+            ref[n].mul_(1 - 0.02 * 0.05).sub_(o, alpha=0.02 * max(1.0, u.shape[0] / u.shape[1]) ** 0.5)
+            change[n] += float((ref[n] - before).norm())
+        opt.step()
+    for seg in opt.arena.plans[dtype].segments:
+        w = opt._weights(dtype)[seg.offset:seg.offset + seg.numel].double()
+        r = ref[seg.name]
+        r = (r.permute(0, 2, 3, 1) if r.dim() == 4 else r).reshape(-1)
+        assert float((w - r).norm()) <= 15 * 2 ** -11 * change[seg.name] + 9 * 2 ** -24 * float(r.norm()) + 1e-12, seg.name
+
+
+def test_captured_in_each_form():
+    from distributeddeeplearning_amd.ops import functional as ops
+
+    xs = [torch.randn(s, device=DEV) for s in FORMS + [(3, 31, 600), (1030, 2050)]]
+    graphs, outs = [], []
+    for x in xs:
+        ops.orthogonalize(x)
+    torch.cuda.synchronize()
+    for x in xs:
+        gr = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(gr):
+            outs.append(ops.orthogonalize(x))
+        graphs.append(gr)
+    side = torch.cuda.Stream()
+    for rep in range(4):
+        for x in xs:
+            x.copy_(torch.randn(x.shape, generator=torch.Generator().manual_seed(rep)))
+        for gr in graphs if rep % 2 else graphs[::-1]:
+            gr.replay()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            eager = [ops.orthogonalize(x) for x in xs]
+        torch.cuda.current_stream().wait_stream(side)
+        torch.cuda.synchronize()
+        for o, e in zip(outs, eager):
+            assert torch.equal(o, e)
+
+
+def test_trained_with_muon_and_served_with_the_8_bit_head():
+    """Both together, as a user has them: some steps, then answers from the head's codes of the trained weights."""
+    from tests.test_int8_linear import check
+    from distributeddeeplearning_amd.ops import functional as ops
+
+    step, opt = _train(False)
+    model = step.model.eval()
+    x = torch.randn(5, 3, 64, 64, device=DEV).to(BF).contiguous(memory_format=torch.channels_last)
+    seen = []
+    with torch.no_grad():
+        model.fc.register_forward_hook(lambda mod, args, out: seen.append(args[0]))
+        model(x)
+        w, b = model.fc.weight.detach().clone(), model.fc.bias.detach().clone()
+        got = model.int8_head()(x)
+    check(got, seen[0], *ops.quantize_int8(w), b)
