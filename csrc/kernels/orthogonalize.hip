@@ -10,8 +10,9 @@
 //   * X is a pair of fp16 values hi + lo; products read hi, the term a X reads both;
 //   * the diagonals of A and P stay in fp32 (near the end A is close to a multiple of 1: its diagonal carries all of
 //     its rounding): with A = D + O,  A^2 = O^2 + (d_i + d_j) O + D^2, and P X = (a + diag P) X + offdiag(P) X_hi.
-// Against 64 bits the result is 2e-4 .. 1e-3 off (2-norm; Gaussian, power-law, exponential, low-rank and gradient-like
-// spectra), below half a bf16 step (1.7e-3 on average); bf16 operands throughout give 8e-3 .. 0.3, plain fp16 1e-3 .. 4e-2.
+// Against 64 bits the result is, before its rounding to bf16 (1.7e-3 itself), 2e-4 .. 7e-4 off on Gaussian and power-law spectra,
+// 1e-3 .. 2.2e-3 on exponential ones (six decades), 1.6e-3 .. 3.1e-3 where all but a sixteenth of the singular values are a
+// thousandth (2-norm); bf16 operands throughout give 8e-3 .. 0.3, plain fp16 1e-3 .. 4e-2.
 //
 // A call takes up to 64 groups of equal matrices; all of them share each launch.  Three forms, by sizes alone:
 //   * every matrix of up to 64 x 512 or 128 x 256: a workgroup a matrix, one launch (ortho_small_kernel);
