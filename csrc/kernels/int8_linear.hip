@@ -226,6 +226,16 @@ constexpr int SKINNY = 16, SKINNY_LDS = 40 * 1024;
 bool skinny(long long M, int K) { return M <= SKINNY && M * ((K + 127LL) / 128 * 128 + 16) <= SKINNY_LDS; }
 bool rows_vec(const void* x, int bf16, long long ldx) { return ddl_aligned16(x) && ldx % (bf16 ? 8 : 4) == 0; }
 
+// (a launch's threads are counted in 32 bits: 2^24 rows at a time)
+template <typename T>
+void launch_rows(const T* x, long long ldx, long long M, int K, int Kp, int vec, signed char* q, float* scale, hipStream_t stream) {
+    constexpr long long AT_ONCE = 1LL << 24;
+    for (long long m = 0; m < M; m += AT_ONCE) {
+        const int rows = (int)(M - m < AT_ONCE ? M - m : AT_ONCE);
+        DDL_KLAUNCH(int8_rows_kernel<T>, dim3((rows + 3) / 4), dim3(256), 0, stream, x + m * ldx, ldx, rows, K, Kp, vec, q + m * Kp, scale + m);
+    }
+}
+
 template <typename T>
 int run(const T* x, long long ldx, const signed char* q, long long ldq, long long q_bytes, const float* s, const float* bias, T* y, long long ldy, int M, int N,
         int K, char* ws, hipStream_t stream) {
@@ -237,12 +247,12 @@ int run(const T* x, long long ldx, const signed char* q, long long ldq, long lon
     }
     signed char* xq = (signed char*)ws;
     float* sx = (float*)(ws + ((long long)M * Kp + 255) / 256 * 256);
-    DDL_KLAUNCH(int8_rows_kernel<T>, dim3((M + 3) / 4), dim3(256), 0, stream, x, ldx, M, K, Kp, vec, xq, sx);
     // 128 x 128 tiles, two a CU, unless they are fewer than the CUs; two groups of waves a tile where even 64 x 64 are.  (256 x 256 in 8 waves is no faster where it fills whole rounds,
     // 4096^3 in 100 / 101 us, and 12 544 x 4096 x 4096 takes 4 rounds for 3.06: 333 / 304 us.  256 x 128: 328; 4 waves of 128 x 128:
     // 396, copies between register halves.)
     const long long t128 = ((M + 127LL) / 128) * ((N + 127) / 128), t64 = ((M + 63LL) / 64) * ((N + 63) / 64);
-    if ((t64 + 7) / 8 * 8 > 0x7fffffffLL) return DDL_EINVAL;
+    if (t128 > 0xffffffLL - 8) return DDL_EINVAL;
+    launch_rows(x, ldx, M, K, Kp, vec, xq, sx, stream);
 #define GEMM(B, W0, W1, NST, KS, t) DDL_KLAUNCH((int8_gemm_kernel<T, B, W0, W1, NST, KS>), dim3((unsigned)((t + 7) / 8 * 8)), dim3(KS * W0 * W1 * 64), 0, stream, xq, sx, q, \
                                             ldq, q_bytes, s, bias, y, ldy, M, N, Kp, (M + B - 1) / B, (N + B - 1) / B)
     if (t128 >= 256) GEMM(128, 2, 2, 2, 1, t128);
@@ -260,9 +270,8 @@ extern "C" int ddl_int8_rows(const void* x, int x_bf16, long long ldx, long long
     if (!x || !q || !scale || M < 0 || M > 0x7fffff00LL || K <= 0 || Kp < K || Kp % 16 || ldx < 0) return DDL_EINVAL;
     if (!ddl_aligned16(q)) return DDL_EALIGN;
     const int vec = rows_vec(x, x_bf16, ldx);
-    const dim3 grid((unsigned)((M + 3) / 4)), block(256);
-    if (x_bf16) DDL_KLAUNCH(int8_rows_kernel<bf16_t>, grid, block, 0, stream, (const bf16_t*)x, ldx, (int)M, K, Kp, vec, (signed char*)q, (float*)scale);
-    else DDL_KLAUNCH(int8_rows_kernel<float>, grid, block, 0, stream, (const float*)x, ldx, (int)M, K, Kp, vec, (signed char*)q, (float*)scale);
+    if (x_bf16) launch_rows((const bf16_t*)x, ldx, M, K, Kp, vec, (signed char*)q, (float*)scale, stream);
+    else launch_rows((const float*)x, ldx, M, K, Kp, vec, (signed char*)q, (float*)scale, stream);
     return ddl_launch_status();
 }
 

@@ -1018,6 +1018,9 @@ __global__ void __launch_bounds__(256) ortho_thin_apply_kernel(const Table* __re
 // one group as the callers describe it: 11 int64 values
 struct Desc { long long src, sb, srs, scs, dst, db, drs, dcs, r, c, batch; };
 
+// most workgroups of a launch: their threads are counted in 32 bits
+constexpr long long most_wgs(int threads) { return 0xffffffffLL / threads; }
+
 struct Plan {
     long long x_elems = 0, a_elems = 0, d_elems = 0, parts = 0, mats = 0;
     long long table, xa_h, xa_l, xb_h, xb_l, o, p, d, pd, part, ex, bytes;
@@ -1058,7 +1061,7 @@ bool plan_of(const Desc* q, int count, bool thin, Plan& pl) {
         pl.mats += s.batch;
         const long long pe = part_elems_of(s.r * s.c);
         pl.parts += s.batch * ((s.r * s.c + pe - 1) / pe);
-        if (pl.x_elems > (1LL << 37) || pl.d_elems > 0x7fffffffLL || pl.parts > 0x7fffffffLL) return false;
+        if (pl.x_elems > (1LL << 37) || pl.d_elems > 0x7fffffffLL || pl.parts >= most_wgs(1024) || pl.mats > most_wgs(512)) return false;
     }
     auto up = [](long long b) { return (b + 255) / 256 * 256; };
     long long at = 0;
@@ -1068,7 +1071,7 @@ bool plan_of(const Desc* q, int count, bool thin, Plan& pl) {
             const long long m = q[i].r > q[i].c ? q[i].r : q[i].c, w = thin_cols(m);
             pl.slabs += q[i].batch * ((m + w - 1) / w);
         }
-        if (pl.slabs > 0x7fffffffLL) return false;
+        if (pl.slabs > most_wgs(256)) return false;
         pl.part = at; at += up(pl.parts * 8);
         pl.o = at; at += up(pl.slabs * pl.thin * pl.thin * 8);
         pl.p = at; at += up(pl.mats * pl.thin * pl.thin * 4);
@@ -1238,7 +1241,6 @@ int run_small(const Desc* q, int count, int kind, const Muon& mu, float a, float
             o.np = (int)pad64(s.r < s.c ? s.r : s.c); o.mp = (int)pad64(s.r < s.c ? s.c : s.r);
             o.fin = (unsigned)grid;
             grid += s.batch;
-            if (grid > 0x7fffffffLL) return DDL_EINVAL;
         }
     }
     return DDL_OK;
@@ -1280,10 +1282,11 @@ int run_all(const Desc* q, int count, int kind, const Muon& mu, float a, float b
         nin += s.batch * parts; nio += s.batch * (pl.thin ? o.chunks : (np / 64) * (mp / 64));
         nsym += s.batch * o.tsym; napp += s.batch * o.tapp;
         xo += s.batch * np * mp; ao += s.batch * np * np; dof += s.batch * np; po += s.batch * parts; mat += s.batch;
-        if (nin > 0x7fffffffLL || nio > 0x7fffffffLL || nsym > 0x0fffffffLL || napp > 0x0fffffffLL) return DDL_EINVAL;
+        if (nio > most_wgs(256) || nsym > most_wgs(512) || napp > most_wgs(512)) return DDL_EINVAL;
     }
     nsym = homes(g, count, true, csym);
     napp = homes(g, count, false, capp);
+    if (nsym > most_wgs(512) || napp > most_wgs(512)) return DDL_EINVAL;
     Table* t = (Table*)(ws + pl.table);
     f16_t *xh = (f16_t*)(ws + pl.xa_h), *xl = (f16_t*)(ws + pl.xa_l), *yh = (f16_t*)(ws + pl.xb_h), *yl = (f16_t*)(ws + pl.xb_l);
     f16_t *O = (f16_t*)(ws + pl.o), *P = (f16_t*)(ws + pl.p);

@@ -307,7 +307,8 @@ class ResNet(nn.Module):
     def int8_head(self):
         """For answering: the classifier head from 8-bit weights (:class:`Int8Linear`), taken from the present ones.  The
         model no longer trains afterwards, and its ``state_dict`` holds codes and scales in the place of ``fc.weight``."""
-        self.fc = Int8Linear.from_linear(self.fc)
+        if not isinstance(self.fc, Int8Linear):
+            self.fc = Int8Linear.from_linear(self.fc)
         return self.eval()
 
 

@@ -61,12 +61,26 @@ class FusedMuon(_ArenaOptimizer):
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
-        g0 = self.param_groups[0]
-        lr, mu, wd, nesterov = g0["lr"], g0["momentum"], g0["weight_decay"], g0["nesterov"]
-        steps, coefficients, eps = g0["steps"], (g0["ortho_a"], g0["ortho_b"], g0["ortho_c"]), g0["eps"]
         from ..ops import kernels
 
         hip = self.arena.device.type == "cuda" and kernels.enabled()
+        if hip:
+            from ..ops import hip_ops
+
+            with hip_ops._on(self.arena.device):
+                self._update(hip)
+        else:
+            self._update(hip)
+        self._step += 1
+        self._notify_weights_changed(hip)
+        return loss
+
+    def _update(self, hip):
+        from ..ops import kernels
+
+        g0 = self.param_groups[0]
+        lr, mu, wd, nesterov = g0["lr"], g0["momentum"], g0["weight_decay"], g0["nesterov"]
+        steps, coefficients, eps = g0["steps"], (g0["ortho_a"], g0["ortho_b"], g0["ortho_c"]), g0["eps"]
         if hip and not kernels.ortho_coefficients_ok(*coefficients, steps):
             raise ValueError("FusedMuon: %d steps with the coefficients %r leave the range of the kernels' 16-bit operands"
                              % (steps, coefficients))
@@ -107,6 +121,3 @@ class FusedMuon(_ArenaOptimizer):
             v.mul_(mu).add_(grad)
             w.add_(grad.add(v, alpha=mu) if nesterov else v, alpha=-lr * g0["vector_lr_scale"])
             self._publish(dt, a, b)
-        self._step += 1
-        self._notify_weights_changed(hip)
-        return loss

@@ -186,3 +186,18 @@ def test_a_row_out_of_range_leaves_the_others():
         assert got[m // 2].isnan().all()
         got[m // 2] = want[m // 2]
         assert torch.equal(got, want)
+
+
+# codes of the input, its values, codes of the weights, results: each beyond 2^31 bytes or values
+@pytest.mark.parametrize("m, n, k", [(270000, 24, 8200), (17000001, 8, 128), (9, 1100000, 2048), (40, 1100000, 2048), (47000, 47000, 64)])
+def test_offsets_beyond_32_bits(m, n, k):
+    from distributeddeeplearning_amd.ops import functional as ops
+
+    gen = torch.Generator(DEV).manual_seed(6)
+    x = torch.randn(m, k, generator=gen, device=DEV, dtype=BF)
+    q, s = ops.quantize_int8(torch.randn(n, k, generator=gen, device=DEV, dtype=BF))
+    b = torch.randn(n, generator=gen, device=DEV)
+    y = ops.linear_int8(x, q, s, b)
+    rows = sorted({0, m // 2, m - 1}) if m < 100 else [0, 1, m // 3, m // 2, m - 2, m - 1]
+    cols = torch.tensor([0, 1, n // 2, n - 2, n - 1], device=DEV)
+    check(y[rows][:, cols], x[rows], q[cols], s[cols], b[cols])

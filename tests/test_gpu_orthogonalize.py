@@ -456,3 +456,19 @@ def test_trained_with_muon_and_served_with_the_8_bit_head():
         w, b = model.fc.weight.detach().clone(), model.fc.bias.detach().clone()
         got = model.int8_head()(x)
     check(got, seen[0], *ops.quantize_int8(w), b)
+
+
+# stacks of more than 2^31 values, in each form: the last matrix is the one that it is alone (another form's launch for the tiles
+# of a large one: both within the tolerance)
+@pytest.mark.parametrize("shape", [(300000, 64, 128), (70000, 32, 1024), (140000, 130, 120)], ids=str)
+def test_offsets_beyond_32_bits(shape):
+    from distributeddeeplearning_amd.ops import functional as ops
+
+    x = torch.zeros(shape, dtype=BF, device=DEV)
+    g = spectrum("gauss", *shape[1:]).to(DEV, BF)
+    for k in (0, shape[0] // 2, shape[0] - 1):
+        x[k] = g
+    out = ops.orthogonalize(x)
+    assert not out[1].any() and not out[shape[0] - 2].any()
+    for k in (0, shape[0] // 2, shape[0] - 1):
+        assert off(out[k], g) < TOL

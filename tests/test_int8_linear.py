@@ -124,3 +124,41 @@ def test_int8_head_of_a_model():
     other.load_state_dict(model.state_dict())
     with torch.no_grad():
         assert torch.equal(other(x), got)
+
+
+def test_int8_head_twice_is_the_same_head():
+    from distributeddeeplearning_amd.models import resnet18
+
+    model = resnet18(num_classes=12).int8_head()
+    head = model.fc
+    assert model.int8_head().fc is head
+
+
+def test_arguments_that_the_kernels_refuse():
+    """The library's own checks: before anything is launched, so they need no GPU."""
+    import ctypes as c
+
+    from distributeddeeplearning_amd.ops import kernels, native
+
+    if not native.kernels_available():
+        pytest.skip("kernel library not built")
+    lib = kernels.lib()
+
+    def rows(x=64, ldx=64, m=4, k=64, kp=64, q=64, scale=64):
+        return lib.ddl_int8_rows(c.c_void_p(x), c.c_int(1), c.c_longlong(ldx), c.c_longlong(m), c.c_int(k), c.c_int(kp), c.c_void_p(q), c.c_void_p(scale),
+                                 c.c_void_p(0))
+
+    for kw in (dict(x=0), dict(q=0), dict(scale=0), dict(m=-1), dict(m=1 << 31), dict(k=0), dict(kp=48), dict(kp=72), dict(ldx=-1), dict(q=72)):
+        assert rows(**kw) != 0, kw
+    assert rows(m=0) == 0
+
+    def product(x=64, ldx=64, q=64, ldq=64, q_bytes=640, s=64, bias=0, y=64, ldy=10, m=20, n=10, k=64, ws=256, nbytes=1 << 40):
+        return lib.ddl_int8_linear(c.c_void_p(x), c.c_int(1), c.c_longlong(ldx), c.c_void_p(q), c.c_longlong(ldq), c.c_longlong(q_bytes), c.c_void_p(s),
+                                   c.c_void_p(bias), c.c_void_p(y), c.c_longlong(ldy), c.c_longlong(m), c.c_int(n), c.c_int(k), c.c_void_p(ws),
+                                   c.c_longlong(nbytes), c.c_void_p(0))
+
+    for kw in (dict(x=0), dict(q=0), dict(s=0), dict(y=0), dict(m=-1), dict(m=1 << 31), dict(n=-1), dict(k=0), dict(k=133145, ldq=133152, q_bytes=1 << 40),
+               dict(ldq=48), dict(ldq=72), dict(ldq=1 << 22, q_bytes=1 << 40), dict(q=72), dict(y=72), dict(ws=64), dict(ws=0), dict(nbytes=100),
+               dict(q_bytes=639), dict(ldy=9), dict(ldx=-1), dict(m=1 << 30, n=1 << 30, ldy=1 << 30, q_bytes=1 << 50)):
+        assert product(**kw) != 0, kw
+    assert product(m=0) == 0 and product(n=0) == 0

@@ -140,3 +140,42 @@ def test_state_round_trip_and_choice_by_name():
     step(b, ob, 2)
     for p, q in zip(a.parameters(), b.parameters()):
         assert torch.equal(p, q)
+
+
+def test_sizes_that_the_kernels_refuse():
+    """The library's own checks: before anything is launched, so they need no GPU."""
+    from distributeddeeplearning_amd.ops import kernels, native
+
+    if not native.kernels_available():
+        pytest.skip("kernel library not built")
+
+    def row(r, c, batch=1):
+        return (64, r * c, c, 1, 64, r * c, c, 1, r, c, batch)
+
+    for rows in ([row(0, 4)], [row(4, -1)], [row(1 << 30, 1)], [row(32768, 32769)], [row(4, 4, 0)], [row(4, 4, 1 << 23)], [row(4, 4, 1 << 40)],
+                 [row(300, 300, 1 << 21)], [row(4, 4)] * 65):
+        table, count = kernels.ortho_table(rows)
+        with pytest.raises(kernels.KernelError, match="out of range"):
+            kernels.ortho_workspace(table, count)
+    # a launch has at most 2^32 - 1 threads: of 1024 for each matrix's sums and for the table
+    table, count = kernels.ortho_table([row(4, 4, (1 << 22) - 3), row(32704, 32704)])
+    with pytest.raises(kernels.KernelError, match="out of range"):      # (the second matrix has 1024 sums)
+        kernels.ortho_workspace(table, count)
+    table, count = kernels.ortho_table([row(4, 4, (1 << 22) - 1026), row(32704, 32704)])
+    assert kernels.ortho_workspace(table, count) > 0
+    lib = kernels.lib()
+    ok = (3.4445, -4.7750, 2.0315)
+    assert kernels.ortho_coefficients_ok(*ok, 5) and not kernels.ortho_coefficients_ok(*ok, 65) and not kernels.ortho_coefficients_ok(*ok, 0)
+
+    def call(steps=5, eps=1e-7, kind=0, ws=256, nbytes=1 << 40, table=kernels.ortho_table([row(8, 8)])[0], count=1, coef=ok):
+        f = lib.ddl_orthogonalize
+        c = __import__("ctypes")
+        return f(table, c.c_int(count), c.c_int(kind), *(c.c_float(v) for v in coef), c.c_int(steps), c.c_float(eps), c.c_void_p(ws),
+                 c.c_longlong(nbytes), c.c_void_p(0))
+
+    no_source = kernels.ortho_table([(0,) + row(8, 8)[1:]])[0]
+    no_stride = kernels.ortho_table([row(8, 8)[:2] + (1 << 31,) + row(8, 8)[3:]])[0]
+    for kw in (dict(steps=0), dict(steps=65), dict(eps=0.0), dict(eps=float("nan")), dict(kind=2), dict(kind=-1), dict(ws=0), dict(ws=64), dict(nbytes=100),
+               dict(count=-1), dict(coef=(100.0, 0.0, 0.0)), dict(table=no_source), dict(table=no_stride)):
+        assert call(**kw) != 0, kw
+    assert call(count=0) == 0
