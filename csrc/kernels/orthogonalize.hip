@@ -48,7 +48,8 @@ struct Group {                      // `batch` equal matrices
     int tsym, tapp;                 // tiles of a matrix in the symmetric products and in P X
     int hsym, happ;                 // the XCD that computes them, -1: all
     unsigned fin, fio;              // first workgroup of the sums, of the packing (thin form: of the chunks)
-    int tcols, chunks;              // thin form: columns of a chunk, chunks of a matrix
+    union { int tcols; int split; };        // thin form: columns of a chunk; tiles: parts of a tile's sum in X X^T (see splits_of)
+    union { int chunks; unsigned slab; };   // thin form: chunks of a matrix; tiles: the first part's slab and counter
 };
 struct Chunk { Group g[CHUNK]; int base, n, last; };
 
@@ -59,7 +60,8 @@ struct Table {
     Group g[MAXG];
     unsigned fin[MAXG], fio[MAXG], fsym[8][MAXG], fapp[8][MAXG];
     int batch[MAXG], np[MAXG], mp[MAXG], tsym[MAXG], tapp[MAXG], hsym[MAXG], happ[MAXG];      // copies out of g: a lane a group (find_tile)
-    unsigned xo[MAXG], ao[MAXG], dof[MAXG], mat[MAXG];
+    unsigned xo[MAXG], ao[MAXG], dof[MAXG], mat[MAXG], slab[MAXG];
+    int split[MAXG];
 };
 
 __host__ __device__ __forceinline__ unsigned run_start(unsigned total, int home, int xcd) {
@@ -68,7 +70,9 @@ __host__ __device__ __forceinline__ unsigned run_start(unsigned total, int home,
 
 // One workgroup writes its chunk's groups; that of the last chunk also where the groups begin on each XCD.  1024 threads: one
 // wave a prefix sum.
-__device__ __forceinline__ void write_table(const Chunk& ch, Table* __restrict__ t) {
+__device__ __forceinline__ void write_table(const Chunk& ch, Table* __restrict__ t, unsigned* __restrict__ counters, int slabs) {
+    if (ch.last)
+        for (int i = threadIdx.x; i < slabs; i += 1024) counters[i] = 0u;
     const unsigned* from = reinterpret_cast<const unsigned*>(ch.g);
     unsigned* to = reinterpret_cast<unsigned*>(t->g + ch.base);
     for (int i = threadIdx.x; i < ch.n * (int)(sizeof(Group) / 4); i += 1024) to[i] = from[i];
@@ -85,6 +89,7 @@ __device__ __forceinline__ void write_table(const Chunk& ch, Table* __restrict__
         t->batch[lane] = g.batch; t->np[lane] = g.np; t->mp[lane] = g.mp;
         t->tsym[lane] = g.tsym; t->tapp[lane] = g.tapp; t->hsym[lane] = g.hsym; t->happ[lane] = g.happ;
         t->xo[lane] = g.xo; t->ao[lane] = g.ao; t->dof[lane] = g.dof; t->mat[lane] = live ? g.mat : 0xffffffffu;
+        t->split[lane] = g.split; t->slab[lane] = g.slab;
     }
     const int xcd = k & 7, home = k < 8 ? g.hsym : g.happ;
     const unsigned total = live ? (unsigned)g.batch * (unsigned)(k < 8 ? g.tsym : g.tapp) : 0u;
@@ -106,15 +111,16 @@ __device__ __forceinline__ int find_group(const unsigned* first, unsigned at) {
 // item of a product -> group, matrix, tile and what the product needs to know.  Every lane reads its group's values at once and
 // the one that is meant is picked afterwards: a tile waits for one load, not for two in a row.
 struct Item {
-    int gi, b, tile, np, mp;
-    unsigned xo, ao, dof, mat;
+    int gi, b, tile, np, mp, part, split;
+    unsigned xo, ao, dof, mat, slab;
     __device__ __forceinline__ bool find(const Table* t, bool sym) {      // false: this XCD has no such item
         const unsigned xcd = blockIdx.x & 7, at = blockIdx.x >> 3;
         const int lane = threadIdx.x & 63;
         const unsigned first = sym ? t->fsym[xcd][lane] : t->fapp[xcd][lane];
         const int l_tiles = sym ? t->tsym[lane] : t->tapp[lane], l_home = sym ? t->hsym[lane] : t->happ[lane];
         const int l_np = t->np[lane], l_mp = t->mp[lane], l_xo = t->xo[lane], l_ao = t->ao[lane], l_dof = t->dof[lane], l_mat = t->mat[lane];
-        const int l_batch = t->batch[lane];
+        const int l_batch = t->batch[lane], l_split = sym ? t->split[lane] : 1;
+        const unsigned l_slab = sym ? t->slab[lane] : 0u;
         gi = __builtin_amdgcn_readfirstlane(__popcll(__ballot(first <= at)) - 1);
         const unsigned tiles = __builtin_amdgcn_readlane(l_tiles, gi);
         const int home = __builtin_amdgcn_readlane(l_home, gi);
@@ -129,6 +135,15 @@ struct Item {
         if (idx >= run_start(total, home, xcd + 1)) return false;
         b = idx / tiles;
         tile = idx - b * tiles;
+        part = 0;
+        split = 1;
+        if (sym) {
+            split = __builtin_amdgcn_readlane(l_split, gi);
+            const int whole = tile / split;
+            part = tile - whole * split;
+            slab = __builtin_amdgcn_readlane(l_slab, gi) + idx - part;
+            tile = whole;
+        }
         return true;
     }
 };
@@ -184,10 +199,11 @@ __device__ __forceinline__ float direction_of(const Muon& mu, float g, float v) 
 // memory-side cache then.)
 // A chunk of groups a launch; its first workgroup writes the table for the kernels behind it.
 template <int KIND>
-__global__ void __launch_bounds__(1024) ortho_sqsum_kernel(const Chunk ch, const Muon mu, double* __restrict__ part, Table* __restrict__ t) {
+__global__ void __launch_bounds__(1024) ortho_sqsum_kernel(const Chunk ch, const Muon mu, double* __restrict__ part, Table* __restrict__ t,
+                                                           unsigned* __restrict__ counters, int slabs) {
     constexpr bool BF = KIND & 1;
     if (blockIdx.x == 0) {
-        write_table(ch, t);
+        write_table(ch, t, counters, slabs);
         return;
     }
     const unsigned wg = blockIdx.x - 1 + ch.g[0].fin;
@@ -411,23 +427,60 @@ __device__ __forceinline__ void tri_tile(int idx, int rows, int& ti, int& tj) {
 template <int B, int W0, int W1, int NST, int KS, bool SQUARE>
 __global__ void __launch_bounds__(KS * W0 * W1 * 64, B == 128 ? 4 : 2) ortho_sym_kernel(const Table* __restrict__ t, const f16_t* __restrict__ in, const float* __restrict__ din,
                                                           f16_t* __restrict__ out, float* __restrict__ dout, const int* __restrict__ ex, int down,
-                                                          float ca, float cb, float cc) {
+                                                          float ca, float cb, float cc, float* __restrict__ slabs, unsigned* __restrict__ counters) {
     typedef TileMul<MulF16, B, B, W0, W1, NST, false, KS> M;
     __shared__ __attribute__((aligned(16))) unsigned char smem[M::LDS];
     Item it;
-    if (!it.find(t, true)) return;
-    const int np = it.np, lda = np, ld = SQUARE ? np : it.mp, K = ld, b = it.b;
+    if (!it.find(t, true) || (SQUARE && it.part > 0)) return;
+    const int np = it.np, lda = np, ld = SQUARE ? np : it.mp, b = it.b;
+    const int each = SQUARE ? np / 64 : (ld / 64 + it.split - 1) / it.split, k0 = SQUARE ? 0 : it.part * each;
+    const int stages = ld / 64 - k0 < each ? ld / 64 - k0 : each;
     int ti, tj;
     tri_tile(it.tile, (np + B - 1) / B, ti, tj);
     const long long ao = (long long)it.ao * 64 + (long long)b * np * lda;
     const f16_t* src = SQUARE ? in + ao : in + (long long)it.xo * 64 + (long long)b * np * ld;
     M m;
-    m.run(smem, src + (long long)ti * B * ld, ld * 2, np - ti * B, DESC_BYTES, src + (long long)tj * B * ld, ld * 2, np - tj * B, DESC_BYTES, K / 64);
+    m.run(smem, src + (long long)ti * B * ld + k0 * 64, ld * 2, np - ti * B, DESC_BYTES, src + (long long)tj * B * ld + k0 * 64, ld * 2, np - tj * B, DESC_BYTES, stages);
     const float* d = SQUARE ? din + it.dof + (long long)b * np : nullptr;
     const float unscale = SQUARE ? USC * USC : ldexpf(USC * USC, -2 * shift_of(ex, it.mat + b, down));
     f16_t* o = out + ao;
     float* dst = dout + it.dof + (long long)b * np;
     float* tile = reinterpret_cast<float*>(smem);
+    // A part of a long sum: the workgroup that ends last adds all parts, in their order, and goes on with the tile.  The parts pass
+    // from XCD to XCD by stores and loads of the device's scope, each wave waiting for its stores before the counter is raised (a
+    // fence would write back and empty a whole L2: 316 us for 512 x 4608 in all).
+    bool joined = false;
+    if constexpr (B == 64 && !SQUARE) {
+        if (it.split > 1) {
+            typedef unsigned long long u64;
+            constexpr int PAIRS = B * B / 2;
+            __shared__ unsigned before;
+            u64* all = reinterpret_cast<u64*>(slabs + (long long)it.slab * (B * B));
+            u64* pairs = reinterpret_cast<u64*>(tile);
+            m.to_lds(tile, 0);
+            __syncthreads();
+            for (int k = threadIdx.x; k < PAIRS; k += M::THREADS)
+                __hip_atomic_store(all + it.part * PAIRS + k, pairs[k], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            __syncthreads();
+            if (threadIdx.x == 0) before = __hip_atomic_fetch_add(counters + it.slab, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            __syncthreads();
+            if (before != (unsigned)it.split - 1u) return;
+            for (int k = threadIdx.x; k < PAIRS; k += M::THREADS) {
+                float s0 = 0.f, s1 = 0.f;
+#pragma unroll 8
+                for (int p = 0; p < it.split; ++p) {
+                    const u64 v = __hip_atomic_load(all + p * PAIRS + k, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                    s0 += __uint_as_float((unsigned)v);
+                    s1 += __uint_as_float((unsigned)(v >> 32));
+                }
+                pairs[k] = (u64)__float_as_uint(s1) << 32 | __float_as_uint(s0);
+            }
+            if (threadIdx.x == 0) counters[it.slab] = 0u;          // for the next step
+            __syncthreads();
+            joined = true;
+        }
+    }
     // value (r, c) of the result from the product's
     auto value = [&](float v, int r, int c, float a, float dr, float dc) {
         v *= unscale;
@@ -440,7 +493,7 @@ __global__ void __launch_bounds__(KS * W0 * W1 * 64, B == 128 ? 4 : 2) ortho_sym
 #pragma unroll
     for (int pass = 0; pass < M::PASSES; ++pass) {
         if (M::PASSES > 1 && pass > 0) __syncthreads();
-        m.to_lds(tile, pass);
+        if (!joined) m.to_lds(tile, pass);
         __syncthreads();
         // block (tj, ti): rows c, 8 of r a thread
         for (int k = threadIdx.x; k < M::ROWS * B / 8; k += M::THREADS) {
@@ -1023,9 +1076,10 @@ constexpr long long most_wgs(int threads) { return 0xffffffffLL / threads; }
 
 struct Plan {
     long long x_elems = 0, a_elems = 0, d_elems = 0, parts = 0, mats = 0;
-    long long table, xa_h, xa_l, xb_h, xb_l, o, p, d, pd, part, ex, bytes;
+    long long table = 0, xa_h = 0, xa_l = 0, xb_h = 0, xb_l = 0, o = 0, p = 0, d = 0, pd = 0, part = 0, ex = 0, bytes = 0;
     int thin = 0;                   // padded rows of the thin form, 0: not taken
-    long long slabs = 0;
+    long long slabs = 0;            // thin form: of all chunks; tiles: of the parts of long sums
+    long long slab = 0, cnt = 0;    // (tiles)
 };
 
 long long part_elems_of(long long numel) {
@@ -1047,6 +1101,9 @@ int thin_rows(const Desc* q, int count) {
 
 // columns of a chunk: a 16-column block for each of a workgroup's waves, but 128 chunks at most
 long long thin_cols(long long m) { return (m + 8191) / 8192 * 64; }
+
+void tiles_of(const Desc* q, int count, int& sym, int& app);
+long long splits_of(const Desc* q, int count, int sym, int* split);
 
 bool plan_of(const Desc* q, int count, bool thin, Plan& pl) {
     if (count < 0 || count > MAXG || (count && !q)) return false;
@@ -1088,6 +1145,11 @@ bool plan_of(const Desc* q, int count, bool thin, Plan& pl) {
     pl.pd = at; at += up(pl.d_elems * 4);
     pl.part = at; at += up(pl.parts * 8);
     pl.ex = at; at += up(pl.mats * 4);
+    int sym, app, split[MAXG];
+    tiles_of(q, count, sym, app);
+    pl.slabs = splits_of(q, count, sym, split);
+    pl.slab = at; at += up(pl.slabs * 64 * 64 * 4);
+    pl.cnt = at; at += up(pl.slabs * 4);
     pl.bytes = at;
     return true;
 }
@@ -1190,6 +1252,41 @@ void tiles_of(const Desc* q, int count, int& sym, int& app) {
     app = a256 >= 512 && a64 >= 12 * a256 ? 256 : (a64 >= 1024 ? 128 : 64);
 }
 
+// Parts of the tiles' sums in X X^T (tiles of 64); returns the parts of all tiles that have more than one.  A workgroup alone on
+// its CU takes 0.15 us per 64 columns, the join 4 us and 0.3 us a part: sqrt(stages / 2) parts from 96 stages on, of at least a
+// 512th of the launch's work each, and no more than leave each workgroup a CU of its own if the tiles do.  Measured, whole calls:
+// 500 x 10000 281 -> 236 us, 128 x 20000 328 -> 166, 64 x 100000 1189 -> 226; shorter sums in parts of 16:
+// 512 x 4608 185 -> 177, 1000 x 2048 164 -> 222, all of ResNet-50 597 -> 632.
+long long splits_of(const Desc* q, int count, int sym, int* split) {
+    long long tiles[MAXG], stages[MAXG], whole = 0, items = 0, slabs = 0;
+    double all = 0.0;
+    for (int i = 0; i < count; ++i) {
+        const long long n64 = ((q[i].r < q[i].c ? q[i].r : q[i].c) + 63) / 64;
+        tiles[i] = q[i].batch * (n64 * (n64 + 1) / 2);
+        stages[i] = ((q[i].r < q[i].c ? q[i].c : q[i].r) + 63) / 64;
+        whole += tiles[i];
+        all += (double)tiles[i] * (double)stages[i];
+    }
+    for (int i = 0; i < count; ++i) {
+        const double most = fmin(64.0, fmin(sqrt(0.5 * (double)stages[i]), 512.0 * (double)stages[i] / all));
+        split[i] = sym == 64 && stages[i] >= 96 && most >= 2.0 ? (int)most : 1;
+        items += tiles[i] * split[i];
+    }
+    while (whole <= 256 && items > 256) {
+        int top = 0;
+        for (int i = 1; i < count; ++i)
+            if (split[i] > split[top]) top = i;
+        --split[top];
+        items -= tiles[top];
+    }
+    for (int i = 0; i < count; ++i) {
+        const long long each = (stages[i] + split[i] - 1) / split[i];
+        split[i] = (int)((stages[i] + each - 1) / each);               // none of them empty
+        if (split[i] > 1) slabs += tiles[i] * split[i];
+    }
+    return slabs;
+}
+
 // Calls that ortho_small_kernel serves: every matrix of up to 64 rows (its shorter side) and 512 columns, or 128 and 256
 int small_class(const Desc& s) {            // 0: none, else 8 * padded rows / 64 + the smallest CB
     const long long n = s.r < s.c ? s.r : s.c, m = s.r < s.c ? s.c : s.r;
@@ -1251,8 +1348,10 @@ int run_all(const Desc* q, int count, int kind, const Muon& mu, float a, float b
     Plan pl;
     if (!plan_of(q, count, thin_steps(a, b, c, steps), pl)) return DDL_EINVAL;
     if (all_small(q, count)) return run_small(q, count, kind, mu, a, b, c, steps, eps, stream);
-    int sb = 64, ab = 64;
+    int sb = 64, ab = 64, split[MAXG];
     tiles_of(q, count, sb, ab);
+    splits_of(q, count, sb, split);
+    long long slabs = 0, squares = 0;
     // the groups with the longest sums first
     int order[MAXG];
     for (int i = 0; i < count; ++i) order[i] = i;
@@ -1273,12 +1372,20 @@ int run_all(const Desc* q, int count, int kind, const Muon& mu, float a, float b
         o.vec = vec_of(s, kind);
         o.part_elems = (int)pe; o.parts = (int)parts;
         o.xo = (unsigned)(xo / 64); o.ao = (unsigned)(ao / 64); o.dof = (unsigned)dof; o.po = (unsigned)po; o.mat = (unsigned)mat;
-        o.tsym = (int)(sn * (sn + 1) / 2); o.tapp = (int)(an * am);
+        const long long whole = sn * (sn + 1) / 2;
+        o.tsym = (int)(whole * (pl.thin ? 1 : split[order[i]])); o.tapp = (int)(an * am);
         o.fin = (unsigned)nin; o.fio = (unsigned)nio;
-        csym[i] = (double)s.batch * o.tsym * (double)(np + mp + 512);      // (512: what a tile costs beside its sum)
+        csym[i] = (double)s.batch * whole * (double)(np + mp + 512);      // (512: what a tile costs beside its sum)
         capp[i] = (double)s.batch * o.tapp * (double)(np + 512);
-        o.tcols = (int)thin_cols(m);
-        o.chunks = (int)((m + o.tcols - 1) / o.tcols);
+        if (pl.thin) {
+            o.tcols = (int)thin_cols(m);
+            o.chunks = (int)((m + o.tcols - 1) / o.tcols);
+        } else {
+            o.split = split[order[i]];
+            o.slab = (unsigned)slabs;
+            if (o.split > 1) slabs += s.batch * o.tsym;
+        }
+        squares += s.batch * whole;
         nin += s.batch * parts; nio += s.batch * (pl.thin ? o.chunks : (np / 64) * (mp / 64));
         nsym += s.batch * o.tsym; napp += s.batch * o.tapp;
         xo += s.batch * np * mp; ao += s.batch * np * np; dof += s.batch * np; po += s.batch * parts; mat += s.batch;
@@ -1293,6 +1400,8 @@ int run_all(const Desc* q, int count, int kind, const Muon& mu, float a, float b
     float *d = (float*)(ws + pl.d), *pd = (float*)(ws + pl.pd);
     double* part = (double*)(ws + pl.part);
     int* ex = (int*)(ws + pl.ex);
+    float* slab = (float*)(ws + pl.slab);
+    unsigned* counters = (unsigned*)(ws + pl.cnt);
     const int fall = growth_bits(a, b, c, steps);
     for (int base = 0; base < count; base += CHUNK) {
         Chunk ch;
@@ -1302,7 +1411,7 @@ int run_all(const Desc* q, int count, int kind, const Muon& mu, float a, float b
         memcpy(ch.g, g + base, ch.n * sizeof(Group));
         memset(ch.g + ch.n, 0, (CHUNK - ch.n) * sizeof(Group));
         const dim3 grid((unsigned)((ch.last ? nin : g[base + CHUNK].fin) - g[base].fin) + 1);
-#define SUMS(K) DDL_KLAUNCH(ortho_sqsum_kernel<K>, grid, dim3(1024), 0, stream, ch, mu, part, t)
+#define SUMS(K) DDL_KLAUNCH(ortho_sqsum_kernel<K>, grid, dim3(1024), 0, stream, ch, mu, part, t, counters, (int)(pl.thin ? 0 : pl.slabs))
         if (kind == 0) SUMS(0); else if (kind == 1) SUMS(1); else if (kind == 2) SUMS(2); else SUMS(3);
 #undef SUMS
     }
@@ -1326,14 +1435,21 @@ int run_all(const Desc* q, int count, int kind, const Muon& mu, float a, float b
 #undef PACK
     for (int k = 0; k < steps; ++k) {
         const int fin = k < steps - 1 ? 0 : (kind < 2 ? 1 : 2);
-#define SYM(B, W0, W1, NST, KS, SQ, IN, DIN, OUTP, DOUT, DOWN) DDL_KLAUNCH((ortho_sym_kernel<B, W0, W1, NST, KS, SQ>), dim3((unsigned)nsym), dim3(KS * W0 * W1 * 64), 0, stream, t, IN, DIN, OUTP, DOUT, ex, DOWN, a, b, c)
-#define SYMS(B, W0, W1, NST, KS) { SYM(B, W0, W1, NST, KS, false, xh, (const float*)nullptr, O, d, k * fall); SYM(B, W0, W1, NST, KS, true, O, d, P, pd, 0); }
+#define SYM(B, W0, W1, NST, KS, SQ, IN, DIN, OUTP, DOUT, DOWN) DDL_KLAUNCH((ortho_sym_kernel<B, W0, W1, NST, KS, SQ>), dim3((unsigned)nsym), dim3(KS * W0 * W1 * 64), 0, stream, t, IN, DIN, OUTP, DOUT, ex, DOWN, a, b, c, slab, counters)
+#define SYM1(B, W0, W1, NST, KS) SYM(B, W0, W1, NST, KS, false, xh, (const float*)nullptr, O, d, k * fall)
+#define SYM2(B, W0, W1, NST, KS) SYM(B, W0, W1, NST, KS, true, O, d, P, pd, 0)
 #define APP1(B, W0, W1, NST, KS, FIN) DDL_KLAUNCH((ortho_apply_kernel<B, B, W0, W1, NST, KS, FIN>), dim3((unsigned)napp), dim3(KS * W0 * W1 * 64), 0, stream, t, mu, P, pd, xh, xl, yh, yl, ex, k * fall, (k + 1) * fall)
 #define APP(B, W0, W1, NST, KS) { if (fin == 0) APP1(B, W0, W1, NST, KS, 0); else if (fin == 1) APP1(B, W0, W1, NST, KS, 1); else APP1(B, W0, W1, NST, KS, 2); }
-        if (sb == 64 && nsym <= 256) SYMS(64, 2, 2, 3, 2)
-        else if (sb == 64) SYMS(64, 2, 2, 3, 1)
-        else if (sb == 128) SYMS(128, 2, 4, 2, 1)
-        else SYMS(256, 2, 4, 2, 1)
+        if (sb == 64) {
+            if (nsym <= 256) SYM1(64, 2, 2, 3, 2); else SYM1(64, 2, 2, 3, 1);
+            if (squares <= 256) SYM2(64, 2, 2, 3, 2); else SYM2(64, 2, 2, 3, 1);
+        } else if (sb == 128) {
+            SYM1(128, 2, 4, 2, 1);
+            SYM2(128, 2, 4, 2, 1);
+        } else {
+            SYM1(256, 2, 4, 2, 1);
+            SYM2(256, 2, 4, 2, 1);
+        }
         if (ab == 64 && napp <= 256) APP(64, 2, 2, 3, 2)
         else if (ab == 64) APP(64, 2, 2, 3, 1)
         else if (ab == 128) APP(128, 2, 4, 2, 1)

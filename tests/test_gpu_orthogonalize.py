@@ -472,3 +472,61 @@ def test_offsets_beyond_32_bits(shape):
     assert not out[1].any() and not out[shape[0] - 2].any()
     for k in (0, shape[0] // 2, shape[0] - 1):
         assert off(out[k], g) < TOL
+
+
+# sums of X X^T that are cut into parts: one tile, several of them ragged, more groups than CUs, stacks; fp16 rounds as elsewhere
+@pytest.mark.parametrize("shapes", [[(64, 6144 + 13)], [(33, 100001)], [(9001, 100), (300, 12345), (40, 7000), (70, 50)], [(3, 65, 9000), (2, 40, 64 * 191)],
+                                    [(500, 6200), (20, 30000), (640, 700), (64, 64)]], ids=str)
+@pytest.mark.parametrize("dtype", [torch.float32, BF], ids=["fp32", "bf16"])
+def test_long_rows(shapes, dtype):
+    from distributeddeeplearning_amd.ops import functional as ops
+
+    gen = torch.Generator(DEV).manual_seed(9)
+    mats = []
+    for s in shapes:
+        x = torch.randn(s, generator=gen, device=DEV) * torch.logspace(0, -3, s[-1], device=DEV)
+        mats += [m.to(dtype) for m in (x if len(s) == 3 else x[None])]
+    if len(shapes[0]) == 3:
+        outs = [o for k in (0, 3) for o in ops.orthogonalize(torch.stack(mats[k:k + 3 - k // 3]))]
+    else:
+        outs = ops.orthogonalize(mats)
+        for _ in range(3):
+            assert all(torch.equal(a, b) for a, b in zip(outs, ops.orthogonalize(mats)))
+    for m, o in zip(mats, outs):
+        want = on_the_card(m)
+        assert float((o.double() - want).norm() / want.norm()) < TOL
+
+
+def test_long_rows_in_graphs_and_in_the_optimizer():
+    from distributeddeeplearning_amd.ops import functional as ops
+    from distributeddeeplearning_amd.optim import FusedMuon
+
+    xs = [torch.randn(130, 8000, device=DEV), torch.randn(2, 50, 20000, device=DEV)]
+    graphs, outs = [], []
+    for x in xs:
+        ops.orthogonalize(x)
+    torch.cuda.synchronize()
+    for x in xs:
+        gr = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(gr):
+            outs.append(ops.orthogonalize(x))
+        graphs.append(gr)
+    for rep in range(4):
+        for x in xs:
+            x.copy_(torch.randn(x.shape, generator=torch.Generator().manual_seed(rep)))
+        for gr in graphs if rep % 2 else graphs[::-1]:
+            gr.replay()
+        eager = [ops.orthogonalize(x) for x in xs]
+        torch.cuda.synchronize()
+        for o, e in zip(outs, eager):
+            assert torch.equal(o, e)
+    # the step is the operator's: w - lr sqrt(max(1, r / c)) O, O in fp32 there (half a bf16 step, 2^-8, from the operator's)
+    named = _params([(130, 8000), (20000, 50)], torch.float32)
+    opt = FusedMuon(named, lr=1.0, momentum=0.0, nesterov=False)
+    before = [p.detach().clone() for _, p in named]
+    for _, p in named:
+        p.grad.copy_(torch.randn(p.shape, generator=torch.Generator(DEV).manual_seed(5), device=DEV))
+    wants = [w - max(1.0, w.shape[0] / w.shape[1]) ** 0.5 * ops.orthogonalize(p.grad).float() for w, (_, p) in zip(before, named)]
+    opt.step()
+    for (_, p), w, b in zip(named, wants, before):
+        assert float((p.detach() - w).norm()) <= 2 ** -8 * float((w - b).norm()) + 2 ** -22 * float(b.norm())
