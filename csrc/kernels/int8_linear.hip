@@ -10,6 +10,7 @@
 // (int8_rows_kernel, bound by memory), then multiplied tile by tile (int8_gemm_kernel, bound by the matrix pipe).
 #include "common.h"
 #include "tile_mul.h"
+#include <math.h>
 
 namespace {
 
@@ -40,16 +41,16 @@ __device__ __forceinline__ void ld_row(const T* __restrict__ row, int k, int K, 
     }
 }
 
-// One wave: the codes of a row (K values, zeros up to Kp, a multiple of 16) to q, which starts at a multiple of 16 bytes; returns
-// its scale.  The first 2048 values are read at once and stay in registers between the two passes.
-template <typename T>
+// One wave (W = 1) or a workgroup of W: the codes of a row (K values, zeros up to Kp, a multiple of 16) to q, which starts at a
+// multiple of 16 bytes; returns its scale.  The first 2048 W values are read at once and stay in registers between the two passes.
+template <int W, typename T>
 __device__ __forceinline__ float quantize_row(const T* __restrict__ row, int K, int Kp, bool vec, signed char* q) {
-    const int lane = threadIdx.x & 63;
+    const int lane = W == 1 ? threadIdx.x & 63 : threadIdx.x;
     constexpr int HOLD = 4;
     float held[HOLD][8], top = 0.f;
     int bad = 0;
 #pragma unroll
-    for (int h = 0; h < HOLD; ++h) ld_row(row, (h * 64 + lane) * 8, K, vec, held[h]);
+    for (int h = 0; h < HOLD; ++h) ld_row(row, (h * 64 * W + lane) * 8, K, vec, held[h]);
     auto see = [&](const float (&v)[8]) {
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
@@ -61,13 +62,28 @@ __device__ __forceinline__ float quantize_row(const T* __restrict__ row, int K, 
 #pragma unroll
     for (int h = 0; h < HOLD; ++h) see(held[h]);
 #pragma unroll 2
-    for (int k = (HOLD * 64 + lane) * 8; k < K; k += 512) {
+    for (int k = (HOLD * 64 * W + lane) * 8; k < K; k += 512 * W) {
         float v[8];
         ld_row(row, k, K, vec, v);
         see(v);
     }
     top = wave_max(top);
     bad = __any(bad);
+    if constexpr (W > 1) {
+        __shared__ float tops[W];
+        __shared__ int bads[W];
+        __syncthreads();                     // (a row before this one)
+        if ((threadIdx.x & 63) == 0) {
+            tops[threadIdx.x >> 6] = top;
+            bads[threadIdx.x >> 6] = bad;
+        }
+        __syncthreads();
+#pragma unroll
+        for (int w = 0; w < W; ++w) {
+            top = fmaxf(top, tops[w]);
+            bad |= bads[w];
+        }
+    }
     const bool zero = bad || top < 1e-30f;
     const float inv = zero ? 0.f : 127.f * (1.f / top);
     auto put = [&](int k, const float (&v)[8]) {
@@ -79,9 +95,9 @@ __device__ __forceinline__ float quantize_row(const T* __restrict__ row, int K, 
         *reinterpret_cast<u32x2*>(q + k) = o;
     };
 #pragma unroll
-    for (int h = 0; h < HOLD; ++h) put((h * 64 + lane) * 8, held[h]);
+    for (int h = 0; h < HOLD; ++h) put((h * 64 * W + lane) * 8, held[h]);
 #pragma unroll 2
-    for (int k = (HOLD * 64 + lane) * 8; k < Kp; k += 512) {
+    for (int k = (HOLD * 64 * W + lane) * 8; k < Kp; k += 512 * W) {
         float v[8];
         ld_row(row, k, K, vec, v);
         put(k, v);
@@ -89,15 +105,17 @@ __device__ __forceinline__ float quantize_row(const T* __restrict__ row, int K, 
     return bad ? __builtin_nanf("") : (zero ? 0.f : top / 127.f);
 }
 
-// a row a wave: codes [M][Kp], scales.  12 544 rows of 4096 bf16 values (154 MB): 31 us (values of a row held in registers between its largest
-// and its codes; read a second time: 94)
-template <typename T>
+// Codes [M][Kp], scales; a row a wave (W = 1) or a workgroup of W waves.  Also clears what int8_gemm_kernel counts with.
+// 12 544 rows of 4096 bf16 values (154 MB): 29 us (values of a row held in registers between its largest and its codes; read a second
+// time: 94)
+template <int W, typename T>
 __global__ void __launch_bounds__(256) int8_rows_kernel(const T* __restrict__ x, long long ldx, int M, int K, int Kp, int vec, signed char* __restrict__ q,
-                                                       float* __restrict__ scale) {
-    const int m = blockIdx.x * 4 + (threadIdx.x >> 6);
+                                                       float* __restrict__ scale, unsigned* __restrict__ counters, int ncount) {
+    if (blockIdx.x == 0 && (int)threadIdx.x < ncount) counters[threadIdx.x] = 0u;
+    const int m = W == 1 ? blockIdx.x * 4 + (threadIdx.x >> 6) : blockIdx.x;
     if (m >= M) return;
-    const float s = quantize_row(x + m * ldx, K, Kp, vec, q + (long long)m * Kp);
-    if ((threadIdx.x & 63) == 0) scale[m] = s;
+    const float s = quantize_row<W>(x + m * ldx, K, Kp, vec, q + (long long)m * Kp);
+    if ((threadIdx.x & (64 * W - 1)) == 0) scale[m] = s;
 }
 
 // B x B tile of y: F = output channels, S = rows of x
@@ -105,23 +123,29 @@ template <typename T, int B, int W0, int W1, int NST, int KS>
 __global__ void __launch_bounds__(KS * W0 * W1 * 64, 2) int8_gemm_kernel(const signed char* __restrict__ xq, const float* __restrict__ sx,
                                                                    const signed char* __restrict__ q, long long ldq, long long q_bytes,
                                                                    const float* __restrict__ s, const float* __restrict__ bias, T* __restrict__ y, long long ldy,
-                                                                   int M, int N, int Kp, int tm, int tn) {
+                                                                   int M, int N, int Kp, int tm, int tn, int split, int* __restrict__ slabs,
+                                                                   unsigned* __restrict__ counters) {
     typedef TileMul<MulI8, B, B, W0, W1, NST, false, KS> Mu;
     __shared__ __attribute__((aligned(16))) unsigned char smem[Mu::LDS];
     // an XCD (workgroup number modulo 8) has a run of tiles, in bands of 8 rows, a band column by column
-    const int all = tm * tn, per = (all + 7) >> 3, idx = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
-    if ((int)(blockIdx.x >> 3) >= per || idx >= all) return;
+    const int all = tm * tn * split, per = (all + 7) >> 3, item = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
+    if ((int)(blockIdx.x >> 3) >= per || item >= all) return;
+    const int idx = item / split, part = item - idx * split, each = (Kp / 128 + split - 1) / split, k0 = part * each;
+    const int stages = Kp / 128 - k0 < each ? Kp / 128 - k0 : each;
     const int band = idx / (8 * tn), rem = idx - band * 8 * tn, h = tm - band * 8 < 8 ? tm - band * 8 : 8;
     const int ni = rem / h, mi = band * 8 + rem - ni * h, m0 = mi * B, n0 = ni * B;
-    const long long left = q_bytes - n0 * ldq;
+    const long long left = q_bytes - n0 * ldq - k0 * 128;
     Mu mu;
-    mu.run(smem, q + n0 * ldq, (unsigned)ldq, N - n0, left < (long long)DESC_BYTES ? (unsigned)left : DESC_BYTES, xq + (long long)m0 * Kp, Kp, M - m0, DESC_BYTES,
-           Kp / 128);
+    mu.run(smem, q + n0 * ldq + k0 * 128, (unsigned)ldq, N - n0, left < (long long)DESC_BYTES ? (unsigned)left : DESC_BYTES, xq + (long long)m0 * Kp + k0 * 128, Kp, M - m0,
+           DESC_BYTES, stages);
+    if constexpr (B == 64) {
+        if (split > 1 && !join_parts<int, Mu>(mu, smem, slabs + (long long)idx * split * (B * B), counters + idx, part, split)) return;
+    }
     const bool vec = (N & 7) == 0 && (ldy & 7) == 0;
 #pragma unroll
     for (int pass = 0; pass < Mu::PASSES; ++pass) {
         if (Mu::PASSES > 1 && pass > 0) __syncthreads();
-        mu.to_lds(smem, pass);
+        if (B > 64 || split == 1) mu.to_lds(smem, pass);
         __syncthreads();
 #pragma unroll 1
         for (int k = threadIdx.x; k < Mu::ROWS * B / 8; k += Mu::THREADS) {
@@ -182,9 +206,16 @@ __global__ void __launch_bounds__(512) int8_skinny_kernel(const T* __restrict__ 
     Pair buf[4];
 #pragma unroll
     for (int u = 0; u < 3; ++u) buf[u] = load(u);
-    for (int m = wid; m < M; m += 8) {
-        const float t = quantize_row(x + m * ldx, K, Kp, vec, xs + m * LD);
-        if (lane == 0) sx[m] = t;
+    if (M <= 4 && K > 2048) {                  // long rows, fewer than waves: 1 x 1000 x 25 088 36 -> 17 us
+        for (int m = 0; m < M; ++m) {
+            const float t = quantize_row<8>(x + m * ldx, K, Kp, vec, xs + m * LD);
+            if (threadIdx.x == 0) sx[m] = t;
+        }
+    } else {
+        for (int m = wid; m < M; m += 8) {
+            const float t = quantize_row<1>(x + m * ldx, K, Kp, vec, xs + m * LD);
+            if (lane == 0) sx[m] = t;
+        }
     }
     __syncthreads();
     const signed char* row = xs + (fr < M ? fr : 0) * LD + fq * 16;        // (columns from M on repeat row 0 and are not stored)
@@ -226,14 +257,32 @@ constexpr int SKINNY = 16, SKINNY_LDS = 40 * 1024;
 bool skinny(long long M, int K) { return M <= SKINNY && M * ((K + 127LL) / 128 * 128 + 16) <= SKINNY_LDS; }
 bool rows_vec(const void* x, int bf16, long long ldx) { return ddl_aligned16(x) && ldx % (bf16 ? 8 : 4) == 0; }
 
-// (a launch's threads are counted in 32 bits: 2^24 rows at a time)
+// (a launch's threads are counted in 32 bits: 2^23 rows at a time)
 template <typename T>
-void launch_rows(const T* x, long long ldx, long long M, int K, int Kp, int vec, signed char* q, float* scale, hipStream_t stream) {
-    constexpr long long AT_ONCE = 1LL << 24;
+void launch_rows(const T* x, long long ldx, long long M, int K, int Kp, int vec, signed char* q, float* scale, unsigned* counters, int ncount, hipStream_t stream) {
+    constexpr long long AT_ONCE = 1LL << 23;
     for (long long m = 0; m < M; m += AT_ONCE) {
         const int rows = (int)(M - m < AT_ONCE ? M - m : AT_ONCE);
-        DDL_KLAUNCH(int8_rows_kernel<T>, dim3((rows + 3) / 4), dim3(256), 0, stream, x + m * ldx, ldx, rows, K, Kp, vec, q + m * Kp, scale + m);
+        // (rows that a wave does not hold: 12 544 of 4096 values 31 -> 29 us, 16 of 25 088 in the whole product 66 -> 43)
+        if (K > 2048)
+            DDL_KLAUNCH((int8_rows_kernel<4, T>), dim3(rows), dim3(256), 0, stream, x + m * ldx, ldx, rows, K, Kp, vec, q + m * Kp, scale + m, counters,
+                        m == 0 ? ncount : 0);
+        else
+            DDL_KLAUNCH((int8_rows_kernel<1, T>), dim3((rows + 3) / 4), dim3(256), 0, stream, x + m * ldx, ldx, rows, K, Kp, vec, q + m * Kp, scale + m, counters,
+                        m == 0 ? ncount : 0);
     }
+}
+
+long long codes_bytes(long long M, int Kp) { return (M * Kp + 255) / 256 * 256 + (M * 4 + 255) / 256 * 256; }
+// Parts of the sums of tiles of 64 (1: none).  A workgroup alone on its CU takes 0.15 us per 128 columns, the join 4 us and 0.3 us a
+// part: sqrt(stages / 2) parts from 96 stages on, while each part has a CU.  64 x 4096 x 25 088 49 -> 38 us, 256 x 1000 x 25 088 50 -> 35,
+// 1 x 1000 x 100 000 147 -> 58; 64 stages, 7 x 4096 x 8192: 17.7 -> 19.6.
+int split_of(long long M, int N, int K) {
+    const long long t64 = ((M + 63) / 64) * ((N + 63LL) / 64), stages = (K + 127) / 128;
+    if (stages < 96 || t64 > 128) return 1;
+    const double most = fmin(256.0 / (double)t64, fmin(32.0, sqrt(0.5 * (double)stages)));
+    const long long each = (stages + (int)most - 1) / (int)most;
+    return (int)((stages + each - 1) / each);
 }
 
 template <typename T>
@@ -252,11 +301,14 @@ int run(const T* x, long long ldx, const signed char* q, long long ldq, long lon
     // 396, copies between register halves.)
     const long long t128 = ((M + 127LL) / 128) * ((N + 127) / 128), t64 = ((M + 63LL) / 64) * ((N + 63) / 64);
     if (t128 > 0xffffffLL - 8) return DDL_EINVAL;
-    launch_rows(x, ldx, M, K, Kp, vec, xq, sx, stream);
+    const int split = split_of(M, N, K);
+    int* slabs = (int*)(ws + codes_bytes(M, Kp));
+    unsigned* counters = (unsigned*)(slabs + t64 * split * 64 * 64);
+    launch_rows(x, ldx, M, K, Kp, vec, xq, sx, counters, split > 1 ? (int)t64 : 0, stream);
 #define GEMM(B, W0, W1, NST, KS, t) DDL_KLAUNCH((int8_gemm_kernel<T, B, W0, W1, NST, KS>), dim3((unsigned)((t + 7) / 8 * 8)), dim3(KS * W0 * W1 * 64), 0, stream, xq, sx, q, \
-                                            ldq, q_bytes, s, bias, y, ldy, M, N, Kp, (M + B - 1) / B, (N + B - 1) / B)
+                                            ldq, q_bytes, s, bias, y, ldy, M, N, Kp, (M + B - 1) / B, (N + B - 1) / B, split, slabs, counters)
     if (t128 >= 256) GEMM(128, 2, 2, 2, 1, t128);
-    else if (t64 <= 256 && Kp > 128) GEMM(64, 2, 2, 3, 2, t64);
+    else if (t64 <= 256 && Kp > 128) GEMM(64, 2, 2, 3, 2, t64 * split);
     else GEMM(64, 2, 2, 3, 1, t64);
 #undef GEMM
     return ddl_launch_status();
@@ -270,8 +322,8 @@ extern "C" int ddl_int8_rows(const void* x, int x_bf16, long long ldx, long long
     if (!x || !q || !scale || M < 0 || M > 0x7fffff00LL || K <= 0 || Kp < K || Kp % 16 || ldx < 0) return DDL_EINVAL;
     if (!ddl_aligned16(q)) return DDL_EALIGN;
     const int vec = rows_vec(x, x_bf16, ldx);
-    if (x_bf16) launch_rows((const bf16_t*)x, ldx, M, K, Kp, vec, (signed char*)q, (float*)scale, stream);
-    else launch_rows((const float*)x, ldx, M, K, Kp, vec, (signed char*)q, (float*)scale, stream);
+    if (x_bf16) launch_rows((const bf16_t*)x, ldx, M, K, Kp, vec, (signed char*)q, (float*)scale, nullptr, 0, stream);
+    else launch_rows((const float*)x, ldx, M, K, Kp, vec, (signed char*)q, (float*)scale, nullptr, 0, stream);
     return ddl_launch_status();
 }
 
@@ -281,7 +333,8 @@ extern "C" int ddl_int8_max_k() { return 133144; }
 extern "C" long long ddl_int8_linear_workspace(long long M, int N, int K) {
     if (skinny(M, K)) return 0;
     const long long Kp = (K + 127LL) / 128 * 128;
-    return (M * Kp + 255) / 256 * 256 + M * 4;
+    const int split = split_of(M, N, K);
+    return codes_bytes(M, (int)Kp) + (split > 1 ? ((M + 63) / 64) * ((N + 63LL) / 64) * (split * 64LL * 64 * 4 + 4) : 0);
 }
 
 // y [M][N] (bf16 or fp32 like x) = x [M][K] times q [N][K]^T with scales; rows of q start at multiples of 16 bytes and may be

@@ -446,40 +446,10 @@ __global__ void __launch_bounds__(KS * W0 * W1 * 64, B == 128 ? 4 : 2) ortho_sym
     f16_t* o = out + ao;
     float* dst = dout + it.dof + (long long)b * np;
     float* tile = reinterpret_cast<float*>(smem);
-    // A part of a long sum: the workgroup that ends last adds all parts, in their order, and goes on with the tile.  The parts pass
-    // from XCD to XCD by stores and loads of the device's scope, each wave waiting for its stores before the counter is raised (a
-    // fence would write back and empty a whole L2: 316 us for 512 x 4608 in all).
     bool joined = false;
     if constexpr (B == 64 && !SQUARE) {
-        if (it.split > 1) {
-            typedef unsigned long long u64;
-            constexpr int PAIRS = B * B / 2;
-            __shared__ unsigned before;
-            u64* all = reinterpret_cast<u64*>(slabs + (long long)it.slab * (B * B));
-            u64* pairs = reinterpret_cast<u64*>(tile);
-            m.to_lds(tile, 0);
-            __syncthreads();
-            for (int k = threadIdx.x; k < PAIRS; k += M::THREADS)
-                __hip_atomic_store(all + it.part * PAIRS + k, pairs[k], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-            __syncthreads();
-            if (threadIdx.x == 0) before = __hip_atomic_fetch_add(counters + it.slab, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-            __syncthreads();
-            if (before != (unsigned)it.split - 1u) return;
-            for (int k = threadIdx.x; k < PAIRS; k += M::THREADS) {
-                float s0 = 0.f, s1 = 0.f;
-#pragma unroll 8
-                for (int p = 0; p < it.split; ++p) {
-                    const u64 v = __hip_atomic_load(all + p * PAIRS + k, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-                    s0 += __uint_as_float((unsigned)v);
-                    s1 += __uint_as_float((unsigned)(v >> 32));
-                }
-                pairs[k] = (u64)__float_as_uint(s1) << 32 | __float_as_uint(s0);
-            }
-            if (threadIdx.x == 0) counters[it.slab] = 0u;          // for the next step
-            __syncthreads();
-            joined = true;
-        }
+        joined = it.split > 1;
+        if (joined && !join_parts<float>(m, tile, slabs + (long long)it.slab * (B * B), counters + it.slab, it.part, it.split)) return;
     }
     // value (r, c) of the result from the product's
     auto value = [&](float v, int r, int c, float a, float dr, float dc) {
@@ -1473,10 +1443,11 @@ extern "C" int ddl_ortho_coefficients_ok(float a, float b, float c, int steps) {
 }
 
 // bytes of workspace of a call with these groups (`desc`: count x 11 int64: source address, its batch / row / column
-// strides, destination address and strides, rows, columns, matrices), -1: sizes out of range
+// strides, destination address and strides, rows, columns, matrices), 0: none, -1: sizes out of range
 extern "C" long long ddl_ortho_workspace(const long long* desc, int count) {
     Plan one, other;               // (which of the forms is taken depends on the steps too)
     if (!plan_of((const Desc*)desc, count, true, one) || !plan_of((const Desc*)desc, count, false, other)) return -1;
+    if (all_small((const Desc*)desc, count)) return 0;
     return one.bytes > other.bytes ? one.bytes : other.bytes;
 }
 
@@ -1486,7 +1457,7 @@ extern "C" int ddl_orthogonalize(const long long* desc, int count, int kind, flo
     if (count == 0) return DDL_OK;
     const Desc* q = (const Desc*)desc;
     const long long need = ddl_ortho_workspace(desc, count);
-    if (kind < 0 || kind > 1 || !ws || need < 0 || ws_bytes < need) return DDL_EINVAL;
+    if (kind < 0 || kind > 1 || need < 0 || ws_bytes < need || (need > 0 && !ws)) return DDL_EINVAL;
     if (!ddl_ortho_coefficients_ok(a, b, c, steps) || !(eps >= 1e-30f)) return DDL_EINVAL;
     if (reinterpret_cast<uintptr_t>(ws) & 255) return DDL_EALIGN;
     for (int i = 0; i < count; ++i)
@@ -1505,7 +1476,7 @@ extern "C" int ddl_muon_step(const long long* desc, int count, void* w, const vo
     if (count == 0) return DDL_OK;
     const Desc* q = (const Desc*)desc;
     const long long need = ddl_ortho_workspace(desc, count);
-    if (!w || !g || !v || !ws || need < 0 || ws_bytes < need) return DDL_EINVAL;
+    if (!w || !g || !v || need < 0 || ws_bytes < need || (need > 0 && !ws)) return DDL_EINVAL;
     if (!ddl_ortho_coefficients_ok(a, b, c, steps) || !(eps >= 1e-30f)) return DDL_EINVAL;
     if ((reinterpret_cast<uintptr_t>(ws) & 255) || !ddl_aligned16(w) || !ddl_aligned16(g) || !ddl_aligned16(v) || (lowp && !ddl_aligned16(lowp)))
         return DDL_EALIGN;

@@ -255,10 +255,11 @@ def orthogonalize(x, steps=5, coefficients=ORTHO_COEFFICIENTS, eps=1e-7):
         if kernels.require():
             from . import hip_ops
 
-            if not kernels.ortho_coefficients_ok(*(float(v) for v in coefficients), steps):
+            a, b, c = map(float, coefficients)
+            if not kernels.ortho_coefficients_ok(a, b, c, steps):
                 raise ValueError("orthogonalize: %d steps with the coefficients %r leave the range of the kernels' 16-bit operands"
                                  % (steps, tuple(coefficients)))
-            out = hip_ops.orthogonalize(mats, steps, tuple(float(v) for v in coefficients), float(eps))
+            out = hip_ops.orthogonalize(mats, steps, (a, b, c), float(eps))
     if out is None:
         with torch.no_grad():
             out = [orthogonalize_plain(m, steps, coefficients, eps).to(torch.bfloat16).contiguous() for m in mats]
@@ -309,29 +310,26 @@ def linear_int8(x, q, scale, bias=None):
     that requires one is refused outside ``torch.no_grad()``.  ``k`` is at most 133 144."""
     if (x.dtype is not torch.float32 and x.dtype is not torch.bfloat16) or x.dim() < 1:
         raise ValueError("linear_int8: fp32 or bf16 rows expected, got %s" % x.dtype)
-    shape, k = x.shape, x.shape[-1]
-    if q.dtype is not torch.int8 or q.dim() != 2 or q.shape[1] != k or not 0 < k <= 133144:
-        raise ValueError("linear_int8: int8 codes [n, %d] of 1 to 133144 columns expected, got %s %s" % (k, q.dtype, tuple(q.shape)))
+    shape, qshape, device = x.shape, q.shape, x.device
+    k = shape[-1]
+    if q.dtype is not torch.int8 or len(qshape) != 2 or qshape[1] != k or not 0 < k <= 133144:
+        raise ValueError("linear_int8: int8 codes [n, %d] of 1 to 133144 columns expected, got %s %s" % (k, q.dtype, tuple(qshape)))
     for name, t in (("scale", scale), ("bias", bias)):
-        if t is None:
-            continue
-        if t.dtype is not torch.float32 or t.dim() != 1 or t.shape[0] != q.shape[0]:
-            raise ValueError("linear_int8: %s must be fp32 [%d], got %s %s" % (name, q.shape[0], t.dtype, tuple(t.shape)))
-        if t.device != x.device:
-            raise ValueError("linear_int8: input, codes, scales and bias must be on one device")
-    if q.device != x.device:
+        if t is not None and (t.dtype is not torch.float32 or t.shape != qshape[:1]):
+            raise ValueError("linear_int8: %s must be fp32 [%d], got %s %s" % (name, qshape[0], t.dtype, tuple(t.shape)))
+    if q.device != device or scale.device != device or (bias is not None and bias.device != device):
         raise ValueError("linear_int8: input, codes, scales and bias must be on one device")
     if torch.is_grad_enabled() and (x.requires_grad or scale.requires_grad or (bias is not None and bias.requires_grad)):
         raise ValueError("linear_int8: no gradient flows through it; call it under torch.no_grad()")
-    x2 = x if x.dim() == 2 else x.reshape(shape[:-1].numel(), k)
-    if x.is_cuda and _FORCED != "aten":
+    x2 = x if len(shape) == 2 else x.reshape(shape[:-1].numel(), k)
+    if device.type == "cuda" and _FORCED != "aten":
         from . import kernels
 
         if kernels.require():
             from . import hip_ops
 
             y = hip_ops.linear_int8(x2, q, scale, bias)
-            return y if x.dim() == 2 else y.view(shape[:-1] + q.shape[:1])
+            return y if len(shape) == 2 else y.view(shape[:-1] + qshape[:1])
     xq, sx = _int8_rows_plain(x2)
     # (fp64 sums: whole numbers up to 2^31 are exact)
     y = (xq.double() @ q.double().t()).float() * (sx[:, None] * scale[None, :])

@@ -1878,18 +1878,22 @@ def linear_int8(x, q, scale, bias):
     """``functional.linear_int8`` of a 2-d input."""
     n, k = q.shape
     ldq, s1 = q.stride()
-    if s1 != 1 or ldq % 16 or ldq >= 1 << 22 or q.data_ptr() % 16 or K.storage_numel_from(q) < (n - 1) * ldq + (k + 15) // 16 * 16:
+    at, readable = q.data_ptr(), q.untyped_storage().nbytes() - q.storage_offset()
+    if s1 != 1 or ldq % 16 or ldq >= 1 << 22 or at % 16 or readable < (n - 1) * ldq + (k + 15) // 16 * 16:
         raise K.KernelError("linear_int8: the rows of the codes must start at multiples of 16 bytes, less than 4 MiB apart, and be readable to "
                             "the next multiple behind their end: take them from quantize_int8 (strides %s)" % (q.stride(),))
-    if x.stride(1) != 1 or x.stride(0) < 0:
+    ldx, s1 = x.stride()
+    if s1 != 1:
         x = x.contiguous()
-    y = torch.empty((x.shape[0], n), dtype=x.dtype, device=x.device)
+        ldx = k
+    m = x.shape[0]
+    y = x.new_empty((m, n))
     if not scale.is_contiguous():
         scale = scale.contiguous()
     if bias is not None and not bias.is_contiguous():
         bias = bias.contiguous()
     with _on(x.device):
-        K.int8_linear(x, q, scale, bias, y)
+        K.int8_linear(x, m, k, ldx, at, n, ldq, readable, scale, bias, y)
     return y
 
 
@@ -1898,22 +1902,30 @@ def linear_int8(x, q, scale, bias):
 # ----------------------------------------------------------------------------------------------
 def orthogonalize(mats, steps, coefficients, eps):
     """``functional.orthogonalize`` of a list: all matrices (and stacks) of a call share its launches."""
-    outs = [torch.empty(m.shape, dtype=_BF16, device=m.device) for m in mats]
-    groups, keep = [], []
-    for m, o in zip(mats, outs):
-        if m.numel() == 0:
+    device, bf16 = mats[0].device, mats[0].dtype == _BF16
+    outs, groups, sizes, keep = [], [], [], []
+    for m in mats:
+        o = torch.empty(m.shape, dtype=_BF16, device=device)
+        outs.append(o)
+        batch, r, c = m.shape if m.dim() == 3 else (1,) + m.shape
+        if batch == 0 or r == 0 or c == 0:
             continue
-        m3, o3 = (m, o) if m.dim() == 3 else (m[None], o[None])
-        if max(m3.stride()[1:]) >= 1 << 31:
-            m3 = m3.contiguous()
-            keep.append(m3)
-        groups.append((m3.data_ptr(),) + m3.stride() + (o.data_ptr(),) + o3.stride() + (m3.shape[1], m3.shape[2], m3.shape[0]))
+        strides = m.stride()
+        if max(strides[-2:]) >= 1 << 31:
+            m = m.contiguous()
+            keep.append(m)
+            strides = m.stride()
+        if len(strides) == 2:
+            strides = (0,) + strides
+        size = (r, c, batch)
+        groups.append((m.data_ptr(),) + strides + (o.data_ptr(), r * c, c, 1) + size)
+        sizes.append(size)
     per = K.ortho_max_groups()
-    with _on(mats[0].device):
+    with _on(device):
         for k in range(0, len(groups), per):
-            table, count = K.ortho_table(groups[k:k + per])
-            work = torch.empty(K.ortho_workspace(table, count), dtype=torch.uint8, device=mats[0].device)
-            K.orthogonalize(table, count, mats[0].dtype == _BF16, coefficients, steps, eps, work)
+            nbytes = K.ortho_workspace_of(tuple(sizes[k:k + per]))
+            work = torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
+            K.orthogonalize(*K.ortho_table(groups[k:k + per]), bf16, coefficients, steps, eps, work)
     return outs
 
 

@@ -260,7 +260,7 @@ def ortho_max_groups():
 def ortho_table(groups):
     """Table of a call: ``groups`` = (source address, its batch / row / column strides, destination address and strides,
     rows, columns, matrices) tuples."""
-    flat = [int(v) for g in groups for v in g]
+    flat = [v for g in groups for v in g]
     return (ctypes.c_longlong * len(flat))(*flat), len(flat) // 11
 
 
@@ -272,6 +272,7 @@ def ortho_coefficients_ok(a, b, c, steps):
 
 
 def ortho_workspace(table, count):
+    """Bytes of workspace of a call; 0: it needs none."""
     f = getattr(lib(), "ddl_ortho_workspace")
     f.restype = ctypes.c_longlong
     n = int(f(table, _i32(count)))
@@ -280,11 +281,17 @@ def ortho_workspace(table, count):
     return n
 
 
+@functools.lru_cache(maxsize=256)
+def ortho_workspace_of(sizes):
+    """The same from the groups' (rows, columns, matrices) alone."""
+    return ortho_workspace(*ortho_table([(0,) * 8 + s for s in sizes]))
+
+
 def orthogonalize(table, count, src_bf16, coefficients, steps, eps, work):
     """bf16 destinations <- the orthogonalised sources of ``table`` (:func:`ortho_table`)."""
     f = _fn("ddl_orthogonalize", "p ii fff i f p q p")
-    check(f(table, count, 1 if src_bf16 else 0, coefficients[0], coefficients[1], coefficients[2], steps, eps, work.data_ptr(),
-            work.numel(), _raw_stream()), "orthogonalize")
+    check(f(table, count, 1 if src_bf16 else 0, coefficients[0], coefficients[1], coefficients[2], steps, eps, _p(work),
+            0 if work is None else work.numel(), _raw_stream()), "orthogonalize")
 
 
 def muon_step_(table, count, w, g, v, lowp, lr, mu, wd, nesterov, lr_scale, coefficients, steps, eps, work):
@@ -300,8 +307,8 @@ def muon_step_(table, count, w, g, v, lowp, lr, mu, wd, nesterov, lr_scale, coef
             raise KernelError("muon_step: matrix %d ends behind the arenas" % i)
     f = _fn("ddl_muon_step", "p i pppp i fff i p fff i f p q p")
     check(f(table, count, w.data_ptr(), g.data_ptr(), v.data_ptr(), _p(lowp), 1 if g.dtype == torch.bfloat16 else 0, lr, mu, wd,
-            1 if nesterov else 0, _p(lr_scale), coefficients[0], coefficients[1], coefficients[2], steps, eps, work.data_ptr(),
-            work.numel(), _raw_stream()), "muon_step")
+            1 if nesterov else 0, _p(lr_scale), coefficients[0], coefficients[1], coefficients[2], steps, eps, _p(work),
+            0 if work is None else work.numel(), _raw_stream()), "muon_step")
 
 
 # ---- dense layer on 8-bit integers (csrc/kernels/int8_linear.hip) -----------------------------
@@ -325,15 +332,14 @@ def _int8_workspace(M, N, Kd):
     return int(f(_i64(M), _i32(N), _i32(Kd)))
 
 
-def int8_linear(x, q, scale, bias, y):
-    """``y`` [M, N] (dense) from ``x`` [M, K] and the codes ``q`` [N, K]; see ``functional.linear_int8``."""
-    M, Kd = x.shape
-    N = q.shape[0]
+def int8_linear(x, M, Kd, ldx, q, N, ldq, q_bytes, scale, bias, y):
+    """``y`` [M, N] (dense) from ``x`` [M, K] (row stride ``ldx``) and the codes ``q`` [N, K] (addresses; row stride ``ldq``,
+    readable for ``q_bytes``); see ``functional.linear_int8``."""
     nbytes = _int8_workspace(M, N, Kd)
     work = torch.empty(nbytes, dtype=torch.uint8, device=x.device) if nbytes else None
     f = _fn("ddl_int8_linear", "p i q p qq pp p q q ii p q p")
-    check(f(x.data_ptr(), 1 if x.dtype == torch.bfloat16 else 0, x.stride(0), q.data_ptr(), q.stride(0), storage_numel_from(q),
-            scale.data_ptr(), _p(bias), y.data_ptr(), N, M, N, Kd, _p(work), nbytes, _raw_stream()), "int8_linear")
+    check(f(x.data_ptr(), x.dtype is torch.bfloat16, ldx, q, ldq, q_bytes, scale.data_ptr(), _p(bias), y.data_ptr(), N, M, N, Kd,
+            _p(work), nbytes, _raw_stream()), "int8_linear")
 
 
 # ---- convolution / GEMM (csrc/kernels/conv_igemm.hip, conv_wgrad.hip) ------------------------

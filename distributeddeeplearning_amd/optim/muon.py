@@ -91,7 +91,7 @@ class FusedMuon(_ArenaOptimizer):
             if hip:
                 lowp = self.arena.params[dt] if dt in self.master else None
                 for table, count, nbytes in self._tables(entry):
-                    work = torch.empty(nbytes, dtype=torch.uint8, device=w.device)
+                    work = torch.empty(nbytes, dtype=torch.uint8, device=w.device) if nbytes else None
                     kernels.muon_step_(table, count, w, g, v, lowp, klr, mu, run_wd, nesterov, kscale, coefficients,
                                        steps, eps, work)
                 continue

@@ -162,19 +162,19 @@ def test_sizes_that_the_kernels_refuse():
     with pytest.raises(kernels.KernelError, match="out of range"):      # (the second matrix has 1024 sums)
         kernels.ortho_workspace(table, count)
     table, count = kernels.ortho_table([row(4, 4, (1 << 22) - 1026), row(32704, 32704)])
-    assert kernels.ortho_workspace(table, count) > 0
+    assert kernels.ortho_workspace(table, count) > 0 and kernels.ortho_workspace(*kernels.ortho_table([row(64, 512), row(100, 256)])) == 0
     lib = kernels.lib()
     ok = (3.4445, -4.7750, 2.0315)
     assert kernels.ortho_coefficients_ok(*ok, 5) and not kernels.ortho_coefficients_ok(*ok, 65) and not kernels.ortho_coefficients_ok(*ok, 0)
 
-    def call(steps=5, eps=1e-7, kind=0, ws=256, nbytes=1 << 40, table=kernels.ortho_table([row(8, 8)])[0], count=1, coef=ok):
+    def call(steps=5, eps=1e-7, kind=0, ws=256, nbytes=1 << 40, table=kernels.ortho_table([row(300, 300)])[0], count=1, coef=ok):
         f = lib.ddl_orthogonalize
         c = __import__("ctypes")
         return f(table, c.c_int(count), c.c_int(kind), *(c.c_float(v) for v in coef), c.c_int(steps), c.c_float(eps), c.c_void_p(ws),
                  c.c_longlong(nbytes), c.c_void_p(0))
 
-    no_source = kernels.ortho_table([(0,) + row(8, 8)[1:]])[0]
-    no_stride = kernels.ortho_table([row(8, 8)[:2] + (1 << 31,) + row(8, 8)[3:]])[0]
+    no_source = kernels.ortho_table([(0,) + row(300, 300)[1:]])[0]
+    no_stride = kernels.ortho_table([row(300, 300)[:2] + (1 << 31,) + row(300, 300)[3:]])[0]
     for kw in (dict(steps=0), dict(steps=65), dict(eps=0.0), dict(eps=float("nan")), dict(kind=2), dict(kind=-1), dict(ws=0), dict(ws=64), dict(nbytes=100),
                dict(count=-1), dict(coef=(100.0, 0.0, 0.0)), dict(table=no_source), dict(table=no_stride)):
         assert call(**kw) != 0, kw
