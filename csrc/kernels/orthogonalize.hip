@@ -197,7 +197,8 @@ __device__ __forceinline__ float direction_of(const Muon& mu, float g, float v) 
 // sums of squares in 64 bits (an fp32 square overflows from 1.8e19 on and vanishes below 1e-23): one partial a workgroup.
 // (The new momentum is not stored here: ortho_pack_kernel computes it again, and what this pass read may still be in the
 // memory-side cache then.)
-// A chunk of groups a launch; its first workgroup writes the table for the kernels behind it.
+// A chunk of groups a launch; its first workgroup writes the table for the kernels behind it.  Bound by memory: ResNet-50's
+// gradients and momentum (153 MB) 37 us.
 template <int KIND>
 __global__ void __launch_bounds__(1024) ortho_sqsum_kernel(const Chunk ch, const Muon mu, double* __restrict__ part, Table* __restrict__ t,
                                                            unsigned* __restrict__ counters, int slabs) {
@@ -271,7 +272,8 @@ __device__ __forceinline__ double inverse_of(double norm, float eps, int& shift)
 }
 
 // hi + lo of the scaled, normalised matrix; one 64 x 64 tile of the padded workspace a workgroup.  A lane's 8 elements run along
-// the source's rows in both orientations.
+// the source's rows in both orientations.  Bound by memory: ResNet-50 from bf16 (51 MB in, 102 MB out) 29 us; with its momentum
+// (153 MB in, 204 MB out) 68 us.
 template <int KIND>
 __global__ void __launch_bounds__(256) ortho_pack_kernel(const Table* __restrict__ t, const Muon mu, const double* __restrict__ part, float eps,
                                                         int* __restrict__ ex, f16_t* __restrict__ xh, f16_t* __restrict__ xl) {
@@ -423,7 +425,9 @@ __device__ __forceinline__ void tri_tile(int idx, int rows, int& ti, int& tj) {
     tj = band * 8 + left - i * (i + 1) / 2;
 }
 
-// SQUARE = false: O, d of A = X X^T.  SQUARE = true: O, d of P = b A + c A^2 (diagonal: + a) from those of A
+// SQUARE = false: O, d of A = X X^T.  SQUARE = true: O, d of P = b A + c A^2 (diagonal: + a) from those of A.
+// Only tiles on and below the diagonal are computed and written twice.  4096 x 8192: 166 and 100 us (tiles of 256, bound by the
+// matrix pipe: 880 TFLOP/s in X X^T); 12 of 512 x 512: 8.6 and 9.8 us (432 tiles of 64, bound by the latency of their 8 stages).
 template <int B, int W0, int W1, int NST, int KS, bool SQUARE>
 __global__ void __launch_bounds__(KS * W0 * W1 * 64, B == 128 ? 4 : 2) ortho_sym_kernel(const Table* __restrict__ t, const f16_t* __restrict__ in, const float* __restrict__ din,
                                                           f16_t* __restrict__ out, float* __restrict__ dout, const int* __restrict__ ex, int down,
@@ -518,7 +522,9 @@ __global__ void __launch_bounds__(KS * W0 * W1 * 64, B == 128 ? 4 : 2) ortho_sym
     }
 }
 
-// X' = pd X + offdiag(P) X_hi; tile: BF columns of X times BS rows of P.  FINAL 0: the next X; 1: the output; 2: the weights (K23)
+// X' = pd X + offdiag(P) X_hi; tile: BF columns of X times BS rows of P.  FINAL 0: the next X; 1: the output; 2: the weights (K23).
+// 4096 x 8192: 250 us (tiles of 256, bound by the matrix pipe: 1100 TFLOP/s); all of ResNet-50: 60 us (tiles of 128, bound by X's
+// pairs, 204 MB in and out), 97 us where it writes the weights; 12 of 512 x 512: 12 us (768 tiles of 64, latency).
 template <int BF, int BS, int W0, int W1, int NST, int KS, int FINAL>
 __global__ void __launch_bounds__(KS * W0 * W1 * 64, BF == 128 ? 4 : 2) ortho_apply_kernel(const Table* __restrict__ t, const Muon mu, const f16_t* __restrict__ P,
                                                             const float* __restrict__ pd, const f16_t* __restrict__ xh, const f16_t* __restrict__ xl,
@@ -597,7 +603,8 @@ __global__ void __launch_bounds__(KS * W0 * W1 * 64, BF == 128 ? 4 : 2) ortho_ap
 // ---- small matrices: all steps in one launch ----------------------------------------------------------------------------
 // One workgroup of 8 waves a matrix: np = NP padded rows, up to 128 CB columns.  X stays in registers in fp32 (in the layout of the
 // products' results: wave w has the 16-column blocks w, w + 8, ..; a lane 4 columns of rows lane % 16 + 16 j), X_hi, O and
-// P in LDS; pd X is the accumulator that P X is added to.  What bounds it is latency: the other path is 19 launches of 4 us.
+// P in LDS; pd X is the accumulator that P X is added to.  What bounds it is latency: 64 x 64 takes 12 us here,
+// and the tiles 17 launches of 5 us.
 template <int NP, int CB, int KIND>
 __global__ void __launch_bounds__(512, 2) ortho_small_kernel(const Chunk ch, const Muon mu, float ca, float cb, float cc, int steps, int fall, float eps) {
     constexpr bool BF = KIND & 1;
@@ -835,9 +842,9 @@ __global__ void __launch_bounds__(512, 2) ortho_small_kernel(const Chunk ch, con
 // long side is read twice and never iterated on: Gram matrix a chunk of columns a workgroup, all steps in one workgroup a matrix,
 // result a chunk of columns a workgroup.  An error of A_0 grows by up to 3e4 where a singular value vanishes, so A and Q are
 // computed in fp64 (its matrix instruction); Q reaches a^steps = 485 with cancelling entries: the result's product is fp32.
-// Bound by the latency of four launches.  Measured against the
-// tiles below: 17 x 2762 105 -> 46 us, 32 x 2048 94 -> 37, 59 of 1 x 3157 209 -> 34, 1000 of 32 x 600 602 -> 192, 32 x 100000
-// 1186 -> 131; 64 rows: 86 -> 80 us in fp32, and too few digits.  Error against 64 bits: 1e-5 before the rounding to bf16.
+// Bound by the latency of four launches.  Measured against the tiles below: 17 x 2762 105 -> 46 us, 32 x 2048 94 -> 37, 59 of
+// 1 x 3157 209 -> 34, 1000 of 32 x 600 602 -> 192, 32 x 100000 226 -> 131; 64 rows: 86 -> 80 us in fp32, and too few digits.
+// Error against 64 bits: 1e-5 before the rounding to bf16.
 typedef double f64x4 __attribute__((ext_vector_type(4)));
 
 // value of X (before its scale) at row r, column c; STORE: the new momentum is stored
@@ -1463,6 +1470,8 @@ extern "C" int ddl_orthogonalize(const long long* desc, int count, int kind, flo
     for (int i = 0; i < count; ++i)
         if (!q[i].src || !q[i].dst || !strides_fit(q[i].srs, q[i].scs) || !strides_fit(q[i].drs, q[i].dcs) || q[i].sb < 0 || q[i].db < 0)
             return DDL_EINVAL;
+    for (int i = 0; i < count; ++i)
+        if (!ddl_aligned16((const void*)q[i].dst)) return DDL_EALIGN;
     return run_all(q, count, kind, Muon{}, a, b, c, steps, eps, (char*)ws, stream);
 }
 

@@ -255,7 +255,7 @@ __device__ __forceinline__ bool join_parts(const M& m, void* tile, V* slabs, uns
         }
         pairs[k] = (u64)__builtin_bit_cast(unsigned, s1) << 32 | __builtin_bit_cast(unsigned, s0);
     }
-    if (threadIdx.x == 0) *counter = 0u;
+    if (threadIdx.x == 0) __hip_atomic_store(counter, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     __syncthreads();
     return true;
 }

@@ -233,7 +233,8 @@ def orthogonalize(x, steps=5, coefficients=ORTHO_COEFFICIENTS, eps=1e-7):
     ``x``: a matrix [r, c], a stack [k, r, c], or a list / tuple of matrices of any shapes (they share the launches), fp32 or
     bf16 of any strides; returns bf16 of the same shape(s).  No gradient flows through it: an input that requires one is
     refused outside ``torch.no_grad()``.  Matrices do not influence each other; one that holds an infinity or a NaN
-    gives NaN, a zero matrix zeros.  ``coefficients`` whose steps leave the range of 16-bit operands are refused."""
+    gives NaN, a zero matrix zeros.  ``coefficients`` whose steps leave the range of 16-bit operands are refused, and on the
+    GPU matrices whose sides, rounded up to 64, have a product of 2^30 or more."""
     many = isinstance(x, (list, tuple))
     mats = list(x) if many else [x]
     _check_steps(steps, coefficients, eps)
