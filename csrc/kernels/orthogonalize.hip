@@ -15,8 +15,8 @@
 // thousandth (2-norm); bf16 operands throughout give 8e-3 .. 0.3, plain fp16 1e-3 .. 4e-2.
 //
 // A call takes up to 64 groups of equal matrices; all of them share each launch.  Three forms, by sizes alone:
-//   * every matrix of up to 64 x 512 or 128 x 256: a workgroup a matrix, one launch (ortho_small_kernel);
-//   * else, every matrix of up to 32 rows: four launches, all steps on the Gram matrix (ortho_thin_*_kernel);
+//   * every matrix of up to 64 x 768 or 128 x 384: a workgroup a matrix, one launch (ortho_small_kernel, all_small);
+//   * else, or from some length on, every matrix of up to 32 rows: four launches, all steps on the Gram matrix (ortho_thin_*_kernel);
 //   * else tiles: sums of squares (whose first workgroup writes the table of shapes and offsets, from the kernel's arguments: a
 //     call can be captured or recorded and copies nothing to the device), packing, three products a step; the last product
 //     writes the result or the weights.
@@ -1264,17 +1264,23 @@ long long splits_of(const Desc* q, int count, int sym, int* split) {
     return slabs;
 }
 
-// Calls that ortho_small_kernel serves: every matrix of up to 64 rows (its shorter side) and 512 columns, or 128 and 256
-int small_class(const Desc& s) {            // 0: none, else 8 * padded rows / 64 + the smallest CB
-    const long long n = s.r < s.c ? s.r : s.c, m = s.r < s.c ? s.c : s.r;
-    if (n <= 64 && m <= 512) return 8 + (m <= 128 ? 0 : m <= 256 ? 1 : 2);
-    if (n <= 128 && m <= 256) return 16 + (m <= 128 ? 0 : 1);
+// Calls that ortho_small_kernel serves: every matrix of up to 64 rows (its shorter side) and 768 columns, or 128 and 384 (more
+// do not fit the registers and, 128 rows, LDS).  Tiles against it: 64 x 576 79 -> 34 us, 64 x 768 80 -> 40, 128 x 384 85 -> 62, 1000 of 64 x 600
+// 651 -> 154, 1000 of 128 x 384 832 -> 294.  All are computed in the largest's size, as each size is a launch of 12 to 70 us, most of it the
+// first run of its code: 64 x 147, 64 x 64, 64 x 576, 256 x 64 and 64 x 256 82 -> 34.  Not where the Gram matrix's form is faster:
+// all up to 32 rows and one of more than 512 columns (32 x 1000 31 us, here 48), up to 16 and more than 256 (1000 of 16 x 300 54, here
+// 89; one 9 x 512 22, here 25).  Returns 0: not served; else 8 * padded rows / 64 + the number of the least columns, 128, 256, ..
+int all_small(const Desc* q, int count) {
+    long long most = 0, wide = 0;
+    for (int i = 0; i < count; ++i) {
+        const long long n = q[i].r < q[i].c ? q[i].r : q[i].c, m = q[i].r < q[i].c ? q[i].c : q[i].r;
+        most = n > most ? n : most;
+        wide = m > wide ? m : wide;
+    }
+    if ((most <= 16 && wide > 256) || (most <= 32 && wide > 512)) return 0;
+    if (most <= 64 && wide <= 768) return 8 + (wide <= 128 ? 0 : wide <= 256 ? 1 : wide <= 512 ? 2 : 3);
+    if (most <= 128 && wide <= 384) return 16 + (wide <= 128 ? 0 : wide <= 256 ? 1 : 2);
     return 0;
-}
-bool all_small(const Desc* q, int count) {
-    for (int i = 0; i < count; ++i)
-        if (!small_class(q[i])) return false;
-    return true;
 }
 template <int KIND>
 int launch_small(int cls, const Chunk& ch, unsigned grid, const Muon& mu, float a, float b, float c, int steps, int fall, float eps, hipStream_t stream) {
@@ -1283,30 +1289,21 @@ int launch_small(int cls, const Chunk& ch, unsigned grid, const Muon& mu, float 
         case 8: SMALL(64, 1); break;
         case 9: SMALL(64, 2); break;
         case 10: SMALL(64, 4); break;
+        case 11: SMALL(64, 6); break;
         case 16: SMALL(128, 1); break;
-        default: SMALL(128, 2); break;
+        case 17: SMALL(128, 2); break;
+        default: SMALL(128, 3); break;
     }
 #undef SMALL
     return ddl_launch_status();
 }
-int run_small(const Desc* q, int count, int kind, const Muon& mu, float a, float b, float c, int steps, float eps, hipStream_t stream) {
+int run_small(const Desc* q, int count, int cls, int kind, const Muon& mu, float a, float b, float c, int steps, float eps, hipStream_t stream) {
     const int fall = growth_bits(a, b, c, steps);
-    static const int classes[5] = {8, 9, 10, 16, 17};
-    for (int k = 0; k < 5; ++k) {
+    for (int base = 0; base < count; base += CHUNK) {
         Chunk ch;
         memset(&ch, 0, sizeof(ch));
         long long grid = 0;
-        for (int i = 0; i <= count; ++i) {
-            if (ch.n && (i == count || ch.n == CHUNK)) {
-                const int rc = kind == 0 ? launch_small<0>(classes[k], ch, (unsigned)grid, mu, a, b, c, steps, fall, eps, stream)
-                             : kind == 1 ? launch_small<1>(classes[k], ch, (unsigned)grid, mu, a, b, c, steps, fall, eps, stream)
-                             : kind == 2 ? launch_small<2>(classes[k], ch, (unsigned)grid, mu, a, b, c, steps, fall, eps, stream)
-                                         : launch_small<3>(classes[k], ch, (unsigned)grid, mu, a, b, c, steps, fall, eps, stream);
-                if (rc != DDL_OK) return rc;
-                ch.n = 0;
-                grid = 0;
-            }
-            if (i == count || small_class(q[i]) != classes[k]) continue;
+        for (int i = base; i < count && i < base + CHUNK; ++i) {
             Group& o = ch.g[ch.n++];
             const Desc& s = q[i];
             o.src = (const void*)s.src; o.dst = (bf16_t*)s.dst; o.sb = s.sb; o.rs = (int)s.srs; o.cs = (int)s.scs;
@@ -1316,6 +1313,11 @@ int run_small(const Desc* q, int count, int kind, const Muon& mu, float a, float
             o.fin = (unsigned)grid;
             grid += s.batch;
         }
+        const int rc = kind == 0 ? launch_small<0>(cls, ch, (unsigned)grid, mu, a, b, c, steps, fall, eps, stream)
+                     : kind == 1 ? launch_small<1>(cls, ch, (unsigned)grid, mu, a, b, c, steps, fall, eps, stream)
+                     : kind == 2 ? launch_small<2>(cls, ch, (unsigned)grid, mu, a, b, c, steps, fall, eps, stream)
+                                 : launch_small<3>(cls, ch, (unsigned)grid, mu, a, b, c, steps, fall, eps, stream);
+        if (rc != DDL_OK) return rc;
     }
     return DDL_OK;
 }
@@ -1324,7 +1326,7 @@ int run_small(const Desc* q, int count, int kind, const Muon& mu, float a, float
 int run_all(const Desc* q, int count, int kind, const Muon& mu, float a, float b, float c, int steps, float eps, char* ws, hipStream_t stream) {
     Plan pl;
     if (!plan_of(q, count, thin_steps(a, b, c, steps), pl)) return DDL_EINVAL;
-    if (all_small(q, count)) return run_small(q, count, kind, mu, a, b, c, steps, eps, stream);
+    if (const int cls = all_small(q, count)) return run_small(q, count, cls, kind, mu, a, b, c, steps, eps, stream);
     int sb = 64, ab = 64, split[MAXG];
     tiles_of(q, count, sb, ab);
     splits_of(q, count, sb, split);

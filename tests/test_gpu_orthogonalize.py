@@ -530,3 +530,43 @@ def test_long_rows_in_graphs_and_in_the_optimizer():
     opt.step()
     for (_, p), w, b in zip(named, wants, before):
         assert float((p.detach() - w).norm()) <= 2 ** -8 * float((w - b).norm()) + 2 ** -22 * float(b.norm())
+
+
+# the largest sizes that a workgroup holds, the next ones, and those that the Gram matrix's form takes before
+@pytest.mark.parametrize("shape", [(64, 576), (33, 577), (64, 768), (50, 767), (64, 769), (128, 257), (65, 384), (128, 384), (127, 383), (128, 385), (129, 384),
+                                   (16, 256), (16, 257), (17, 512), (17, 513), (300, 64, 600), (260, 20, 300), (260, 16, 300), (3, 100, 380)], ids=str)
+@pytest.mark.parametrize("dtype", [torch.float32, BF], ids=["fp32", "bf16"])
+def test_borders_of_one_workgroup(shape, dtype):
+    from distributeddeeplearning_amd.ops import functional as ops
+
+    for kind in ("gauss", "exp"):
+        g = spectrum(kind, *shape[-2:], seed=10).to(DEV, dtype)
+        x = g if len(shape) == 2 else torch.stack([g * (k + 1) for k in range(shape[0])])
+        for y in (x, x.transpose(-2, -1), x.transpose(-2, -1).contiguous()):
+            out = ops.orthogonalize(y)
+            for k in (0,) if len(shape) == 2 else (0, 1, shape[0] - 1):
+                o, v = (out, y) if len(shape) == 2 else (out[k], y[k])
+                assert off(o, v) < TOL
+
+
+# one size for all: lists whose rows, columns and classes differ; more than one launch's groups
+@pytest.mark.parametrize("shapes", [[(64, 147), (64, 64), (64, 576), (256, 64), (64, 256)], [(64, 147), (128, 64), (100, 300), (5, 5), (384, 1)],
+                                    [(100, 100), (64, 700)], [(16, 256), (3, 2)], [(16, 300), (64, 64)], [(9 + i, 700 - 8 * i) for i in range(50)]], ids=str)
+def test_lists_of_small_matrices(shapes):
+    from distributeddeeplearning_amd.ops import functional as ops
+    from distributeddeeplearning_amd.optim import FusedMuon
+
+    mats = [spectrum("power", *s, seed=i).to(DEV) for i, s in enumerate(shapes)]
+    outs = ops.orthogonalize(mats)
+    for m, o in zip(mats, outs):
+        assert off(o, m) < TOL
+    named = _params(shapes, torch.float32)
+    opt = FusedMuon(named, lr=1.0, momentum=0.0, nesterov=False)
+    before = [p.detach().clone() for _, p in named]
+    for (_, p), m in zip(named, mats):
+        p.grad.copy_(m)
+    opt.step()
+    # the operator's result before its rounding to bf16: half a step, 2^-8, from it
+    for (_, p), w, o in zip(named, before, outs):
+        want = w - max(1.0, w.shape[0] / w.shape[1]) ** 0.5 * o.float()
+        assert float((p.detach() - want).norm()) <= 2 ** -8 * float((want - w).norm()) + 2 ** -22 * float(w.norm())
