@@ -42,7 +42,7 @@ struct Group {                      // `batch` equal matrices
     int rs, cs;                     // strides of a row, of a column of src
     int r, c, np, mp;               // sizes; padded shorter and longer side
     int batch;
-    int vec;                        // src (K23: the arenas) can be read 8 elements of a row at a time
+    short vec, flat;                // src (K23: the arenas) can be read 8 elements of a row at a time; src is one array from 16 bytes on
     int part_elems, parts;          // elements of a partial sum of squares, partial sums of a matrix
     unsigned xo, ao, dof, po, mat;  // first matrix in the X and square workspaces (64 elements), in the diagonals, the partial sums, among all
     int tsym, tapp;                 // tiles of a matrix in the symmetric products and in P X
@@ -110,11 +110,35 @@ __device__ __forceinline__ int find_group(const unsigned* first, unsigned at) {
 }
 // item of a product -> group, matrix, tile and what the product needs to know.  Every lane reads its group's values at once and
 // the one that is meant is picked afterwards: a tile waits for one load, not for two in a row.
+// What Item needs of a call's only group (ONE, tiles of 64): it travels in the arguments, a round trip to memory less in each launch
+// (301 x 410 105 -> 101 us, 12 of 512 x 512 153 -> 149)
+struct Single { int np, mp, batch, tsym, tapp, split; };
+template <bool ONE>
 struct Item {
     int gi, b, tile, np, mp, part, split;
     unsigned xo, ao, dof, mat, slab;
-    __device__ __forceinline__ bool find(const Table* t, bool sym) {      // false: this XCD has no such item
+    __device__ __forceinline__ bool find(const Table* t, const Single& one, bool sym) {      // false: this XCD has no such item
         const unsigned xcd = blockIdx.x & 7, at = blockIdx.x >> 3;
+        part = 0;
+        split = 1;
+        if (ONE) {
+            gi = 0;
+            np = one.np;
+            mp = one.mp;
+            xo = ao = dof = mat = slab = 0u;
+            const unsigned tiles = sym ? one.tsym : one.tapp, total = (unsigned)one.batch * tiles, idx = at + run_start(total, -1, xcd);
+            if (idx >= run_start(total, -1, xcd + 1)) return false;
+            b = idx / tiles;
+            tile = idx - b * tiles;
+            if (sym) {
+                split = one.split;
+                const int whole = tile / split;
+                part = tile - whole * split;
+                slab = idx - part;
+                tile = whole;
+            }
+            return true;
+        }
         const int lane = threadIdx.x & 63;
         const unsigned first = sym ? t->fsym[xcd][lane] : t->fapp[xcd][lane];
         const int l_tiles = sym ? t->tsym[lane] : t->tapp[lane], l_home = sym ? t->hsym[lane] : t->happ[lane];
@@ -135,8 +159,6 @@ struct Item {
         if (idx >= run_start(total, home, xcd + 1)) return false;
         b = idx / tiles;
         tile = idx - b * tiles;
-        part = 0;
-        split = 1;
         if (sym) {
             split = __builtin_amdgcn_readlane(l_split, gi);
             const int whole = tile / split;
@@ -234,7 +256,7 @@ __global__ void __launch_bounds__(1024) ortho_sqsum_kernel(const Chunk ch, const
             const float gr = load1<BF>(mu.g, e), u = direction_of(mu, gr, momentum_of(mu, gr, mu.v[e]));
             s += (double)u * (double)u;
         }
-    } else if (g.vec && g.rs == g.c) {       // dense
+    } else if (g.flat) {
         const long long end8 = lo + ((hi - lo) & ~7LL);
         for (long long e = lo + threadIdx.x * 8; e < end8; e += 8192) {
             float u[8];
@@ -248,7 +270,7 @@ __global__ void __launch_bounds__(1024) ortho_sqsum_kernel(const Chunk ch, const
         }
     } else {
         for (long long e = lo + threadIdx.x; e < hi; e += 1024) {
-            const int i = (int)(e / g.c), j = (int)(e - (long long)i * g.c);
+            const unsigned i = (unsigned)e / (unsigned)g.c, j = (unsigned)e - i * (unsigned)g.c;
             const float u = load1<BF>(g.src, b * g.sb + (long long)i * g.rs + (long long)j * g.cs);
             s += (double)u * (double)u;
         }
@@ -428,14 +450,14 @@ __device__ __forceinline__ void tri_tile(int idx, int rows, int& ti, int& tj) {
 // SQUARE = false: O, d of A = X X^T.  SQUARE = true: O, d of P = b A + c A^2 (diagonal: + a) from those of A.
 // Only tiles on and below the diagonal are computed and written twice.  4096 x 8192: 166 and 100 us (tiles of 256, bound by the
 // matrix pipe: 880 TFLOP/s in X X^T); 12 of 512 x 512: 8.6 and 9.8 us (432 tiles of 64, bound by the latency of their 8 stages).
-template <int B, int W0, int W1, int NST, int KS, bool SQUARE>
-__global__ void __launch_bounds__(KS * W0 * W1 * 64, B == 128 ? 4 : 2) ortho_sym_kernel(const Table* __restrict__ t, const f16_t* __restrict__ in, const float* __restrict__ din,
+template <int B, int W0, int W1, int NST, int KS, bool SQUARE, bool ONE>
+__global__ void __launch_bounds__(KS * W0 * W1 * 64, B == 128 ? 4 : 2) ortho_sym_kernel(const Table* __restrict__ t, const Single one, const f16_t* __restrict__ in, const float* __restrict__ din,
                                                           f16_t* __restrict__ out, float* __restrict__ dout, const int* __restrict__ ex, int down,
                                                           float ca, float cb, float cc, float* __restrict__ slabs, unsigned* __restrict__ counters) {
     typedef TileMul<MulF16, B, B, W0, W1, NST, false, KS> M;
     __shared__ __attribute__((aligned(16))) unsigned char smem[M::LDS];
-    Item it;
-    if (!it.find(t, true) || (SQUARE && it.part > 0)) return;
+    Item<ONE> it;
+    if (!it.find(t, one, true) || (SQUARE && it.part > 0)) return;
     const int np = it.np, lda = np, ld = SQUARE ? np : it.mp, b = it.b;
     const int each = SQUARE ? np / 64 : (ld / 64 + it.split - 1) / it.split, k0 = SQUARE ? 0 : it.part * each;
     const int stages = ld / 64 - k0 < each ? ld / 64 - k0 : each;
@@ -525,15 +547,15 @@ __global__ void __launch_bounds__(KS * W0 * W1 * 64, B == 128 ? 4 : 2) ortho_sym
 // X' = pd X + offdiag(P) X_hi; tile: BF columns of X times BS rows of P.  FINAL 0: the next X; 1: the output; 2: the weights (K23).
 // 4096 x 8192: 250 us (tiles of 256, bound by the matrix pipe: 1100 TFLOP/s); all of ResNet-50: 60 us (tiles of 128, bound by X's
 // pairs, 204 MB in and out), 97 us where it writes the weights; 12 of 512 x 512: 12 us (768 tiles of 64, latency).
-template <int BF, int BS, int W0, int W1, int NST, int KS, int FINAL>
-__global__ void __launch_bounds__(KS * W0 * W1 * 64, BF == 128 ? 4 : 2) ortho_apply_kernel(const Table* __restrict__ t, const Muon mu, const f16_t* __restrict__ P,
+template <int BF, int BS, int W0, int W1, int NST, int KS, int FINAL, bool ONE>
+__global__ void __launch_bounds__(KS * W0 * W1 * 64, BF == 128 ? 4 : 2) ortho_apply_kernel(const Table* __restrict__ t, const Single one, const Muon mu, const f16_t* __restrict__ P,
                                                             const float* __restrict__ pd, const f16_t* __restrict__ xh, const f16_t* __restrict__ xl,
                                                             f16_t* __restrict__ yh, f16_t* __restrict__ yl,
                                                             const int* __restrict__ ex, int down, int down1) {
     typedef TileMul<MulF16, BF, BS, W0, W1, NST, true, KS> M;
     __shared__ __attribute__((aligned(16))) unsigned char smem[M::LDS];
-    Item it;
-    if (!it.find(t, false)) return;
+    Item<ONE> it;
+    if (!it.find(t, one, false)) return;
     const int np = it.np, mp = it.mp, b = it.b;
     int ti, tj;
     band_tile(it.tile, (np + BS - 1) / BS, (mp + BF - 1) / BF, ti, tj);
@@ -1349,6 +1371,7 @@ int run_all(const Desc* q, int count, int kind, const Muon& mu, float a, float b
         o.src = (const void*)s.src; o.dst = (bf16_t*)s.dst; o.sb = s.sb; o.rs = (int)s.srs; o.cs = (int)s.scs;
         o.r = (int)s.r; o.c = (int)s.c; o.np = (int)np; o.mp = (int)mp; o.batch = (int)s.batch;
         o.vec = vec_of(s, kind);
+        o.flat = s.scs == 1 && s.srs == s.c && (s.batch == 1 || s.sb % 8 == 0) && ((uintptr_t)s.src & 15) == 0;
         o.part_elems = (int)pe; o.parts = (int)parts;
         o.xo = (unsigned)(xo / 64); o.ao = (unsigned)(ao / 64); o.dof = (unsigned)dof; o.po = (unsigned)po; o.mat = (unsigned)mat;
         const long long whole = sn * (sn + 1) / 2;
@@ -1373,6 +1396,7 @@ int run_all(const Desc* q, int count, int kind, const Muon& mu, float a, float b
     nsym = homes(g, count, true, csym);
     napp = homes(g, count, false, capp);
     if (nsym > most_wgs(512) || napp > most_wgs(512)) return DDL_EINVAL;
+    const Single one = count == 1 ? Single{g[0].np, g[0].mp, g[0].batch, g[0].tsym, g[0].tapp, g[0].split} : Single{};
     Table* t = (Table*)(ws + pl.table);
     f16_t *xh = (f16_t*)(ws + pl.xa_h), *xl = (f16_t*)(ws + pl.xa_l), *yh = (f16_t*)(ws + pl.xb_h), *yl = (f16_t*)(ws + pl.xb_l);
     f16_t *O = (f16_t*)(ws + pl.o), *P = (f16_t*)(ws + pl.p);
@@ -1414,25 +1438,30 @@ int run_all(const Desc* q, int count, int kind, const Muon& mu, float a, float b
 #undef PACK
     for (int k = 0; k < steps; ++k) {
         const int fin = k < steps - 1 ? 0 : (kind < 2 ? 1 : 2);
-#define SYM(B, W0, W1, NST, KS, SQ, IN, DIN, OUTP, DOUT, DOWN) DDL_KLAUNCH((ortho_sym_kernel<B, W0, W1, NST, KS, SQ>), dim3((unsigned)nsym), dim3(KS * W0 * W1 * 64), 0, stream, t, IN, DIN, OUTP, DOUT, ex, DOWN, a, b, c, slab, counters)
-#define SYM1(B, W0, W1, NST, KS) SYM(B, W0, W1, NST, KS, false, xh, (const float*)nullptr, O, d, k * fall)
-#define SYM2(B, W0, W1, NST, KS) SYM(B, W0, W1, NST, KS, true, O, d, P, pd, 0)
-#define APP1(B, W0, W1, NST, KS, FIN) DDL_KLAUNCH((ortho_apply_kernel<B, B, W0, W1, NST, KS, FIN>), dim3((unsigned)napp), dim3(KS * W0 * W1 * 64), 0, stream, t, mu, P, pd, xh, xl, yh, yl, ex, k * fall, (k + 1) * fall)
-#define APP(B, W0, W1, NST, KS) { if (fin == 0) APP1(B, W0, W1, NST, KS, 0); else if (fin == 1) APP1(B, W0, W1, NST, KS, 1); else APP1(B, W0, W1, NST, KS, 2); }
-        if (sb == 64) {
-            if (nsym <= 256) SYM1(64, 2, 2, 3, 2); else SYM1(64, 2, 2, 3, 1);
-            if (squares <= 256) SYM2(64, 2, 2, 3, 2); else SYM2(64, 2, 2, 3, 1);
-        } else if (sb == 128) {
-            SYM1(128, 2, 4, 2, 1);
-            SYM2(128, 2, 4, 2, 1);
-        } else {
-            SYM1(256, 2, 4, 2, 1);
-            SYM2(256, 2, 4, 2, 1);
+#define SYM(B, W0, W1, NST, KS, SQ, ONE, IN, DIN, OUTP, DOUT, DOWN) DDL_KLAUNCH((ortho_sym_kernel<B, W0, W1, NST, KS, SQ, ONE>), dim3((unsigned)nsym), dim3(KS * W0 * W1 * 64), 0, stream, t, one, IN, DIN, OUTP, DOUT, ex, DOWN, a, b, c, slab, counters)
+#define SYM1(B, W0, W1, NST, KS, ONE) SYM(B, W0, W1, NST, KS, false, ONE, xh, (const float*)nullptr, O, d, k * fall)
+#define SYM2(B, W0, W1, NST, KS, ONE) SYM(B, W0, W1, NST, KS, true, ONE, O, d, P, pd, 0)
+#define APP1(B, W0, W1, NST, KS, FIN, ONE) DDL_KLAUNCH((ortho_apply_kernel<B, B, W0, W1, NST, KS, FIN, ONE>), dim3((unsigned)napp), dim3(KS * W0 * W1 * 64), 0, stream, t, one, mu, P, pd, xh, xl, yh, yl, ex, k * fall, (k + 1) * fall)
+#define APP(B, W0, W1, NST, KS, ONE) { if (fin == 0) APP1(B, W0, W1, NST, KS, 0, ONE); else if (fin == 1) APP1(B, W0, W1, NST, KS, 1, ONE); else APP1(B, W0, W1, NST, KS, 2, ONE); }
+#define TILES64(ONE)                                                                                                         \
+        {                                                                                                                    \
+            if (sb == 64) {                                                                                                  \
+                if (nsym <= 256) SYM1(64, 2, 2, 3, 2, ONE); else SYM1(64, 2, 2, 3, 1, ONE);                                  \
+                if (squares <= 256) SYM2(64, 2, 2, 3, 2, ONE); else SYM2(64, 2, 2, 3, 1, ONE);                               \
+            }                                                                                                                \
         }
-        if (ab == 64 && napp <= 256) APP(64, 2, 2, 3, 2)
-        else if (ab == 64) APP(64, 2, 2, 3, 1)
-        else if (ab == 128) APP(128, 2, 4, 2, 1)
-        else APP(256, 2, 4, 2, 1)
+        if (one.np) TILES64(true) else TILES64(false)
+        if (sb == 128) {
+            SYM1(128, 2, 4, 2, 1, false);
+            SYM2(128, 2, 4, 2, 1, false);
+        } else if (sb == 256) {
+            SYM1(256, 2, 4, 2, 1, false);
+            SYM2(256, 2, 4, 2, 1, false);
+        }
+        if (ab == 64 && one.np) { if (napp <= 256) APP(64, 2, 2, 3, 2, true) else APP(64, 2, 2, 3, 1, true) }
+        else if (ab == 64) { if (napp <= 256) APP(64, 2, 2, 3, 2, false) else APP(64, 2, 2, 3, 1, false) }
+        else if (ab == 128) APP(128, 2, 4, 2, 1, false)
+        else APP(256, 2, 4, 2, 1, false)
         f16_t* s = xh; xh = yh; yh = s;
         s = xl; xl = yl; yl = s;
     }

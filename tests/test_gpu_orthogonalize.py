@@ -570,3 +570,20 @@ def test_lists_of_small_matrices(shapes):
     for (_, p), w, o in zip(named, before, outs):
         want = w - max(1.0, w.shape[0] / w.shape[1]) ** 0.5 * o.float()
         assert float((p.detach() - want).norm()) <= 2 ** -8 * float((want - w).norm()) + 2 ** -22 * float(w.norm())
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, BF], ids=["fp32", "bf16"])
+@pytest.mark.parametrize("shape", [(40, 90), (20, 700), (200, 301), (300, 200), (3, 130, 201)], ids=str)
+def test_arrays_that_start_anywhere(shape, dtype):
+    from distributeddeeplearning_amd.ops import functional as ops
+
+    n = math.prod(shape)
+    x = torch.randn(n, generator=torch.Generator().manual_seed(3)).to(DEV, dtype)
+    want = ops.orthogonalize(x.view(shape))
+    store = torch.full((n + 16,), float("nan"), device=DEV, dtype=dtype)
+    for at in (1, 4, 7):
+        store.fill_(float("nan"))
+        store[at:at + n] = x
+        got = ops.orthogonalize(store[at:at + n].view(shape))
+        for w, o, v in zip(want.view(-1, *shape[-2:]), got.view(-1, *shape[-2:]), x.view(-1, *shape[-2:])):
+            assert off(o, v) < TOL and off(w, v) < TOL
