@@ -118,8 +118,8 @@ __global__ void __launch_bounds__(256) int8_rows_kernel(const T* __restrict__ x,
     if ((threadIdx.x & (64 * W - 1)) == 0) scale[m] = s;
 }
 
-// B x B tile of y (or a part of its sum): F = output channels, S = rows of x.  12 544 x 4096 x 4096: 290 us (tiles of 128, bound by the
-// matrix pipe: 1450 TOPS); 256 x 1000 x 2047: 8.6 us (64 tiles of 64, two groups of waves each, bound by the latency of 8 stages).
+// B x B tile of y (or a part of its sum): F = output channels, S = rows of x.  12 544 x 4096 x 4096: 250 to 290 us (tiles of 128, bound by the
+// matrix pipe: 1450 to 1680 TOPS); 256 x 1000 x 2047: 8.6 us (64 tiles of 64, two groups of waves each, bound by the latency of 16 stages).
 template <typename T, int B, int W0, int W1, int NST, int KS>
 __global__ void __launch_bounds__(KS * W0 * W1 * 64, 2) int8_gemm_kernel(const signed char* __restrict__ xq, const float* __restrict__ sx,
                                                                    const signed char* __restrict__ q, long long ldq, long long q_bytes,
@@ -142,40 +142,19 @@ __global__ void __launch_bounds__(KS * W0 * W1 * 64, 2) int8_gemm_kernel(const s
     if constexpr (B == 64) {
         if (split > 1 && !join_parts<int, Mu>(mu, smem, slabs + (long long)idx * split * (B * B), counters + idx, part, split)) return;
     }
-    const bool vec = (N & 7) == 0 && (ldy & 7) == 0;
 #pragma unroll
     for (int pass = 0; pass < Mu::PASSES; ++pass) {
         if (Mu::PASSES > 1 && pass > 0) __syncthreads();
         if (B > 64 || split == 1) mu.to_lds(smem, pass);
         __syncthreads();
+        // a lane an element: a wave's loads of s and bias and its stores are side by side, whatever N is (8 elements a lane, 16-byte
+        // stores: 12 544 x 4096 x 64 122 us, so 97; where rows begin anywhere, 770 x 6171 x 26 28.8, so 20.4; 12 544 x 4096 x 4096 291, so 279)
 #pragma unroll 1
-        for (int k = threadIdx.x; k < Mu::ROWS * B / 8; k += Mu::THREADS) {
-            const int r = k / (B / 8), c = (k % (B / 8)) * 2, m = m0 + Mu::tile_row(r, pass), n = n0 + c * 4;
+        for (int k = threadIdx.x; k < Mu::ROWS * B; k += Mu::THREADS) {
+            const int r = k / B, c = k % B, m = m0 + Mu::tile_row(r, pass), n = n0 + c;
             if (m >= M || n >= N) continue;
-            const i32x4 v0 = Mu::at(smem, r, c), v1 = Mu::at(smem, r, c + 1);
-            const float rs = sx[m];
-            float o[8];
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                const int ne = n + e < N ? n + e : N - 1;
-                o[e] = (float)(e < 4 ? v0[e & 3] : v1[e & 3]) * (rs * s[ne]) + (bias ? bias[ne] : 0.f);
-            }
-            T* out = y + m * ldy + n;
-            if (vec) {
-                if constexpr (sizeof(T) == 2) {
-                    bf16x8 w;
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) w[e] = f2bf(o[e]);
-                    *reinterpret_cast<bf16x8*>(out) = w;
-                } else {
-                    *reinterpret_cast<f32x4*>(out) = f32x4{o[0], o[1], o[2], o[3]};
-                    *reinterpret_cast<f32x4*>(out + 4) = f32x4{o[4], o[5], o[6], o[7]};
-                }
-            } else {
-#pragma unroll
-                for (int e = 0; e < 8; ++e)
-                    if (n + e < N) st1(out + e, o[e]);
-            }
+            const int v = __float_as_int(Mu::at1(reinterpret_cast<const float*>(smem), r, c));
+            st1(y + m * ldy + n, (float)v * (sx[m] * s[n]) + (bias ? bias[n] : 0.f));
         }
     }
 }
