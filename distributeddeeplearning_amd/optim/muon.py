@@ -44,6 +44,14 @@ class FusedMuon(_ArenaOptimizer):
                         for s in r["segments"] if s.numel > 0]
                 if segs:
                     self._matrices.append({"dtype": dt, "decay": decay, "segments": segs, "calls": None})
+        if self._hip():
+            for entry in self._matrices:      # refuses a matrix that the kernels do not take
+                self._tables(entry)
+
+    def _hip(self):
+        from ..ops import kernels
+
+        return self.arena.device.type == "cuda" and kernels.enabled()
 
     def _tables(self, entry):
         if entry["calls"] is None:
@@ -61,9 +69,7 @@ class FusedMuon(_ArenaOptimizer):
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
-        from ..ops import kernels
-
-        hip = self.arena.device.type == "cuda" and kernels.enabled()
+        hip = self._hip()
         if hip:
             from ..ops import hip_ops
 

@@ -587,3 +587,15 @@ def test_arrays_that_start_anywhere(shape, dtype):
         got = ops.orthogonalize(store[at:at + n].view(shape))
         for w, o, v in zip(want.view(-1, *shape[-2:]), got.view(-1, *shape[-2:]), x.view(-1, *shape[-2:])):
             assert off(o, v) < TOL and off(w, v) < TOL
+
+
+def test_matrices_that_are_too_large_are_refused():
+    from distributeddeeplearning_amd.ops import functional as ops
+    from distributeddeeplearning_amd.ops.kernels import KernelError
+    from distributeddeeplearning_amd.optim import FusedMuon
+
+    g = torch.zeros(32705, 32705, dtype=BF, device=DEV)          # rounded up to 64: 32768^2 = 2^30
+    with pytest.raises(KernelError, match="out of range"):
+        ops.orthogonalize(g)
+    with pytest.raises(KernelError, match="out of range"):
+        FusedMuon([("w", torch.nn.Parameter(g))])
