@@ -122,9 +122,9 @@ __global__ void __launch_bounds__(256) int8_rows_kernel(const T* __restrict__ x,
 // matrix pipe: 1450 to 1680 TOPS); 256 x 1000 x 2047: 8.6 us (64 tiles of 64, two groups of waves each, bound by the latency of 16 stages).
 template <typename T, int B, int W0, int W1, int NST, int KS>
 __global__ void __launch_bounds__(KS * W0 * W1 * 64, 2) int8_gemm_kernel(const signed char* __restrict__ xq, const float* __restrict__ sx,
-                                                                   const signed char* __restrict__ q, long long ldq, long long q_bytes,
+                                                                   const signed char* __restrict__ q, long long ldq,
                                                                    const float* __restrict__ s, const float* __restrict__ bias, T* __restrict__ y, long long ldy,
-                                                                   int M, int N, int Kp, int tm, int tn, int split, int* __restrict__ slabs,
+                                                                   int M, int N, int K, int Kp, int tm, int tn, int split, int* __restrict__ slabs,
                                                                    unsigned* __restrict__ counters) {
     typedef TileMul<MulI8, B, B, W0, W1, NST, false, KS> Mu;
     __shared__ __attribute__((aligned(16))) unsigned char smem[Mu::LDS];
@@ -135,10 +135,10 @@ __global__ void __launch_bounds__(KS * W0 * W1 * 64, 2) int8_gemm_kernel(const s
     const int stages = Kp / 128 - k0 < each ? Kp / 128 - k0 : each;
     const int band = idx / (8 * tn), rem = idx - band * 8 * tn, h = tm - band * 8 < 8 ? tm - band * 8 : 8;
     const int ni = rem / h, mi = band * 8 + rem - ni * h, m0 = mi * B, n0 = ni * B;
-    const long long left = q_bytes - n0 * ldq - k0 * 128;
     Mu mu;
-    mu.run(smem, q + n0 * ldq + k0 * 128, (unsigned)ldq, N - n0, left < (long long)DESC_BYTES ? (unsigned)left : DESC_BYTES, xq + (long long)m0 * Kp + k0 * 128, Kp, M - m0,
-           DESC_BYTES, stages);
+    // (the codes' rows may be read up to the next multiple of 16 bytes behind K, the workspace's are whole stages)
+    mu.run(smem, q + n0 * ldq + k0 * 128, (unsigned)ldq, N - n0, xq + (long long)m0 * Kp + k0 * 128, Kp, M - m0, stages,
+           k0 + stages == Kp / 128 ? ((K + 15) & ~15) - (Kp - 128) : 128);
     if constexpr (B == 64) {
         if (split > 1 && !join_parts<int, Mu>(mu, smem, slabs + (long long)idx * split * (B * B), counters + idx, part, split)) return;
     }
@@ -267,8 +267,8 @@ int split_of(long long M, int N, int K) {
 }
 
 template <typename T>
-int run(const T* x, long long ldx, const signed char* q, long long ldq, long long q_bytes, const float* s, const float* bias, T* y, long long ldy, int M, int N,
-        int K, char* ws, hipStream_t stream) {
+int run(const T* x, long long ldx, const signed char* q, long long ldq, const float* s, const float* bias, T* y, long long ldy, int M, int N, int K,
+        char* ws, hipStream_t stream) {
     const int vec = rows_vec(x, sizeof(T) == 2, ldx), Kp = (K + 127) / 128 * 128;
     if (skinny(M, K)) {
         const int tiles = (N + 15) / 16, grid = tiles < 512 ? tiles : 512;
@@ -287,7 +287,7 @@ int run(const T* x, long long ldx, const signed char* q, long long ldq, long lon
     unsigned* counters = (unsigned*)(slabs + t64 * split * 64 * 64);
     launch_rows(x, ldx, M, K, Kp, vec, xq, sx, counters, split > 1 ? (int)t64 : 0, stream);
 #define GEMM(B, W0, W1, NST, KS, t) DDL_KLAUNCH((int8_gemm_kernel<T, B, W0, W1, NST, KS>), dim3((unsigned)((t + 7) / 8 * 8)), dim3(KS * W0 * W1 * 64), 0, stream, xq, sx, q, \
-                                            ldq, q_bytes, s, bias, y, ldy, M, N, Kp, (M + B - 1) / B, (N + B - 1) / B, split, slabs, counters)
+                                            ldq, s, bias, y, ldy, M, N, K, Kp, (M + B - 1) / B, (N + B - 1) / B, split, slabs, counters)
     if (t128 >= 256) GEMM(128, 2, 2, 2, 1, t128);
     else if (t64 <= 256 && Kp > 128) GEMM(64, 2, 2, 3, 2, t64 * split);
     else GEMM(64, 2, 2, 3, 1, t64);
@@ -331,6 +331,6 @@ extern "C" int ddl_int8_linear(const void* x, int x_bf16, long long ldx, const v
     const long long need = ddl_int8_linear_workspace(M, N, K);
     if (need > 0 && (!ws || ws_bytes < need)) return DDL_EINVAL;
     if (x_bf16)
-        return run((const bf16_t*)x, ldx, (const signed char*)q, ldq, q_bytes, (const float*)s, (const float*)bias, (bf16_t*)y, ldy, (int)M, N, K, (char*)ws, stream);
-    return run((const float*)x, ldx, (const signed char*)q, ldq, q_bytes, (const float*)s, (const float*)bias, (float*)y, ldy, (int)M, N, K, (char*)ws, stream);
+        return run((const bf16_t*)x, ldx, (const signed char*)q, ldq, (const float*)s, (const float*)bias, (bf16_t*)y, ldy, (int)M, N, K, (char*)ws, stream);
+    return run((const float*)x, ldx, (const signed char*)q, ldq, (const float*)s, (const float*)bias, (float*)y, ldy, (int)M, N, K, (char*)ws, stream);
 }

@@ -466,7 +466,7 @@ __global__ void __launch_bounds__(KS * W0 * W1 * 64, B == 128 ? 4 : 2) ortho_sym
     const long long ao = (long long)it.ao * 64 + (long long)b * np * lda;
     const f16_t* src = SQUARE ? in + ao : in + (long long)it.xo * 64 + (long long)b * np * ld;
     M m;
-    m.run(smem, src + (long long)ti * B * ld + k0 * 64, ld * 2, np - ti * B, DESC_BYTES, src + (long long)tj * B * ld + k0 * 64, ld * 2, np - tj * B, DESC_BYTES, stages);
+    m.run(smem, src + (long long)ti * B * ld + k0 * 64, ld * 2, np - ti * B, src + (long long)tj * B * ld + k0 * 64, ld * 2, np - tj * B, stages);
     const float* d = SQUARE ? din + it.dof + (long long)b * np : nullptr;
     const float unscale = SQUARE ? USC * USC : ldexpf(USC * USC, -2 * shift_of(ex, it.mat + b, down));
     f16_t* o = out + ao;
@@ -562,7 +562,7 @@ __global__ void __launch_bounds__(KS * W0 * W1 * 64, BF == 128 ? 4 : 2) ortho_ap
     const f16_t* A = P + (long long)it.ao * 64 + ((long long)b * np + ti * BS) * np;
     const long long xo = (long long)it.xo * 64 + (long long)b * np * mp;
     M m;
-    m.run(smem, xh + xo + tj * BF, mp * 2, mp - tj * BF, DESC_BYTES, A, np * 2, np - ti * BS, DESC_BYTES, np / 64);
+    m.run(smem, xh + xo + tj * BF, mp * 2, mp - tj * BF, A, np * 2, np - ti * BS, np / 64);
     const int e0 = shift_of(ex, it.mat + b, down), e1 = shift_of(ex, it.mat + b, down1);
     const float rescale = FINAL ? ldexpf(USC, -e0) : ldexpf(1.f, e1 - e0);
     const float* d = pd + it.dof + (long long)b * np;

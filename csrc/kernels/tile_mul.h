@@ -20,24 +20,37 @@ namespace {
 
 typedef __fp16 half4 __attribute__((ext_vector_type(4)));      // (the type that the transposing load is declared with)
 typedef __attribute__((address_space(3))) half4* lds_half4_ptr;
-constexpr unsigned OUT = 0x80000000u, DESC_BYTES = OUT - 16;      // an offset behind every descriptor's range (reads as zero); the longest range
+// Whether the scalar offset of a buffer load counts in its range check is left open here: every descriptor has the same range, longer than
+// any sum of both offsets; lanes that must not read have OUT as their own offset, behind that range (zeros); all others are inside
+// their array.
+constexpr unsigned OUT = 0x80000000u, DESC_BYTES = OUT - 16;
 
 __device__ __forceinline__ int nt_off(int row, int ch) { return row * 128 + ((ch ^ ((row >> 1) & 7)) << 4); }
 template <int B>
-__device__ __forceinline__ int tr_swz(int row) {
+__host__ __device__ __forceinline__ int tr_swz(int row) {
     return B >= 128 ? (row & 3) | ((row >> 1) & 4) : ((row >> 1) & 1) | ((row >> 2) & 2);
 }
 
 struct MulF16 {
     typedef f16x8 frag;
     typedef f32x4 acc;
+    static constexpr bool CUT = false;         // rows of f are whole stages
     static __device__ __forceinline__ acc mma(frag a, frag b, acc c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
 };
 struct MulI8 {
     typedef i32x4 frag;
     typedef i32x4 acc;
+    static constexpr bool CUT = true;          // rows of f are the caller's: they end inside the last stage
     static __device__ __forceinline__ acc mma(frag a, frag b, acc c) { return __builtin_amdgcn_mfma_i32_16x16x64_i8(a, b, c, 0, 0, 0); }
 };
+
+// Stages of a group of waves: it issues the loads of `count`, of which `live` exist and `last` (if any) is the sum's last one.
+struct Stages { int first, count, live, last; };
+__host__ __device__ __forceinline__ Stages stages_of(int total, int ks, int group) {
+    if (ks == 1) return Stages{0, total, total, total - 1};
+    const int half = (total + 1) >> 1;                  // (the second group may have a stage less)
+    return group ? Stages{half, half, total - half, total - 1 - half} : Stages{0, half, half, total - 1};
+}
 
 // KS = 2: two such groups of waves with stages of their own take half of the sum each and are added at the end - a tile
 // that has a CU to itself is bound by the latency of its stages, one after another, not by their bytes.
@@ -58,50 +71,54 @@ struct TileMul {
         for (int i = 0; i < 4; ++i) r[i] = __builtin_amdgcn_readfirstlane(r[i]);
         return r;
     }
-    static __device__ __forceinline__ unsigned behind(unsigned bytes, unsigned by) { return bytes > by ? bytes - by : 0u; }
-    // f: first row (TRF: first column) of the tile, ldf bytes from a row to the next, fleft rows (columns) that exist, fbytes: what
-    // may be read from f on (behind it and behind the rows that exist: zeros); s likewise; `total` stages.  All offsets < 2^31.
-    __device__ __forceinline__ void run(unsigned char* smem, const void* f, unsigned ldf, int fleft, unsigned fbytes, const void* s, unsigned lds, int sleft,
-                                        unsigned sbytes, int total) {
-        int KT = total;
+    // The lane's offset of a wave's i-th load of f and of s (the same in every stage), and what is or-ed to f's in the last stage: OUT
+    // where the 16 bytes begin at or behind byte `fend` of the stage's 128 (the swizzle has whole turns in WAVES * 8 rows: any i).
+    static __host__ __device__ __forceinline__ unsigned f_offset(int i, int wid, int lane, unsigned ldf, int fleft) {
+        const int slot = (i * WAVES + wid) * 64 + lane;
+        if (TRF) {
+            constexpr int CPR = BF / 8;
+            const int row = slot / CPR, ch = slot % CPR, c = (((ch >> 1) ^ tr_swz<BF>(row)) << 1) | (ch & 1);
+            return c * 8 < fleft ? row * ldf + c * 16 : OUT;
+        }
+        const int row = slot >> 3, c = (slot & 7) ^ ((row >> 1) & 7);
+        return row < fleft ? row * ldf + c * 16 : OUT;
+    }
+    static __host__ __device__ __forceinline__ unsigned s_offset(int i, int wid, int lane, unsigned lds, int sleft) {
+        const int slot = (i * WAVES + wid) * 64 + lane, row = slot >> 3, c = (slot & 7) ^ ((row >> 1) & 7);
+        return row < sleft ? row * lds + c * 16 : OUT;
+    }
+    static __host__ __device__ __forceinline__ unsigned f_behind(int wid, int lane, int fend) {
+        static_assert(WAVES % 2 == 0, "swizzle");
+        const int slot = wid * 64 + lane, c = (slot & 7) ^ ((slot >> 4) & 7);
+        return c * 16 < fend ? 0u : OUT;
+    }
+    // f: first row (TRF: first column) of the tile, ldf bytes from a row to the next, fleft rows (columns) that exist (behind them:
+    // zeros), of which the last stage is read up to byte `fend` (a multiple of 16; OP::CUT: behind it zeros, else 128); s likewise, in
+    // whole stages; `total` stages.  All offsets < 2^31 - 16.
+    __device__ __forceinline__ void run(unsigned char* smem, const void* f, unsigned ldf, int fleft, const void* s, unsigned lds, int sleft, int total,
+                                        int fend = 128) {
         const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), wid = wave % WAVES, w0 = wid / W1, w1 = wid % W1;
-        int live = KT;                                                         // stages of this group that exist
-        if (KS == 2) {
-            live = KT = (KT + 1) >> 1;
-            if (wave >= WAVES) {
-                live = total - KT;
-                smem += NST * STAGE;
-                f = (const char*)f + (size_t)KT * (TRF ? ldf * 64u : 128u);
-                s = (const char*)s + (size_t)KT * 128u;
-                fbytes = behind(fbytes, KT * (TRF ? ldf * 64u : 128u));
-                sbytes = behind(sbytes, KT * 128u);
-            }
+        const Stages mine = stages_of(total, KS, wave / WAVES);
+        const int KT = mine.count, live = mine.live;
+        if (KS == 2 && wave >= WAVES) {
+            smem += NST * STAGE;
+            f = (const char*)f + (size_t)mine.first * (TRF ? ldf * 64u : 128u);
+            s = (const char*)s + (size_t)mine.first * 128u;
         }
         const int fr = lane & 15, fq = lane >> 4;
         const unsigned lds0 = (unsigned)(uintptr_t)(__attribute__((address_space(3))) void*)smem;
         unsigned vo[L];
 #pragma unroll
-        for (int i = 0; i < FL; ++i) {
-            const int slot = (i * WAVES + wid) * 64 + lane;
-            if (TRF) {
-                constexpr int CPR = BF / 8;
-                const int row = slot / CPR, ch = slot % CPR, c = (((ch >> 1) ^ tr_swz<BF>(row)) << 1) | (ch & 1);
-                vo[i] = c * 8 < fleft ? row * ldf + c * 16 : OUT;
-            } else {
-                const int row = slot >> 3, c = (slot & 7) ^ ((row >> 1) & 7);
-                vo[i] = row < fleft ? row * ldf + c * 16 : OUT;
-            }
-        }
+        for (int i = 0; i < FL; ++i) vo[i] = f_offset(i, wid, lane, ldf, fleft);
 #pragma unroll
-        for (int i = 0; i < SL; ++i) {
-            const int slot = (i * WAVES + wid) * 64 + lane, row = slot >> 3, c = (slot & 7) ^ ((row >> 1) & 7);
-            vo[FL + i] = row < sleft ? row * lds + c * 16 : OUT;
-        }
-        const u32x4 rf = uniform(raw_rsrc(f, fbytes)), rs = uniform(raw_rsrc(s, sbytes));
+        for (int i = 0; i < SL; ++i) vo[FL + i] = s_offset(i, wid, lane, lds, sleft);
+        const unsigned cut = OP::CUT ? f_behind(wid, lane, fend) : 0u;
+        const u32x4 rf = uniform(raw_rsrc(f, DESC_BYTES)), rs = uniform(raw_rsrc(s, DESC_BYTES));
         const unsigned fstep = TRF ? ldf * 64u : 128u;                         // bytes from a tile to the next
         // every stage is exactly L instructions a wave (behind the end: the last tile again): the counted waits rely on it
         auto piece = [&](unsigned kt, unsigned at, int i) {                    // at: LDS address of the wave's part of the stage
-            const unsigned o = KS == 1 || (int)kt < live ? vo[i] : OUT;        // (the second group may have a stage less: zeros)
+            unsigned o = KS == 1 || (int)kt < live ? vo[i] : OUT;              // (a stage that the second group does not have: zeros)
+            if (OP::CUT && i < FL && (int)kt == mine.last) o |= cut;
             if (i < FL) lds_dma16(rf, at + i * WAVES * 1024, o, kt * fstep);
             else lds_dma16(rs, at + FBYTES + (i - FL) * WAVES * 1024, o, kt * 128u);
         };
