@@ -7,12 +7,12 @@
 // with a = 3.4445), so where the products round decides the result's accuracy.  The matrix pipe runs fp16 at bf16's
 // rate with three more bits, and every quantity here is bounded, so the operands are fp16, scaled by 2^12 (off the
 // subnormals); two things are kept apart from them at no extra product:
-//   * X is a pair of fp16 values hi + lo; products read hi, the term a X reads both;
+//   * X is a pair of fp16 values hi + lo; products read hi, the term a X and, in the last two steps, diag(P) X read both (see low_by_a);
 //   * the diagonals of A and P stay in fp32 (near the end A is close to a multiple of 1: its diagonal carries all of
 //     its rounding): with A = D + O,  A^2 = O^2 + (d_i + d_j) O + D^2, and P X = (a + diag P) X + offdiag(P) X_hi.
-// Against 64 bits the result is, before its rounding to bf16 (1.7e-3 itself), 2e-4 .. 7e-4 off on Gaussian and power-law spectra,
-// 1e-3 .. 2.2e-3 on exponential ones (six decades), 1.6e-3 .. 3.1e-3 where all but a sixteenth of the singular values are a
-// thousandth (2-norm); bf16 operands throughout give 8e-3 .. 0.3, plain fp16 1e-3 .. 4e-2.
+// Against 64 bits the result is, before its rounding to bf16 (1.7e-3 itself), at most this much off (2-norm; Gaussian, power-law,
+// exponential over six decades, rank 1, all but a sixteenth of the singular values a thousandth, gradient-like): 1e-4 .. 1.3e-3 from 32 rows
+// on, 4e-4 .. 1.9e-3 with 8 and 16, 3.2e-3 with 2; bf16 operands throughout give 8e-3 .. 0.3, plain fp16 1e-3 .. 4e-2.
 //
 // A call takes up to 64 groups of equal matrices; all of them share each launch.  Three forms, by sizes alone:
 //   * every matrix of up to 64 x 768 or 128 x 384: a workgroup a matrix, one launch (ortho_small_kernel, all_small);
@@ -175,6 +175,12 @@ __device__ __forceinline__ double wave_sum_d(double v) {
     for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
     return v;
 }
+
+// What X_lo is multiplied with in the place of P = a + (P - a), whose product reads X_hi alone.  a leaves out (P - a) X_lo, which lies
+// in the directions of large singular values: it is not amplified by later steps.  diag(P) comes nearer to P where P is almost a diagonal,
+// but leaves out offdiag(P) X_lo, which later steps amplify by a each where singular values are small.  So: a, and diag(P) in
+// the last two steps.  Rank 1, 2 x 64: 2e-3 (diag(P) throughout 4.3e-2); Gaussian 512 x 512: 8e-4 (a throughout 1.2e-3).
+__host__ __device__ __forceinline__ bool low_by_a(int step, int steps) { return step < steps - 2; }
 
 struct Muon {                       // K23: arenas of one parameter dtype
     const void* g;
@@ -544,14 +550,14 @@ __global__ void __launch_bounds__(KS * W0 * W1 * 64, B == 128 ? 4 : 2) ortho_sym
     }
 }
 
-// X' = pd X + offdiag(P) X_hi; tile: BF columns of X times BS rows of P.  FINAL 0: the next X; 1: the output; 2: the weights (K23).
+// X' = pd X_hi + (pd or a) X_lo + offdiag(P) X_hi; tile: BF columns of X times BS rows of P.  FINAL 0: the next X; 1: the output; 2: the weights (K23).
 // 4096 x 8192: 250 us (tiles of 256, bound by the matrix pipe: 1100 TFLOP/s); all of ResNet-50: 60 us (tiles of 128, bound by X's
 // pairs, 204 MB in and out), 97 us where it writes the weights; 12 of 512 x 512: 12 us (768 tiles of 64, latency).
 template <int BF, int BS, int W0, int W1, int NST, int KS, int FINAL, bool ONE>
 __global__ void __launch_bounds__(KS * W0 * W1 * 64, BF == 128 ? 4 : 2) ortho_apply_kernel(const Table* __restrict__ t, const Single one, const Muon mu, const f16_t* __restrict__ P,
                                                             const float* __restrict__ pd, const f16_t* __restrict__ xh, const f16_t* __restrict__ xl,
                                                             f16_t* __restrict__ yh, f16_t* __restrict__ yl,
-                                                            const int* __restrict__ ex, int down, int down1) {
+                                                            const int* __restrict__ ex, int down, int down1, int by_a, float ca) {
     typedef TileMul<MulF16, BF, BS, W0, W1, NST, true, KS> M;
     __shared__ __attribute__((aligned(16))) unsigned char smem[M::LDS];
     Item<ONE> it;
@@ -585,11 +591,11 @@ __global__ void __launch_bounds__(KS * W0 * W1 * 64, BF == 128 ? 4 : 2) ortho_ap
             if ((BS > 64 && r >= np) || (BF > 64 && c >= mp)) continue;
             const long long at = xo + (long long)r * mp + c;
             const f16x8 h0 = *reinterpret_cast<const f16x8*>(xh + at), l0 = *reinterpret_cast<const f16x8*>(xl + at);
-            const float dr = d[r];
+            const float dr = d[r], dl = by_a ? ca : dr;
             const f32x4 v0 = M::at(tile, s, q), v1 = M::at(tile, s, q + 1);
             float v[8];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) v[e] = (dr * ((float)h0[e] + (float)l0[e]) + (e < 4 ? v0[e & 3] : v1[e & 3]) * USC) * rescale;
+            for (int e = 0; e < 8; ++e) v[e] = (dr * (float)h0[e] + dl * (float)l0[e] + (e < 4 ? v0[e & 3] : v1[e & 3]) * USC) * rescale;
             if (FINAL == 0) {
                 f16x8 h, l;
 #pragma unroll
@@ -625,7 +631,7 @@ __global__ void __launch_bounds__(KS * W0 * W1 * 64, BF == 128 ? 4 : 2) ortho_ap
 // ---- small matrices: all steps in one launch ----------------------------------------------------------------------------
 // One workgroup of 8 waves a matrix: np = NP padded rows, up to 128 CB columns.  X stays in registers in fp32 (in the layout of the
 // products' results: wave w has the 16-column blocks w, w + 8, ..; a lane 4 columns of rows lane % 16 + 16 j), X_hi, O and
-// P in LDS; pd X is the accumulator that P X is added to.  What bounds it is latency: 64 x 64 takes 12 us here,
+// P in LDS; pd X (lo: by a) is the accumulator that P X is added to.  What bounds it is latency: 64 x 64 takes 12 us here,
 // and the tiles 17 launches of 5 us.
 template <int NP, int CB, int KIND>
 __global__ void __launch_bounds__(512, 2) ortho_small_kernel(const Chunk ch, const Muon mu, float ca, float cb, float cc, int steps, int fall, float eps) {
@@ -783,8 +789,19 @@ __global__ void __launch_bounds__(512, 2) ortho_small_kernel(const Chunk ch, con
 #pragma unroll
         for (int j = 0; j < NS; ++j) {
             const float pd = pds[j * 16 + fr] * SC;
+            if (low_by_a(step, steps)) {
+                const float pa = ca * SC;
 #pragma unroll
-            for (int k = 0; k < CB; ++k) x[k][j] *= pd;
+                for (int k = 0; k < CB; ++k)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const float hi = (float)(f16_t)x[k][j][e];
+                        x[k][j][e] = pd * hi + pa * (x[k][j][e] - hi);
+                    }
+            } else {
+#pragma unroll
+                for (int k = 0; k < CB; ++k) x[k][j] *= pd;
+            }
         }
 #pragma unroll
         for (int h = 0; h < NP / 32; ++h) {
@@ -1441,7 +1458,7 @@ int run_all(const Desc* q, int count, int kind, const Muon& mu, float a, float b
 #define SYM(B, W0, W1, NST, KS, SQ, ONE, IN, DIN, OUTP, DOUT, DOWN) DDL_KLAUNCH((ortho_sym_kernel<B, W0, W1, NST, KS, SQ, ONE>), dim3((unsigned)nsym), dim3(KS * W0 * W1 * 64), 0, stream, t, one, IN, DIN, OUTP, DOUT, ex, DOWN, a, b, c, slab, counters)
 #define SYM1(B, W0, W1, NST, KS, ONE) SYM(B, W0, W1, NST, KS, false, ONE, xh, (const float*)nullptr, O, d, k * fall)
 #define SYM2(B, W0, W1, NST, KS, ONE) SYM(B, W0, W1, NST, KS, true, ONE, O, d, P, pd, 0)
-#define APP1(B, W0, W1, NST, KS, FIN, ONE) DDL_KLAUNCH((ortho_apply_kernel<B, B, W0, W1, NST, KS, FIN, ONE>), dim3((unsigned)napp), dim3(KS * W0 * W1 * 64), 0, stream, t, one, mu, P, pd, xh, xl, yh, yl, ex, k * fall, (k + 1) * fall)
+#define APP1(B, W0, W1, NST, KS, FIN, ONE) DDL_KLAUNCH((ortho_apply_kernel<B, B, W0, W1, NST, KS, FIN, ONE>), dim3((unsigned)napp), dim3(KS * W0 * W1 * 64), 0, stream, t, one, mu, P, pd, xh, xl, yh, yl, ex, k * fall, (k + 1) * fall, low_by_a(k, steps), a)
 #define APP(B, W0, W1, NST, KS, ONE) { if (fin == 0) APP1(B, W0, W1, NST, KS, 0, ONE); else if (fin == 1) APP1(B, W0, W1, NST, KS, 1, ONE); else APP1(B, W0, W1, NST, KS, 2, ONE); }
 #define TILES64(ONE)                                                                                                         \
         {                                                                                                                    \

@@ -599,3 +599,33 @@ def test_matrices_that_are_too_large_are_refused():
         ops.orthogonalize(g)
     with pytest.raises(KernelError, match="out of range"):
         FusedMuon([("w", torch.nn.Parameter(g))])
+
+
+# What the steps' roundings may leave, before the result's own to bf16: each step rounds X_hi, offdiag(A) and offdiag(P) to fp16, at most
+# 2^-11 of a value each, 2^-11 / sqrt(3) in the mean of many; a value's error enters by P - a (|b s^2 + c s^4| < 3 here) and is not
+# amplified by the later steps, whatever the spectrum; 15 independent ones: sqrt(15) 3 2^-11 / sqrt(3).  Of few values: without the mean.
+def direction_limit(shape):
+    return math.sqrt(15) * 3 * 2 ** -11 / (math.sqrt(3) if min(shape) >= 16 else 1)
+
+
+@pytest.mark.parametrize("kind", ["gauss", "power", "exp", "rank1", "lowrank"])
+@pytest.mark.parametrize("shape", [(2, 8), (2, 64), (4, 64), (64, 3), (8, 256), (16, 256), (32, 512), (64, 64), (64, 768), (768, 64), (33, 1000), (128, 384),
+                                   (1000, 40), (129, 300), (256, 1024), (520, 512), (2040, 2001)], ids=str)
+def test_the_direction_of_any_spectrum(shape, kind):
+    """The fp32 weights that a step from zero leaves: the direction itself, in each form."""
+    from distributeddeeplearning_amd.ops import functional as ops
+    from distributeddeeplearning_amd.optim import FusedMuon
+
+    if max(shape) > 2000 and kind not in ("gauss", "rank1"):
+        pytest.skip("the large one: two spectra")
+    p = torch.nn.Parameter(torch.zeros(shape, device=DEV))
+    opt = FusedMuon([("w", p)], lr=1.0, momentum=0.0, nesterov=False)
+    g = spectrum(kind, *shape, seed=11).to(DEV)
+    p.grad.copy_(g)
+    opt.step()
+    want = -max(1.0, shape[0] / shape[1]) ** 0.5 * (on_the_card(g) if max(shape) > 2000 else oracle(g.cpu()).to(DEV))
+    err = float((p.detach().double() - want).norm() / want.norm())
+    assert err < direction_limit(shape), err
+    out = ops.orthogonalize(g.to(BF))                 # a bf16 input has a spectrum of its own
+    want = on_the_card(g.to(BF)) if max(shape) > 2000 else oracle(g.to(BF).cpu()).to(DEV)
+    assert float((out.double() - want).norm() / want.norm()) < direction_limit(shape) + 2 ** -8
