@@ -15,6 +15,7 @@ import argparse
 import concurrent.futures as cf
 import glob
 import os
+import re
 import shutil
 import subprocess
 import sys
@@ -33,6 +34,11 @@ def _hipcc():
         if cand and os.path.exists(cand):
             return cand
     raise RuntimeError("hipcc not found")
+
+
+# kernels that must not use scratch memory, by source: ortho_small_kernel<64, 8> (64 x 1024 in one workgroup, not built) spilled
+# registers and gave NaN for a reason that is not known, so none of its sizes is built with spills
+NO_SCRATCH = {"orthogonalize.hip": "ortho_small_kernel"}
 
 
 def _newer(target, deps):
@@ -57,6 +63,16 @@ def _made(target, cmd):
         f.write(" ".join(cmd))
 
 
+def _check_scratch(remarks, kernel):
+    """Raises unless the compiler's resource remarks name instances of ``kernel`` and none of them uses scratch memory."""
+    seen = re.findall(r"Function Name: (\S*%s\S*).*?ScratchSize \[bytes/lane\]: (\d+)" % kernel, remarks, re.S)
+    if not seen:
+        raise RuntimeError("the compiler reported no %s" % kernel)
+    bad = [name for name, size in seen if int(size)]
+    if bad:
+        raise RuntimeError("%s spills registers: %s" % (kernel, ", ".join(bad)))
+
+
 def _run(cmd):
     proc = subprocess.run(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)
     if proc.returncode != 0:
@@ -79,13 +95,20 @@ def build_kernels(force=False, jobs=8, verbose=True):
     for s in srcs:
         o = os.path.join(BUILD, "kernels", os.path.basename(s) + ".o")
         objs.append(o)
-        cmd = [hipcc] + flags + ["-c", s, "-o", o]
+        kernel = NO_SCRATCH.get(os.path.basename(s))
+        cmd = [hipcc] + flags + (["-Rpass-analysis=kernel-resource-usage"] if kernel else []) + ["-c", s, "-o", o]
         if force or _stale(o, [s] + hdrs, cmd):
-            todo.append((s, o, cmd))
+            todo.append((s, o, cmd, kernel))
 
     def compile_one(job):
-        s, o, cmd = job
-        _run(cmd)
+        s, o, cmd, kernel = job
+        text = _run(cmd)
+        if kernel:
+            try:
+                _check_scratch(text, kernel)
+            except RuntimeError:
+                os.remove(o)
+                raise
         _made(o, cmd)
         return s
 
