@@ -1506,7 +1506,7 @@ extern "C" long long ddl_ortho_workspace(const long long* desc, int count) {
     return one.bytes > other.bytes ? one.bytes : other.bytes;
 }
 
-// kind 0 / 1: fp32 / bf16 sources; destinations are bf16
+// kind 0 / 1: fp32 / bf16 sources; destinations are dense bf16 (other strides are refused)
 extern "C" int ddl_orthogonalize(const long long* desc, int count, int kind, float a, float b, float c, int steps, float eps, void* ws,
                                  long long ws_bytes, hipStream_t stream) {
     if (count == 0) return DDL_OK;
@@ -1516,7 +1516,8 @@ extern "C" int ddl_orthogonalize(const long long* desc, int count, int kind, flo
     if (!ddl_ortho_coefficients_ok(a, b, c, steps) || !(eps >= 1e-30f)) return DDL_EINVAL;
     if (reinterpret_cast<uintptr_t>(ws) & 255) return DDL_EALIGN;
     for (int i = 0; i < count; ++i)
-        if (!q[i].src || !q[i].dst || !strides_fit(q[i].srs, q[i].scs) || !strides_fit(q[i].drs, q[i].dcs) || q[i].sb < 0 || q[i].db < 0)
+        if (!q[i].src || !q[i].dst || !strides_fit(q[i].srs, q[i].scs) || q[i].sb < 0 || q[i].drs != q[i].c || q[i].dcs != 1 ||
+            (q[i].batch > 1 && q[i].db != q[i].r * q[i].c))
             return DDL_EINVAL;
     for (int i = 0; i < count; ++i)
         if (!ddl_aligned16((const void*)q[i].dst)) return DDL_EALIGN;

@@ -179,3 +179,21 @@ def test_sizes_that_the_kernels_refuse():
                dict(count=-1), dict(coef=(100.0, 0.0, 0.0)), dict(table=no_source), dict(table=no_stride)):
         assert call(**kw) != 0, kw
     assert call(count=0) == 0
+
+
+def test_destinations_that_are_not_dense_are_refused():
+    """Every form writes dense results; refused before anything is launched, so it needs no GPU."""
+    import ctypes as c
+
+    from distributeddeeplearning_amd.ops import kernels, native
+
+    if not native.kernels_available():
+        pytest.skip("kernel library not built")
+    refused = -1                                          # DDL_EINVAL
+    for r, cols in ((300, 400), (20, 700), (40, 90)):
+        for db, drs, dcs, batch in ((r * cols, cols + 8, 1, 1), (r * cols, 1, r, 1), (r * cols, cols, 2, 1), (r * cols + 64, cols, 1, 3),
+                                    (0, cols, 1, 2), (-1, cols, 1, 2), (r * cols, -cols, 1, 1)):
+            table, count = kernels.ortho_table([(64, r * cols, cols, 1, 64, db, drs, dcs, r, cols, batch)])
+            rc = kernels.lib().ddl_orthogonalize(table, c.c_int(count), c.c_int(0), c.c_float(3.4445), c.c_float(-4.7750), c.c_float(2.0315), c.c_int(5),
+                                                 c.c_float(1e-7), c.c_void_p(256), c.c_longlong(1 << 40), c.c_void_p(0))
+            assert rc == refused, (r, cols, db, drs, dcs, batch, rc)
