@@ -36,6 +36,7 @@ class FusedMuon(_ArenaOptimizer):
         defaults = dict(lr=lr, momentum=momentum, weight_decay=weight_decay, nesterov=nesterov, steps=steps,
                         ortho_a=a, ortho_b=b, ortho_c=c, eps=eps, vector_lr_scale=vector_lr_scale)
         super().__init__(named_parameters, defaults, weight_decay_filter, engine_config)
+        self._vector_lr = None            # (frozen learning rate: the vectors')
         # matrices of one arena and one decay flag, in calls of at most ortho_max_groups
         self._matrices = []
         for dt in self.arena.plans:
@@ -62,6 +63,23 @@ class FusedMuon(_ArenaOptimizer):
             tables = [kernels.ortho_table(rows[k:k + per]) for k in range(0, len(rows), per)]
             entry["calls"] = [(t, n, kernels.ortho_workspace(t, n)) for t, n in tables]
         return entry["calls"]
+
+    # the vectors' rate is a device scalar of its own: lr * vector_lr_scale is rounded to fp32 once, as where it is passed by value
+    def freeze_lr(self):
+        out = super().freeze_lr()
+        if self._vector_lr is None:
+            self._vector_written = self._vector_rate()
+            self._vector_lr = torch.full((1,), self._vector_written, dtype=torch.float32, device=self.arena.device)
+        return out
+
+    def sync_lr(self):
+        super().sync_lr()
+        if self._vector_lr is not None and self._vector_rate() != self._vector_written:
+            self._vector_written = self._vector_rate()
+            self._vector_lr.fill_(self._vector_written)
+
+    def _vector_rate(self):
+        return float(self.param_groups[0]["lr"]) * self.param_groups[0]["vector_lr_scale"]
 
     @torch.no_grad()
     def step(self, closure=None):
@@ -119,11 +137,12 @@ class FusedMuon(_ArenaOptimizer):
             w, g, v = self._weights(dt)[a:b], self.arena.grads[dt][a:b], self.momentum_buf[dt][a:b]
             if hip:
                 lowp = self.arena.params[dt][a:b] if dt in self.master else None
-                kernels.fused_sgd_(w, g, v, lowp, klr * g0["vector_lr_scale"], mu, run_wd, nesterov, kscale)
+                rate = self._vector_rate() if kscale is None else self._frozen_lr
+                kernels.fused_sgd_(w, g, v, lowp, rate, mu, run_wd, nesterov, None if kscale is None else self._vector_lr)
                 continue
             grad = g.to(torch.float32)
             if run_wd:
                 grad = grad.add(w, alpha=run_wd)
             v.mul_(mu).add_(grad)
-            w.add_(grad.add(v, alpha=mu) if nesterov else v, alpha=-lr * g0["vector_lr_scale"])
+            w.add_(grad.add(v, alpha=mu) if nesterov else v, alpha=-self._vector_rate())
             self._publish(dt, a, b)

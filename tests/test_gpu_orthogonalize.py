@@ -629,3 +629,26 @@ def test_the_direction_of_any_spectrum(shape, kind):
     out = ops.orthogonalize(g.to(BF))                 # a bf16 input has a spectrum of its own
     want = on_the_card(g.to(BF)) if max(shape) > 2000 else oracle(g.to(BF).cpu()).to(DEV)
     assert float((out.double() - want).norm() / want.norm()) < direction_limit(shape) + 2 ** -8
+
+
+@pytest.mark.parametrize("scale", [0.3, 1.7, 0.0])
+def test_muon_frozen_lr_with_a_scale_for_vectors_is_bit_identical(scale):
+    """As test_muon_frozen_lr_follows_the_schedule_bit_for_bit, with scales whose product with the learning rate has to be rounded."""
+    from distributeddeeplearning_amd.optim import FusedMuon
+
+    results = []
+    for frozen in (False, True):
+        named = _params(MUON_SHAPES, BF)
+        opt = FusedMuon(named, lr=0.02, weight_decay=0.01, vector_lr_scale=scale)
+        for step, lr in enumerate((0.02, 0.013, 0.0041, 0.0007)):
+            opt.param_groups[0]["lr"] = lr
+            opt.param_groups[0]["vector_lr_scale"] = scale if step < 3 else 0.9
+            if frozen:
+                opt.freeze_lr() if step == 1 else opt.sync_lr()
+            gen = torch.Generator().manual_seed(step)
+            for _, p in named:
+                p.grad.copy_(torch.randn(p.shape, generator=gen))
+            opt.step()
+        results.append([opt.master[BF].clone(), opt.arena.params[torch.float32].clone()])
+    for a, b in zip(*results):
+        assert torch.equal(a, b)
