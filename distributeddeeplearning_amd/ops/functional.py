@@ -19,6 +19,9 @@ pool (``:287-289``), dense head (``:293-296``), mean softmax cross-entropy
 """
 from __future__ import annotations
 
+import ctypes
+import functools
+import math
 import os
 
 import torch
@@ -203,11 +206,41 @@ def linear(x, weight, bias=None):
 ORTHO_COEFFICIENTS = (3.4445, -4.7750, 2.0315)   # five steps take singular values from about 0.002 on into [0.7, 1.2]
 
 
+@functools.lru_cache(maxsize=256)
+def _steps_in_range(a, b, c, steps):
+    """True when these steps keep every operand of the kernels in the range of scaled fp16 values: the largest |s (a + b s^2 + c s^4)| and
+    |b s^2 + c s^4| over [0, top], top = what the step before leaves (1 at first), at the ends or where a derivative vanishes.
+    The library has the same rule (``ddl_ortho_coefficients_ok``); here it holds on every device."""
+    a, b, c = (ctypes.c_float(v).value for v in (a, b, c))
+    if not all(map(math.isfinite, (a, b, c))):
+        return False
+    top = 1.0
+    for _ in range(steps):
+        end = top * top
+        at, root = [0.0, end], 9.0 * b * b - 20.0 * a * c
+        if c != 0.0:
+            if root >= 0.0:
+                at += [(-3.0 * b + math.sqrt(root)) / (10.0 * c), (-3.0 * b - math.sqrt(root)) / (10.0 * c)]
+        elif b != 0.0:
+            at.append(-a / (3.0 * b))
+        f = max(math.sqrt(s) * abs(a + b * s + c * s * s) for s in at if 0.0 <= s <= end)
+        mid = -b / (2.0 * c) if c != 0.0 and 0.0 < -b / (2.0 * c) < end else 0.0
+        p = max(abs(b * s + c * s * s) for s in (end, mid))
+        q = max(abs(a + b * s + c * s * s) for s in (0.0, end, mid))
+        if not (f * 1.02 <= 8.0 and p * 1.02 <= 15.0 and end <= 15.0 and q <= 1024.0):
+            return False
+        top = max(f * 1.02, 1.0)
+    return True
+
+
 def _check_steps(steps, coefficients, eps):
     if not isinstance(steps, int) or not 1 <= steps <= 64:
         raise ValueError("orthogonalize: steps must be an integer from 1 to 64, got %r" % (steps,))
     if len(coefficients) != 3:
         raise ValueError("orthogonalize: three coefficients expected, got %r" % (coefficients,))
+    if not _steps_in_range(*map(float, coefficients), steps):
+        raise ValueError("orthogonalize: %d steps with the coefficients %r leave the range of the kernels' 16-bit operands"
+                         % (steps, tuple(coefficients)))
     if not eps >= 1e-30:
         raise ValueError("orthogonalize: eps must be at least 1e-30, got %r" % (eps,))
 
@@ -233,7 +266,7 @@ def orthogonalize(x, steps=5, coefficients=ORTHO_COEFFICIENTS, eps=1e-7):
     ``x``: a matrix [r, c], a stack [k, r, c], or a list / tuple of matrices of any shapes (they share the launches), fp32 or
     bf16 of any strides; returns bf16 of the same shape(s).  No gradient flows through it: an input that requires one is
     refused outside ``torch.no_grad()``.  Matrices do not influence each other; one that holds an infinity or a NaN
-    gives NaN, a zero matrix zeros.  ``coefficients`` whose steps leave the range of 16-bit operands are refused, and on the
+    gives NaN, a zero matrix zeros.  ``coefficients`` whose steps leave the range of 16-bit operands are refused on any device, and on the
     GPU matrices whose sides, rounded up to 64, have a product of 2^30 or more."""
     many = isinstance(x, (list, tuple))
     mats = list(x) if many else [x]
@@ -256,11 +289,7 @@ def orthogonalize(x, steps=5, coefficients=ORTHO_COEFFICIENTS, eps=1e-7):
         if kernels.require():
             from . import hip_ops
 
-            a, b, c = map(float, coefficients)
-            if not kernels.ortho_coefficients_ok(a, b, c, steps):
-                raise ValueError("orthogonalize: %d steps with the coefficients %r leave the range of the kernels' 16-bit operands"
-                                 % (steps, tuple(coefficients)))
-            out = hip_ops.orthogonalize(mats, steps, (a, b, c), float(eps))
+            out = hip_ops.orthogonalize(mats, steps, tuple(map(float, coefficients)), float(eps))
     if out is None:
         with torch.no_grad():
             out = [orthogonalize_plain(m, steps, coefficients, eps).to(torch.bfloat16).contiguous() for m in mats]

@@ -105,9 +105,7 @@ class FusedMuon(_ArenaOptimizer):
         g0 = self.param_groups[0]
         lr, mu, wd, nesterov = g0["lr"], g0["momentum"], g0["weight_decay"], g0["nesterov"]
         steps, coefficients, eps = g0["steps"], (g0["ortho_a"], g0["ortho_b"], g0["ortho_c"]), g0["eps"]
-        if hip and not kernels.ortho_coefficients_ok(*coefficients, steps):
-            raise ValueError("FusedMuon: %d steps with the coefficients %r leave the range of the kernels' 16-bit operands"
-                             % (steps, coefficients))
+        ops._check_steps(steps, coefficients, eps)        # (the group's values may have been changed)
         klr, kscale = self._kernel_lr(lr)
         for entry in self._matrices:
             dt, run_wd = entry["dtype"], wd if entry["decay"] else 0.0

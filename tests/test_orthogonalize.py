@@ -197,3 +197,42 @@ def test_destinations_that_are_not_dense_are_refused():
             rc = kernels.lib().ddl_orthogonalize(table, c.c_int(count), c.c_int(0), c.c_float(3.4445), c.c_float(-4.7750), c.c_float(2.0315), c.c_int(5),
                                                  c.c_float(1e-7), c.c_void_p(256), c.c_longlong(1 << 40), c.c_void_p(0))
             assert rc == refused, (r, cols, db, drs, dcs, batch, rc)
+
+
+OUT_OF_RANGE = [(50.0, 0.0, 0.0), (3.0, 3.0, 3.0), (float("nan"), 0.0, 0.0), (1.0, -40.0, 0.0), (1e39, 0.0, 0.0), (float("inf"), 0.0, 0.0)]
+
+
+@pytest.mark.parametrize("coef", OUT_OF_RANGE, ids=str)
+def test_coefficients_are_refused_on_the_cpu_and_when_the_optimizer_is_made(coef):
+    with pytest.raises(ValueError, match="range"):
+        ops.orthogonalize(torch.zeros(4, 4), coefficients=coef)
+    p = torch.nn.Parameter(torch.zeros(2, 3))
+    before = p.data_ptr()
+    with pytest.raises(ValueError, match="range"):
+        FusedMuon([("w", p)], coefficients=coef)
+    assert p.data_ptr() == before and p.grad is None
+    opt = FusedMuon([("w", p)])
+    opt.param_groups[0]["ortho_a"], opt.param_groups[0]["ortho_b"], opt.param_groups[0]["ortho_c"] = coef
+    with pytest.raises(ValueError, match="range"):
+        opt.step()
+
+
+def test_the_range_of_coefficients_is_the_librarys():
+    from distributeddeeplearning_amd.ops import kernels, native
+
+    if not native.kernels_available():
+        pytest.skip("kernel library not built")
+    gen = torch.Generator().manual_seed(5)
+    taken = 0
+    for i in range(4000):
+        a, b, c = (torch.randn(3, generator=gen) * torch.tensor([3.0, 4.0, 2.0])).tolist()
+        if i % 5 == 0:
+            c = 0.0
+        if i % 7 == 0:
+            a, b, c = 3.4445 + 0.1 * a, -4.7750 + 0.1 * b, 2.0315 + 0.1 * c
+        steps = 1 + i % 12
+        taken += ops._steps_in_range(a, b, c, steps)
+        assert ops._steps_in_range(a, b, c, steps) == kernels.ortho_coefficients_ok(a, b, c, steps), (a, b, c, steps)
+    assert 500 < taken < 3500
+    for coef in OUT_OF_RANGE + [(3.4445, -4.7750, 2.0315), (1.5, -0.5, 0.0), (2.0, -1.5, 0.5)]:
+        assert ops._steps_in_range(*coef, 5) == kernels.ortho_coefficients_ok(*coef, 5)
