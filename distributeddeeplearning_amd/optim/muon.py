@@ -32,10 +32,12 @@ class FusedMuon(_ArenaOptimizer):
         if lr < 0 or momentum < 0 or weight_decay < 0 or vector_lr_scale < 0:
             raise ValueError("negative hyper-parameter")
         ops._check_steps(steps, coefficients, eps)
+        named = list(named_parameters)
+        self._refuse_sizes(named)
         a, b, c = (float(v) for v in coefficients)
         defaults = dict(lr=lr, momentum=momentum, weight_decay=weight_decay, nesterov=nesterov, steps=steps,
                         ortho_a=a, ortho_b=b, ortho_c=c, eps=eps, vector_lr_scale=vector_lr_scale)
-        super().__init__(named_parameters, defaults, weight_decay_filter, engine_config)
+        super().__init__(named, defaults, weight_decay_filter, engine_config)
         self._vector_lr = None            # (frozen learning rate: the vectors')
         # matrices of one arena and one decay flag, in calls of at most ortho_max_groups
         self._matrices = []
@@ -45,9 +47,16 @@ class FusedMuon(_ArenaOptimizer):
                         for s in r["segments"] if s.numel > 0]
                 if segs:
                     self._matrices.append({"dtype": dt, "decay": decay, "segments": segs, "calls": None})
-        if self._hip():
-            for entry in self._matrices:      # refuses a matrix that the kernels do not take
-                self._tables(entry)
+
+    @staticmethod
+    def _refuse_sizes(named):
+        """Refuses a matrix that the kernels do not take, before the parameters are moved into the arenas."""
+        from ..ops import kernels
+
+        for entry in named:
+            p = entry[1] if isinstance(entry, tuple) else entry
+            if p.is_cuda and p.requires_grad and p.dim() > 1 and p.numel() > 0 and kernels.enabled():
+                kernels.ortho_workspace_of(((p.shape[0], p.numel() // p.shape[0], 1),))
 
     def _hip(self):
         from ..ops import kernels

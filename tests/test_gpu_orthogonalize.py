@@ -652,3 +652,15 @@ def test_muon_frozen_lr_with_a_scale_for_vectors_is_bit_identical(scale):
         results.append([opt.master[BF].clone(), opt.arena.params[torch.float32].clone()])
     for a, b in zip(*results):
         assert torch.equal(a, b)
+
+
+def test_a_refused_optimizer_leaves_the_parameters_where_they_were():
+    from distributeddeeplearning_amd.ops.kernels import KernelError
+    from distributeddeeplearning_amd.optim import FusedMuon
+
+    small = torch.nn.Parameter(torch.ones(4, 4, device=DEV))
+    large = torch.nn.Parameter(torch.zeros(1, 1 << 24, dtype=BF, device=DEV))       # rounded up to 64 rows: 2^30
+    at = small.data_ptr(), large.data_ptr()
+    with pytest.raises(KernelError, match="out of range"):
+        FusedMuon(p for p in [("a", small), ("b", large)])
+    assert (small.data_ptr(), large.data_ptr()) == at and small.grad is None and large.grad is None
