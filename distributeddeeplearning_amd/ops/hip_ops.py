@@ -1917,10 +1917,13 @@ def orthogonalize(mats, steps, coefficients, eps):
             strides = m.stride()
         if len(strides) == 2:
             strides = (0,) + strides
-        size = (r, c, batch)
-        groups.append((m.data_ptr(),) + strides + (o.data_ptr(), r * c, c, 1) + size)
-        sizes.append(size)
-    per = K.ortho_max_groups()
+        # (a stack of more matrices than a launch takes: several groups, each in a call of its own)
+        most = K.ortho_most_matrices(r, c)
+        for at in range(0, batch, most):
+            size = (r, c, min(most, batch - at))
+            groups.append((m.data_ptr() + at * strides[0] * m.element_size(),) + strides + (o.data_ptr() + at * r * c * 2, r * c, c, 1) + size)
+            sizes.append(size)
+    per = K.ortho_max_groups() if len(groups) <= len(mats) else 1
     with _on(device):
         for k in range(0, len(groups), per):
             nbytes = K.ortho_workspace_of(tuple(sizes[k:k + per]))

@@ -257,6 +257,11 @@ def ortho_max_groups():
     return int(lib().ddl_ortho_max_groups())
 
 
+def ortho_most_matrices(r, c):
+    """Most equal matrices of a group: the launches' threads are counted in 32 bits, up to 1024 for each 64 x 64 tile."""
+    return max(1, min(1 << 20, (1 << 21) // (((r + 63) // 64) * ((c + 63) // 64))))
+
+
 def ortho_table(groups):
     """Table of a call: ``groups`` = (source address, its batch / row / column strides, destination address and strides,
     rows, columns, matrices) tuples."""

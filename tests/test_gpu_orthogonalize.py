@@ -664,3 +664,33 @@ def test_a_refused_optimizer_leaves_the_parameters_where_they_were():
     with pytest.raises(KernelError, match="out of range"):
         FusedMuon(p for p in [("a", small), ("b", large)])
     assert (small.data_ptr(), large.data_ptr()) == at and small.grad is None and large.grad is None
+
+
+# more equal matrices than a launch takes: 2^20 of one tile a call, fewer of more tiles
+@pytest.mark.parametrize("shape", [(4_300_000, 4, 4), (300_000, 2, 900), (60_000, 130, 960)], ids=str)
+def test_stacks_of_more_matrices_than_a_launch_takes(shape):
+    from distributeddeeplearning_amd.ops import functional as ops, kernels
+
+    most = kernels.ortho_most_matrices(*shape[1:])
+    assert most < shape[0]
+    x = torch.zeros(shape, dtype=BF, device=DEV)
+    g = spectrum("gauss", *shape[1:]).to(DEV, BF)
+    at = [0, most - 1, most, 2 * most - 1, shape[0] - 1]
+    at = [k for k in at if k < shape[0]]
+    for k in at:
+        x[k] = g
+    out = ops.orthogonalize(x)
+    assert out.shape == x.shape
+    for k in at:
+        assert off(out[k], g) < TOL
+    assert int(out.flatten(1).any(1).sum()) == len(at)
+    every = ops.orthogonalize(g.expand(shape))            # a stack of strides 0
+    assert torch.equal(every[shape[0] - 1], out[0]) and torch.equal(every[most - 1], every[0])
+
+
+def test_the_most_matrices_of_a_call_are_within_the_launches():
+    from distributeddeeplearning_amd.ops import kernels
+
+    for r, c in ((1, 1), (64, 64), (65, 1), (1, 1000), (33, 1 << 20), (1000, 1000), (128, 130000), (32000, 32000), (1, 1 << 23), (4000, 100000)):
+        n = kernels.ortho_most_matrices(r, c)
+        assert kernels.ortho_workspace_of(((r, c, n),)) >= 0 and kernels.ortho_workspace_of(((c, r, n),)) >= 0
