@@ -1513,7 +1513,7 @@ extern "C" int ddl_orthogonalize(const long long* desc, int count, int kind, flo
     const Desc* q = (const Desc*)desc;
     const long long need = ddl_ortho_workspace(desc, count);
     if (kind < 0 || kind > 1 || need < 0 || ws_bytes < need || (need > 0 && !ws)) return DDL_EINVAL;
-    if (!ddl_ortho_coefficients_ok(a, b, c, steps) || !(eps >= 1e-30f)) return DDL_EINVAL;
+    if (!ddl_ortho_coefficients_ok(a, b, c, steps) || !(eps >= 1e-30f && eps <= 3.1e38f)) return DDL_EINVAL;
     if (reinterpret_cast<uintptr_t>(ws) & 255) return DDL_EALIGN;
     for (int i = 0; i < count; ++i)
         if (!q[i].src || !q[i].dst || !strides_fit(q[i].srs, q[i].scs) || q[i].sb < 0 || q[i].drs != q[i].c || q[i].dcs != 1 ||
@@ -1535,7 +1535,7 @@ extern "C" int ddl_muon_step(const long long* desc, int count, void* w, const vo
     const Desc* q = (const Desc*)desc;
     const long long need = ddl_ortho_workspace(desc, count);
     if (!w || !g || !v || need < 0 || ws_bytes < need || (need > 0 && !ws)) return DDL_EINVAL;
-    if (!ddl_ortho_coefficients_ok(a, b, c, steps) || !(eps >= 1e-30f)) return DDL_EINVAL;
+    if (!ddl_ortho_coefficients_ok(a, b, c, steps) || !(eps >= 1e-30f && eps <= 3.1e38f)) return DDL_EINVAL;
     if ((reinterpret_cast<uintptr_t>(ws) & 255) || !ddl_aligned16(w) || !ddl_aligned16(g) || !ddl_aligned16(v) || (lowp && !ddl_aligned16(lowp)))
         return DDL_EALIGN;
     for (int i = 0; i < count; ++i)

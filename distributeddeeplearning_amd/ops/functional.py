@@ -241,8 +241,8 @@ def _check_steps(steps, coefficients, eps):
     if not _steps_in_range(*map(float, coefficients), steps):
         raise ValueError("orthogonalize: %d steps with the coefficients %r leave the range of the kernels' 16-bit operands"
                          % (steps, tuple(coefficients)))
-    if not eps >= 1e-30:
-        raise ValueError("orthogonalize: eps must be at least 1e-30, got %r" % (eps,))
+    if not 1e-30 <= eps <= 3e38:
+        raise ValueError("orthogonalize: eps must be from 1e-30 to 3e38, got %r" % (eps,))
 
 
 def orthogonalize_plain(x, steps=5, coefficients=ORTHO_COEFFICIENTS, eps=1e-7):

@@ -236,3 +236,19 @@ def test_the_range_of_coefficients_is_the_librarys():
     assert 500 < taken < 3500
     for coef in OUT_OF_RANGE + [(3.4445, -4.7750, 2.0315), (1.5, -0.5, 0.0), (2.0, -1.5, 0.5)]:
         assert ops._steps_in_range(*coef, 5) == kernels.ortho_coefficients_ok(*coef, 5)
+
+
+@pytest.mark.parametrize("eps", [float("inf"), 1e39, -1.0, 1e-31])
+def test_eps_that_fp32_does_not_hold_is_refused(eps):
+    import ctypes as c
+
+    from distributeddeeplearning_amd.ops import kernels, native
+
+    with pytest.raises(ValueError, match="eps"):
+        ops.orthogonalize(torch.zeros(4, 4), eps=eps)
+    with pytest.raises(ValueError, match="eps"):
+        FusedMuon([("w", torch.nn.Parameter(torch.zeros(2, 3)))], eps=eps)
+    if native.kernels_available():
+        table, count = kernels.ortho_table([(64, 90, 9, 1, 64, 90, 9, 1, 10, 9, 1)])
+        assert kernels.lib().ddl_orthogonalize(table, c.c_int(count), c.c_int(0), c.c_float(3.4445), c.c_float(-4.7750), c.c_float(2.0315), c.c_int(5),
+                                               c.c_float(eps), c.c_void_p(256), c.c_longlong(1 << 40), c.c_void_p(0)) == -1
