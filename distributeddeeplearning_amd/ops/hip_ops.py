@@ -1914,7 +1914,7 @@ def orthogonalize(mats, steps, coefficients, eps):
         if max(strides[-2:]) >= 1 << 31:
             m = m.contiguous()
             keep.append(m)
-            strides = m.stride()
+            strides = (r * c, c, 1)[3 - m.dim():]         # (dense; the stride of a dimension of one may be anything)
         if len(strides) == 2:
             strides = (0,) + strides
         # (a stack of more matrices than a launch takes: several groups, each in a call of its own)

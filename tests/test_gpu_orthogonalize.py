@@ -694,3 +694,13 @@ def test_the_most_matrices_of_a_call_are_within_the_launches():
     for r, c in ((1, 1), (64, 64), (65, 1), (1, 1000), (33, 1 << 20), (1000, 1000), (128, 130000), (32000, 32000), (1, 1 << 23), (4000, 100000)):
         n = kernels.ortho_most_matrices(r, c)
         assert kernels.ortho_workspace_of(((r, c, n),)) >= 0 and kernels.ortho_workspace_of(((c, r, n),)) >= 0
+
+
+def test_a_stride_that_is_never_taken_may_be_anything():
+    from distributeddeeplearning_amd.ops import functional as ops
+
+    x = torch.randn(700, generator=torch.Generator().manual_seed(1)).to(DEV)
+    for size, strides in (((1, 700), (1 << 31, 1)), ((700, 1), (1, 1 << 40)), ((1, 1), (1 << 33, 1 << 33)), ((1, 1, 700), (1 << 50, 1 << 31, 1)),
+                          ((7, 1, 100), (100, 1 << 31, 1)), ((1, 7, 100), (1 << 40, 100, 1))):
+        v = x.as_strided(size, strides)
+        assert torch.equal(ops.orthogonalize(v), ops.orthogonalize(v.clone(memory_format=torch.contiguous_format)))
