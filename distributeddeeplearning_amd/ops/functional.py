@@ -26,6 +26,7 @@ import os
 
 import torch
 import torch.nn.functional as F
+from torch.autograd import forward_ad
 
 __all__ = ["use_hip", "conv2d", "conv_bn_act", "residual_block", "batchnorm_act", "maxpool3x3s2", "global_avgpool", "linear",
            "orthogonalize", "quantize_int8", "linear_int8", "softmax_cross_entropy", "topk_correct", "topk_hits", "NoHipKernel", "set_backend", "backend"]
@@ -203,6 +204,11 @@ def linear(x, weight, bias=None):
     return F.linear(x, weight.to(x.dtype), None if bias is None else bias.to(x.dtype))
 
 
+def _has_tangent(t):
+    """True for a dual tensor of forward-mode differentiation."""
+    return forward_ad._current_level >= 0 and forward_ad.unpack_dual(t).tangent is not None
+
+
 ORTHO_COEFFICIENTS = (3.4445, -4.7750, 2.0315)   # five steps take singular values from about 0.002 on into [0.7, 1.2]
 
 
@@ -265,7 +271,7 @@ def orthogonalize(x, steps=5, coefficients=ORTHO_COEFFICIENTS, eps=1e-7):
 
     ``x``: a matrix [r, c], a stack [k, r, c], or a list / tuple of matrices of any shapes (they share the launches), fp32 or
     bf16 of any strides; returns bf16 of the same shape(s).  No gradient flows through it: an input that requires one is
-    refused outside ``torch.no_grad()``.  Matrices do not influence each other; one that holds an infinity or a NaN
+    refused outside ``torch.no_grad()``, a dual tensor always.  Matrices do not influence each other; one that holds an infinity or a NaN
     gives NaN, a zero matrix zeros.  ``coefficients`` whose steps leave the range of 16-bit operands are refused on any device, and on the
     GPU matrices whose sides, rounded up to 64, have a product of 2^30 or more."""
     many = isinstance(x, (list, tuple))
@@ -280,6 +286,8 @@ def orthogonalize(x, steps=5, coefficients=ORTHO_COEFFICIENTS, eps=1e-7):
             raise ValueError("orthogonalize: the matrices of a list must share device and dtype")
         if m.requires_grad and torch.is_grad_enabled():
             raise ValueError("orthogonalize: no gradient flows through it; detach the input or call it under torch.no_grad()")
+        if _has_tangent(m):
+            raise ValueError("orthogonalize: no tangent flows through it; take the primal of the input")
     if not mats:
         return []
     out = None
@@ -303,10 +311,12 @@ def quantize_int8(w):
     """8-bit codes of the rows of ``w`` [n, k] (fp32 or bf16): ``(q, scale)`` with ``q`` int8 [n, k], ``scale`` fp32 [n] and
     ``w ~ q * scale[:, None]``; ``scale = max|row| / 127``, ``q = round(row * (127 * (1 / max|row|)))`` to even, in fp32.  Rows of ``q`` start
     at multiples of 64 bytes, as :func:`linear_int8` reads them.  A row below 1e-30 counts as zero; one that holds an
-    infinity or a NaN has the scale NaN."""
+    infinity or a NaN has the scale NaN.  No gradient and no tangent flows through it."""
     if w.dim() != 2 or w.dtype not in (torch.float32, torch.bfloat16) or w.shape[1] == 0:
         raise ValueError("quantize_int8: an fp32 or bf16 matrix with columns expected, got %s %s" % (w.dtype, tuple(w.shape)))
     w = w.detach()
+    if _has_tangent(w):                       # (detach keeps it)
+        w = forward_ad.unpack_dual(w).primal
     n, k = w.shape
     if w.is_cuda and _FORCED != "aten":
         from . import kernels
@@ -337,7 +347,7 @@ def linear_int8(x, q, scale, bias=None):
     :func:`quantize_int8` does, each with a scale of its own, multiplied with the codes ``q`` [n, k] and ``scale`` [n] of the weights
     and summed exactly: ``y = (xq q^T) * sx * scale + bias`` in fp32, returned in ``x``'s dtype [..., n].  ``bias``: fp32 [n].
     ``q`` as :func:`quantize_int8` returns it (rows start at multiples of 16 bytes).  No gradient flows through it: an input
-    that requires one is refused outside ``torch.no_grad()``.  ``k`` is at most 133 144."""
+    that requires one is refused outside ``torch.no_grad()``, a dual tensor always.  ``k`` is at most 133 144."""
     if (x.dtype is not torch.float32 and x.dtype is not torch.bfloat16) or x.dim() < 1:
         raise ValueError("linear_int8: fp32 or bf16 rows expected, got %s" % x.dtype)
     shape, qshape, device = x.shape, q.shape, x.device
@@ -351,6 +361,8 @@ def linear_int8(x, q, scale, bias=None):
         raise ValueError("linear_int8: input, codes, scales and bias must be on one device")
     if torch.is_grad_enabled() and (x.requires_grad or scale.requires_grad or (bias is not None and bias.requires_grad)):
         raise ValueError("linear_int8: no gradient flows through it; call it under torch.no_grad()")
+    if _has_tangent(x) or _has_tangent(scale) or (bias is not None and _has_tangent(bias)):
+        raise ValueError("linear_int8: no tangent flows through it; take the primal of the input")
     x2 = x if len(shape) == 2 else x.reshape(shape[:-1].numel(), k)
     if device.type == "cuda" and _FORCED != "aten":
         from . import kernels

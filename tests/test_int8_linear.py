@@ -162,3 +162,26 @@ def test_arguments_that_the_kernels_refuse():
                dict(q_bytes=639), dict(ldy=9), dict(ldx=-1), dict(m=1 << 30, n=1 << 30, ldy=1 << 30, q_bytes=1 << 50)):
         assert product(**kw) != 0, kw
     assert product(m=0) == 0 and product(n=0) == 0
+
+
+def test_dual_tensors_are_refused():
+    """Forward-mode differentiation: nothing is passed by silently."""
+    from torch.autograd import forward_ad
+
+    x, w, b = torch.randn(3, 8), torch.randn(5, 8), torch.randn(5)
+    q, s = ops.quantize_int8(w)
+    with forward_ad.dual_level():
+        dual = forward_ad.make_dual
+        for args in ((dual(x, x), q, s, b), (x, q, dual(s, s), b), (x, q, s, dual(b, b))):
+            with pytest.raises(ValueError, match="tangent"):
+                ops.linear_int8(*args)
+        assert torch.equal(ops.linear_int8(x, q, s, b), ops.linear_int8(forward_ad.unpack_dual(dual(x, x)).primal, q, s, b))
+        codes, scale = ops.quantize_int8(dual(w, w))
+        assert forward_ad.unpack_dual(scale).tangent is None and torch.equal(codes, q)
+        for m in (dual(x, x), [w, dual(x, x)]):
+            with pytest.raises(ValueError, match="tangent"):
+                ops.orthogonalize(m)
+    with pytest.raises(ValueError, match="tangent"):
+        torch.func.jvp(lambda t: ops.linear_int8(t, q, s, b), (x,), (x,))
+    with pytest.raises(ValueError, match="tangent"):
+        torch.func.jvp(ops.orthogonalize, (x,), (x,))
