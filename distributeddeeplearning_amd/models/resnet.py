@@ -139,7 +139,8 @@ class Linear(nn.Module):
 
 class Int8Linear(nn.Module):
     """Dense layer that answers from 8-bit weights (``ops.linear_int8``): codes with a scale for each output channel,
-    the input's rows quantised on the way.  Buffers only: it does not train."""
+    the input's rows quantised on the way.  Buffers only: it does not train.  Scales and bias stay fp32 whatever dtype the module is
+    moved to: the codes' exact sums are multiplied with them."""
 
     def __init__(self, cin, cout, bias=True):
         super().__init__()
@@ -148,6 +149,14 @@ class Int8Linear(nn.Module):
         self.register_buffer("codes", torch.zeros(cout, (cin + 63) // 64 * 64, dtype=torch.int8))
         self.register_buffer("scale", torch.zeros(cout))
         self.register_buffer("bias", torch.zeros(cout) if bias else None)
+
+    def _apply(self, fn, recurse=True):
+        kept = {n: self._buffers[n] for n in ("scale", "bias") if self._buffers[n] is not None}
+        super()._apply(fn, recurse)
+        for n, t in kept.items():
+            if self._buffers[n].dtype != torch.float32:
+                self._buffers[n] = t.to(self._buffers[n].device)
+        return self
 
     @classmethod
     def from_linear(cls, linear):

@@ -185,3 +185,19 @@ def test_dual_tensors_are_refused():
         torch.func.jvp(lambda t: ops.linear_int8(t, q, s, b), (x,), (x,))
     with pytest.raises(ValueError, match="tangent"):
         torch.func.jvp(ops.orthogonalize, (x,), (x,))
+
+
+@pytest.mark.parametrize("move", [lambda m: m.to(torch.bfloat16), lambda m: m.half(), lambda m: m.double().float(), lambda m: m.bfloat16().cpu()],
+                         ids=["bf16", "half", "double-float", "bf16-cpu"])
+@pytest.mark.parametrize("bias", [True, False])
+def test_the_layer_keeps_its_scales_when_it_is_moved_to_another_type(move, bias):
+    from distributeddeeplearning_amd.models import Int8Linear
+
+    gen = torch.Generator().manual_seed(2)
+    linear = torch.nn.Linear(70, 9, bias=bias)
+    linear.weight.data = torch.randn(9, 70, generator=gen)
+    layer, x = Int8Linear.from_linear(linear), torch.randn(4, 70, generator=gen)
+    want = layer(x)
+    moved = move(torch.nn.Sequential(layer))
+    assert moved[0].scale.dtype == torch.float32 and torch.equal(moved(x), want)
+    assert moved(x.to(torch.bfloat16)).dtype == torch.bfloat16
