@@ -159,8 +159,12 @@ class Int8Linear(nn.Module):
         return self
 
     @classmethod
-    def from_linear(cls, linear):
-        w = linear.weight.detach()
+    def from_linear(cls, linear, weight=None):
+        """``weight``: what the codes are taken from (default: the layer's own weight)."""
+        w = linear.weight.detach() if weight is None else weight.detach()
+        if w.shape != linear.weight.shape:
+            raise ValueError("Int8Linear: weight %s does not fit the layer's %s" % (tuple(w.shape), tuple(linear.weight.shape)))
+        w = w.to(linear.weight.device)
         m = cls(w.shape[1], w.shape[0], linear.bias is not None).to(w.device)
         q, scale = ops.quantize_int8(w)
         m.codes[:, :w.shape[1]].copy_(q)
@@ -313,11 +317,13 @@ class ResNet(nn.Module):
         return self
 
 
-    def int8_head(self):
+    def int8_head(self, masters=None):
         """For answering: the classifier head from 8-bit weights (:class:`Int8Linear`), taken from the present ones.  The
-        model no longer trains afterwards, and its ``state_dict`` holds codes and scales in the place of ``fc.weight``."""
+        model no longer trains afterwards, and its ``state_dict`` holds codes and scales in the place of ``fc.weight``.
+        ``masters``: the optimizer's ``master_state_dict(model)``; the codes then come from the fp32 weights, not from their
+        bf16 copy, so they are rounded once."""
         if not isinstance(self.fc, Int8Linear):
-            self.fc = Int8Linear.from_linear(self.fc)
+            self.fc = Int8Linear.from_linear(self.fc, None if masters is None else masters.get("fc.weight"))
         return self.eval()
 
 

@@ -201,3 +201,24 @@ def test_the_layer_keeps_its_scales_when_it_is_moved_to_another_type(move, bias)
     moved = move(torch.nn.Sequential(layer))
     assert moved[0].scale.dtype == torch.float32 and torch.equal(moved(x), want)
     assert moved(x.to(torch.bfloat16)).dtype == torch.bfloat16
+
+
+def test_int8_head_from_the_masters():
+    """The codes of the fp32 weights that the optimizer holds, not of their bf16 copy."""
+    from distributeddeeplearning_amd.models import Int8Linear, resnet18
+    from distributeddeeplearning_amd.optim import FusedMuon
+
+    torch.manual_seed(0)
+    model = resnet18(num_classes=12).to_compute("cpu", torch.bfloat16)
+    opt = FusedMuon(model.named_parameters(), lr=0.01)
+    for _, p in model.named_parameters():
+        p.grad.copy_(torch.randn(p.shape))
+    opt.step()
+    masters = opt.master_state_dict(model)
+    q, s = ops.quantize_int8(masters["fc.weight"])
+    rounded = ops.quantize_int8(model.fc.weight)
+    assert not torch.equal(s, rounded[1])
+    with pytest.raises(ValueError, match="fit"):
+        Int8Linear.from_linear(model.fc, masters["fc.weight"][:3])
+    head = model.int8_head(masters).fc
+    assert torch.equal(head.codes[:, :q.shape[1]], q) and torch.equal(head.scale, s)
