@@ -11,12 +11,13 @@
 //   * the diagonals of A and P stay in fp32 (near the end A is close to a multiple of 1: its diagonal carries all of
 //     its rounding): with A = D + O,  A^2 = O^2 + (d_i + d_j) O + D^2, and P X = (a + diag P) X + offdiag(P) X_hi.
 // Against 64 bits the result is, before its rounding to bf16 (1.7e-3 itself), at most this much off (2-norm; Gaussian, power-law,
-// exponential over six decades, rank 1, all but a sixteenth of the singular values a thousandth, gradient-like): 1e-4 .. 1.3e-3 from 32 rows
-// on, 4e-4 .. 1.9e-3 with 8 and 16, 3.2e-3 with 2; bf16 operands throughout give 8e-3 .. 0.3, plain fp16 1e-3 .. 4e-2.
+// exponential over six decades, rank 1, all but a sixteenth of the singular values a thousandth, gradient-like): 1e-4 .. 1.3e-3 from 33 rows
+// on (bf16 operands throughout give 8e-3 .. 0.3, plain fp16 1e-3 .. 4e-2); up to 32 rows, which run in fp64, 1e-7 .. 5e-5.
 //
-// A call takes up to 64 groups of equal matrices; all of them share each launch.  Three forms, by sizes alone:
-//   * every matrix of up to 64 x 768 or 128 x 384: a workgroup a matrix, one launch (ortho_small_kernel, all_small);
-//   * else, or from some length on, every matrix of up to 32 rows: four launches, all steps on the Gram matrix (ortho_thin_*_kernel);
+// A call takes up to 64 groups of equal matrices.  The forms, by sizes alone; the groups of one form share its launches:
+//   * up to 32 rows: all steps on the Gram matrix in fp64, a workgroup a matrix in one launch (ortho_few_kernel), long ones in four
+//     (ortho_thin_*_kernel); see forms_of;
+//   * if all others are of up to 64 x 768 or 128 x 384: a workgroup a matrix, one launch (ortho_small_kernel, all_small);
 //   * else tiles: sums of squares (whose first workgroup writes the table of shapes and offsets, from the kernel's arguments: a
 //     call can be captured or recorded and copies nothing to the device), packing, three products a step; the last product
 //     writes the result or the weights.
@@ -61,7 +62,7 @@ struct Table {
     unsigned fin[MAXG], fio[MAXG], fsym[8][MAXG], fapp[8][MAXG];
     int batch[MAXG], np[MAXG], mp[MAXG], tsym[MAXG], tapp[MAXG], hsym[MAXG], happ[MAXG];      // copies out of g: a lane a group (find_tile)
     unsigned xo[MAXG], ao[MAXG], dof[MAXG], mat[MAXG], slab[MAXG];
-    int split[MAXG];
+    int split[MAXG], lone[MAXG];
 };
 
 __host__ __device__ __forceinline__ unsigned run_start(unsigned total, int home, int xcd) {
@@ -89,7 +90,7 @@ __device__ __forceinline__ void write_table(const Chunk& ch, Table* __restrict__
         t->batch[lane] = g.batch; t->np[lane] = g.np; t->mp[lane] = g.mp;
         t->tsym[lane] = g.tsym; t->tapp[lane] = g.tapp; t->hsym[lane] = g.hsym; t->happ[lane] = g.happ;
         t->xo[lane] = g.xo; t->ao[lane] = g.ao; t->dof[lane] = g.dof; t->mat[lane] = live ? g.mat : 0xffffffffu;
-        t->split[lane] = g.split; t->slab[lane] = g.slab;
+        t->split[lane] = g.split; t->slab[lane] = g.slab; t->lone[lane] = g.r == 1 || g.c == 1;
     }
     const int xcd = k & 7, home = k < 8 ? g.hsym : g.happ;
     const unsigned total = live ? (unsigned)g.batch * (unsigned)(k < 8 ? g.tsym : g.tapp) : 0u;
@@ -112,10 +113,10 @@ __device__ __forceinline__ int find_group(const unsigned* first, unsigned at) {
 // the one that is meant is picked afterwards: a tile waits for one load, not for two in a row.
 // What Item needs of a call's only group (ONE, tiles of 64): it travels in the arguments, a round trip to memory less in each launch
 // (301 x 410 105 -> 101 us, 12 of 512 x 512 153 -> 149)
-struct Single { int np, mp, batch, tsym, tapp, split; };
+struct Single { int np, mp, batch, tsym, tapp, split, lone; };
 template <bool ONE>
 struct Item {
-    int gi, b, tile, np, mp, part, split;
+    int gi, b, tile, np, mp, part, split, lone;
     unsigned xo, ao, dof, mat, slab;
     __device__ __forceinline__ bool find(const Table* t, const Single& one, bool sym) {      // false: this XCD has no such item
         const unsigned xcd = blockIdx.x & 7, at = blockIdx.x >> 3;
@@ -124,6 +125,7 @@ struct Item {
         if (ONE) {
             gi = 0;
             np = one.np;
+            lone = one.lone;
             mp = one.mp;
             xo = ao = dof = mat = slab = 0u;
             const unsigned tiles = sym ? one.tsym : one.tapp, total = (unsigned)one.batch * tiles, idx = at + run_start(total, -1, xcd);
@@ -143,13 +145,14 @@ struct Item {
         const unsigned first = sym ? t->fsym[xcd][lane] : t->fapp[xcd][lane];
         const int l_tiles = sym ? t->tsym[lane] : t->tapp[lane], l_home = sym ? t->hsym[lane] : t->happ[lane];
         const int l_np = t->np[lane], l_mp = t->mp[lane], l_xo = t->xo[lane], l_ao = t->ao[lane], l_dof = t->dof[lane], l_mat = t->mat[lane];
-        const int l_batch = t->batch[lane], l_split = sym ? t->split[lane] : 1;
+        const int l_batch = t->batch[lane], l_split = sym ? t->split[lane] : 1, l_lone = sym ? 0 : t->lone[lane];
         const unsigned l_slab = sym ? t->slab[lane] : 0u;
         gi = __builtin_amdgcn_readfirstlane(__popcll(__ballot(first <= at)) - 1);
         const unsigned tiles = __builtin_amdgcn_readlane(l_tiles, gi);
         const int home = __builtin_amdgcn_readlane(l_home, gi);
         np = __builtin_amdgcn_readlane(l_np, gi);
         mp = __builtin_amdgcn_readlane(l_mp, gi);
+        lone = __builtin_amdgcn_readlane(l_lone, gi);
         xo = __builtin_amdgcn_readlane(l_xo, gi);
         ao = __builtin_amdgcn_readlane(l_ao, gi);
         dof = __builtin_amdgcn_readlane(l_dof, gi);
@@ -179,7 +182,7 @@ __device__ __forceinline__ double wave_sum_d(double v) {
 // What X_lo is multiplied with in the place of P = a + (P - a), whose product reads X_hi alone.  a leaves out (P - a) X_lo, which lies
 // in the directions of large singular values: it is not amplified by later steps.  diag(P) comes nearer to P where P is almost a diagonal,
 // but leaves out offdiag(P) X_lo, which later steps amplify by a each where singular values are small.  So: a, and diag(P) in
-// the last two steps.  Rank 1, 2 x 64: 2e-3 (diag(P) throughout 4.3e-2); Gaussian 512 x 512: 8e-4 (a throughout 1.2e-3).
+// the last two steps.  Rank 1, 64 x 768: 6e-4 (diag(P) throughout 9e-3); Gaussian 512 x 512: 8e-4 (a throughout 1.2e-3).
 __host__ __device__ __forceinline__ bool low_by_a(int step, int steps) { return step < steps - 2; }
 
 struct Muon {                       // K23: arenas of one parameter dtype
@@ -591,7 +594,7 @@ __global__ void __launch_bounds__(KS * W0 * W1 * 64, BF == 128 ? 4 : 2) ortho_ap
             if ((BS > 64 && r >= np) || (BF > 64 && c >= mp)) continue;
             const long long at = xo + (long long)r * mp + c;
             const f16x8 h0 = *reinterpret_cast<const f16x8*>(xh + at), l0 = *reinterpret_cast<const f16x8*>(xl + at);
-            const float dr = d[r], dl = by_a ? ca : dr;
+            const float dr = d[r], dl = by_a && !it.lone ? ca : dr;
             const f32x4 v0 = M::at(tile, s, q), v1 = M::at(tile, s, q + 1);
             float v[8];
 #pragma unroll
@@ -788,20 +791,13 @@ __global__ void __launch_bounds__(512, 2) ortho_small_kernel(const Chunk ch, con
         const float rescale = ldexpf(USC, e1 - e0);
 #pragma unroll
         for (int j = 0; j < NS; ++j) {
-            const float pd = pds[j * 16 + fr] * SC;
-            if (low_by_a(step, steps)) {
-                const float pa = ca * SC;
+            const float pd = pds[j * 16 + fr] * SC, pl = low_by_a(step, steps) && n > 1 ? ca * SC : pd;
 #pragma unroll
-                for (int k = 0; k < CB; ++k)
+            for (int k = 0; k < CB; ++k)
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const float hi = (float)(f16_t)x[k][j][e];
-                        x[k][j][e] = pd * hi + pa * (x[k][j][e] - hi);
-                    }
-            } else {
-#pragma unroll
-                for (int k = 0; k < CB; ++k) x[k][j] *= pd;
-            }
+                for (int e = 0; e < 4; ++e) {
+                    x[k][j][e] = pl * x[k][j][e] + (pd - pl) * (float)(f16_t)x[k][j][e];
+                }
         }
 #pragma unroll
         for (int h = 0; h < NP / 32; ++h) {
@@ -879,10 +875,9 @@ __global__ void __launch_bounds__(512, 2) ortho_small_kernel(const Chunk ch, con
 // ---- thin matrices: all steps on the Gram matrix ------------------------------------------------------------------------
 // Up to 32 rows of any length.  X_k = Q_k X_0 with Q_k and A_k polynomials in A_0: A <- P A P, Q <- P Q on np x np matrices, so the
 // long side is read twice and never iterated on: Gram matrix a chunk of columns a workgroup, all steps in one workgroup a matrix,
-// result a chunk of columns a workgroup.  An error of A_0 grows by up to 3e4 where a singular value vanishes, so A and Q are
+// result a chunk of columns a workgroup.  An error of A_0 grows by up to a^(2 steps) = 2.3e5 where a singular value vanishes, so A and Q are
 // computed in fp64 (its matrix instruction); Q reaches a^steps = 485 with cancelling entries: the result's product is fp32.
-// Bound by the latency of four launches.  Measured against the tiles below: 17 x 2762 105 -> 46 us, 32 x 2048 94 -> 37, 59 of
-// 1 x 3157 209 -> 34, 1000 of 32 x 600 602 -> 192, 32 x 100000 226 -> 131; 64 rows: 86 -> 80 us in fp32, and too few digits.
+// Bound by latency: of four launches, or of a workgroup's loads and fp64 products (ortho_few_kernel; which one: forms_of).
 // Error against 64 bits: 1e-5 before the rounding to bf16.
 typedef double f64x4 __attribute__((ext_vector_type(4)));
 
@@ -986,6 +981,27 @@ __device__ __forceinline__ void thin_mul(const double (*M)[NP + 2], const double
     __syncthreads();
 }
 
+// All steps on np x np matrices in LDS: A holds A_0; returns which of Q holds their product.
+template <int NP, typename Mat>
+__device__ __forceinline__ int thin_steps_of(Mat& A, Mat& P, Mat& T, Mat* Q, float ca, float cb, float cc, int steps) {
+    const double da = ca, db = cb, dc = cc;
+    auto same = [](int, int, double v) { return v; };
+    auto poly = [&](int r, int c, double v) { return db * A[r][c] + dc * v + (r == c ? da : 0.0); };
+    thin_mul<NP>(A, A, Q[0], poly);
+    int at = 0;
+#pragma unroll 1
+    for (int k = 1; k < steps; ++k) {
+        // A <- P A P; P of the first step is Q
+        const Mat& last = k == 1 ? Q[0] : P;
+        thin_mul<NP>(A, last, T, same);
+        thin_mul<NP>(last, T, A, same);
+        thin_mul<NP>(A, A, P, poly);
+        thin_mul<NP>(P, Q[at], Q[at ^ 1], same);
+        at ^= 1;
+    }
+    return at;
+}
+
 template <int NP>
 __global__ void __launch_bounds__(256) ortho_thin_steps_kernel(const Table* __restrict__ t, const double* __restrict__ slabs, float* __restrict__ Qout, float ca,
                                                               float cb, float cc, int steps) {
@@ -1002,49 +1018,23 @@ __global__ void __launch_bounds__(256) ortho_thin_steps_kernel(const Table* __re
         A[k / NP][k % NP] = s;
     }
     __syncthreads();
-    const double da = ca, db = cb, dc = cc;
-    auto same = [](int, int, double v) { return v; };
-    auto poly = [&](int r, int c, double v) { return db * A[r][c] + dc * v + (r == c ? da : 0.0); };
-    thin_mul<NP>(A, A, Q[0], poly);
-    int at = 0;
-#pragma unroll 1
-    for (int k = 1; k < steps; ++k) {
-        // A <- P A P; P of the first step is Q
-        const Mat& last = k == 1 ? Q[0] : P;
-        thin_mul<NP>(A, last, T, same);
-        thin_mul<NP>(last, T, A, same);
-        thin_mul<NP>(A, A, P, poly);
-        thin_mul<NP>(P, Q[at], Q[at ^ 1], same);
-        at ^= 1;
-    }
+    const int at = thin_steps_of<NP>(A, P, T, Q, ca, cb, cc, steps);
     float* out = Qout + (long long)blockIdx.x * NP * NP;
     for (int k = threadIdx.x; k < NP * NP; k += 256) out[k] = (float)Q[at][k / NP][k % NP];
 }
 
-// result = Q X: D rows = columns of X (4 a lane), D columns = rows
+// result = Q X, columns k0, k0 + stride, .. (16 each) before `end`: D rows = columns of X (4 a lane), D columns = rows
 template <int NP, int KIND>
-__global__ void __launch_bounds__(256) ortho_thin_apply_kernel(const Table* __restrict__ t, const Muon mu, const double* __restrict__ part, float eps,
-                                                              const float* __restrict__ Qin) {
+__device__ __forceinline__ void thin_columns(const Group& g, const Muon& mu, int b, bool turn, const float (*Q)[NP + 4], double scale, int k0, int stride, int end) {
     constexpr int NS = NP / 16;
-    __shared__ __attribute__((aligned(16))) float Q[NP][NP + 4];
-    const int gi = find_group(t->fio, blockIdx.x);
-    const Group& g = t->g[gi];
-    const bool turn = g.r > g.c;
-    const int n = turn ? g.c : g.r, m = turn ? g.r : g.c, chunks = g.chunks, width = g.tcols;
-    const unsigned idx = blockIdx.x - t->fio[gi];
-    const int b = idx / chunks, c0 = (idx - b * chunks) * width, end = c0 + width < m ? c0 + width : m;
-    const int lane = threadIdx.x & 63, wid = threadIdx.x >> 6, fr = lane & 15, fq = lane >> 4;
-    const float* from = Qin + ((long long)g.mat + b) * NP * NP;
-    for (int k = threadIdx.x; k < NP * NP; k += 256) Q[k / NP][k % NP] = from[k];
-    const double scale = thin_scale(g, part, b, eps);
+    const int n = turn ? g.c : g.r, lane = threadIdx.x & 63, fr = lane & 15, fq = lane >> 4;
     float lr = 0.f, by = 0.f;
     if (KIND >= 2) {
         lr = mu.lr_scale ? mu.lr * *mu.lr_scale : mu.lr;
         by = lr * sqrtf(turn ? (float)g.r / (float)g.c : 1.f);
     }
-    __syncthreads();
 #pragma unroll 1
-    for (int k = c0 + wid * 16; k < end; k += 64) {
+    for (int k = k0; k < end; k += stride) {
         f32x4 acc[NS];
         float x[NS][4];
 #pragma unroll
@@ -1081,6 +1071,105 @@ __global__ void __launch_bounds__(256) ortho_thin_apply_kernel(const Table* __re
                 }
             }
     }
+}
+
+template <int NP, int KIND>
+__global__ void __launch_bounds__(256) ortho_thin_apply_kernel(const Table* __restrict__ t, const Muon mu, const double* __restrict__ part, float eps,
+                                                              const float* __restrict__ Qin) {
+    __shared__ __attribute__((aligned(16))) float Q[NP][NP + 4];
+    const int gi = find_group(t->fio, blockIdx.x);
+    const Group& g = t->g[gi];
+    const bool turn = g.r > g.c;
+    const int m = turn ? g.r : g.c, chunks = g.chunks, width = g.tcols;
+    const unsigned idx = blockIdx.x - t->fio[gi];
+    const int b = idx / chunks, c0 = (idx - b * chunks) * width, end = c0 + width < m ? c0 + width : m;
+    const float* from = Qin + ((long long)g.mat + b) * NP * NP;
+    for (int k = threadIdx.x; k < NP * NP; k += 256) Q[k / NP][k % NP] = from[k];
+    const double scale = thin_scale(g, part, b, eps);
+    __syncthreads();
+    thin_columns<NP, KIND>(g, mu, b, turn, Q, scale, c0 + (threadIdx.x >> 6) * 16, 64, end);
+}
+
+// The same in one launch, a workgroup of 8 waves a matrix: the Gram matrix of the values as they are (products of fp32 values are exact
+// in fp64), whose trace is the square of the norm; all steps; the result from a second read.
+template <int NP, int KIND>
+__global__ void __launch_bounds__(512) ortho_few_kernel(const Chunk ch, const Muon mu, float ca, float cb, float cc, int steps, float eps) {
+    constexpr int NS = NP / 16, W = 8, EL = (NP * NP + 511) / 512;
+    typedef double Mat[NP][NP + 2];
+    __shared__ Mat mats[W];                              // the waves' sums; then A, P, T, Q[2]
+    __shared__ __attribute__((aligned(16))) float Qf[NP][NP + 4];
+    const int lane = threadIdx.x & 63, wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), fr = lane & 15, fq = lane >> 4;
+    const bool mine = lane < ch.n && ch.g[lane < CHUNK ? lane : 0].fin <= blockIdx.x;
+    const int gi = __builtin_amdgcn_readfirstlane(__popcll(__ballot(mine)) - 1);
+    const Group g = ch.g[gi];
+    const int b = blockIdx.x - g.fin;
+    const bool turn = g.r > g.c;
+    const int n = turn ? g.c : g.r, m = turn ? g.r : g.c;
+    f64x4 acc[NS][NS];
+#pragma unroll
+    for (int i = 0; i < NS; ++i)
+#pragma unroll
+        for (int j = 0; j < NS; ++j) acc[i][j] = f64x4{0.0, 0.0, 0.0, 0.0};
+    struct Cols { float x[NS][4]; };
+    auto load = [&](int k) {
+        Cols v;
+#pragma unroll
+        for (int i = 0; i < NS; ++i)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int r = i * 16 + fr, c = k + fq * 4 + e;
+                v.x[i][e] = r < n && c < m ? thin_value<KIND, false>(g, mu, b, turn, r, c) : 0.f;
+            }
+        return v;
+    };
+    Cols now = load(wid * 16);
+    for (int k = wid * 16; k < m; k += W * 16) {
+        const Cols next = load(k + W * 16);              // (behind the end: zeros)
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+#pragma unroll
+            for (int i = 0; i < NS; ++i)
+#pragma unroll
+                for (int j = 0; j <= i; ++j) acc[i][j] = __builtin_amdgcn_mfma_f64_16x16x4f64((double)now.x[i][e], (double)now.x[j][e], acc[i][j], 0, 0, 0);
+        now = next;
+    }
+#pragma unroll
+    for (int i = 0; i < NS; ++i)
+#pragma unroll
+        for (int j = 0; j <= i; ++j)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int r = i * 16 + fq + 4 * e, c = j * 16 + fr;
+                mats[wid][r][c] = acc[i][j][e];
+                if (i != j) mats[wid][c][r] = acc[i][j][e];
+            }
+    __syncthreads();
+    double sum[EL];
+#pragma unroll
+    for (int q = 0; q < EL; ++q) {
+        const int k = threadIdx.x + q * 512, r = k / NP, c = k % NP;
+        sum[q] = 0.0;
+        if (k < NP * NP)
+#pragma unroll
+            for (int w = 0; w < W; ++w) sum[q] += mats[w][r][c];
+    }
+    double trace = 0.0;
+    if (lane < NP)
+#pragma unroll
+        for (int w = 0; w < W; ++w) trace += mats[w][lane][lane];
+    const double norm = sqrt(wave_sum_d(trace)), scale = 1.0 / (norm > (double)eps ? norm : (norm == norm ? (double)eps : norm));
+    __syncthreads();
+    Mat& A = mats[0];
+#pragma unroll
+    for (int q = 0; q < EL; ++q) {
+        const int k = threadIdx.x + q * 512;
+        if (k < NP * NP) A[k / NP][k % NP] = sum[q] * scale * scale;
+    }
+    __syncthreads();
+    const int at = thin_steps_of<NP>(A, mats[1], mats[2], mats + 3, ca, cb, cc, steps);
+    for (int k = threadIdx.x; k < NP * NP; k += 512) Qf[k / NP][k % NP] = (float)mats[3 + at][k / NP][k % NP];
+    __syncthreads();
+    thin_columns<NP, KIND>(g, mu, b, turn, Qf, scale, wid * 16, W * 16, m);
 }
 
 // ---- host -------------------------------------------------------------------------------------------------------------
@@ -1306,9 +1395,8 @@ long long splits_of(const Desc* q, int count, int sym, int* split) {
 // Calls that ortho_small_kernel serves: every matrix of up to 64 rows (its shorter side) and 768 columns, or 128 and 384 (more
 // do not fit the registers and, 128 rows, LDS).  Tiles against it: 64 x 576 79 -> 34 us, 64 x 768 80 -> 40, 128 x 384 85 -> 62, 1000 of 64 x 600
 // 651 -> 154, 1000 of 128 x 384 832 -> 294.  All are computed in the largest's size, as each size is a launch of 12 to 70 us, most of it the
-// first run of its code: 64 x 147, 64 x 64, 64 x 576, 256 x 64 and 64 x 256 82 -> 34.  Not where the Gram matrix's form is faster:
-// all up to 32 rows and one of more than 512 columns (32 x 1000 31 us, here 48), up to 16 and more than 256 (1000 of 16 x 300 54, here
-// 89; one 9 x 512 22, here 25).  Returns 0: not served; else 8 * padded rows / 64 + the number of the least columns, 128, 256, ..
+// first run of its code: 64 x 147, 64 x 64, 64 x 576, 256 x 64 and 64 x 256 82 -> 34.  Returns 0: not served; else 8 * padded rows / 64 + the number
+// of the least columns, 128, 256, ..
 int all_small(const Desc* q, int count) {
     long long most = 0, wide = 0;
     for (int i = 0; i < count; ++i) {
@@ -1316,7 +1404,6 @@ int all_small(const Desc* q, int count) {
         most = n > most ? n : most;
         wide = m > wide ? m : wide;
     }
-    if ((most <= 16 && wide > 256) || (most <= 32 && wide > 512)) return 0;
     if (most <= 64 && wide <= 768) return 8 + (wide <= 128 ? 0 : wide <= 256 ? 1 : wide <= 512 ? 2 : 3);
     if (most <= 128 && wide <= 384) return 16 + (wide <= 128 ? 0 : wide <= 256 ? 1 : 2);
     return 0;
@@ -1361,11 +1448,63 @@ int run_small(const Desc* q, int count, int cls, int kind, const Muon& mu, float
     return DDL_OK;
 }
 
-// kind as in load8
-int run_all(const Desc* q, int count, int kind, const Muon& mu, float a, float b, float c, int steps, float eps, char* ws, hipStream_t stream) {
+// matrices that ortho_few_kernel serves, whatever their number
+int run_few(const Desc* q, int count, int kind, const Muon& mu, float a, float b, float c, int steps, float eps, hipStream_t stream) {
+    const int rows = thin_rows(q, count);
+    for (int base = 0; base < count; base += CHUNK) {
+        Chunk ch;
+        memset(&ch, 0, sizeof(ch));
+        long long grid = 0;
+        for (int i = base; i < count && i < base + CHUNK; ++i) {
+            Group& o = ch.g[ch.n++];
+            const Desc& s = q[i];
+            o.src = (const void*)s.src; o.dst = (bf16_t*)s.dst; o.sb = s.sb; o.rs = (int)s.srs; o.cs = (int)s.scs;
+            o.r = (int)s.r; o.c = (int)s.c; o.batch = (int)s.batch;
+            o.fin = (unsigned)grid;
+            grid += s.batch;
+        }
+        if (grid > most_wgs(512)) return DDL_EINVAL;
+#define FEW(NP, K) DDL_KLAUNCH((ortho_few_kernel<NP, K>), dim3((unsigned)grid), dim3(512), 0, stream, ch, mu, a, b, c, steps, eps)
+#define FEW1(K) { if (rows == 16) FEW(16, K); else FEW(32, K); }
+        if (kind == 0) FEW1(0) else if (kind == 1) FEW1(1) else if (kind == 2) FEW1(2) else FEW1(3)
+#undef FEW1
+#undef FEW
+        const int rc = ddl_launch_status();
+        if (rc != DDL_OK) return rc;
+    }
+    return DDL_OK;
+}
+
+// A call's groups by form.  Up to 32 rows the fp16 products of the other forms would leave 1e-3 .. 3e-3 (few values to average over), so
+// where the steps allow it (thin_steps) such matrices always run on their Gram matrix: `few` in one launch, `thin` in four that spread
+// long rows over the chip.  Measured (us, few / thin): 16 x 64 8.5 / 15.7, 16 x 512 17 / 18, 16 x 1024 26 / 19, 32 x 256 23 / 28,
+// 32 x 512 32 / 28, 64 of 16 x 2048 45 / 30, 1000 of 16 x 2048 128 / 212, 1000 of 32 x 8192 1370 / 2380: few up to 512 columns (above 16 rows
+// 256) or where a stack has a matrix for each CU; the rest of a call's then share thin's launches.
+// One row has no offdiagonal values: it is exact in every form and goes along with the others, if they are of one form.
+struct Forms {
+    Desc few[MAXG], thin[MAXG], rest[MAXG];
+    int nfew = 0, nthin = 0, nrest = 0;
+};
+void forms_of(const Desc* q, int count, bool steps_fit, Forms& f) {
+    bool gram = false, other = false, spread = false;
+    for (int i = 0; i < count; ++i) {
+        const long long n = q[i].r < q[i].c ? q[i].r : q[i].c, m = q[i].r < q[i].c ? q[i].c : q[i].r;
+        gram = gram || (n > 1 && n <= 32);
+        other = other || n > 32;
+        spread = spread || (n <= 32 && q[i].batch < 256 && m > (n > 16 ? 256 : 512));
+    }
+    for (int i = 0; i < count; ++i) {
+        const long long n = q[i].r < q[i].c ? q[i].r : q[i].c;
+        if (!steps_fit || n > 32 || (n == 1 && other && !gram)) f.rest[f.nrest++] = q[i];
+        else if (q[i].batch >= 256 || !spread) f.few[f.nfew++] = q[i];
+        else f.thin[f.nthin++] = q[i];
+    }
+}
+
+// the forms that have a table in the workspace: thin, or tiles; kind as in load8
+int run_table(const Desc* q, int count, bool thin, int kind, const Muon& mu, float a, float b, float c, int steps, float eps, char* ws, hipStream_t stream) {
     Plan pl;
-    if (!plan_of(q, count, thin_steps(a, b, c, steps), pl)) return DDL_EINVAL;
-    if (const int cls = all_small(q, count)) return run_small(q, count, cls, kind, mu, a, b, c, steps, eps, stream);
+    if (!plan_of(q, count, thin, pl)) return DDL_EINVAL;
     int sb = 64, ab = 64, split[MAXG];
     tiles_of(q, count, sb, ab);
     splits_of(q, count, sb, split);
@@ -1413,7 +1552,7 @@ int run_all(const Desc* q, int count, int kind, const Muon& mu, float a, float b
     nsym = homes(g, count, true, csym);
     napp = homes(g, count, false, capp);
     if (nsym > most_wgs(512) || napp > most_wgs(512)) return DDL_EINVAL;
-    const Single one = count == 1 ? Single{g[0].np, g[0].mp, g[0].batch, g[0].tsym, g[0].tapp, g[0].split} : Single{};
+    const Single one = count == 1 ? Single{g[0].np, g[0].mp, g[0].batch, g[0].tsym, g[0].tapp, g[0].split, g[0].r == 1 || g[0].c == 1} : Single{};
     Table* t = (Table*)(ws + pl.table);
     f16_t *xh = (f16_t*)(ws + pl.xa_h), *xl = (f16_t*)(ws + pl.xa_l), *yh = (f16_t*)(ws + pl.xb_h), *yl = (f16_t*)(ws + pl.xb_l);
     f16_t *O = (f16_t*)(ws + pl.o), *P = (f16_t*)(ws + pl.p);
@@ -1485,6 +1624,32 @@ int run_all(const Desc* q, int count, int kind, const Muon& mu, float a, float b
     return ddl_launch_status();
 }
 
+int run_all(const Desc* q, int count, int kind, const Muon& mu, float a, float b, float c, int steps, float eps, char* ws, hipStream_t stream) {
+    Forms f;
+    forms_of(q, count, thin_steps(a, b, c, steps), f);
+    int rc = DDL_OK;
+    // (one after another in the stream: they share the workspace)
+    if (f.nfew) rc = run_few(f.few, f.nfew, kind, mu, a, b, c, steps, eps, stream);
+    if (rc == DDL_OK && f.nthin) rc = run_table(f.thin, f.nthin, true, kind, mu, a, b, c, steps, eps, ws, stream);
+    if (rc == DDL_OK && f.nrest) {
+        if (const int cls = all_small(f.rest, f.nrest)) rc = run_small(f.rest, f.nrest, cls, kind, mu, a, b, c, steps, eps, stream);
+        else rc = run_table(f.rest, f.nrest, false, kind, mu, a, b, c, steps, eps, ws, stream);
+    }
+    return rc;
+}
+
+// -1: sizes out of range
+long long workspace_of(const Desc* q, int count, float a, float b, float c, int steps) {
+    Plan whole, gram;              // (of one form each: what either takes)
+    if (!plan_of(q, count, true, gram) || !plan_of(q, count, false, whole)) return -1;
+    Forms f;
+    forms_of(q, count, thin_steps(a, b, c, steps), f);
+    Plan thin, tiles;
+    if (f.nthin && !plan_of(f.thin, f.nthin, true, thin)) return -1;
+    if (f.nrest && !all_small(f.rest, f.nrest) && !plan_of(f.rest, f.nrest, false, tiles)) return -1;
+    return thin.bytes > tiles.bytes ? thin.bytes : tiles.bytes;
+}
+
 bool strides_fit(long long rs, long long cs) { return rs >= 0 && cs >= 0 && rs < (1LL << 31) && cs < (1LL << 31); }
 
 }  // namespace
@@ -1498,12 +1663,9 @@ extern "C" int ddl_ortho_coefficients_ok(float a, float b, float c, int steps) {
 }
 
 // bytes of workspace of a call with these groups (`desc`: count x 11 int64: source address, its batch / row / column
-// strides, destination address and strides, rows, columns, matrices), 0: none, -1: sizes out of range
-extern "C" long long ddl_ortho_workspace(const long long* desc, int count) {
-    Plan one, other;               // (which of the forms is taken depends on the steps too)
-    if (!plan_of((const Desc*)desc, count, true, one) || !plan_of((const Desc*)desc, count, false, other)) return -1;
-    if (all_small((const Desc*)desc, count)) return 0;
-    return one.bytes > other.bytes ? one.bytes : other.bytes;
+// strides, destination address and strides, rows, columns, matrices) and steps, 0: none, -1: sizes out of range
+extern "C" long long ddl_ortho_workspace(const long long* desc, int count, float a, float b, float c, int steps) {
+    return workspace_of((const Desc*)desc, count, a, b, c, steps);
 }
 
 // kind 0 / 1: fp32 / bf16 sources; destinations are dense bf16 (other strides are refused)
@@ -1511,7 +1673,7 @@ extern "C" int ddl_orthogonalize(const long long* desc, int count, int kind, flo
                                  long long ws_bytes, hipStream_t stream) {
     if (count == 0) return DDL_OK;
     const Desc* q = (const Desc*)desc;
-    const long long need = ddl_ortho_workspace(desc, count);
+    const long long need = workspace_of(q, count, a, b, c, steps);
     if (kind < 0 || kind > 1 || need < 0 || ws_bytes < need || (need > 0 && !ws)) return DDL_EINVAL;
     if (!ddl_ortho_coefficients_ok(a, b, c, steps) || !(eps >= 1e-30f && eps <= 3.1e38f)) return DDL_EINVAL;
     if (reinterpret_cast<uintptr_t>(ws) & 255) return DDL_EALIGN;
@@ -1533,7 +1695,7 @@ extern "C" int ddl_muon_step(const long long* desc, int count, void* w, const vo
                              long long ws_bytes, hipStream_t stream) {
     if (count == 0) return DDL_OK;
     const Desc* q = (const Desc*)desc;
-    const long long need = ddl_ortho_workspace(desc, count);
+    const long long need = workspace_of(q, count, a, b, c, steps);
     if (!w || !g || !v || need < 0 || ws_bytes < need || (need > 0 && !ws)) return DDL_EINVAL;
     if (!ddl_ortho_coefficients_ok(a, b, c, steps) || !(eps >= 1e-30f && eps <= 3.1e38f)) return DDL_EINVAL;
     if ((reinterpret_cast<uintptr_t>(ws) & 255) || !ddl_aligned16(w) || !ddl_aligned16(g) || !ddl_aligned16(v) || (lowp && !ddl_aligned16(lowp)))

@@ -1926,7 +1926,7 @@ def orthogonalize(mats, steps, coefficients, eps):
     per = K.ortho_max_groups() if len(groups) <= len(mats) else 1
     with _on(device):
         for k in range(0, len(groups), per):
-            nbytes = K.ortho_workspace_of(tuple(sizes[k:k + per]))
+            nbytes = K.ortho_workspace_of(tuple(sizes[k:k + per]), coefficients, steps)
             work = torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
             K.orthogonalize(*K.ortho_table(groups[k:k + per]), bf16, coefficients, steps, eps, work)
     return outs

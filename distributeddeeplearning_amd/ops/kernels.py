@@ -276,20 +276,21 @@ def ortho_coefficients_ok(a, b, c, steps):
     return bool(f(a, b, c, steps))
 
 
-def ortho_workspace(table, count):
-    """Bytes of workspace of a call; 0: it needs none."""
+def ortho_workspace(table, count, coefficients=(3.4445, -4.7750, 2.0315), steps=5):
+    """Bytes of workspace of a call with these steps; 0: it needs none."""
     f = getattr(lib(), "ddl_ortho_workspace")
     f.restype = ctypes.c_longlong
-    n = int(f(table, _i32(count)))
+    a, b, c = map(ctypes.c_float, coefficients)
+    n = int(f(table, _i32(count), a, b, c, _i32(steps)))
     if n < 0:
         raise KernelError("orthogonalize: sizes out of range")
     return n
 
 
 @functools.lru_cache(maxsize=256)
-def ortho_workspace_of(sizes):
+def ortho_workspace_of(sizes, *steps):
     """The same from the groups' (rows, columns, matrices) alone."""
-    return ortho_workspace(*ortho_table([(0,) * 8 + s for s in sizes]))
+    return ortho_workspace(*ortho_table([(0,) * 8 + s for s in sizes]), *steps)
 
 
 def orthogonalize(table, count, src_bf16, coefficients, steps, eps, work):

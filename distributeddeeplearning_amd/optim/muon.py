@@ -70,8 +70,18 @@ class FusedMuon(_ArenaOptimizer):
             rows = [(0, s.offset, 0, 0, 0, 0, 0, 0, s.shape[0], s.numel // s.shape[0], 1) for s in entry["segments"]]
             per = kernels.ortho_max_groups()
             tables = [kernels.ortho_table(rows[k:k + per]) for k in range(0, len(rows), per)]
-            entry["calls"] = [(t, n, kernels.ortho_workspace(t, n)) for t, n in tables]
+            entry["calls"] = [(t, n, {}) for t, n in tables]
         return entry["calls"]
+
+    @staticmethod
+    def _workspace(table, count, known, coefficients, steps):
+        """Bytes of a call's workspace (``known``: what earlier steps found)."""
+        from ..ops import kernels
+
+        key = (coefficients, steps)
+        if key not in known:
+            known[key] = kernels.ortho_workspace(table, count, coefficients, steps)
+        return known[key]
 
     # the vectors' rate is a device scalar of its own: lr * vector_lr_scale is rounded to fp32 once, as where it is passed by value
     def freeze_lr(self):
@@ -121,7 +131,8 @@ class FusedMuon(_ArenaOptimizer):
             w, g, v = self._weights(dt), self.arena.grads[dt], self.momentum_buf[dt]
             if hip:
                 lowp = self.arena.params[dt] if dt in self.master else None
-                for table, count, nbytes in self._tables(entry):
+                for table, count, known in self._tables(entry):
+                    nbytes = self._workspace(table, count, known, coefficients, steps)
                     work = torch.empty(nbytes, dtype=torch.uint8, device=w.device) if nbytes else None
                     kernels.muon_step_(table, count, w, g, v, lowp, klr, mu, run_wd, nesterov, kscale, coefficients,
                                        steps, eps, work)

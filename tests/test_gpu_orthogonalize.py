@@ -704,3 +704,62 @@ def test_a_stride_that_is_never_taken_may_be_anything():
                           ((7, 1, 100), (100, 1 << 31, 1)), ((1, 7, 100), (1 << 40, 100, 1))):
         v = x.as_strided(size, strides)
         assert torch.equal(ops.orthogonalize(v), ops.orthogonalize(v.clone(memory_format=torch.contiguous_format)))
+
+
+# Up to 32 rows the direction is Q X_0 in fp32, a sum of up to 32 terms whose two factors are rounded: 34 * 2^-24 |Q| |X_0| with |Q| <= 3.4445^5 = 485
+# and |X_0| = 1, against a result of 0.68 at least in its largest direction.  (Q's own error: 2^-53 * 485^2.)
+FEW_LIMIT = 34 * 485 * 2 ** -24 / 0.68
+FEW = [(2, 8), (8, 2), (2, 64), (3, 16), (4, 64), (5, 9), (16, 16), (16, 512), (16, 513), (17, 256), (17, 257), (32, 256), (32, 700), (700, 30), (31, 3000)]
+BESIDE = {"alone": [], "small": [(64, 147), (100, 90)], "tiles": [(300, 200), (40, 900)]}
+
+
+def directions(mats):
+    """fp32 directions of one FusedMuon step from zero, all in one call."""
+    from distributeddeeplearning_amd.optim import FusedMuon
+
+    ps = [torch.nn.Parameter(torch.zeros(m.shape, device=DEV)) for m in mats]
+    opt = FusedMuon([("w%d" % i, p) for i, p in enumerate(ps)], lr=1.0, momentum=0.0, nesterov=False)
+    for p, m in zip(ps, mats):
+        p.grad.copy_(m)
+    opt.step()
+    return [-p.detach() / max(1.0, p.shape[0] / p.shape[1]) ** 0.5 for p in ps]
+
+
+@pytest.mark.parametrize("beside", sorted(BESIDE))
+@pytest.mark.parametrize("kind", ["gauss", "rank1", "exp"])
+def test_few_rows_keep_their_digits_in_any_call(kind, beside):
+    from distributeddeeplearning_amd.ops import functional as ops
+
+    small = [s for s in FEW if max(s) <= (512 if min(s) <= 16 else 256)]
+    for shapes in ([[s] for s in FEW] if beside == "alone" else []) + [FEW, small]:
+        mats = [spectrum(kind, *s, seed=i).to(DEV) for i, s in enumerate(shapes + BESIDE[beside])]
+        for m, d, o in zip(mats, directions(mats), ops.orthogonalize(mats)):
+            want = oracle(m.cpu()).to(DEV)
+            limit = FEW_LIMIT if min(m.shape) <= 32 else direction_limit(m.shape)
+            assert float((d.double() - want).norm() / want.norm()) < limit, tuple(m.shape)
+            assert float((o.double() - want).norm() / want.norm()) < limit + 2 ** -8, tuple(m.shape)
+
+
+@pytest.mark.parametrize("beside", [[], [(64, 147)], [(300, 200)], [(300, 200), (5, 40)]], ids=str)
+def test_one_row_keeps_its_digits_in_any_call(beside):
+    # beside larger ones: A is a sum of squares of values rounded to fp16, off by 2 * 2^-11 / sqrt(3) sqrt(3 / 300) = 5.6e-5 of it in the mean; a
+    # step's factor a + b A + c A^2 by 0.71 of that (A near 1), five of them added up: 2e-4 of a result of 0.7
+    shapes = [(1, 300), (2000, 1), (1, 1), (1, 5000)]
+    mats = [spectrum("gauss", *s, seed=i).to(DEV) for i, s in enumerate(shapes + beside)]
+    for m, d in list(zip(mats, directions(mats)))[:4]:
+        want = oracle(m.cpu()).to(DEV)
+        limit = 3e-4 * max(1.0, (300 / max(m.shape)) ** 0.5) if beside else FEW_LIMIT
+        assert float((d.double() - want).norm() / want.norm()) < limit, tuple(m.shape)
+
+
+def test_stacks_of_few_rows():
+    """A matrix for each CU: one launch whatever the length; beside strides."""
+    from distributeddeeplearning_amd.ops import functional as ops
+
+    for dtype in (torch.float32, BF):
+        x = spectrum("gauss", 300 * 20, 1100, 3).to(DEV, dtype).view(300, 20, 1100)
+        for s in (x, x.transpose(1, 2), x[:, 3:, 1::2], x[:1].expand(260, 20, 1100)):
+            out = ops.orthogonalize(s)
+            for k in (0, 1, s.shape[0] - 1):
+                want = oracle(s[k].cpu()).to(DEV)
+                assert float((out[k].double() - want).norm() / want.norm()) < FEW_LIMIT + 2 ** -8
