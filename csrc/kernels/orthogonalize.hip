@@ -634,7 +634,7 @@ __global__ void __launch_bounds__(KS * W0 * W1 * 64, BF == 128 ? 4 : 2) ortho_ap
 // ---- small matrices: all steps in one launch ----------------------------------------------------------------------------
 // One workgroup of 8 waves a matrix: np = NP padded rows, up to 128 CB columns.  X stays in registers in fp32 (in the layout of the
 // products' results: wave w has the 16-column blocks w, w + 8, ..; a lane 4 columns of rows lane % 16 + 16 j), X_hi, O and
-// P in LDS; pd X (lo: by a) is the accumulator that P X is added to.  What bounds it is latency: 64 x 64 takes 12 us here,
+// P in LDS; pd X (lo: by a) is the accumulator that P X is added to.  What bounds it is latency: 64 x 64 takes 13 us here,
 // and the tiles 17 launches of 5 us.
 template <int NP, int CB, int KIND>
 __global__ void __launch_bounds__(512, 2) ortho_small_kernel(const Chunk ch, const Muon mu, float ca, float cb, float cc, int steps, int fall, float eps) {
@@ -1393,9 +1393,9 @@ long long splits_of(const Desc* q, int count, int sym, int* split) {
 }
 
 // Calls that ortho_small_kernel serves: every matrix of up to 64 rows (its shorter side) and 768 columns, or 128 and 384 (more
-// do not fit the registers and, 128 rows, LDS).  Tiles against it: 64 x 576 79 -> 34 us, 64 x 768 80 -> 40, 128 x 384 85 -> 62, 1000 of 64 x 600
-// 651 -> 154, 1000 of 128 x 384 832 -> 294.  All are computed in the largest's size, as each size is a launch of 12 to 70 us, most of it the
-// first run of its code: 64 x 147, 64 x 64, 64 x 576, 256 x 64 and 64 x 256 82 -> 34.  Returns 0: not served; else 8 * padded rows / 64 + the number
+// do not fit the registers and, 128 rows, LDS).  Tiles against it: 64 x 576 79 -> 37 us, 64 x 768 80 -> 43, 128 x 384 85 -> 66, 1000 of 64 x 600
+// 651 -> 169, 1000 of 128 x 384 832 -> 309.  All are computed in the largest's size, as each size is a launch that takes as long as its steps
+// (64 x 64 1.8 us a step and 4.3, 64 x 576 4.9 and 12, 128 x 384 10.3 and 14): 64 x 147, 64 x 64, 64 x 576, 256 x 64 and 64 x 256 82 -> 36.  Returns 0: not served; else 8 * padded rows / 64 + the number
 // of the least columns, 128, 256, ..
 int all_small(const Desc* q, int count) {
     long long most = 0, wide = 0;

@@ -269,6 +269,8 @@ def orthogonalize(x, steps=5, coefficients=ORTHO_COEFFICIENTS, eps=1e-7):
     """Newton-Schulz orthogonalisation: ``X = G / max(|G|_F, eps)``, then ``steps`` times ``X <- a X + (b A + c A^2) X``
     with ``A = X X^T`` over the shorter side - every singular value of ``G`` is driven towards 1, its vectors stay.
 
+    On the GPU the result is, before its rounding to bf16, about 1e-3 off where both sides are above 32 (products of 16-bit operands), 1e-5 else.
+
     ``x``: a matrix [r, c], a stack [k, r, c], or a list / tuple of matrices of any shapes (they share the launches), fp32 or
     bf16 of any strides; returns bf16 of the same shape(s).  No gradient flows through it: an input that requires one is
     refused outside ``torch.no_grad()``, a dual tensor always.  Matrices do not influence each other; one that holds an infinity or a NaN

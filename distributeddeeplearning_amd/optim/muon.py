@@ -9,7 +9,8 @@ For vectors: the rule of ``FusedSGD`` with ``vector_lr_scale*lr``.
 
 The reference has plain momentum SGD only (``imagenet_pytorch_horovod.py:333``); a third optimizer next to ``FusedSGD`` and
 ``FusedLARS``, with the same arenas, checkpoints, launch tape and learning-rate handling.  All matrices of a step share the
-launches (up to 64 matrices each).  Like ``FusedLARS`` it updates after the last gradient bucket: a bucket at a time would
+launches of their form (up to 64 matrices a call).  Their products are those of ``orthogonalize``: 16-bit operands above 32 rows,
+for fp32 parameters too.  Like ``FusedLARS`` it updates after the last gradient bucket: a bucket at a time would
 leave the products of a few matrices alone on the chip.  Every rank orthogonalises every matrix, in a fixed order: replicas
 stay equal bit for bit.
 """
