@@ -1334,7 +1334,7 @@ int growth_bits(float a, float b, float c, int steps) {
 // 2^18 for five steps of the usual coefficients), and Q, rounded to fp32, by what X grows by (485)
 bool thin_steps(float a, float b, float c, int steps) {
     double growth;
-    return range_of(a, b, c, steps, growth) && steps * log2(growth) <= 10.0;
+    return steps >= 1 && steps <= 64 && range_of(a, b, c, steps, growth) && steps * log2(growth) <= 10.0;
 }
 
 // Tile sizes of a call.  Larger tiles need less LDS and L2 traffic a product (256 CUs full: 64 x 64 650, 128 x 128 890, 256 x 256

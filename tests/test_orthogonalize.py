@@ -252,3 +252,19 @@ def test_eps_that_fp32_does_not_hold_is_refused(eps):
         table, count = kernels.ortho_table([(64, 90, 9, 1, 64, 90, 9, 1, 10, 9, 1)])
         assert kernels.lib().ddl_orthogonalize(table, c.c_int(count), c.c_int(0), c.c_float(3.4445), c.c_float(-4.7750), c.c_float(2.0315), c.c_int(5),
                                                c.c_float(eps), c.c_void_p(256), c.c_longlong(1 << 40), c.c_void_p(0)) == -1
+
+
+def test_any_number_of_steps_is_answered_at_once():
+    """The library's checks are not as long as the number of steps that they refuse."""
+    import time
+
+    from distributeddeeplearning_amd.ops import kernels, native
+
+    if not native.kernels_available():
+        pytest.skip("kernel library not built")
+    table, count = kernels.ortho_table([(64, 90, 9, 1, 64, 90, 9, 1, 10, 9, 1)])
+    start = time.perf_counter()
+    for steps in (2 ** 31 - 1, 10 ** 9, -1, -(2 ** 31)):
+        kernels.ortho_workspace(table, count, (1.5, -0.5, 0.0), steps)
+        assert not kernels.ortho_coefficients_ok(1.5, -0.5, 0.0, steps)
+    assert time.perf_counter() - start < 1.0
