@@ -608,16 +608,14 @@ def direction_limit(shape):
     return math.sqrt(15) * 3 * 2 ** -11 / (math.sqrt(3) if min(shape) >= 16 else 1)
 
 
-@pytest.mark.parametrize("kind", ["gauss", "power", "exp", "rank1", "lowrank"])
-@pytest.mark.parametrize("shape", [(2, 8), (2, 64), (4, 64), (64, 3), (8, 256), (16, 256), (32, 512), (64, 64), (64, 768), (768, 64), (33, 1000), (128, 384),
-                                   (1000, 40), (129, 300), (256, 1024), (520, 512), (2040, 2001)], ids=str)
+@pytest.mark.parametrize("shape, kind", [(s, k) for k in ["gauss", "power", "exp", "rank1", "lowrank"] for s in
+                                         [(2, 8), (2, 64), (4, 64), (64, 3), (8, 256), (16, 256), (32, 512), (64, 64), (64, 768), (768, 64), (33, 1000), (128, 384),
+                                          (1000, 40), (129, 300), (256, 1024), (520, 512)] + ([(2040, 2001)] if k in ("gauss", "rank1") else [])], ids=str)
 def test_the_direction_of_any_spectrum(shape, kind):
     """The fp32 weights that a step from zero leaves: the direction itself, in each form."""
     from distributeddeeplearning_amd.ops import functional as ops
     from distributeddeeplearning_amd.optim import FusedMuon
 
-    if max(shape) > 2000 and kind not in ("gauss", "rank1"):
-        pytest.skip("the large one: two spectra")
     p = torch.nn.Parameter(torch.zeros(shape, device=DEV))
     opt = FusedMuon([("w", p)], lr=1.0, momentum=0.0, nesterov=False)
     g = spectrum(kind, *shape, seed=11).to(DEV)
